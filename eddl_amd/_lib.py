@@ -9,7 +9,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("EDDLHIP_LIBRARY") or os.path.join(_HERE, "libeddlhip.so")
 
-c_int, c_float, c_size_t, c_void_p = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_int, c_float, c_size_t, c_void_p, c_longlong = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_longlong
 P = c_void_p  # device pointers travel as integers
 intp = ctypes.POINTER(c_int)
 
@@ -86,6 +86,13 @@ PROTOTYPES = {
     "eddlhip_mult2d": [c_int, P, P, P, c_int, c_int, c_int, c_int],
     "eddlhip_sum2d_rowwise": [c_int, P, P, P, c_int, c_int],
     "eddlhip_dense_fwd": [c_int, P, P, P, P, c_int, c_int, c_int, c_int],
+    "eddlhip_rotary_axes": [c_int, P, c_longlong, P, c_longlong, c_int, c_int, c_int, P, c_int, c_int, c_int, P, P],
+    "eddlhip_paged_append": [c_int] + [P, c_longlong] * 4 + [c_int] * 4 + [P, c_int, c_int, c_int, P, P, P, P] + [c_int] * 3
+                            + [P, c_int, P, P, c_int, c_int],
+    "eddlhip_paged_attention": [c_int, P, c_longlong, P, c_longlong, c_int, P, P] + [c_int] * 6 + [P, c_int, P, P] + [c_int] * 3
+                               + [c_float, c_int, c_int],
+    "eddlhip_norm_residual": [c_int, P, c_longlong, P, c_longlong, c_float, P, c_longlong, P, c_longlong, c_int, c_int, c_int, P, P, c_float, P, c_int,
+                              c_int, P, P, c_float, P, P, c_int],
 }
 _RESTYPE = {"eddlhip_version": ctypes.c_char_p, "eddlhip_last_error": ctypes.c_char_p,
             "eddlhip_conv2d_last_kernel": ctypes.c_char_p}

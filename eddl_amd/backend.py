@@ -15,14 +15,23 @@ class EddlHipError(RuntimeError):
     """A C ABI call returned a negative code; the text is eddlhip_last_error()."""
 
 
-class DeviceTensor:
-    """A float32 tensor in HBM owned by this object (freed when collected)."""
+# bytes of an element, and the numpy type that host copies have (bfloat16 travels as its 16 bits)
+_TYPES = {"float32": (4, np.float32), "int32": (4, np.int32), "bfloat16": (2, np.uint16)}
 
-    def __init__(self, backend, shape):
+
+class DeviceTensor:
+    """A tensor in HBM owned by this object (freed when collected): float32, or, where an operator asks for them, int32 and bfloat16."""
+    dtype = "float32"
+
+    def __init__(self, backend, shape, dtype="float32"):
         self.backend = backend
         self.shape = tuple(int(d) for d in shape)
         self.size = int(np.prod(self.shape)) if len(self.shape) else 1
-        self.nbytes = self.size * 4
+        if dtype not in _TYPES:
+            raise ValueError("no tensors of type %s: %s" % (dtype, ", ".join(_TYPES)))
+        if dtype != "float32":
+            self.dtype = dtype
+        self.nbytes = self.size * _TYPES[dtype][0]
         self.ptr = backend._malloc(self.nbytes)
 
     def __del__(self):
@@ -34,12 +43,12 @@ class DeviceTensor:
             pass
 
     def numpy(self):
-        out = np.empty(self.shape, np.float32)
+        out = np.empty(self.shape, _TYPES[self.dtype][1])
         self.backend._check(self.backend.lib.eddlhip_memcpy_d2h(self.backend.dev, out.ctypes.data, self.ptr, self.nbytes))
         return out
 
     def copy_from(self, host):
-        host = np.ascontiguousarray(host, dtype=np.float32)
+        host = np.ascontiguousarray(host, dtype=_TYPES[self.dtype][1])
         if host.size != self.size:
             raise ValueError("size mismatch: %s vs %s" % (host.shape, self.shape))
         self.backend._check(self.backend.lib.eddlhip_memcpy_h2d(self.backend.dev, self.ptr, host.ctypes.data, self.nbytes))
@@ -53,13 +62,35 @@ class DeviceTensor:
         if int(np.prod(view.shape)) != self.size:
             raise ValueError("reshape changes the size")
         view._base = self  # keeps the owner alive
+        if self.dtype != "float32":
+            view.dtype = self.dtype
         view.__class__ = _View
         return view
+
+    def columns(self, start, stop):
+        """Columns ``start`` .. ``stop - 1`` of a float32 matrix [rows, columns], for the operators that take rows of any distance."""
+        if len(self.shape) != 2 or self.dtype != "float32" or not 0 <= start < stop <= self.shape[1]:
+            raise ValueError("columns %d to %d of a %s tensor of shape %s" % (start, stop, self.dtype, self.shape))
+        return Columns(self, start, stop)
 
 
 class _View(DeviceTensor):
     def __del__(self):  # storage belongs to the base tensor
         pass
+
+
+class _Foreign(DeviceTensor):
+    def __del__(self):  # storage belongs to the object that lent it
+        pass
+
+
+class Columns:
+    """Some columns of a float32 matrix: its rows lie ``ld`` floats apart (``DeviceTensor.columns``).  Not a DeviceTensor: the operators
+    that walk whole tensors do not take it."""
+
+    def __init__(self, base, start, stop):
+        self._base = base  # keeps the owner alive
+        self.at, self.ld, self.shape = base.ptr + 4 * start, base.shape[1], (base.shape[0], stop - start)
 
 
 class PinnedArray:
@@ -131,6 +162,15 @@ class Graph:
 
 def _ptr(t):
     return None if t is None else t.ptr
+
+
+def _rows(t, what):
+    """(pointer, distance of two rows, shape) of a float32 matrix or some of its columns."""
+    if isinstance(t, Columns):
+        return t.at, t.ld, t.shape
+    if len(t.shape) != 2 or t.dtype != "float32":
+        raise ValueError("%s takes float32 matrices [rows, columns], not %s %s" % (what, t.dtype, t.shape))
+    return t.ptr, t.shape[1], t.shape
 
 
 class Backend:
@@ -243,12 +283,31 @@ class Backend:
         self._check(self._probe_lib().eddlhip_probe_hbm(self.dev, int(nbytes), ctypes.byref(r), ctypes.byref(w), ctypes.byref(c)))
         return r.value, w.value, c.value
 
-    def empty(self, shape):
-        return DeviceTensor(self, shape)
+    def empty(self, shape, dtype="float32"):
+        return DeviceTensor(self, shape, dtype)
 
-    def array(self, host):
-        host = np.ascontiguousarray(host, dtype=np.float32)
-        return DeviceTensor(self, host.shape).copy_from(host)
+    def wrap(self, owner, dtype=None):
+        """Device memory that another library holds (an object with ``__cuda_array_interface__``, contiguous) as a tensor, without a copy; keeps
+        ``owner`` alive.  ``dtype`` says what the memory holds where the interface has no name for it ("bfloat16")."""
+        spec = owner.__cuda_array_interface__
+        kind = dtype or {"<f4": "float32", "<i4": "int32"}.get(spec["typestr"])
+        shape = tuple(int(d) for d in spec["shape"])
+        if kind not in _TYPES or _TYPES[kind][0] != int(spec["typestr"][2:]):
+            raise ValueError("no tensors of type %s over elements of %s" % (kind, spec["typestr"]))
+        steps, expect = spec.get("strides"), _TYPES[kind][0]
+        for d, step in reversed(list(zip(shape, steps or ()))):
+            if d > 1 and step != expect:
+                raise ValueError("the memory of a wrapped tensor is contiguous: shape %s, strides %s" % (shape, steps))
+            expect *= d
+        t = object.__new__(_Foreign)
+        t.backend, t.shape, t.dtype, t._owner, t.ptr = self, shape, kind, owner, spec["data"][0]
+        t.size = int(np.prod(shape)) if shape else 1
+        t.nbytes = t.size * _TYPES[kind][0]
+        return t
+
+    def array(self, host, dtype="float32"):
+        host = np.ascontiguousarray(host, dtype=_TYPES[dtype][1])
+        return DeviceTensor(self, host.shape, dtype).copy_from(host)
 
     def full(self, shape, v):
         t = DeviceTensor(self, shape)
@@ -452,3 +511,63 @@ class Backend:
 
     def sum2D_rowwise(self, A, B, C):
         self._check(self.lib.eddlhip_sum2d_rowwise(self.dev, A.ptr, B.ptr, C.ptr, A.shape[0], A.shape[1]))
+
+    # ---- attention blocks (eddl_amd.attention holds the cache, the batch and the plan that these take)
+    def rotary_axes(self, X, Y, plan, positions):
+        """Rotary positions: ``X``, ``Y`` [rows, heads * head_dim] (``Y`` may be ``X``), ``plan`` a RotaryPlan, ``positions`` [rows, axes]."""
+        (x, ldx, shape), (y, ldy, yshape) = _rows(X, "rotary_axes"), _rows(Y, "rotary_axes")
+        if shape != yshape or shape[1] % plan.head_dim or positions.shape != (shape[0], plan.axes) or positions.dtype != "float32":
+            raise ValueError("rotary_axes shapes %s -> %s, heads of %d, positions %s" % (shape, yshape, plan.head_dim, positions.shape))
+        self._check(self.lib.eddlhip_rotary_axes(self.dev, x, ldx, y, ldy, shape[0], shape[1] // plan.head_dim, plan.head_dim, positions.ptr,
+                                                 *plan.arguments))
+
+    def paged_append(self, Q, K, V, Qout, cache, batch, rotary=None, positions=None):
+        """Writes the new tokens' keys (turned by ``rotary``, a RotaryPlan, or as they are) and values into ``cache`` and the turned queries
+        into ``Qout`` (``Q`` and ``Qout`` may be None, or the same)."""
+        (k, ldk, shape), (v, ldv, vshape) = _rows(K, "paged_append"), _rows(V, "paged_append")
+        q, ldq, qshape = _rows(Q, "paged_append") if Q is not None else (None, 0, (shape[0], 0))
+        o, ldo, oshape = _rows(Qout, "paged_append") if Qout is not None else (None, 0, (shape[0], 0))
+        if shape != vshape or shape[1] != cache.kv_heads * cache.head_dim or qshape != oshape or qshape[0] != shape[0] or qshape[1] % cache.head_dim:
+            raise ValueError("paged_append shapes q %s -> %s, k %s, v %s, %d heads of %d" % (qshape, oshape, shape, vshape, cache.kv_heads, cache.head_dim))
+        if (rotary is None) != (positions is None):
+            raise ValueError("paged_append: a rotary plan and positions come together")
+        if rotary is not None and (rotary.head_dim != cache.head_dim or positions.shape != (shape[0], rotary.axes) or positions.dtype != "float32"):
+            raise ValueError("paged_append: a plan for heads of %d and positions %s for %s rows" % (rotary.head_dim, positions.shape, shape[0]))
+        self._check(self.lib.eddlhip_paged_append(self.dev, q, ldq, o, ldo, k, ldk, v, ldv, shape[0], qshape[1] // cache.head_dim, cache.kv_heads,
+                                                  cache.head_dim, _ptr(positions), *(rotary.arguments if rotary is not None else (0, 0, 0, None, None)),
+                                                  *cache.arguments, *batch.arguments, batch.max_new))
+
+    def paged_attention(self, Q, O, cache, batch, scale=None, causal=True, window=0):
+        """Attention of the new tokens ``Q`` -> ``O`` [rows, heads * head_dim] over the cache; ``scale`` is 1 / sqrt(head_dim) unless given."""
+        (q, ldq, shape), (o, ldo, oshape) = _rows(Q, "paged_attention"), _rows(O, "paged_attention")
+        if shape != oshape or shape[1] % (cache.kv_heads * cache.head_dim):
+            raise ValueError("paged_attention shapes %s -> %s, %d key heads of %d" % (shape, oshape, cache.kv_heads, cache.head_dim))
+        self._check(self.lib.eddlhip_paged_attention(self.dev, q, ldq, o, ldo, shape[0], *cache.arguments, shape[1] // cache.head_dim, cache.kv_heads,
+                                                     cache.head_dim, *batch.arguments, batch.max_new, batch.max_length,
+                                                     cache.head_dim ** -0.5 if scale is None else scale, int(causal), window))
+
+    def norm_residual(self, X, R, S, H, post=(None, None, None, 0.0), pre=(None, None, None, 0.0), gate=None, residual_scale=1.0, mod=None, shift=None,
+                      group_rows=None):
+        """S = residual_scale * R + gate * post(X), H = pre(S) * (1 + mod) + shift.  ``post`` and ``pre``: (kind, weight, bias, eps), kind
+        None, "layer" or "rms", weight and bias [columns] or None.
+        ``gate`` [groups, columns] (or one row for all), ``mod``, ``shift`` [groups, columns] belong to ``group_rows`` rows side by side (all, unless
+        given).  R, S, H may be None."""
+        x, ldx, shape = _rows(X, "norm_residual")
+        (r, ldr, rs), (s, lds, ss), (h, ldh, hs) = (_rows(t, "norm_residual") if t is not None else (None, 0, shape) for t in (R, S, H))
+        if group_rows is None:
+            group_rows = max(shape[0], 1)
+        groups = -(-shape[0] // group_rows) if group_rows > 0 else 0
+        if not rs == ss == hs == shape:
+            raise ValueError("norm_residual shapes x %s, residual %s, sum %s, normed %s" % (shape, rs, ss, hs))
+        for t in (post[1], post[2], pre[1], pre[2]):
+            if t is not None and (t.size != shape[1] or t.dtype != "float32"):
+                raise ValueError("norm_residual: weights %s %s for %d columns" % (t.dtype, t.shape, shape[1]))
+        for t in (gate, mod, shift):
+            if t is not None and (t.dtype != "float32" or t.size != max(groups, 1) * shape[1] and not (t is gate and t.size == shape[1])):
+                raise ValueError("norm_residual: gate, mod or shift %s for %d groups of %d columns" % (t.shape, groups, shape[1]))
+        self._check(self.lib.eddlhip_norm_residual(self.dev, x, ldx, r, ldr, residual_scale, s, lds, h, ldh, shape[0], shape[1], _NORMS[post[0]], _ptr(post[1]),
+                                                   _ptr(post[2]), post[3], _ptr(gate), gate.size // shape[1] if gate is not None else 0, _NORMS[pre[0]],
+                                                   _ptr(pre[1]), _ptr(pre[2]), pre[3], _ptr(mod), _ptr(shift), group_rows))
+
+
+_NORMS = {None: 0, "layer": 1, "rms": 2}

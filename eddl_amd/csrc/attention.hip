@@ -1,0 +1,511 @@
+// Attention of new tokens over a paged cache, in fp32 accuracy on the bf16 matrix instructions.
+//
+// Row i of a sequence's `new` query rows stands at position p = length - new + i.  With the visible tokens j (j < length; causal:
+// j <= p; window: j > p - window)
+//     s_j = scale q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j,   and o = 0 where nothing is visible.
+// One pass over the tokens with running maximum, sum and output; all three in fp32.  The exponentials are powers of two: log2(e)
+// goes into the queries together with the scale.
+//
+// The two products run on v_mfma_f32_32x32x16_bf16.  Every fp32 operand (queries, weights, an fp32 cache) is the sum of three bf16
+// numbers (split_parts.h); a bf16 cache is its own single part.  An fp32 cache takes the six largest of nine products, a bf16
+// cache three, whose sum is the product of a bf16 and an fp32 number without any rounding but the accumulator's.  Parts of
+// numbers below 2^-110 lose bits: absolute errors of 2^-133, nothing beside a softmax's other terms.
+//
+// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a query is a column: lane l holds the scores of query
+// l % 32 in registers, the maximum and the sum of a query are those of two lanes (one shuffle), the rescaling of the output is
+// one factor a lane.  And S^T is the second product's operand as it stands: a lane needs eight consecutive tokens of its query, which
+// it has when row r = 8a + 4h + i of the first product is token 16 (a / 2) + 8h + 4 (a % 2) + i.  The rows of K are read in that
+// order; no score ever moves between lanes.
+//
+// The cache is kept in the order in which these operands are read (eddlhip.h): a lane's operand is 16 (32) bytes side by side, and
+// the lanes' operands are side by side too.
+//
+// Infinities and NaN: what is not visible has no influence.  Masked scores are replaced, values behind the last token are
+// replaced by zeros; a NaN or infinity in a visible or masked place of a tile otherwise reaches the sums as NaN (0 * inf, or the parts
+// of an infinity), and rows whose sums are not finite are computed again one token at a time (attend_row_again), with what
+// the formula gives.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "split_parts.h"
+
+using namespace eddlhip;
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+constexpr int TILE_Q = 32;   // rows (a token's query heads of one key head, side by side) of a wavefront
+constexpr int TILE_KV = 32;  // tokens of a step
+constexpr int MAX_TOKENS = 1 << 30;
+constexpr float NEG_INF = -__builtin_inff();
+
+struct AttendParams {
+    const float *Q;
+    float *O;
+    const void *K, *V;
+    const int *table, *offsets, *lengths;
+    float *part_o;   // [splits][rows * q_heads][D]
+    float2 *part_s;  // [splits][rows * q_heads] maximum and sum
+    long long ldq, ldo;
+    int rows, q_heads, kv_heads, group, D, pages, page_shift, width, seqs, causal, window, splits, q_tiles, vec;
+    float scale;  // with log2(e)
+};
+
+// A sequence's part of the batch, from the device's arrays, kept within the buffers whatever those hold.
+struct Sequence {
+    int row0, fresh, length;
+    bool bad;  // longer than its row of the table, or negative
+};
+__device__ __forceinline__ Sequence sequence_of(const AttendParams &p, int s) {
+    Sequence q;
+    q.row0 = max(p.offsets[s], 0);
+    q.fresh = q.row0 < p.rows ? max(0, min(p.offsets[s + 1], p.rows) - q.row0) : 0;
+    q.length = p.lengths[s];
+    q.bad = q.length < 0 || (long long)q.length > ((long long)p.width << p.page_shift);
+    if (q.bad) q.length = 0;
+    return q;
+}
+
+// Element offset of 16 tokens of a key head; a page that is not in the pool gives `bad` and the place of page 0.
+__device__ __forceinline__ size_t block_base(const AttendParams &p, int page, int block16, int head, bool &bad) {
+    if ((unsigned)page >= (unsigned)p.pages) {
+        bad = true;
+        page = 0;
+    }
+    const int in_page = block16 & ((1 << (p.page_shift - 4)) - 1);
+    return ((((size_t)page * p.kv_heads + head) << (p.page_shift - 4)) + in_page) * (16 * p.D);
+}
+
+template <bool F32>
+struct Raw;
+template <>
+struct Raw<false> {
+    uintx4 v;
+    __device__ __forceinline__ void load(const void *base, size_t at) { v = *reinterpret_cast<const uintx4 *>((const unsigned short *)base + at); }
+    // tokens from `count` of the eight on are zeros
+    __device__ __forceinline__ void keep(int count) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = 2 * i + 1 < count ? v[i] : 2 * i < count ? v[i] & 0xffffu : 0u;
+    }
+};
+template <>
+struct Raw<true> {
+    floatx4 lo, hi;
+    __device__ __forceinline__ void load(const void *base, size_t at) {
+        const floatx4 *src = reinterpret_cast<const floatx4 *>((const float *)base + at);
+        lo = src[0];
+        hi = src[1];
+    }
+    __device__ __forceinline__ void keep(int count) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            lo[i] = i < count ? lo[i] : 0.0f;
+            hi[i] = 4 + i < count ? hi[i] : 0.0f;
+        }
+    }
+};
+
+struct Parts {
+    uintx4 p[3];
+};
+__device__ __forceinline__ Parts split8(const float (&x)[8]) {
+    Parts s;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned h, m, l;
+        split_pair(x[2 * i], x[2 * i + 1], h, m, l);
+        s.p[0][i] = h;
+        s.p[1][i] = m;
+        s.p[2][i] = l;
+    }
+    return s;
+}
+__device__ __forceinline__ floatx16 mfma(uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// large += the product of the largest parts, small += the others, the smallest first
+template <bool F32>
+__device__ __forceinline__ void multiply(const Raw<F32> &a, const uintx4 &b0, const uintx4 &b1, const uintx4 &b2, floatx16 &large, floatx16 &small) {
+    if constexpr (F32) {
+        const float x[8] = {a.lo[0], a.lo[1], a.lo[2], a.lo[3], a.hi[0], a.hi[1], a.hi[2], a.hi[3]};
+        const Parts s = split8(x);
+        small = mfma(s.p[0], b2, small);
+        small = mfma(s.p[1], b1, small);
+        small = mfma(s.p[2], b0, small);
+        small = mfma(s.p[0], b1, small);
+        small = mfma(s.p[1], b0, small);
+        large = mfma(s.p[0], b0, large);
+    } else {
+        small = mfma(a.v, b2, small);
+        small = mfma(a.v, b1, small);
+        large = mfma(a.v, b0, large);
+    }
+}
+
+__device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float element(const AttendParams &p, const void *base, size_t at, bool f32) {
+    return f32 ? ((const float *)base)[at] : __builtin_bit_cast(float, (unsigned)((const unsigned short *)base)[at] << 16);
+}
+
+// Where a row's result goes: the output, or its partial result.
+__device__ __forceinline__ void store_scale(const AttendParams &p, float m, float l, float &factor) {
+    // (no visible token: m = -inf, l = 0, o = 0; visible ones that are all -inf: l > 0 and o = NaN, as the formula)
+    factor = m == NEG_INF && l == 0.0f ? 0.0f : 1.0f / l;
+}
+
+// One row over the tokens [lo, hi), a wavefront together, one token at a time: lanes hold the dimensions lane, lane + 64, ...
+template <bool F32>
+__device__ void attend_row_again(const AttendParams &p, const Sequence &q, int seq, int kv_head, int token, int head, int lo, int hi, int split, bool bad) {
+    const int lane = threadIdx.x & 63, pos = q.length - q.fresh + token;
+    if (p.causal) hi = min(hi, pos + 1);
+    if (p.window > 0) lo = max(lo, pos - p.window + 1);
+    const float *qrow = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * p.D;
+    float x[4], o[4] = {0.0f, 0.0f, 0.0f, 0.0f}, m = NEG_INF, l = 0.0f;
+    for (int i = 0; i < 4; i++) x[i] = lane + 64 * i < p.D ? qrow[lane + 64 * i] * p.scale : 0.0f;
+    for (int j = lo; j < hi; j++) {
+        const size_t base = block_base(p, p.table[(size_t)seq * p.width + (j >> p.page_shift)], j >> 4, kv_head, bad);
+        float s = 0.0f;
+        for (int i = 0; i < 4; i++) {
+            const int d = lane + 64 * i;
+            if (d < p.D) s += x[i] * element(p, p.K, base + (d >> 3) * 128 + (j & 15) * 8 + (d & 7), F32);
+        }
+        for (int step = 32; step > 0; step >>= 1) s += __shfl_xor(s, step);
+        const float top = s > m || s != s ? s : m;  // a NaN stays
+        const float keep = top == NEG_INF ? 1.0f : power2(m - top), w = top == NEG_INF ? 0.0f : power2(s - top);
+        l = l * keep + (top == NEG_INF ? 1.0f : w);
+        if (top != NEG_INF && m == NEG_INF) l = w;
+        for (int i = 0; i < 4; i++) {
+            const int d = lane + 64 * i;
+            if (d < p.D) o[i] = (m == NEG_INF ? 0.0f : o[i] * keep) + w * element(p, p.V, base + ((j >> 3) & 1) * 8 * p.D + d * 8 + (j & 7), F32);
+        }
+        m = top;
+    }
+    if (bad) l = __builtin_nanf("");
+    const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
+    if (p.splits > 1) {
+        const size_t slot = (size_t)split * p.rows * p.q_heads + at;
+        if (lane == 0) p.part_s[slot] = make_float2(m, l);
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < p.D) p.part_o[slot * p.D + lane + 64 * i] = o[i];
+    } else {
+        float factor;
+        store_scale(p, m, l, factor);
+        if (m == NEG_INF && l > 0.0f) factor = __builtin_nanf("");
+        for (int i = 0; i < 4; i++)
+            if (lane + 64 * i < p.D) p.O[(size_t)(q.row0 + token) * p.ldo + (size_t)head * p.D + lane + 64 * i] = o[i] * factor;
+    }
+}
+
+// The tokens that any row of a tile sees, and the bounds that all of them share.
+struct Range {
+    int lo, hi;            // tokens of the tile's rows (lo on a boundary of TILE_KV)
+    int all_lo, all_hi;    // every row sees [all_lo, all_hi)
+};
+__device__ __forceinline__ Range range_of(const AttendParams &p, const Sequence &q, int row_lo, int row_hi) {
+    const int first = q.length - q.fresh + row_lo / p.group, last = q.length - q.fresh + (row_hi - 1) / p.group;
+    Range r;
+    r.hi = p.causal ? min(q.length, last + 1) : q.length;
+    r.all_hi = p.causal ? min(q.length, first + 1) : q.length;
+    r.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    r.all_lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
+    r.lo &= ~(TILE_KV - 1);
+    return r;
+}
+
+// A wavefront: 32 rows over its part of the tokens, operands straight from the cache into registers.  grid (q_tiles * splits, kv_heads, seqs).
+template <int DP, bool F32>
+__global__ __launch_bounds__(64, DP > 128 ? 1 : 2) void attend_wave_kernel(const AttendParams p) {
+    constexpr int KS = DP / 16, DT = DP / 32;
+    __shared__ uintx4 q_parts[3][KS][64];
+    const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
+    const int split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
+    const Sequence q = sequence_of(p, seq);
+    const int rows = q.fresh * p.group, ks_n = p.D >> 4;
+    const int *pages = p.table + (size_t)seq * p.width;
+    // K's lane order: row col of the product is token `k_token` of the step
+    const int a = col >> 3, k_token = 16 * (a >> 1) + 8 * ((col >> 2) & 1) + 4 * (a & 1) + (col & 3);
+
+    for (int tile = blockIdx.x / p.splits; tile * TILE_Q < rows; tile += p.q_tiles) {
+        const int row_lo = tile * TILE_Q, row_hi = min(rows, row_lo + TILE_Q);
+        const Range range = range_of(p, q, row_lo, row_hi);
+        const int steps_all = max(0, (range.hi - range.lo + TILE_KV - 1) / TILE_KV);
+        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
+        const int lo = range.lo + step_lo * TILE_KV, hi = min(range.hi, range.lo + step_hi * TILE_KV);
+
+        // ---- queries: parts of 8 dimensions of a row a lane, in LDS
+        const int row = min(row_lo + col, row_hi - 1), token = row / p.group, head = kv_head * p.group + row % p.group;
+        const int pos = q.length - q.fresh + token;
+        const float *qrow = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * p.D;
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+            if (ks < ks_n) {
+                float x[8];
+                if (p.vec) {
+                    const floatx4 *src = reinterpret_cast<const floatx4 *>(qrow + 16 * ks + 8 * half);
+                    const floatx4 u = src[0], v = src[1];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x[j] = u[j] * p.scale;
+                        x[4 + j] = v[j] * p.scale;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = qrow[16 * ks + 8 * half + j] * p.scale;
+                }
+                const Parts s = split8(x);
+#pragma unroll
+                for (int k = 0; k < 3; k++) q_parts[k][ks][lane] = s.p[k];
+            }
+        __syncthreads();
+
+        floatx16 o[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+        float m = NEG_INF, l = 0.0f;
+        bool bad = q.bad;
+        const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
+
+        // ---- the pages of 64 blocks of 16 tokens at a time, one a lane
+        int page_lane = 0, page_from = -1;
+        auto bases = [&](int j0, size_t (&base)[2]) __attribute__((always_inline)) {
+            const int b = j0 >> 4;
+            if (page_from < 0 || b + 1 >= page_from + 64) {
+                page_from = b;
+                const int j = min((b + lane) << 4, hi - 1);  // (behind the last token: its page again, whose values do not count)
+                page_lane = pages[j >> p.page_shift];
+            }
+            base[0] = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
+            base[1] = block_base(p, __builtin_amdgcn_readlane(page_lane, b + 1 - page_from), b + 1, kv_head, bad);
+        };
+        for (int j0 = lo; j0 < hi; j0 += TILE_KV) {
+            size_t base[2];
+            bases(j0, base);
+            const size_t k_base = (k_token < 16 ? base[0] : base[1]) + (k_token & 15) * 8 + half * 128;
+            Raw<F32> k[KS], v[2][DT];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                if (ks < ks_n) k[ks].load(p.K, k_base + ks * 256);
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    if (32 * dt < p.D) v[b][dt].load(p.V, base[b] + (size_t)half * 8 * p.D + min(32 * dt + col, p.D - 1) * 8);
+            floatx16 s_large, s_small;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s_large[r] = s_small[r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                if (ks < ks_n) multiply<F32>(k[ks], q_parts[0][ks][lane], q_parts[1][ks][lane], q_parts[2][ks][lane], s_large, s_small);
+            float s[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = s_large[r] + s_small[r];
+            if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
+                    s[r] = j >= see_lo && j < see_hi ? s[r] : NEG_INF;
+                }
+                if (j0 + TILE_KV > q.length) {
+#pragma unroll
+                    for (int b = 0; b < 2; b++)
+#pragma unroll
+                        for (int dt = 0; dt < DT; dt++) v[b][dt].keep(q.length - (j0 + 16 * b + 8 * half));
+                }
+            }
+            float top = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            top = fmaxf(top, m);
+            if (__any(top > m)) {
+                const float keep = m == NEG_INF ? 0.0f : power2(m - top);
+                l *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[dt][r] *= keep;
+                m = top;
+            }
+            const float from = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[r] = power2(s[r] - from);
+                l += s[r];
+            }
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float w[8] = {s[8 * b], s[8 * b + 1], s[8 * b + 2], s[8 * b + 3], s[8 * b + 4], s[8 * b + 5], s[8 * b + 6], s[8 * b + 7]};
+                const Parts ws = split8(w);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    if (32 * dt < p.D) multiply<F32>(v[b][dt], ws.p[0], ws.p[1], ws.p[2], o[dt], o[dt]);
+            }
+        }
+        l += __shfl_xor(l, 32);
+
+        // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one
+        float worst = l - l;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+            if (32 * dt < p.D) {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (32 * dt + 8 * (r >> 2) + 4 * half + (r & 3) < p.D) worst += o[dt][r] - o[dt][r];
+            }
+        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi));
+        again = again && row_lo + col < row_hi;
+        unsigned long long todo = __ballot(again);
+        todo = (todo | (todo >> 32)) & 0xffffffffull;
+        const bool redo = (todo >> col) & 1;
+        for (unsigned long long t = todo; t != 0; t &= t - 1) {
+            const int r = row_lo + __builtin_ctzll(t);
+            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, bad);
+        }
+        if (bad) l = __builtin_nanf("");
+
+        if (row_lo + col < row_hi && !redo) {
+            const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
+            const size_t slot = (size_t)split * p.rows * p.q_heads + at;
+            float factor = 1.0f, *dst;
+            if (p.splits > 1) {
+                if (half == 0) p.part_s[slot] = make_float2(m, l);
+                dst = p.part_o + slot * p.D;
+            } else {
+                store_scale(p, m, l, factor);
+                dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)head * p.D;
+            }
+            const bool whole = p.splits > 1 || p.vec;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int d = 32 * dt + 8 * g + 4 * half;
+                    if (d < p.D) {
+                        const floatx4 x = {o[dt][4 * g] * factor, o[dt][4 * g + 1] * factor, o[dt][4 * g + 2] * factor, o[dt][4 * g + 3] * factor};
+                        if (whole) {
+                            *reinterpret_cast<floatx4 *>(dst + d) = x;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) dst[d + i] = x[i];
+                        }
+                    }
+                }
+        }
+    }
+}
+
+// Joins the parts of a row in the order of the tokens; a wavefront a row.
+__global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
+    const int lane = threadIdx.x & 63;
+    const long long total = (long long)p.rows * p.q_heads;
+    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
+    for (long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += (long long)gridDim.x * 4) {
+        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
+        if (row < first || row >= end) continue;
+        float m = NEG_INF;
+        for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_s[(size_t)s * total + at].x);
+        for (int step = 32; step > 0; step >>= 1) m = fmaxf(m, __shfl_xor(m, step));
+        float l = 0.0f;
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < p.splits; s++) {
+            const float2 ms = p.part_s[(size_t)s * total + at];
+            if (ms.x == NEG_INF && ms.y == 0.0f) continue;  // saw nothing
+            const float w = m == NEG_INF ? 1.0f : power2(ms.x - m);
+            l += w * ms.y;
+            if (4 * lane < p.D) {
+                const floatx4 x = *reinterpret_cast<const floatx4 *>(p.part_o + ((size_t)s * total + at) * p.D + 4 * lane);
+                o += x * w;
+            }
+        }
+        float factor;
+        store_scale(p, m, l, factor);
+        if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
+        float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + 4 * lane;
+        if (4 * lane < p.D)
+            for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
+    }
+}
+
+}  // namespace
+
+extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, long long ldo, int rows, const void *k_pages, const void *v_pages,
+                                       int cache_type, int pages, int page_size, int q_heads, int kv_heads, int head_dim, const int *table, int table_width,
+                                       const int *offsets, const int *lengths, int seqs, int max_new, int max_length, float scale, int causal, int window) {
+    EH_REQUIRE(rows >= 0 && seqs >= 0 && seqs <= 65535, "paged_attention: %d rows of %d sequences (at most 65535)", rows, seqs);
+    EH_REQUIRE(cache_type == EDDLHIP_CACHE_F32 || cache_type == EDDLHIP_CACHE_BF16, "paged_attention: unknown cache type %d", cache_type);
+    EH_REQUIRE(head_dim >= 16 && head_dim <= 256 && head_dim % 16 == 0, "paged_attention: head_dim %d is not a multiple of 16 up to 256", head_dim);
+    EH_REQUIRE(kv_heads > 0 && kv_heads <= 65535 && q_heads > 0 && q_heads % kv_heads == 0, "paged_attention: %d query heads do not share %d key heads evenly",
+               q_heads, kv_heads);
+    EH_REQUIRE(page_size >= 16 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0, "paged_attention: page size %d is not a power of two from 16 on",
+               page_size);
+    EH_REQUIRE(pages > 0 && table_width > 0 && (long long)table_width * page_size <= MAX_TOKENS, "paged_attention: a pool of %d pages, a table of %d columns", pages,
+               table_width);
+    EH_REQUIRE(rows <= MAX_TOKENS && (long long)rows * q_heads <= 1LL << 30, "paged_attention: %d rows of %d heads are out of range", rows, q_heads);
+    EH_REQUIRE(ldq >= (long long)q_heads * head_dim && ldo >= (long long)q_heads * head_dim, "paged_attention: rows of %lld and %lld floats do not hold %d heads of %d",
+               ldq, ldo, q_heads, head_dim);
+    EH_REQUIRE(max_new >= 0 && max_length >= 0 && window >= 0, "paged_attention: negative max_new, max_length or window");
+    if (rows == 0 || seqs == 0) return 0;
+    EH_REQUIRE(Q && O && k_pages && v_pages && table && offsets && lengths, "paged_attention: NULL tensor");
+    EH_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "paged_attention: the cache is not aligned to 16 bytes");
+    EH_TRY(use_device(dev));
+    AttendParams p;
+    p.Q = Q;
+    p.O = O;
+    p.K = k_pages;
+    p.V = v_pages;
+    p.table = table;
+    p.offsets = offsets;
+    p.lengths = lengths;
+    p.ldq = ldq;
+    p.ldo = ldo;
+    p.rows = rows;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.group = q_heads / kv_heads;
+    p.D = head_dim;
+    p.pages = pages;
+    p.page_shift = __builtin_ctz((unsigned)page_size);
+    p.width = table_width;
+    p.seqs = seqs;
+    p.causal = causal != 0;
+    p.window = std::min(window, MAX_TOKENS);  // (no sequence is longer)
+    p.vec = (((uintptr_t)Q | (uintptr_t)O) & 15) == 0 && ldq % 4 == 0 && ldo % 4 == 0;
+    p.scale = scale * 1.44269504088896340736f;
+    // The launch goes by the bounds max_new and max_length; what is beyond them is still computed, by the same wavefronts.
+    const long long fresh = std::min(max_new > 0 ? max_new : 1, rows);
+    const long long tiles = std::min<long long>((fresh * p.group + TILE_Q - 1) / TILE_Q, 1 << 20);
+    p.q_tiles = (int)tiles;
+    const long long waves = tiles * kv_heads * seqs, want = 8LL * state(dev).num_cu;
+    long long seen = max_length > 0 ? max_length : 1;
+    if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
+    const long long steps = (seen + TILE_KV - 1) / TILE_KV;
+    p.splits = (int)std::max(1LL, std::min(want / waves, steps / 4));
+    p.part_o = nullptr;
+    p.part_s = nullptr;
+    if (p.splits > 1) {
+        const size_t slots = (size_t)p.splits * rows * q_heads;
+        void *ws = nullptr;
+        EH_TRY(get_workspace(dev, slots * (head_dim + 2) * sizeof(float), &ws));
+        p.part_o = (float *)ws;
+        p.part_s = (float2 *)((char *)ws + slots * head_dim * sizeof(float));
+    }
+    EH_REQUIRE(tiles * p.splits < (1LL << 31), "paged_attention: shape out of range");
+    typedef void (*kernel)(AttendParams);
+    static const kernel kernels[2][3] = {{attend_wave_kernel<64, true>, attend_wave_kernel<128, true>, attend_wave_kernel<256, true>},
+                                         {attend_wave_kernel<64, false>, attend_wave_kernel<128, false>, attend_wave_kernel<256, false>}};
+    const int size = head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2;
+    hipLaunchKernelGGL(kernels[cache_type == EDDLHIP_CACHE_F32 ? 0 : 1][size], dim3((unsigned)(tiles * p.splits), kv_heads, seqs), dim3(64), 0, state(dev).stream, p);
+    EH_CHECK_LAUNCH();
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 4, 65536)), dim3(256), 0, state(dev).stream, p);
+        EH_CHECK_LAUNCH();
+    }
+    return 0;
+}

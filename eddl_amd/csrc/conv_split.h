@@ -18,25 +18,12 @@
 // fp32 instruction too, from the original filters (split_tile_again), and every sum that is not finite takes that value: the
 // others keep theirs, whatever stands beside them in the tile.
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float floatx2 __attribute__((ext_vector_type(2)));
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+#include "split_parts.h"
 
 constexpr int SPLIT_K = 32;                   // channels of a K-step (of one filter tap): two matrix instructions deep
 constexpr int SPLIT_UNIT = 3 * 64 * 16;       // bytes of 32 filters x 16 channels: [part][lane][8 bf16]
 
-__device__ __forceinline__ unsigned split_round(float a, float b) {  // two bf16, rounded to nearest even
-    return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2){a, b}, bf16x2));
-}
-__device__ __forceinline__ void split_pair(float a, float b, unsigned &hi, unsigned &mid, unsigned &lo) {
-    hi = split_round(a, b);
-    const float ra = a - __builtin_bit_cast(float, hi << 16), rb = b - __builtin_bit_cast(float, hi & 0xffff0000u);
-    mid = split_round(ra, rb);
-    lo = split_round(ra - __builtin_bit_cast(float, mid << 16), rb - __builtin_bit_cast(float, mid & 0xffff0000u));
-}
-
-// The same of numbers that are known in 64 bits (transformed filters): the three parts, each rounded to nearest, hold 26 bits of them.
+// split_pair of numbers that are known in 64 bits (transformed filters): the three parts, each rounded to nearest, hold 26 bits of them.
 __device__ __forceinline__ void split_pair(double a, double b, unsigned &hi, unsigned &mid, unsigned &lo) {
     hi = split_round((float)a, (float)b);
     const double ra = a - (double)__builtin_bit_cast(float, hi << 16), rb = b - (double)__builtin_bit_cast(float, hi & 0xffff0000u);

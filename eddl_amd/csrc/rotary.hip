@@ -1,0 +1,313 @@
+// Rotary positions with several axes (time, row, column of a token of an image or a video), and the write of keys and values into
+// the paged cache that goes with them.
+//
+// Pair n of a head's first rot_dim dimensions turns by the angle a = position[axis[n]] * frequency[n]:
+//     y_i = x_i cos a - x_j sin a,   y_j = x_j cos a + x_i sin a,    (i, j) = (n, n + rot_dim / 2) or (2n, 2n + 1);
+// the dimensions behind rot_dim are copied.  Axis and frequency of every pair come from the host and travel as the kernel's
+// arguments.  Angles of far positions lose their meaning in 32 bits (position 1e5 at frequency 1: steps of 0.008), so the angle is
+// formed in 64 bits, in turns, and only its fraction of a turn goes into the fp32 sine and cosine.  They are computed
+// once for a token and pair and kept in LDS for all heads.
+//
+// Bound: memory, 8 bytes a number.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "split_parts.h"
+
+using namespace eddlhip;
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+constexpr int TPB = 256;
+constexpr int MAX_PAIRS = 128;
+
+struct Rotary {
+    double turns[MAX_PAIRS];  // frequency / (2 pi)
+    unsigned char axis[MAX_PAIRS];
+    const float *positions;  // [rows][axes]
+    int pairs, axes, adjacent;
+};
+
+__device__ __forceinline__ float2 turn(const Rotary &r, int row, int n) {
+    const double t = (double)r.positions[(size_t)row * r.axes + r.axis[n]] * r.turns[n];
+    const float part = (float)(t - rint(t));  // of a turn, -0.5 ... 0.5
+    float2 cs;
+    sincospif(2.0f * part, &cs.y, &cs.x);
+    return cs;
+}
+
+__device__ __forceinline__ floatx4 load4(const float *p, bool vec) {
+    if (vec) return *reinterpret_cast<const floatx4 *>(p);
+    return floatx4{p[0], p[1], p[2], p[3]};
+}
+__device__ __forceinline__ void store4(float *p, floatx4 x, bool vec) {
+    if (vec) {
+        *reinterpret_cast<floatx4 *>(p) = x;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = x[i];
+    }
+}
+
+// A head is cut into pieces of four pairs (8 numbers) and, behind rot_dim, of eight numbers: pieces = head_dim / 8.
+// Dimensions of piece n: (d0 .. d0 + 3) and (d1 .. d1 + 3).
+__device__ __forceinline__ void piece_at(const Rotary &r, int n, int &d0, int &d1) {
+    const bool halves = 4 * n < r.pairs && !r.adjacent;
+    d0 = halves ? 4 * n : 8 * n;
+    d1 = halves ? 4 * n + r.pairs : 8 * n + 4;
+}
+__device__ __forceinline__ void turn_piece(const Rotary &r, int n, const float2 *cs, floatx4 &x, floatx4 &y) {
+    if (4 * n >= r.pairs) return;
+    floatx4 a, b;
+    if (r.adjacent) {
+        a = floatx4{x[0], x[2], y[0], y[2]};
+        b = floatx4{x[1], x[3], y[1], y[3]};
+    } else {
+        a = x;
+        b = y;
+    }
+    floatx4 u, v;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 t = cs[4 * n + i];
+        u[i] = a[i] * t.x - b[i] * t.y;
+        v[i] = b[i] * t.x + a[i] * t.y;
+    }
+    if (r.adjacent) {
+        x = floatx4{u[0], v[0], u[1], v[1]};
+        y = floatx4{u[2], v[2], u[3], v[3]};
+    } else {
+        x = u;
+        y = v;
+    }
+}
+
+// grid: groups of ROWS rows, looping
+template <int ROWS>
+__global__ __launch_bounds__(TPB) void rotary_kernel(const Rotary r, const float *X, float *Y, long long ldx, long long ldy, int rows, int heads, int D, int vec) {
+    __shared__ float2 cs[ROWS][MAX_PAIRS];
+    const int pieces = D / 8, per_row = heads * pieces;
+    for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+        const int n_rows = min(ROWS, rows - row0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * r.pairs; i += TPB) cs[i / r.pairs][i % r.pairs] = turn(r, row0 + i / r.pairs, i % r.pairs);
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * per_row; i += TPB) {
+            const int at = i / per_row, rest = i - at * per_row, head = rest / pieces, n = rest - head * pieces;
+            int d0, d1;
+            piece_at(r, n, d0, d1);
+            const float *src = X + (size_t)(row0 + at) * ldx + (size_t)head * D;
+            floatx4 x = load4(src + d0, vec), y = load4(src + d1, vec);
+            turn_piece(r, n, cs[at], x, y);
+            float *dst = Y + (size_t)(row0 + at) * ldy + (size_t)head * D;
+            store4(dst + d0, x, vec);
+            store4(dst + d1, y, vec);
+        }
+    }
+}
+
+struct AppendParams {
+    const float *Q, *K, *V;
+    float *Qout;
+    void *k_pages, *v_pages;
+    const int *table, *offsets, *lengths;
+    long long ldq, ldk, ldv, ldo;
+    int rows, q_heads, kv_heads, D, pages, page_shift, width, f32, vec, head_groups;
+};
+
+__device__ __forceinline__ void put4(void *base, size_t at, floatx4 x, int f32) {
+    if (f32) {
+        *reinterpret_cast<floatx4 *>((float *)base + at) = x;
+    } else {  // (rounded to nearest even: the cache's type)
+        *reinterpret_cast<uint2 *>((unsigned short *)base + at) = make_uint2(split_round(x[0], x[1]), split_round(x[2], x[3]));
+    }
+}
+
+// The new tokens of a sequence that lie in one block of 16 places of the cache, and a part of the heads.
+// grid (blocks of 16 places, looping; head_groups; seqs)
+__global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const AppendParams p) {
+    __shared__ float2 cs[16][MAX_PAIRS];
+    const int seq = blockIdx.z, row0 = max(p.offsets[seq], 0), fresh = row0 < p.rows ? min(p.offsets[seq + 1], p.rows) - row0 : 0, length = p.lengths[seq];
+    const int start = length - fresh;  // place of row row0 (below 0: the first rows have none)
+    if (fresh <= 0) return;
+    const int D = p.D, pieces = D / 8;
+    // blocks of 16 rows of the sequence, aligned to the places
+    const int shift = start & 15;
+    for (int b = blockIdx.x; 16 * b < shift + fresh; b += gridDim.x) {
+        const int first = max(0, 16 * b - shift), n_rows = min(fresh, 16 * b - shift + 16) - first;  // of the sequence's rows
+        __syncthreads();
+        for (int i = threadIdx.x; i < n_rows * r.pairs; i += TPB) cs[i / r.pairs][i % r.pairs] = turn(r, row0 + first + i / r.pairs, i % r.pairs);
+        __syncthreads();
+        // the block's place in the cache; nothing is written where there is none
+        const int place = start + first;
+        int page = -1;
+        if (place >= 0 && length > 0 && (place >> p.page_shift) < p.width) page = p.table[(size_t)seq * p.width + (place >> p.page_shift)];
+        const bool stored = (unsigned)page < (unsigned)p.pages;
+        const size_t block = ((size_t)page * p.kv_heads << (p.page_shift - 4)) + ((place >> 4) & ((1 << (p.page_shift - 4)) - 1));
+        const size_t head_stride = (size_t)16 * D << (p.page_shift - 4);
+        const int t0 = place & 15;
+        const int q_items = p.Q ? p.q_heads : 0, head_lo = (int)((long long)(q_items + 2 * p.kv_heads) * blockIdx.y / p.head_groups),
+                  head_hi = (int)((long long)(q_items + 2 * p.kv_heads) * (blockIdx.y + 1) / p.head_groups);
+        for (int h = head_lo; h < head_hi; h++) {
+            if (h < q_items) {
+                for (int i = threadIdx.x; i < n_rows * pieces; i += TPB) {
+                    const int at = i / pieces, n = i - at * pieces;
+                    const size_t row = row0 + first + at;
+                    int d0, d1;
+                    piece_at(r, n, d0, d1);
+                    const float *src = p.Q + row * p.ldq + (size_t)h * D;
+                    floatx4 x = load4(src + d0, p.vec), y = load4(src + d1, p.vec);
+                    turn_piece(r, n, cs[at], x, y);
+                    float *dst = p.Qout + row * p.ldo + (size_t)h * D;
+                    store4(dst + d0, x, p.vec);
+                    store4(dst + d1, y, p.vec);
+                }
+            } else if (!stored) {
+                continue;
+            } else if (h < q_items + p.kv_heads) {
+                const int kv = h - q_items;
+                const size_t base = block * 16 * D + kv * head_stride;
+                for (int i = threadIdx.x; i < n_rows * pieces; i += TPB) {
+                    const int at = i % n_rows, n = i / n_rows;  // (tokens side by side: theirs are the neighbouring places)
+                    int d0, d1;
+                    piece_at(r, n, d0, d1);
+                    const float *src = p.K + (size_t)(row0 + first + at) * p.ldk + (size_t)kv * D;
+                    floatx4 x = load4(src + d0, p.vec), y = load4(src + d1, p.vec);
+                    turn_piece(r, n, cs[at], x, y);
+                    const size_t t = base + (t0 + at) * 8;
+                    put4(p.k_pages, t + (d0 >> 3) * 128 + (d0 & 7), x, p.f32);
+                    put4(p.k_pages, t + (d1 >> 3) * 128 + (d1 & 7), y, p.f32);
+                }
+            } else {
+                const int kv = h - q_items - p.kv_heads;
+                const size_t base = block * 16 * D + kv * head_stride;
+                for (int i = threadIdx.x; i < 4 * D; i += TPB) {  // four tokens of a dimension
+                    const int quarter = i / D, d = i - quarter * D, at = 4 * quarter - t0;  // (row of the block's token 4 quarter)
+                    if (at + 4 <= 0 || at >= n_rows) continue;
+                    const float *src = p.V + (size_t)kv * D + d;
+                    floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (at + k >= 0 && at + k < n_rows) x[k] = src[(size_t)(row0 + first + at + k) * p.ldv];
+                    const size_t t = base + (size_t)(quarter >> 1) * 8 * D + d * 8 + (quarter & 1) * 4;
+                    if (at >= 0 && at + 4 <= n_rows) {
+                        put4(p.v_pages, t, x, p.f32);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            if (at + k >= 0 && at + k < n_rows) {
+                                if (p.f32) ((float *)p.v_pages)[t + k] = x[k];
+                                else ((unsigned short *)p.v_pages)[t + k] = (unsigned short)split_round(x[k], x[k]);
+                            }
+                    }
+                }
+            }
+        }
+    }
+}
+
+int rotary_plan(Rotary &r, const char *what, const float *positions, int head_dim, int rot_dim, int adjacent, int axes, const int *host_axis,
+                const double *host_freq) {
+    EH_REQUIRE(head_dim >= 8 && head_dim % 8 == 0, "%s: head_dim %d is not a multiple of 8", what, head_dim);
+    EH_REQUIRE(rot_dim >= 0 && rot_dim % 8 == 0 && rot_dim <= head_dim && rot_dim <= 2 * MAX_PAIRS, "%s: rot_dim %d is not a multiple of 8 up to %d of a head of %d",
+               what, rot_dim, 2 * MAX_PAIRS, head_dim);
+    r.pairs = rot_dim / 2;
+    r.adjacent = adjacent != 0;
+    r.positions = positions;
+    r.axes = axes;
+    if (rot_dim == 0) return 0;
+    EH_REQUIRE(positions && host_axis && host_freq, "%s: NULL positions, axes or frequencies", what);
+    EH_REQUIRE(axes > 0 && axes <= 256, "%s: %d axes", what, axes);
+    for (int n = 0; n < r.pairs; n++) {
+        EH_REQUIRE(host_axis[n] >= 0 && host_axis[n] < axes, "%s: pair %d turns by axis %d of %d", what, n, host_axis[n], axes);
+        r.axis[n] = (unsigned char)host_axis[n];
+        r.turns[n] = host_freq[n] * 0.15915494309189533576888;  // 1 / (2 pi)
+    }
+    return 0;
+}
+
+bool aligned16(const void *p, long long ld) { return ((uintptr_t)p & 15) == 0 && ld % 4 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long long ldy, int rows, int heads, int head_dim, const float *positions, int rot_dim,
+                        int adjacent, int axes, const int *host_axis, const double *host_freq) {
+    EH_REQUIRE(rows >= 0 && heads > 0, "rotary_axes: %d rows of %d heads", rows, heads);
+    Rotary r;
+    EH_TRY(rotary_plan(r, "rotary_axes", positions, head_dim, rot_dim, adjacent, axes, host_axis, host_freq));
+    EH_REQUIRE((long long)heads * head_dim <= (1 << 24) && ldx >= (long long)heads * head_dim && ldy >= (long long)heads * head_dim,
+               "rotary_axes: rows of %lld and %lld floats do not hold %d heads of %d", ldx, ldy, heads, head_dim);
+    if (rows == 0) return 0;
+    EH_REQUIRE(X && Y, "rotary_axes: NULL tensor");
+    EH_REQUIRE(X != Y || ldx == ldy, "rotary_axes: in place, but rows of %lld and %lld floats", ldx, ldy);
+    EH_TRY(use_device(dev));
+    const int vec = aligned16(X, ldx) && aligned16(Y, ldy);
+    if (rows >= 4 * 4 * state(dev).num_cu)
+        hipLaunchKernelGGL(rotary_kernel<4>, dim3(std::min((rows + 3) / 4, 1 << 20)), dim3(TPB), 0, state(dev).stream, r, X, Y, ldx, ldy, rows, heads, head_dim, vec);
+    else
+        hipLaunchKernelGGL(rotary_kernel<1>, dim3(std::min(rows, 1 << 20)), dim3(TPB), 0, state(dev).stream, r, X, Y, ldx, ldy, rows, heads, head_dim, vec);
+    EH_CHECK_LAUNCH();
+    return 0;
+}
+
+int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, long long ldo, const float *K, long long ldk, const float *V, long long ldv, int rows,
+                         int q_heads, int kv_heads, int head_dim, const float *positions, int rot_dim, int adjacent, int axes, const int *host_axis,
+                         const double *host_freq, void *k_pages, void *v_pages, int cache_type, int pages, int page_size, const int *table, int table_width,
+                         const int *offsets, const int *lengths, int seqs, int max_new) {
+    EH_REQUIRE(rows >= 0 && seqs >= 0 && seqs <= 65535, "paged_append: %d rows of %d sequences (at most 65535)", rows, seqs);
+    EH_REQUIRE(cache_type == EDDLHIP_CACHE_F32 || cache_type == EDDLHIP_CACHE_BF16, "paged_append: unknown cache type %d", cache_type);
+    EH_REQUIRE(head_dim >= 16 && head_dim <= 256 && head_dim % 16 == 0, "paged_append: head_dim %d is not a multiple of 16 up to 256", head_dim);
+    EH_REQUIRE(kv_heads > 0 && (Q == nullptr || q_heads > 0) && q_heads >= 0 && (long long)q_heads + 2LL * kv_heads <= (1 << 20), "paged_append: %d query and %d key heads",
+               q_heads, kv_heads);
+    EH_REQUIRE((Q == nullptr) == (Qout == nullptr), "paged_append: queries and their output come together");
+    EH_REQUIRE(page_size >= 16 && page_size <= (1 << 20) && (page_size & (page_size - 1)) == 0, "paged_append: page size %d is not a power of two from 16 on", page_size);
+    EH_REQUIRE(pages > 0 && table_width > 0 && max_new >= 0, "paged_append: a pool of %d pages, a table of %d columns, max_new %d", pages, table_width, max_new);
+    Rotary r;
+    EH_TRY(rotary_plan(r, "paged_append", positions, head_dim, rot_dim, adjacent, axes, host_axis, host_freq));
+    EH_REQUIRE(ldk >= (long long)kv_heads * head_dim && ldv >= (long long)kv_heads * head_dim &&
+                   (Q == nullptr || (ldq >= (long long)q_heads * head_dim && ldo >= (long long)q_heads * head_dim)),
+               "paged_append: rows of %lld, %lld, %lld and %lld floats do not hold %d and %d heads of %d", ldq, ldo, ldk, ldv, q_heads, kv_heads, head_dim);
+    if (rows == 0 || seqs == 0) return 0;
+    EH_REQUIRE(K && V && k_pages && v_pages && table && offsets && lengths, "paged_append: NULL tensor");
+    EH_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "paged_append: the cache is not aligned to 16 bytes");
+    EH_REQUIRE(Q != Qout || ldq == ldo, "paged_append: queries in place, but rows of %lld and %lld floats", ldq, ldo);
+    EH_TRY(use_device(dev));
+    AppendParams p;
+    p.Q = Q;
+    p.K = K;
+    p.V = V;
+    p.Qout = Qout;
+    p.k_pages = k_pages;
+    p.v_pages = v_pages;
+    p.table = table;
+    p.offsets = offsets;
+    p.lengths = lengths;
+    p.ldq = ldq;
+    p.ldk = ldk;
+    p.ldv = ldv;
+    p.ldo = ldo;
+    p.rows = rows;
+    p.q_heads = q_heads;
+    p.kv_heads = kv_heads;
+    p.D = head_dim;
+    p.pages = pages;
+    p.page_shift = __builtin_ctz((unsigned)page_size);
+    p.width = table_width;
+    p.f32 = cache_type == EDDLHIP_CACHE_F32;
+    p.vec = aligned16(K, ldk) && aligned16(V, ldv) && (Q == nullptr || (aligned16(Q, ldq) && aligned16(Qout, ldo)));
+    // The launch goes by the bound max_new; sequences with more new tokens loop.
+    const int fresh = std::min(max_new > 0 ? max_new : 1, rows), blocks = (fresh + 14) / 16 + 1;
+    const long long items = (Q ? q_heads : 0) + 2LL * kv_heads, there = (long long)blocks * seqs;
+    p.head_groups = (int)std::max(1LL, std::min({items, (8LL * state(dev).num_cu + there - 1) / there, 65535LL}));
+    hipLaunchKernelGGL(paged_append_kernel, dim3(blocks, p.head_groups, seqs), dim3(TPB), 0, state(dev).stream, r, p);
+    EH_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // extern "C"

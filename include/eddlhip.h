@@ -480,6 +480,81 @@ int eddlhip_sum2d_rowwise(int dev, const float *A, const float *B, float *C, int
  * row's bits do not depend on their number; beyond they may. */
 int eddlhip_dense_fwd(int dev, const float *A, const float *W, const float *bias, float *C, int m, int k, int n, int relu);
 
+/* ------------------------------------------------------------------ attention blocks on image and video tokens
+ * What a network of attention blocks needs beside the dense layers: rotary positions, a paged cache of keys and values, the
+ * attention of new tokens over it, and the norms around a block.  No counterpart in the reference.  Inference only.
+ *
+ * Activations are fp32 rows, one token a row, whose heads lie side by side: [rows][heads * head_dim].  `ld*` is the distance of two
+ * rows in floats, so that queries, keys and values may be columns of one tensor (a dense layer's output).  Rows whose
+ * pointers and distances are multiples of 16 bytes are read 16 bytes at a time, others four.
+ *
+ * The cache is a pool of `pages` pages of `page_size` tokens (a power of two, 16 or more) in two tensors of the caller's, of
+ * fp32 numbers (EDDLHIP_CACHE_F32) or bf16 numbers (EDDLHIP_CACHE_BF16), aligned to 16 bytes:
+ *     k_pages [pages][kv_heads][page_size / 16][head_dim / 8][16 tokens][8 dimensions]
+ *     v_pages [pages][kv_heads][page_size / 16][2][head_dim][8 tokens]
+ * head_dim is a multiple of 16 up to 256.  Tokens are written by eddlhip_paged_append, in the order above.
+ *
+ * A batch is described by three int tensors on the device, read when the kernels run, so that a recorded graph follows them:
+ *     table [seqs][table_width]   the pages of each sequence, in the order of its tokens (entries behind its length are not read)
+ *     offsets [seqs + 1]          rows offsets[s] .. offsets[s + 1] - 1 are the new tokens of sequence s (maybe none)
+ *     lengths [seqs]              tokens of the sequence in the cache, the new ones included
+ * New token i of `new` stands at place lengths[s] - new + i.  Rows before offsets[0] and from offsets[seqs] on are neither read
+ * nor written.  max_new and max_length are the host's bounds of the new tokens and the length of a sequence: they size the
+ * launch, and sequences beyond them come out right too, only slower.  No access leaves the buffers whatever the three tensors
+ * hold; the rows of sequences must not overlap. */
+#define EDDLHIP_CACHE_F32 0
+#define EDDLHIP_CACHE_BF16 1
+
+/* Rotary positions with several axes.  positions[rows][axes] are fp32 numbers (whole or not).  Pair n of the first rot_dim
+ * dimensions of every head (a multiple of 8, up to head_dim and 256) turns by the angle a = positions[row][host_axis[n]] * host_freq[n]:
+ *     y_i = x_i cos a - x_j sin a,  y_j = x_j cos a + x_i sin a,
+ * (i, j) = (n, n + rot_dim / 2), or (2n, 2n + 1) when `adjacent` != 0.  The other dimensions are copied.  Angles are formed in
+ * 64 bits.  host_axis (0 .. axes - 1) and host_freq are host arrays of rot_dim / 2 entries, read during the call.  Y may be X (ldx == ldy).
+ * Negative frequencies turn back.  head_dim is a multiple of 8. */
+int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long long ldy, int rows, int heads, int head_dim,
+                        const float *positions, int rot_dim, int adjacent, int axes, const int *host_axis, const double *host_freq);
+
+/* The new tokens' keys (turned as above; rot_dim == 0: as they are) and values to their places in the cache, and the turned
+ * queries to Qout (Q and Qout NULL: no queries; Qout may be Q).  A bf16 cache rounds to nearest even.  A token without a place - before
+ * place 0, behind the table's row, on a page that is not in the pool - is not written; eddlhip_paged_attention reports its
+ * sequence.  No page may be written by two sequences of a call. */
+int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, long long ldo, const float *K, long long ldk,
+                         const float *V, long long ldv, int rows, int q_heads, int kv_heads, int head_dim,
+                         const float *positions, int rot_dim, int adjacent, int axes, const int *host_axis, const double *host_freq,
+                         void *k_pages, void *v_pages, int cache_type, int pages, int page_size,
+                         const int *table, int table_width, const int *offsets, const int *lengths, int seqs, int max_new);
+
+/* Attention of the new tokens over the cache: query head h of a row at place p reads key head h / (q_heads / kv_heads),
+ *     s_j = scale q . k_j,   o = sum_j softmax(s)_j v_j   over the visible tokens
+ * j < length, with causal != 0 also j <= p, with window > 0 also j > p - window.  A row that sees nothing is 0.  What is not
+ * visible has no influence, infinities and NaN included; among visible tokens they come out as the formula brings them.
+ * Both products have the accuracy of fp32 (sums of bf16 products, as the split form of the convolutions), softmax
+ * and sums are fp32.  The cache's length may be divided over workgroups, whose parts are joined in the order of the tokens: the
+ * same call gives the same bits, calls of other bounds (max_new, max_length, seqs) may differ by rounding.
+ * A sequence longer than its row of the table, or that reads a page outside the pool, comes out as NaN, in all of its rows that
+ * would have read there.  O must not overlap Q or the cache.  Workspace: the parts of a divided length. */
+int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, long long ldo, int rows,
+                            const void *k_pages, const void *v_pages, int cache_type, int pages, int page_size,
+                            int q_heads, int kv_heads, int head_dim, const int *table, int table_width,
+                            const int *offsets, const int *lengths, int seqs, int max_new, int max_length,
+                            float scale, int causal, int window);
+
+/* The norm behind a block, its gate, the residual sum and the norm before the next block, in one pass over the rows:
+ *     n = post(X),   S = residual_scale R + gate n,   H = pre(S) (1 + mod) + shift
+ * post and pre are EDDLHIP_NORM_NONE, _LAYER ((x - mean) / sqrt(variance + eps) w + b) or _RMS (x / sqrt(mean(x^2) + eps) w + b)
+ * over the columns; w and b [cols] may be NULL.  gate [gate_groups][cols] belongs to groups of group_rows rows side by side (an image's
+ * tokens), or to all rows with gate_groups == 1; NULL: 1.  mod and shift [groups][cols], NULL: 0, with groups = ceil(rows / group_rows).
+ * R NULL: no residual.  S or H may be NULL where nobody needs them.  S or H may be X or R (rows of the same distance), not each other.
+ * Up to 32768 columns. */
+#define EDDLHIP_NORM_NONE 0
+#define EDDLHIP_NORM_LAYER 1
+#define EDDLHIP_NORM_RMS 2
+int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R, long long ldr, float residual_scale,
+                          float *S, long long lds, float *H, long long ldh, int rows, int cols,
+                          int post_kind, const float *post_w, const float *post_b, float post_eps, const float *gate, int gate_groups,
+                          int pre_kind, const float *pre_w, const float *pre_b, float pre_eps, const float *mod, const float *shift,
+                          int group_rows);
+
 #ifdef __cplusplus
 }
 #endif
