@@ -401,36 +401,356 @@ __global__ __launch_bounds__(64, DP > 128 ? 1 : 2) void attend_wave_kernel(const
     }
 }
 
-// Joins the parts of a row in the order of the tokens; a wavefront a row.
-__global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
-    const int lane = threadIdx.x & 63;
-    const long long total = (long long)p.rows * p.q_heads;
-    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
-    for (long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += (long long)gridDim.x * 4) {
-        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
-        if (row < first || row >= end) continue;
-        float m = NEG_INF;
-        for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_s[(size_t)s * total + at].x);
-        for (int step = 32; step > 0; step >>= 1) m = fmaxf(m, __shfl_xor(m, step));
-        float l = 0.0f;
-        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < p.splits; s++) {
-            const float2 ms = p.part_s[(size_t)s * total + at];
-            if (ms.x == NEG_INF && ms.y == 0.0f) continue;  // saw nothing
-            const float w = m == NEG_INF ? 1.0f : power2(ms.x - m);
-            l += w * ms.y;
-            if (4 * lane < p.D) {
-                const floatx4 x = *reinterpret_cast<const floatx4 *>(p.part_o + ((size_t)s * total + at) * p.D + 4 * lane);
-                o += x * w;
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to 16 NQ rows of a sequence and key head (single tokens, short drafts): bound by the cache's bytes.  A workgroup takes a part of the
+// tokens, its four wavefronts take steps of 32 tokens in turn, operands straight from the cache into registers: every byte is read
+// once, by one wavefront, so LDS would only add a trip.  Keys of the next step are asked for as soon as the products have
+// used this step's, values likewise, into the same registers: a step's loads are on their way while the other half of a step is
+// computed, 16 (32) KB a wavefront.  The 16x16x32 instruction keeps the queries that are not there at 15 of 16 columns
+// instead of 31 of 32, and the registers at half.  The wavefronts' sums meet in LDS once.
+// Rows of the product K Q^T: row 4g + i of tile t is token 8g + 4t + i of the step, so that lane group g holds tokens 8g .. 8g + 7.
+constexpr int FEW_WAVES = 4;
+
+__device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <bool F32>
+struct Operand;
+template <>
+struct Operand<false> {
+    uintx4 v;
+    __device__ __forceinline__ explicit Operand(const Raw<false> &r) : v(r.v) {}
+    __device__ __forceinline__ void multiply(const uintx4 &b0, const uintx4 &b1, const uintx4 &b2, floatx4 &large, floatx4 &small) const {
+        small = mfma16(v, b2, small);
+        small = mfma16(v, b1, small);
+        large = mfma16(v, b0, large);
+    }
+};
+template <>
+struct Operand<true> {
+    Parts s;
+    __device__ __forceinline__ explicit Operand(const Raw<true> &r) {
+        const float x[8] = {r.lo[0], r.lo[1], r.lo[2], r.lo[3], r.hi[0], r.hi[1], r.hi[2], r.hi[3]};
+        s = split8(x);
+    }
+    __device__ __forceinline__ void multiply(const uintx4 &b0, const uintx4 &b1, const uintx4 &b2, floatx4 &large, floatx4 &small) const {
+        small = mfma16(s.p[0], b2, small);
+        small = mfma16(s.p[1], b1, small);
+        small = mfma16(s.p[2], b0, small);
+        small = mfma16(s.p[0], b1, small);
+        small = mfma16(s.p[1], b0, small);
+        large = mfma16(s.p[0], b0, large);
+    }
+};
+
+// FULL: head_dim is DP.  grid (q_tiles * splits, kv_heads, seqs)
+template <int DP, bool F32, int NQ, bool FULL>
+__global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ > 1) ? 1 : 2) void attend_few_kernel(const AttendParams p) {
+    constexpr int KS = DP / 32, DT = DP / 16, W = FEW_WAVES, COLS = 16 * NQ, PITCH = DP + 4;
+    constexpr int Q_BYTES = 3 * KS * NQ * 64 * 16, O_BYTES = W * COLS * PITCH * 4;
+    __shared__ __attribute__((aligned(16))) char lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
+    __shared__ float sums[W][COLS][2];
+    __shared__ unsigned redo_columns;
+    uintx4(*q_parts)[KS][NQ][64] = reinterpret_cast<uintx4(*)[KS][NQ][64]>(lds);
+    float(*o_lds)[COLS][PITCH] = reinterpret_cast<float(*)[COLS][PITCH]>(lds);
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
+    const int D = FULL ? DP : p.D, ks_n = FULL ? KS : (D + 31) >> 5, dt_n = FULL ? DT : D >> 4;
+    const int split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
+    const Sequence q = sequence_of(p, seq);
+    const int rows = q.fresh * p.group;
+    const int *pages = p.table + (size_t)seq * p.width;
+
+    for (int tile = blockIdx.x / p.splits; tile * COLS < rows; tile += p.q_tiles) {
+        const int row_lo = tile * COLS, row_hi = min(rows, row_lo + COLS);
+        const Range range = range_of(p, q, row_lo, row_hi);
+        const int steps_all = max(0, (range.hi - range.lo + TILE_KV - 1) / TILE_KV);
+        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
+        const int lo = range.lo + step_lo * TILE_KV, hi = min(range.hi, range.lo + step_hi * TILE_KV);
+        __syncthreads();  // (the tile before has been stored)
+
+        // ---- the cache's operands of a step
+        bool bad = q.bad;
+        int page_lane = 0, page_it = -64;
+        Raw<F32> k[2][KS], v[DT];
+        size_t base[2];
+        auto find = [&](int it) __attribute__((always_inline)) {  // the wavefront's step `it`: 16 tokens' places, twice
+            if (it >= page_it + 32) {
+                page_it = it;
+                const int j = lo + ((wave + W * (it + (lane >> 1))) * 2 + (lane & 1)) * 16;
+                page_lane = pages[min(j, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
+            }
+            const int b = (lo >> 4) + (wave + W * it) * 2, at = 2 * (it - page_it);
+            base[0] = block_base(p, __builtin_amdgcn_readlane(page_lane, at), b, kv_head, bad);
+            base[1] = block_base(p, __builtin_amdgcn_readlane(page_lane, at + 1), b + 1, kv_head, bad);
+        };
+        auto load_keys = [&]() __attribute__((always_inline)) {
+            const size_t from = (col >> 3 ? base[1] : base[0]);
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int token = (8 * (col >> 2) + 4 * t + (col & 3)) & 15;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+                    if (FULL || ks < ks_n) k[t][ks].load(p.K, from + token * 8 + (FULL ? 4 * ks + g : min(4 * ks + g, (D >> 3) - 1)) * 128);
+            }
+        };
+        auto load_values = [&]() __attribute__((always_inline)) {
+            const size_t from = (g & 2 ? base[1] : base[0]) + (size_t)(g & 1) * 8 * D + col * 8;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+                if (FULL || dt < dt_n) v[dt].load(p.V, from + dt * 128);
+        };
+        const int its = (step_hi - step_lo - wave + W - 1) / W;  // steps of this wavefront
+        if (its > 0 && hi > lo) {
+            find(0);
+            load_keys();
+            load_values();
+        }
+
+        // ---- queries: parts of 8 dimensions of a row a lane, in LDS, made by all wavefronts together
+        for (int i = wave; i < ks_n * NQ; i += W) {
+            const int ks = i / NQ, nq = i % NQ, row = min(row_lo + 16 * nq + col, row_hi - 1), token = row / p.group, head = kv_head * p.group + row % p.group;
+            const int d = 32 * ks + 8 * g;
+            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (d < D) {
+                const float *src = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D + d;
+                if (p.vec) {
+                    const floatx4 a = *reinterpret_cast<const floatx4 *>(src), b = *reinterpret_cast<const floatx4 *>(src + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x[j] = a[j] * p.scale;
+                        x[4 + j] = b[j] * p.scale;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = src[j] * p.scale;
+                }
+            }
+            const Parts s = split8(x);
+#pragma unroll
+            for (int n = 0; n < 3; n++) q_parts[n][ks][nq][lane] = s.p[n];
+        }
+        if (tid == 0) redo_columns = 0;
+        int see_lo[NQ], see_hi[NQ];
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            const int pos = q.length - q.fresh + min(row_lo + 16 * nq + col, row_hi - 1) / p.group;
+            see_lo[nq] = p.window > 0 ? pos - p.window + 1 : 0;
+            see_hi[nq] = p.causal ? min(q.length, pos + 1) : q.length;
+        }
+        __syncthreads();
+
+        floatx4 o[NQ][DT];
+        float m[NQ], l[NQ];
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            m[nq] = NEG_INF;
+            l[nq] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) o[nq][dt] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        for (int it = 0; it < its; it++) {
+            const int j0 = lo + (wave + W * it) * TILE_KV;
+            const bool more = it + 1 < its;
+            floatx4 large[NQ][2], small[NQ][2];
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++)
+#pragma unroll
+                for (int t = 0; t < 2; t++) large[nq][t] = small[nq][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                if (FULL || ks < ks_n) {
+                    const Operand<F32> a0(k[0][ks]), a1(k[1][ks]);
+#pragma unroll
+                    for (int nq = 0; nq < NQ; nq++) {
+                        const uintx4 b0 = q_parts[0][ks][nq][lane], b1 = q_parts[1][ks][nq][lane], b2 = q_parts[2][ks][nq][lane];
+                        a0.multiply(b0, b1, b2, large[nq][0], small[nq][0]);
+                        a1.multiply(b0, b1, b2, large[nq][1], small[nq][1]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);  // (one operand's parts at a time: registers)
+                }
+            if (more) {
+                find(it + 1);
+                load_keys();
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (j0 + TILE_KV > q.length) {
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) v[dt].keep(q.length - (j0 + 8 * g));
+            }
+            Parts ws[NQ];
+#pragma unroll
+            for (int nq = 0; nq < NQ; nq++) {
+                float s[8];
+#pragma unroll
+                for (int r = 0; r < 8; r++) s[r] = large[nq][r >> 2][r & 3] + small[nq][r >> 2][r & 3];
+                if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        const int j = j0 + 8 * g + r;
+                        s[r] = j >= see_lo[nq] && j < see_hi[nq] ? s[r] : NEG_INF;
+                    }
+                }
+                float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                top = fmaxf(top, m[nq]);
+                if (__any(top > m[nq])) {
+                    const float keep = m[nq] == NEG_INF ? 0.0f : power2(m[nq] - top);
+                    l[nq] *= keep;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) o[nq][dt] *= keep;
+                    m[nq] = top;
+                }
+                const float from = m[nq] == NEG_INF ? 0.0f : m[nq];
+#pragma unroll
+                for (int r = 0; r < 8; r++) {
+                    s[r] = power2(s[r] - from);
+                    l[nq] += s[r];
+                }
+                ws[nq] = split8(s);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+                if (FULL || dt < dt_n) {
+                    const Operand<F32> a(v[dt]);
+#pragma unroll
+                    for (int nq = 0; nq < NQ; nq++) a.multiply(ws[nq].p[0], ws[nq].p[1], ws[nq].p[2], o[nq][dt], o[nq][dt]);
+                    if (F32) __builtin_amdgcn_sched_barrier(0);
+                }
+            if (more) load_values();
+        }
+        __syncthreads();  // (the queries have been read: their place takes the outputs)
+#pragma unroll
+        for (int nq = 0; nq < NQ; nq++) {
+            l[nq] += __shfl_xor(l[nq], 16);
+            l[nq] += __shfl_xor(l[nq], 32);
+            if (bad) l[nq] = __builtin_nanf("");
+            if (g == 0) {
+                sums[wave][16 * nq + col][0] = m[nq];
+                sums[wave][16 * nq + col][1] = l[nq];
+            }
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+                if (FULL || dt < dt_n) *reinterpret_cast<floatx4 *>(&o_lds[wave][16 * nq + col][16 * dt + 4 * g]) = o[nq][dt];
+        }
+        __syncthreads();
+
+        // ---- the wavefronts' sums together, four dimensions of a row a thread
+        const int quads = D >> 2, items = (row_hi - row_lo) * quads;
+        for (int i0 = 0; i0 < items; i0 += 64 * W) {
+            const int i = i0 + tid, c = i / quads, d = 4 * (i - c * quads);
+            if (i < items) {
+                float top = sums[0][c][0];
+#pragma unroll
+                for (int w = 1; w < W; w++) top = fmaxf(top, sums[w][c][0]);
+                float sum = 0.0f;
+                floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const float f = sums[w][c][0] == NEG_INF ? (sums[w][c][1] == 0.0f ? 0.0f : sums[w][c][1]) : power2(sums[w][c][0] - top);
+                    sum += f * sums[w][c][1];
+                    x += *reinterpret_cast<const floatx4 *>(&o_lds[w][c][d]) * f;
+                }
+                const int row = row_lo + c, token = row / p.group, head = kv_head * p.group + row % p.group;
+                const int pos = q.length - q.fresh + token, from = p.window > 0 ? max(lo, pos - p.window + 1) : lo, to = p.causal ? min(hi, pos + 1) : hi;
+                const float worst = (sum - sum) + ((x[0] - x[0]) + (x[1] - x[1])) + ((x[2] - x[2]) + (x[3] - x[3]));
+                if (worst != 0.0f || (top == NEG_INF && from < to)) {
+                    atomicOr(&redo_columns, 1u << c);
+                }
+                const size_t at = (size_t)(q.row0 + token) * p.q_heads + head, slot = (size_t)split * p.rows * p.q_heads + at;
+                if (p.splits > 1) {
+                    if (d == 0) p.part_s[slot] = make_float2(top, sum);
+                    *reinterpret_cast<floatx4 *>(p.part_o + slot * D + d) = x;
+                } else {
+                    float factor;
+                    store_scale(p, top, sum, factor);
+                    float *dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)head * D + d;
+                    x *= factor;
+                    if (p.vec) {
+                        *reinterpret_cast<floatx4 *>(dst) = x;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) dst[j] = x[j];
+                    }
+                }
             }
         }
-        float factor;
-        store_scale(p, m, l, factor);
-        if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
-        float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + 4 * lane;
-        if (4 * lane < p.D)
-            for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
+        // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one (behind the stores above)
+        __syncthreads();
+        const bool any_bad = q.bad;
+        for (unsigned todo = redo_columns; todo != 0; todo &= todo - 1) {
+            const int c = __builtin_ctz(todo), r = row_lo + c;
+            if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, any_bad);
+        }
     }
+}
+
+// Joins the parts of a row, a workgroup a row: the weights of all parts first, then four dimensions and every (1024 / head_dim)th part a
+// thread, then those together, in an order that the shape alone fixes.
+constexpr int MAX_SPLITS = 512;
+__global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
+    __shared__ float weights[MAX_SPLITS], red[8];
+    __shared__ floatx4 sums[256];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quads = p.D >> 2, lanes = 256 / quads;
+    const long long total = (long long)p.rows * p.q_heads;
+    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
+    for (long long at = blockIdx.x; at < total; at += gridDim.x) {
+        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
+        if (row < first || row >= end) continue;
+        float2 ms[MAX_SPLITS / 256];
+        float m = NEG_INF, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 256; i++) {
+            const int s = tid + 256 * i;
+            ms[i] = s < p.splits ? p.part_s[(size_t)s * total + at] : make_float2(NEG_INF, 0.0f);
+            m = fmaxf(m, ms[i].x);
+        }
+        for (int step = 32; step > 0; step >>= 1) m = fmaxf(m, __shfl_xor(m, step));
+        __syncthreads();  // (the row before has been read)
+        if (lane == 0) red[wave] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 256; i++) {
+            const int s = tid + 256 * i;
+            const float w = ms[i].x == NEG_INF && ms[i].y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(ms[i].x - m);
+            l += w * ms[i].y;
+            if (s < p.splits) weights[s] = w;
+        }
+        for (int step = 32; step > 0; step >>= 1) l += __shfl_xor(l, step);
+        if (lane == 0) red[4 + wave] = l;
+        __syncthreads();
+        l = (red[4] + red[5]) + (red[6] + red[7]);
+        const int part = tid / quads, d = 4 * (tid - part * quads);
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (part < lanes) {
+            const float *src = p.part_o + (size_t)at * p.D + d;
+            const size_t step = (size_t)total * p.D;
+#pragma unroll 4
+            for (int s = part; s < p.splits; s += lanes) o += *reinterpret_cast<const floatx4 *>(src + s * step) * weights[s];
+            sums[tid] = o;
+        }
+        __syncthreads();
+        if (part == 0) {
+            for (int n = 1; n < lanes; n++) o += sums[n * quads + tid];
+            float factor;
+            store_scale(p, m, l, factor);
+            if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
+            float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + d;
+#pragma unroll
+            for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
+        }
+    }
+}
+
+template <int DP, bool FULL>
+void launch_few(const AttendParams &p, bool f32, int nq, dim3 grid, hipStream_t st) {
+    typedef void (*kernel)(AttendParams);
+    constexpr int MOST = DP <= 128 ? 2 : 1;
+    static const kernel kernels[2][2] = {{attend_few_kernel<DP, false, 1, FULL>, attend_few_kernel<DP, false, MOST, FULL>},
+                                         {attend_few_kernel<DP, true, 1, FULL>, attend_few_kernel<DP, true, MOST, FULL>}};
+    hipLaunchKernelGGL(kernels[f32][nq - 1], grid, dim3(64 * FEW_WAVES), 0, st, p);
 }
 
 }  // namespace
@@ -479,14 +799,15 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     p.vec = (((uintptr_t)Q | (uintptr_t)O) & 15) == 0 && ldq % 4 == 0 && ldo % 4 == 0;
     p.scale = scale * 1.44269504088896340736f;
     // The launch goes by the bounds max_new and max_length; what is beyond them is still computed, by the same wavefronts.
-    const long long fresh = std::min(max_new > 0 ? max_new : 1, rows);
-    const long long tiles = std::min<long long>((fresh * p.group + TILE_Q - 1) / TILE_Q, 1 << 20);
+    const long long fresh = std::min(max_new > 0 ? max_new : 1, rows), tile_rows = fresh * p.group;
+    const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : TILE_Q;
+    const long long tiles = (tile_rows + per_tile - 1) / per_tile;
     p.q_tiles = (int)tiles;
-    const long long waves = tiles * kv_heads * seqs, want = 8LL * state(dev).num_cu;
+    const long long groups = tiles * kv_heads * seqs, want = (nq ? 3LL : 8LL) * state(dev).num_cu;
     long long seen = max_length > 0 ? max_length : 1;
     if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
-    p.splits = (int)std::max(1LL, std::min(want / waves, steps / 4));
+    p.splits = (int)std::max(1LL, std::min({want / groups, steps / (nq ? 8 : 4), (long long)MAX_SPLITS}));
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
@@ -497,14 +818,25 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
         p.part_s = (float2 *)((char *)ws + slots * head_dim * sizeof(float));
     }
     EH_REQUIRE(tiles * p.splits < (1LL << 31), "paged_attention: shape out of range");
-    typedef void (*kernel)(AttendParams);
-    static const kernel kernels[2][3] = {{attend_wave_kernel<64, true>, attend_wave_kernel<128, true>, attend_wave_kernel<256, true>},
-                                         {attend_wave_kernel<64, false>, attend_wave_kernel<128, false>, attend_wave_kernel<256, false>}};
-    const int size = head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2;
-    hipLaunchKernelGGL(kernels[cache_type == EDDLHIP_CACHE_F32 ? 0 : 1][size], dim3((unsigned)(tiles * p.splits), kv_heads, seqs), dim3(64), 0, state(dev).stream, p);
+    const dim3 grid((unsigned)(tiles * p.splits), kv_heads, seqs);
+    const hipStream_t st = state(dev).stream;
+    const bool f32 = cache_type == EDDLHIP_CACHE_F32;
+    if (nq) {
+        if (head_dim == 64) launch_few<64, true>(p, f32, nq, grid, st);
+        else if (head_dim == 128) launch_few<128, true>(p, f32, nq, grid, st);
+        else if (head_dim == 256) launch_few<256, true>(p, f32, nq, grid, st);
+        else if (head_dim < 64) launch_few<64, false>(p, f32, nq, grid, st);
+        else if (head_dim < 128) launch_few<128, false>(p, f32, nq, grid, st);
+        else launch_few<256, false>(p, f32, nq, grid, st);
+    } else {
+        typedef void (*kernel)(AttendParams);
+        static const kernel kernels[2][3] = {{attend_wave_kernel<64, false>, attend_wave_kernel<128, false>, attend_wave_kernel<256, false>},
+                                             {attend_wave_kernel<64, true>, attend_wave_kernel<128, true>, attend_wave_kernel<256, true>}};
+        hipLaunchKernelGGL(kernels[f32][head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2], grid, dim3(64), 0, st, p);
+    }
     EH_CHECK_LAUNCH();
     if (p.splits > 1) {
-        hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 4, 65536)), dim3(256), 0, state(dev).stream, p);
+        hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 1, 65536)), dim3(256), 0, st, p);
         EH_CHECK_LAUNCH();
     }
     return 0;
