@@ -38,7 +38,6 @@ namespace {
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
-constexpr int TILE_Q = 32;   // rows (a token's query heads of one key head, side by side) of a wavefront
 constexpr int TILE_KV = 32;  // tokens of a step
 constexpr int MAX_TOKENS = 1 << 30;
 constexpr float NEG_INF = -__builtin_inff();
@@ -128,22 +127,16 @@ __device__ __forceinline__ floatx16 mfma(uintx4 a, uintx4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 // large += the product of the largest parts, small += the others, the smallest first
-template <bool F32>
-__device__ __forceinline__ void multiply(const Raw<F32> &a, const uintx4 &b0, const uintx4 &b1, const uintx4 &b2, floatx16 &large, floatx16 &small) {
-    if constexpr (F32) {
-        const float x[8] = {a.lo[0], a.lo[1], a.lo[2], a.lo[3], a.hi[0], a.hi[1], a.hi[2], a.hi[3]};
-        const Parts s = split8(x);
-        small = mfma(s.p[0], b2, small);
-        small = mfma(s.p[1], b1, small);
-        small = mfma(s.p[2], b0, small);
-        small = mfma(s.p[0], b1, small);
-        small = mfma(s.p[1], b0, small);
-        large = mfma(s.p[0], b0, large);
-    } else {
-        small = mfma(a.v, b2, small);
-        small = mfma(a.v, b1, small);
-        large = mfma(a.v, b0, large);
+template <int NP>
+__device__ __forceinline__ void multiply(const uintx4 (&a)[NP], const uintx4 (&b)[3], floatx16 &large, floatx16 &small) {
+    small = mfma(a[0], b[2], small);
+    if constexpr (NP == 3) {
+        small = mfma(a[1], b[1], small);
+        small = mfma(a[2], b[0], small);
     }
+    small = mfma(a[0], b[1], small);
+    if constexpr (NP == 3) small = mfma(a[1], b[0], small);
+    large = mfma(a[0], b[0], large);
 }
 
 __device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -214,191 +207,6 @@ __device__ __forceinline__ Range range_of(const AttendParams &p, const Sequence 
     r.all_lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
     r.lo &= ~(TILE_KV - 1);
     return r;
-}
-
-// A wavefront: 32 rows over its part of the tokens, operands straight from the cache into registers.  grid (q_tiles * splits, kv_heads, seqs).
-template <int DP, bool F32>
-__global__ __launch_bounds__(64, DP > 128 ? 1 : 2) void attend_wave_kernel(const AttendParams p) {
-    constexpr int KS = DP / 16, DT = DP / 32;
-    __shared__ uintx4 q_parts[3][KS][64];
-    const int lane = threadIdx.x, col = lane & 31, half = lane >> 5;
-    const int split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
-    const Sequence q = sequence_of(p, seq);
-    const int rows = q.fresh * p.group, ks_n = p.D >> 4;
-    const int *pages = p.table + (size_t)seq * p.width;
-    // K's lane order: row col of the product is token `k_token` of the step
-    const int a = col >> 3, k_token = 16 * (a >> 1) + 8 * ((col >> 2) & 1) + 4 * (a & 1) + (col & 3);
-
-    for (int tile = blockIdx.x / p.splits; tile * TILE_Q < rows; tile += p.q_tiles) {
-        const int row_lo = tile * TILE_Q, row_hi = min(rows, row_lo + TILE_Q);
-        const Range range = range_of(p, q, row_lo, row_hi);
-        const int steps_all = max(0, (range.hi - range.lo + TILE_KV - 1) / TILE_KV);
-        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
-        const int lo = range.lo + step_lo * TILE_KV, hi = min(range.hi, range.lo + step_hi * TILE_KV);
-
-        // ---- queries: parts of 8 dimensions of a row a lane, in LDS
-        const int row = min(row_lo + col, row_hi - 1), token = row / p.group, head = kv_head * p.group + row % p.group;
-        const int pos = q.length - q.fresh + token;
-        const float *qrow = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * p.D;
-        __syncthreads();
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-            if (ks < ks_n) {
-                float x[8];
-                if (p.vec) {
-                    const floatx4 *src = reinterpret_cast<const floatx4 *>(qrow + 16 * ks + 8 * half);
-                    const floatx4 u = src[0], v = src[1];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        x[j] = u[j] * p.scale;
-                        x[4 + j] = v[j] * p.scale;
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = qrow[16 * ks + 8 * half + j] * p.scale;
-                }
-                const Parts s = split8(x);
-#pragma unroll
-                for (int k = 0; k < 3; k++) q_parts[k][ks][lane] = s.p[k];
-            }
-        __syncthreads();
-
-        floatx16 o[DT];
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
-        float m = NEG_INF, l = 0.0f;
-        bool bad = q.bad;
-        const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
-
-        // ---- the pages of 64 blocks of 16 tokens at a time, one a lane
-        int page_lane = 0, page_from = -1;
-        auto bases = [&](int j0, size_t (&base)[2]) __attribute__((always_inline)) {
-            const int b = j0 >> 4;
-            if (page_from < 0 || b + 1 >= page_from + 64) {
-                page_from = b;
-                const int j = min((b + lane) << 4, hi - 1);  // (behind the last token: its page again, whose values do not count)
-                page_lane = pages[j >> p.page_shift];
-            }
-            base[0] = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
-            base[1] = block_base(p, __builtin_amdgcn_readlane(page_lane, b + 1 - page_from), b + 1, kv_head, bad);
-        };
-        for (int j0 = lo; j0 < hi; j0 += TILE_KV) {
-            size_t base[2];
-            bases(j0, base);
-            const size_t k_base = (k_token < 16 ? base[0] : base[1]) + (k_token & 15) * 8 + half * 128;
-            Raw<F32> k[KS], v[2][DT];
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                if (ks < ks_n) k[ks].load(p.K, k_base + ks * 256);
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    if (32 * dt < p.D) v[b][dt].load(p.V, base[b] + (size_t)half * 8 * p.D + min(32 * dt + col, p.D - 1) * 8);
-            floatx16 s_large, s_small;
-#pragma unroll
-            for (int r = 0; r < 16; r++) s_large[r] = s_small[r] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                if (ks < ks_n) multiply<F32>(k[ks], q_parts[0][ks][lane], q_parts[1][ks][lane], q_parts[2][ks][lane], s_large, s_small);
-            float s[16];
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = s_large[r] + s_small[r];
-            if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
-                    s[r] = j >= see_lo && j < see_hi ? s[r] : NEG_INF;
-                }
-                if (j0 + TILE_KV > q.length) {
-#pragma unroll
-                    for (int b = 0; b < 2; b++)
-#pragma unroll
-                        for (int dt = 0; dt < DT; dt++) v[b][dt].keep(q.length - (j0 + 16 * b + 8 * half));
-                }
-            }
-            float top = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(top, m);
-            if (__any(top > m)) {
-                const float keep = m == NEG_INF ? 0.0f : power2(m - top);
-                l *= keep;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[dt][r] *= keep;
-                m = top;
-            }
-            const float from = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[r] = power2(s[r] - from);
-                l += s[r];
-            }
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const float w[8] = {s[8 * b], s[8 * b + 1], s[8 * b + 2], s[8 * b + 3], s[8 * b + 4], s[8 * b + 5], s[8 * b + 6], s[8 * b + 7]};
-                const Parts ws = split8(w);
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    if (32 * dt < p.D) multiply<F32>(v[b][dt], ws.p[0], ws.p[1], ws.p[2], o[dt], o[dt]);
-            }
-        }
-        l += __shfl_xor(l, 32);
-
-        // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one
-        float worst = l - l;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-            if (32 * dt < p.D) {
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (32 * dt + 8 * (r >> 2) + 4 * half + (r & 3) < p.D) worst += o[dt][r] - o[dt][r];
-            }
-        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi));
-        again = again && row_lo + col < row_hi;
-        unsigned long long todo = __ballot(again);
-        todo = (todo | (todo >> 32)) & 0xffffffffull;
-        const bool redo = (todo >> col) & 1;
-        for (unsigned long long t = todo; t != 0; t &= t - 1) {
-            const int r = row_lo + __builtin_ctzll(t);
-            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, bad);
-        }
-        if (bad) l = __builtin_nanf("");
-
-        if (row_lo + col < row_hi && !redo) {
-            const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
-            const size_t slot = (size_t)split * p.rows * p.q_heads + at;
-            float factor = 1.0f, *dst;
-            if (p.splits > 1) {
-                if (half == 0) p.part_s[slot] = make_float2(m, l);
-                dst = p.part_o + slot * p.D;
-            } else {
-                store_scale(p, m, l, factor);
-                dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)head * p.D;
-            }
-            const bool whole = p.splits > 1 || p.vec;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    const int d = 32 * dt + 8 * g + 4 * half;
-                    if (d < p.D) {
-                        const floatx4 x = {o[dt][4 * g] * factor, o[dt][4 * g + 1] * factor, o[dt][4 * g + 2] * factor, o[dt][4 * g + 3] * factor};
-                        if (whole) {
-                            *reinterpret_cast<floatx4 *>(dst + d) = x;
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; i++) dst[d + i] = x[i];
-                        }
-                    }
-                }
-        }
-    }
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -686,6 +494,250 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
     }
 }
 
+// ------------------------------------------------------------------------------------------------ many rows
+// A workgroup takes 128 rows, 32 a wavefront, and walks through its part of the tokens 32 at a time, which all four wavefronts read
+// from LDS.  Bound by the matrix instruction.  The cache's order is the operands' order, so a tile is copied as it lies: a bf16
+// cache by loads into LDS (two tiles, one filled while the other is used, one barrier a tile), an fp32 cache through registers,
+// where its numbers are split once for all four wavefronts.  Every LDS access is 16 bytes a lane of 16 lanes side by side.
+// The queries' parts stay in registers (3 head_dim / 4 of them).
+constexpr int CHUNK_ROWS = 128;
+
+// FULL: head_dim is DP.  grid: a multiple of 8 workgroups
+template <int DP, bool F32, bool FULL>
+__global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
+    constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 3 : 1, BUFS = F32 ? 1 : 2, UNITS = 4 * DP;  // units: 8 numbers of a tile's keys or values
+    __shared__ uintx4 kv[BUFS][2][NP][UNITS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
+    const int D = FULL ? DP : p.D, ks_n = D >> 4;
+    // workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps
+    const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD, vid = (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD;
+    if (vid >= total || blockIdx.x / EDDLHIP_NUM_XCD >= per) return;
+    const int split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
+    const Sequence q = sequence_of(p, seq);
+    const int rows = q.fresh * p.group;
+    const int *pages = p.table + (size_t)seq * p.width;
+    // K's lane order: row col of the product is token `k_token` of the tile
+    const int a8 = col >> 3, k_token = 16 * (a8 >> 1) + 8 * ((col >> 2) & 1) + 4 * (a8 & 1) + (col & 3);
+    const int k_unit = (k_token >> 4) * 2 * D + half * 16 + (k_token & 15);
+
+    for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * CHUNK_ROWS < rows; tile += p.q_tiles) {
+        const Range all = range_of(p, q, tile * CHUNK_ROWS, min(rows, (tile + 1) * CHUNK_ROWS));
+        const int steps_all = max(0, (all.hi - all.lo + TILE_KV - 1) / TILE_KV);
+        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
+        const int lo = all.lo + step_lo * TILE_KV, hi = min(all.hi, all.lo + step_hi * TILE_KV);
+        const int row_lo = min(rows, tile * CHUNK_ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
+        const bool works = row_lo < row_hi;
+        const Range range = works ? range_of(p, q, row_lo, row_hi) : Range{0, 0, 0, 0};
+
+        const int row = works ? min(row_lo + col, row_hi - 1) : 0, token = row / p.group, head = kv_head * p.group + row % p.group;
+        const int pos = q.length - q.fresh + token;
+        uintx4 qp[KS][3];
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const float *src = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D + 16 * ks + 8 * half;
+            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (FULL || ks < ks_n) {
+                if (p.vec) {
+                    const floatx4 u = *reinterpret_cast<const floatx4 *>(src), v = *reinterpret_cast<const floatx4 *>(src + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        x[j] = u[j] * p.scale;
+                        x[4 + j] = v[j] * p.scale;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] = src[j] * p.scale;
+                }
+            }
+            const Parts s = split8(x);
+#pragma unroll
+            for (int n = 0; n < 3; n++) qp[ks][n] = s.p[n];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        floatx16 o[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+        float m = NEG_INF, l = 0.0f;
+        bool bad = q.bad;
+        const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
+
+        // ---- the tiles' way into LDS
+        int page_lane = 0, page_from = -1;
+        size_t base0 = 0, base1 = 0;
+        auto find = [&](int j0) __attribute__((always_inline)) {
+            const int b = j0 >> 4;
+            if (page_from < 0 || b + 1 >= page_from + 64) {
+                page_from = b;
+                page_lane = pages[min((b + lane) << 4, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
+            }
+            base0 = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
+            base1 = block_base(p, __builtin_amdgcn_readlane(page_lane, b + 1 - page_from), b + 1, kv_head, bad);
+        };
+        constexpr int RAW = F32 ? (8 * DP + 255) / 256 : 1;
+        Raw<true> raw[RAW];
+        auto fetch = [&](int j0, int buf) __attribute__((always_inline)) {
+            find(j0);
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < RAW; i++) {
+                    const int u = tid + 256 * i, values = u >= 4 * D, in = u - values * 4 * D, b = in >= 2 * D;
+                    if (FULL || u < 8 * D) raw[i].load(values ? p.V : p.K, (b ? base1 : base0) + (size_t)(in - b * 2 * D) * 8);
+                }
+            } else {  // (a wavefront copies one block's keys or values: 2 D units side by side)
+                const int values = wave >> 1, b = wave & 1;
+                const char *src = (const char *)(values ? p.V : p.K) + (b ? base1 : base0) * 2;
+#pragma unroll
+                for (int i = 0; i < DP / 32; i++)
+                    if (FULL || 64 * i + lane < 2 * D)
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (64 * i + lane) * 16),
+                                                         (__attribute__((address_space(3))) void *)&kv[buf][values][0][b * 2 * D + 64 * i], 16, 0, 0);
+            }
+        };
+        auto place = [&](int j0) __attribute__((always_inline)) {  // (fp32: from the registers, in parts)
+            if constexpr (F32) {
+#pragma unroll
+                for (int i = 0; i < RAW; i++) {
+                    const int u = tid + 256 * i, values = u >= 4 * D, in = u - values * 4 * D, b = in >= 2 * D;
+                    if (FULL || u < 8 * D) {
+                        if (values && j0 + TILE_KV > q.length) raw[i].keep(q.length - (j0 + 16 * b + (in - b * 2 * D >= D ? 8 : 0)));
+                        const float x[8] = {raw[i].lo[0], raw[i].lo[1], raw[i].lo[2], raw[i].lo[3], raw[i].hi[0], raw[i].hi[1], raw[i].hi[2], raw[i].hi[3]};
+                        const Parts s = split8(x);
+#pragma unroll
+                        for (int n = 0; n < NP; n++) kv[0][values][n][in] = s.p[n];
+                    }
+                }
+            }
+        };
+        __syncthreads();  // (the tile of rows before has read its last operands)
+        if (lo < hi) fetch(lo, 0);
+        for (int j0 = lo, buf = 0; j0 < hi; j0 += TILE_KV, buf = BUFS - 1 - buf) {
+            if constexpr (F32) {
+                if (j0 > lo) __syncthreads();
+                place(j0);
+                __syncthreads();
+                if (j0 + TILE_KV < hi) fetch(j0 + TILE_KV, 0);
+            } else {
+                __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile is in LDS
+                __syncthreads();
+                if (j0 + TILE_KV < hi) fetch(j0 + TILE_KV, 1 - buf);
+            }
+            if (j0 >= range.hi || j0 + TILE_KV <= range.lo) continue;  // (none of this wavefront's rows sees the tile)
+            floatx16 large, small;
+#pragma unroll
+            for (int r = 0; r < 16; r++) large[r] = small[r] = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                if (FULL || ks < ks_n) {
+                    uintx4 k[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; n++) k[n] = kv[buf][0][n][k_unit + 32 * ks];
+                    multiply<NP>(k, qp[ks], large, small);
+                }
+            float s[16];
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = large[r] + small[r];
+            if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
+                    s[r] = j >= see_lo && j < see_hi ? s[r] : NEG_INF;
+                }
+            }
+            float top = s[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            top = fmaxf(top, m);
+            if (__any(top > m)) {
+                const float keep = m == NEG_INF ? 0.0f : power2(m - top);
+                l *= keep;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) o[dt][r] *= keep;
+                m = top;
+            }
+            const float from = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[r] = power2(s[r] - from);
+                l += s[r];
+            }
+            const bool tail = !F32 && j0 + TILE_KV > q.length;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float w[8] = {s[8 * b], s[8 * b + 1], s[8 * b + 2], s[8 * b + 3], s[8 * b + 4], s[8 * b + 5], s[8 * b + 6], s[8 * b + 7]};
+                const Parts ws = split8(w);
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+                    if (FULL || 32 * dt < D) {
+                        uintx4 v[NP];
+#pragma unroll
+                        for (int n = 0; n < NP; n++) v[n] = kv[buf][1][n][b * 2 * D + half * D + (FULL ? 32 * dt + col : min(32 * dt + col, D - 1))];
+                        if constexpr (!F32) {
+                            if (tail) {
+                                Raw<false> x;
+                                x.v = v[0];
+                                x.keep(q.length - (j0 + 16 * b + 8 * half));
+                                v[0] = x.v;
+                            }
+                        }
+                        multiply<NP>(v, ws.p, o[dt], o[dt]);
+                    }
+            }
+        }
+        l += __shfl_xor(l, 32);
+
+        // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one
+        float worst = l - l;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (FULL || 32 * dt + 8 * (r >> 2) + 4 * half + (r & 3) < D) worst += o[dt][r] - o[dt][r];
+        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi)) || bad;
+        again = again && row_lo + col < row_hi;
+        unsigned long long todo = __ballot(again);
+        todo = (todo | (todo >> 32)) & 0xffffffffull;
+        const bool redo = (todo >> col) & 1;
+        for (unsigned long long t = todo; t != 0; t &= t - 1) {
+            const int r = row_lo + __builtin_ctzll(t);
+            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, q.bad);
+        }
+
+        if (row_lo + col < row_hi && !redo) {
+            const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
+            const size_t slot = (size_t)split * p.rows * p.q_heads + at;
+            float factor = 1.0f, *dst;
+            if (p.splits > 1) {
+                if (half == 0) p.part_s[slot] = make_float2(m, l);
+                dst = p.part_o + slot * D;
+            } else {
+                store_scale(p, m, l, factor);
+                dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)head * D;
+            }
+            const bool whole = p.splits > 1 || p.vec;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int d = 32 * dt + 8 * g + 4 * half;
+                    if (FULL || d < D) {
+                        const floatx4 x = {o[dt][4 * g] * factor, o[dt][4 * g + 1] * factor, o[dt][4 * g + 2] * factor, o[dt][4 * g + 3] * factor};
+                        if (whole) {
+                            *reinterpret_cast<floatx4 *>(dst + d) = x;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) dst[d + i] = x[i];
+                        }
+                    }
+                }
+        }
+    }
+}
+
 // Joins the parts of a row, a workgroup a row: the weights of all parts first, then four dimensions and every (1024 / head_dim)th part a
 // thread, then those together, in an order that the shape alone fixes.
 constexpr int MAX_SPLITS = 512;
@@ -753,6 +805,13 @@ void launch_few(const AttendParams &p, bool f32, int nq, dim3 grid, hipStream_t 
     hipLaunchKernelGGL(kernels[f32][nq - 1], grid, dim3(64 * FEW_WAVES), 0, st, p);
 }
 
+template <int DP, bool FULL>
+void launch_chunk(const AttendParams &p, bool f32, int total, hipStream_t st) {
+    const dim3 grid((total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD);
+    if (f32) hipLaunchKernelGGL((attend_chunk_kernel<DP, true, FULL>), grid, dim3(256), 0, st, p, total);
+    else hipLaunchKernelGGL((attend_chunk_kernel<DP, false, FULL>), grid, dim3(256), 0, st, p, total);
+}
+
 }  // namespace
 
 extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, long long ldo, int rows, const void *k_pages, const void *v_pages,
@@ -800,14 +859,14 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     p.scale = scale * 1.44269504088896340736f;
     // The launch goes by the bounds max_new and max_length; what is beyond them is still computed, by the same wavefronts.
     const long long fresh = std::min(max_new > 0 ? max_new : 1, rows), tile_rows = fresh * p.group;
-    const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : TILE_Q;
+    const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : CHUNK_ROWS;
     const long long tiles = (tile_rows + per_tile - 1) / per_tile;
     p.q_tiles = (int)tiles;
-    const long long groups = tiles * kv_heads * seqs, want = (nq ? 3LL : 8LL) * state(dev).num_cu;
+    const long long groups = tiles * kv_heads * seqs, want = (nq ? 3LL : 2LL) * state(dev).num_cu;
     long long seen = max_length > 0 ? max_length : 1;
     if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
-    p.splits = (int)std::max(1LL, std::min({want / groups, steps / (nq ? 8 : 4), (long long)MAX_SPLITS}));
+    p.splits = (int)std::max(1LL, std::min({want / groups, steps / 8, (long long)MAX_SPLITS}));
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
@@ -817,7 +876,7 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
         p.part_o = (float *)ws;
         p.part_s = (float2 *)((char *)ws + slots * head_dim * sizeof(float));
     }
-    EH_REQUIRE(tiles * p.splits < (1LL << 31), "paged_attention: shape out of range");
+    EH_REQUIRE(groups * p.splits < (1LL << 30), "paged_attention: shape out of range");
     const dim3 grid((unsigned)(tiles * p.splits), kv_heads, seqs);
     const hipStream_t st = state(dev).stream;
     const bool f32 = cache_type == EDDLHIP_CACHE_F32;
@@ -829,10 +888,13 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
         else if (head_dim < 128) launch_few<128, false>(p, f32, nq, grid, st);
         else launch_few<256, false>(p, f32, nq, grid, st);
     } else {
-        typedef void (*kernel)(AttendParams);
-        static const kernel kernels[2][3] = {{attend_wave_kernel<64, false>, attend_wave_kernel<128, false>, attend_wave_kernel<256, false>},
-                                             {attend_wave_kernel<64, true>, attend_wave_kernel<128, true>, attend_wave_kernel<256, true>}};
-        hipLaunchKernelGGL(kernels[f32][head_dim <= 64 ? 0 : head_dim <= 128 ? 1 : 2], grid, dim3(64), 0, st, p);
+        const int total = (int)(groups * p.splits);
+        if (head_dim == 64) launch_chunk<64, true>(p, f32, total, st);
+        else if (head_dim == 128) launch_chunk<128, true>(p, f32, total, st);
+        else if (head_dim == 256) launch_chunk<256, true>(p, f32, total, st);
+        else if (head_dim < 64) launch_chunk<64, false>(p, f32, total, st);
+        else if (head_dim < 128) launch_chunk<128, false>(p, f32, total, st);
+        else launch_chunk<256, false>(p, f32, total, st);
     }
     EH_CHECK_LAUNCH();
     if (p.splits > 1) {
