@@ -27,6 +27,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "split_parts.h"
@@ -209,6 +210,12 @@ __device__ __forceinline__ Range range_of(const AttendParams &p, const Sequence 
     return r;
 }
 
+// Step at which part `n` of `parts` begins: parts differ by at most one step.
+__device__ __forceinline__ int part_at(int steps, int n, int parts) {
+    const int each = (int)((unsigned)steps / (unsigned)parts), more = steps - each * parts;
+    return n * each + min(n, more);
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 NQ rows of a sequence and key head (single tokens, short drafts): bound by the cache's bytes.  A workgroup takes a part of the
 // tokens, its four wavefronts take steps of 32 tokens in turn, operands straight from the cache into registers: every byte is read
@@ -251,7 +258,8 @@ struct Operand<true> {
     }
 };
 
-// FULL: head_dim is DP.  grid (q_tiles * splits, kv_heads, seqs)
+// FULL: head_dim is DP; otherwise DP - 64 < head_dim < DP: dimensions past the last are zeros of the queries, which meet the last 8
+// dimensions of the keys again, and outputs that nobody reads.  grid (q_tiles * splits, kv_heads, seqs)
 template <int DP, bool F32, int NQ, bool FULL>
 __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ > 1) ? 1 : 2) void attend_few_kernel(const AttendParams p) {
     constexpr int KS = DP / 32, DT = DP / 16, W = FEW_WAVES, COLS = 16 * NQ, PITCH = DP + 4;
@@ -263,7 +271,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
     float(*o_lds)[COLS][PITCH] = reinterpret_cast<float(*)[COLS][PITCH]>(lds);
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
-    const int D = FULL ? DP : p.D, ks_n = FULL ? KS : (D + 31) >> 5, dt_n = FULL ? DT : D >> 4;
+    const int D = FULL ? DP : p.D;
     const int split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
     const Sequence q = sequence_of(p, seq);
     const int rows = q.fresh * p.group;
@@ -273,7 +281,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
         const int row_lo = tile * COLS, row_hi = min(rows, row_lo + COLS);
         const Range range = range_of(p, q, row_lo, row_hi);
         const int steps_all = max(0, (range.hi - range.lo + TILE_KV - 1) / TILE_KV);
-        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
+        const int step_lo = part_at(steps_all, split, p.splits), step_hi = part_at(steps_all, split + 1, p.splits);
         const int lo = range.lo + step_lo * TILE_KV, hi = min(range.hi, range.lo + step_hi * TILE_KV);
         __syncthreads();  // (the tile before has been stored)
 
@@ -299,14 +307,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
                 const int token = (8 * (col >> 2) + 4 * t + (col & 3)) & 15;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++)
-                    if (FULL || ks < ks_n) k[t][ks].load(p.K, from + token * 8 + (FULL ? 4 * ks + g : min(4 * ks + g, (D >> 3) - 1)) * 128);
+                    k[t][ks].load(p.K, from + token * 8 + (FULL ? 4 * ks + g : min(4 * ks + g, (D >> 3) - 1)) * 128);
             }
         };
         auto load_values = [&]() __attribute__((always_inline)) {
-            const size_t from = (g & 2 ? base[1] : base[0]) + (size_t)(g & 1) * 8 * D + col * 8;
+            const size_t from = (g & 2 ? base[1] : base[0]) + (size_t)(g & 1) * 8 * D;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-                if (FULL || dt < dt_n) v[dt].load(p.V, from + dt * 128);
+            for (int dt = 0; dt < DT; dt++) v[dt].load(p.V, from + (FULL ? 16 * dt + col : min(16 * dt + col, D - 1)) * 8);
         };
         const int its = (step_hi - step_lo - wave + W - 1) / W;  // steps of this wavefront
         if (its > 0 && hi > lo) {
@@ -316,7 +323,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
         }
 
         // ---- queries: parts of 8 dimensions of a row a lane, in LDS, made by all wavefronts together
-        for (int i = wave; i < ks_n * NQ; i += W) {
+        for (int i = wave; i < KS * NQ; i += W) {
             const int ks = i / NQ, nq = i % NQ, row = min(row_lo + 16 * nq + col, row_hi - 1), token = row / p.group, head = kv_head * p.group + row % p.group;
             const int d = 32 * ks + 8 * g;
             float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -366,17 +373,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
 #pragma unroll
                 for (int t = 0; t < 2; t++) large[nq][t] = small[nq][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                if (FULL || ks < ks_n) {
-                    const Operand<F32> a0(k[0][ks]), a1(k[1][ks]);
+            for (int ks = 0; ks < KS; ks++) {
+                const Operand<F32> a0(k[0][ks]), a1(k[1][ks]);
 #pragma unroll
-                    for (int nq = 0; nq < NQ; nq++) {
-                        const uintx4 b0 = q_parts[0][ks][nq][lane], b1 = q_parts[1][ks][nq][lane], b2 = q_parts[2][ks][nq][lane];
-                        a0.multiply(b0, b1, b2, large[nq][0], small[nq][0]);
-                        a1.multiply(b0, b1, b2, large[nq][1], small[nq][1]);
-                    }
-                    __builtin_amdgcn_sched_barrier(0);  // (one operand's parts at a time: registers)
+                for (int nq = 0; nq < NQ; nq++) {
+                    const uintx4 b0 = q_parts[0][ks][nq][lane], b1 = q_parts[1][ks][nq][lane], b2 = q_parts[2][ks][nq][lane];
+                    a0.multiply(b0, b1, b2, large[nq][0], small[nq][0]);
+                    a1.multiply(b0, b1, b2, large[nq][1], small[nq][1]);
                 }
+                __builtin_amdgcn_sched_barrier(0);  // (one operand's parts at a time: registers)
+            }
             if (more) {
                 find(it + 1);
                 load_keys();
@@ -419,13 +425,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
                 ws[nq] = split8(s);
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-                if (FULL || dt < dt_n) {
-                    const Operand<F32> a(v[dt]);
+            for (int dt = 0; dt < DT; dt++) {
+                const Operand<F32> a(v[dt]);
 #pragma unroll
-                    for (int nq = 0; nq < NQ; nq++) a.multiply(ws[nq].p[0], ws[nq].p[1], ws[nq].p[2], o[nq][dt], o[nq][dt]);
-                    if (F32) __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int nq = 0; nq < NQ; nq++) a.multiply(ws[nq].p[0], ws[nq].p[1], ws[nq].p[2], o[nq][dt], o[nq][dt]);
+                if (F32) __builtin_amdgcn_sched_barrier(0);
+            }
             if (more) load_values();
         }
         __syncthreads();  // (the queries have been read: their place takes the outputs)
@@ -439,8 +444,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
                 sums[wave][16 * nq + col][1] = l[nq];
             }
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-                if (FULL || dt < dt_n) *reinterpret_cast<floatx4 *>(&o_lds[wave][16 * nq + col][16 * dt + 4 * g]) = o[nq][dt];
+            for (int dt = 0; dt < DT; dt++) *reinterpret_cast<floatx4 *>(&o_lds[wave][16 * nq + col][16 * dt + 4 * g]) = o[nq][dt];
         }
         __syncthreads();
 
@@ -502,13 +506,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
 // The queries' parts stay in registers (3 head_dim / 4 of them).
 constexpr int CHUNK_ROWS = 128;
 
-// FULL: head_dim is DP.  grid: a multiple of 8 workgroups
+// FULL: head_dim is DP; otherwise the dimensions past the last are zeros in LDS.  grid: a multiple of 8 workgroups
 template <int DP, bool F32, bool FULL>
 __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
     constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 3 : 1, BUFS = F32 ? 1 : 2, UNITS = 4 * DP;  // units: 8 numbers of a tile's keys or values
     __shared__ uintx4 kv[BUFS][2][NP][UNITS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
-    const int D = FULL ? DP : p.D, ks_n = D >> 4;
+    const int D = FULL ? DP : p.D;
     // workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps
     const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD, vid = (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD;
     if (vid >= total || blockIdx.x / EDDLHIP_NUM_XCD >= per) return;
@@ -518,12 +522,16 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
     const int *pages = p.table + (size_t)seq * p.width;
     // K's lane order: row col of the product is token `k_token` of the tile
     const int a8 = col >> 3, k_token = 16 * (a8 >> 1) + 8 * ((col >> 2) & 1) + 4 * (a8 & 1) + (col & 3);
-    const int k_unit = (k_token >> 4) * 2 * D + half * 16 + (k_token & 15);
+    const int k_unit = (k_token >> 4) * 2 * DP + half * 16 + (k_token & 15);
+
+    if constexpr (!FULL) {
+        for (int i = tid; i < BUFS * 2 * NP * UNITS; i += 256) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
+    }
 
     for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * CHUNK_ROWS < rows; tile += p.q_tiles) {
         const Range all = range_of(p, q, tile * CHUNK_ROWS, min(rows, (tile + 1) * CHUNK_ROWS));
         const int steps_all = max(0, (all.hi - all.lo + TILE_KV - 1) / TILE_KV);
-        const int step_lo = (int)((long long)steps_all * split / p.splits), step_hi = (int)((long long)steps_all * (split + 1) / p.splits);
+        const int step_lo = part_at(steps_all, split, p.splits), step_hi = part_at(steps_all, split + 1, p.splits);
         const int lo = all.lo + step_lo * TILE_KV, hi = min(all.hi, all.lo + step_hi * TILE_KV);
         const int row_lo = min(rows, tile * CHUNK_ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
         const bool works = row_lo < row_hi;
@@ -536,7 +544,7 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
         for (int ks = 0; ks < KS; ks++) {
             const float *src = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D + 16 * ks + 8 * half;
             float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (FULL || ks < ks_n) {
+            if (FULL || 16 * ks < D) {
                 if (p.vec) {
                     const floatx4 u = *reinterpret_cast<const floatx4 *>(src), v = *reinterpret_cast<const floatx4 *>(src + 4);
 #pragma unroll
@@ -588,11 +596,20 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
             } else {  // (a wavefront copies one block's keys or values: 2 D units side by side)
                 const int values = wave >> 1, b = wave & 1;
                 const char *src = (const char *)(values ? p.V : p.K) + (b ? base1 : base0) * 2;
+                auto copy = [&](int from, int to, int units) __attribute__((always_inline)) {
+                    if (FULL || lane < units)
+                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (from + lane) * 16),
+                                                         (__attribute__((address_space(3))) void *)&kv[buf][values][0][b * 2 * DP + to], 16, 0, 0);
+                };
+                if (FULL || !values) {
 #pragma unroll
-                for (int i = 0; i < DP / 32; i++)
-                    if (FULL || 64 * i + lane < 2 * D)
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (64 * i + lane) * 16),
-                                                         (__attribute__((address_space(3))) void *)&kv[buf][values][0][b * 2 * D + 64 * i], 16, 0, 0);
+                    for (int i = 0; i < DP / 32; i++) copy(64 * i, 64 * i, 2 * D - 64 * i);
+                } else {  // (two runs of D units)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int i = 0; i < (DP + 63) / 64; i++) copy(h * D + 64 * i, h * DP + 64 * i, D - 64 * i);
+                }
             }
         };
         auto place = [&](int j0) __attribute__((always_inline)) {  // (fp32: from the registers, in parts)
@@ -605,7 +622,7 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
                         const float x[8] = {raw[i].lo[0], raw[i].lo[1], raw[i].lo[2], raw[i].lo[3], raw[i].hi[0], raw[i].hi[1], raw[i].hi[2], raw[i].hi[3]};
                         const Parts s = split8(x);
 #pragma unroll
-                        for (int n = 0; n < NP; n++) kv[0][values][n][in] = s.p[n];
+                        for (int n = 0; n < NP; n++) kv[0][values][n][b * 2 * DP + (in - b * 2 * D) + (values && in - b * 2 * D >= D ? DP - D : 0)] = s.p[n];
                     }
                 }
             }
@@ -628,13 +645,12 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
 #pragma unroll
             for (int r = 0; r < 16; r++) large[r] = small[r] = 0.0f;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                if (FULL || ks < ks_n) {
-                    uintx4 k[NP];
+            for (int ks = 0; ks < KS; ks++) {
+                uintx4 k[NP];
 #pragma unroll
-                    for (int n = 0; n < NP; n++) k[n] = kv[buf][0][n][k_unit + 32 * ks];
-                    multiply<NP>(k, qp[ks], large, small);
-                }
+                for (int n = 0; n < NP; n++) k[n] = kv[buf][0][n][k_unit + 32 * ks];
+                multiply<NP>(k, qp[ks], large, small);
+            }
             float s[16];
 #pragma unroll
             for (int r = 0; r < 16; r++) s[r] = large[r] + small[r];
@@ -671,21 +687,20 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
                 const float w[8] = {s[8 * b], s[8 * b + 1], s[8 * b + 2], s[8 * b + 3], s[8 * b + 4], s[8 * b + 5], s[8 * b + 6], s[8 * b + 7]};
                 const Parts ws = split8(w);
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-                    if (FULL || 32 * dt < D) {
-                        uintx4 v[NP];
+                for (int dt = 0; dt < DT; dt++) {
+                    uintx4 v[NP];
 #pragma unroll
-                        for (int n = 0; n < NP; n++) v[n] = kv[buf][1][n][b * 2 * D + half * D + (FULL ? 32 * dt + col : min(32 * dt + col, D - 1))];
-                        if constexpr (!F32) {
-                            if (tail) {
-                                Raw<false> x;
-                                x.v = v[0];
-                                x.keep(q.length - (j0 + 16 * b + 8 * half));
-                                v[0] = x.v;
-                            }
+                    for (int n = 0; n < NP; n++) v[n] = kv[buf][1][n][(b * 2 + half) * DP + 32 * dt + col];
+                    if constexpr (!F32) {
+                        if (tail) {
+                            Raw<false> x;
+                            x.v = v[0];
+                            x.keep(q.length - (j0 + 16 * b + 8 * half));
+                            v[0] = x.v;
                         }
-                        multiply<NP>(v, ws.p, o[dt], o[dt]);
                     }
+                    multiply<NP>(v, ws.p, o[dt], o[dt]);
+                }
             }
         }
         l += __shfl_xor(l, 32);
@@ -695,8 +710,7 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-            for (int r = 0; r < 16; r++)
-                if (FULL || 32 * dt + 8 * (r >> 2) + 4 * half + (r & 3) < D) worst += o[dt][r] - o[dt][r];
+            for (int r = 0; r < 16; r++) worst += o[dt][r] - o[dt][r];
         bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi)) || bad;
         again = again && row_lo + col < row_hi;
         unsigned long long todo = __ballot(again);
@@ -738,7 +752,41 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
     }
 }
 
-// Joins the parts of a row, a workgroup a row: the weights of all parts first, then four dimensions and every (1024 / head_dim)th part a
+// Joins the few parts of a row, a wavefront a row: every lane reads all weights and four dimensions of every part.
+constexpr int JOIN_FEW = 16;
+__global__ __launch_bounds__(256) void attend_join_few_kernel(const AttendParams p) {
+    const int lane = threadIdx.x & 63, d = 4 * lane;
+    const long long total = (long long)p.rows * p.q_heads;
+    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
+    for (long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += (long long)gridDim.x * 4) {
+        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
+        if (row < first || row >= end) continue;
+        float m = NEG_INF, l = 0.0f;
+        for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_s[(size_t)s * total + at].x);
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int s = 0; s < p.splits; s++) {
+            const float2 ms = p.part_s[(size_t)s * total + at];
+            const float w = ms.x == NEG_INF && ms.y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(ms.x - m);
+            l += w * ms.y;
+            if (d < p.D) o += *reinterpret_cast<const floatx4 *>(p.part_o + ((size_t)s * total + at) * p.D + d) * w;
+        }
+        float factor;
+        store_scale(p, m, l, factor);
+        if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
+        float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + d;
+        if (d < p.D) {
+            if (p.vec) {
+                *reinterpret_cast<floatx4 *>(dst) = o * factor;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
+            }
+        }
+    }
+}
+
+// Joins the many parts of a row, a workgroup a row: the weights of all parts first, then four dimensions and every (1024 / head_dim)th part a
 // thread, then those together, in an order that the shape alone fixes.
 constexpr int MAX_SPLITS = 512;
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
@@ -880,25 +928,24 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     const dim3 grid((unsigned)(tiles * p.splits), kv_heads, seqs);
     const hipStream_t st = state(dev).stream;
     const bool f32 = cache_type == EDDLHIP_CACHE_F32;
-    if (nq) {
-        if (head_dim == 64) launch_few<64, true>(p, f32, nq, grid, st);
-        else if (head_dim == 128) launch_few<128, true>(p, f32, nq, grid, st);
-        else if (head_dim == 256) launch_few<256, true>(p, f32, nq, grid, st);
-        else if (head_dim < 64) launch_few<64, false>(p, f32, nq, grid, st);
-        else if (head_dim < 128) launch_few<128, false>(p, f32, nq, grid, st);
-        else launch_few<256, false>(p, f32, nq, grid, st);
-    } else {
-        const int total = (int)(groups * p.splits);
-        if (head_dim == 64) launch_chunk<64, true>(p, f32, total, st);
-        else if (head_dim == 128) launch_chunk<128, true>(p, f32, total, st);
-        else if (head_dim == 256) launch_chunk<256, true>(p, f32, total, st);
-        else if (head_dim < 64) launch_chunk<64, false>(p, f32, total, st);
-        else if (head_dim < 128) launch_chunk<128, false>(p, f32, total, st);
-        else launch_chunk<256, false>(p, f32, total, st);
-    }
+    const int total = (int)(groups * p.splits);
+    auto launch = [&](auto size, auto full) {
+        if (nq) launch_few<size(), full()>(p, f32, nq, grid, st);
+        else launch_chunk<size(), full()>(p, f32, total, st);
+    };
+    auto sized = [&](auto size) {
+        if (head_dim == size()) launch(size, std::true_type());
+        else launch(size, std::false_type());
+    };
+    if (head_dim <= 64) sized(std::integral_constant<int, 64>());
+    else if (head_dim <= 96) sized(std::integral_constant<int, 96>());
+    else if (head_dim <= 128) sized(std::integral_constant<int, 128>());
+    else if (head_dim <= 192) sized(std::integral_constant<int, 192>());
+    else sized(std::integral_constant<int, 256>());
     EH_CHECK_LAUNCH();
     if (p.splits > 1) {
-        hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 1, 65536)), dim3(256), 0, st, p);
+        if (p.splits <= JOIN_FEW) hipLaunchKernelGGL(attend_join_few_kernel, dim3(eh_blocks((size_t)rows * q_heads, 4, 65536)), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 1, 65536)), dim3(256), 0, st, p);
         EH_CHECK_LAUNCH();
     }
     return 0;
