@@ -24,9 +24,8 @@
 // replaced by zeros; a NaN or infinity in a visible or masked place of a tile otherwise reaches the sums as NaN (0 * inf, or the parts
 // of an infinity), and rows whose sums are not finite are computed again one token at a time (attend_row_again), with what
 // the formula gives.
-#include <math.h>
-
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "common.h"
@@ -38,6 +37,7 @@ namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef unsigned short ushortx2 __attribute__((ext_vector_type(2)));
 
 constexpr int TILE_KV = 32;  // tokens of a step
 constexpr int MAX_TOKENS = 1 << 30;
@@ -91,6 +91,19 @@ struct Raw<false> {
 #pragma unroll
         for (int i = 0; i < 4; i++) v[i] = 2 * i + 1 < count ? v[i] : 2 * i < count ? v[i] & 0xffffu : 0u;
     }
+    __device__ __forceinline__ void numbers(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __builtin_bit_cast(float, v[i] << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, v[i] & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ unsigned largest() const {  // the bits of the largest magnitude (of a NaN, if there is one)
+        ushortx2 m = __builtin_bit_cast(ushortx2, v[0] & 0x7fff7fffu);
+#pragma unroll
+        for (int i = 1; i < 4; i++) m = __builtin_elementwise_max(m, __builtin_bit_cast(ushortx2, v[i] & 0x7fff7fffu));
+        return (unsigned)max(m[0], m[1]) << 16;
+    }
 };
 template <>
 struct Raw<true> {
@@ -106,6 +119,19 @@ struct Raw<true> {
             lo[i] = i < count ? lo[i] : 0.0f;
             hi[i] = 4 + i < count ? hi[i] : 0.0f;
         }
+    }
+    __device__ __forceinline__ void numbers(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[i] = lo[i];
+            x[4 + i] = hi[i];
+        }
+    }
+    __device__ __forceinline__ unsigned largest() const {  // the bits of the largest magnitude, NaN left out
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = fmaxf(fmaxf(m, fabsf(lo[i])), fabsf(hi[i]));
+        return __builtin_bit_cast(unsigned, m);
     }
 };
 
@@ -124,22 +150,6 @@ __device__ __forceinline__ Parts split8(const float (&x)[8]) {
     }
     return s;
 }
-__device__ __forceinline__ floatx16 mfma(uintx4 a, uintx4 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-// large += the product of the largest parts, small += the others, the smallest first
-template <int NP>
-__device__ __forceinline__ void multiply(const uintx4 (&a)[NP], const uintx4 (&b)[3], floatx16 &large, floatx16 &small) {
-    small = mfma(a[0], b[2], small);
-    if constexpr (NP == 3) {
-        small = mfma(a[1], b[1], small);
-        small = mfma(a[2], b[0], small);
-    }
-    small = mfma(a[0], b[1], small);
-    if constexpr (NP == 3) small = mfma(a[1], b[0], small);
-    large = mfma(a[0], b[0], large);
-}
-
 __device__ __forceinline__ float power2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float element(const AttendParams &p, const void *base, size_t at, bool f32) {
     return f32 ? ((const float *)base)[at] : __builtin_bit_cast(float, (unsigned)((const unsigned short *)base)[at] << 16);
@@ -500,22 +510,92 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
 
 // ------------------------------------------------------------------------------------------------ many rows
 // A workgroup takes 128 rows, 32 a wavefront, and walks through its part of the tokens 32 at a time, which all four wavefronts read
-// from LDS.  Bound by the matrix instruction.  The cache's order is the operands' order, so a tile is copied as it lies: a bf16
-// cache by loads into LDS (two tiles, one filled while the other is used, one barrier a tile), an fp32 cache through registers,
-// where its numbers are split once for all four wavefronts.  Every LDS access is 16 bytes a lane of 16 lanes side by side.
-// The queries' parts stay in registers (3 head_dim / 4 of them).
+// from LDS.  Bound by the matrix instruction, so its operands are pairs of fp16 numbers here and not three bf16 numbers:
+// x 2^e = hi + lo, hi = fp16(x 2^e), lo = fp16(x 2^e - hi), with e such that the largest number of a row of queries, or of 16 tokens'
+// keys or values of a head, lies in 2^14 .. 2^15.  Each half brings 11 bits and its sign: a pair is off by at most 2^-23 of x, or, where
+// lo runs out of fp16's range, by 2^-25 of 2^-14 of the largest number, 2^-39.  A bf16 number is its own hi down to 2^-31 of the largest.
+// Two pairs take three products (lo lo is below 2^-24 of the whole), a pair and a bf16 number two, where the bf16 parts take six and
+// three; and a pair costs 4 instructions for two numbers where three parts cost 11.  The rows' and blocks' exponents go into the scores as
+// factors, and the blocks' exponents of values into the weights: a weight is exp2(s - m + c) with c = 14 + (the block's exponent) - (the largest so
+// far), the output carries the largest, a whole number of doublings like m.  (14: weights of 2^-28 still have eleven bits in hi.)
+// A block whose largest number is infinite takes a NaN as its factor, so that its rows are computed again.
+// Tiles: a wavefront brings the keys or the values of 16 tokens, their numbers go through its registers (the largest, the pairs) into LDS;
+// two tiles, one filled while the other is used, one barrier a tile.  The cache's order is the operands' order: every LDS
+// access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
 constexpr int CHUNK_ROWS = 128;
+
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ floatx16 mfma(uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ unsigned round_half(float a, float b) {  // two fp16, rounded to nearest even
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2){a, b}, halfx2));
+}
+// Two numbers as pairs; the differences are exact, one instruction each.
+__device__ __forceinline__ void pair_up(float a, float b, unsigned &hi, unsigned &lo) {
+    float ra, rb;
+    hi = round_half(a, b);
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
+    lo = round_half(ra, rb);
+}
+struct Pair {
+    uintx4 hi, lo;
+};
+__device__ __forceinline__ Pair pair8(const float (&x)[8]) {
+    Pair r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        unsigned h, l;
+        pair_up(x[2 * i], x[2 * i + 1], h, l);
+        r.hi[i] = h;
+        r.lo[i] = l;
+    }
+    return r;
+}
+// Factor 2^(14 - exponent) of numbers whose largest magnitude is given by its bits, its inverse, and that as a power of two.
+struct Scale {
+    float up, down, power;
+};
+__device__ __forceinline__ Scale scale_of(unsigned bits) {
+    unsigned e = bits >> 23;
+    const bool whole = e < 255u;
+    e = bits == 0u ? 141u : max(e, 15u);
+    Scale s;
+    s.up = whole ? __builtin_bit_cast(float, (268u - e) << 23) : 1.0f;
+    s.down = whole ? __builtin_bit_cast(float, (e - 14u) << 23) : __builtin_nanf("");
+    s.power = whole ? (float)((int)e - 141) : __builtin_nanf("");
+    return s;
+}
+__device__ __forceinline__ unsigned wave_max(unsigned v) {  // in lane 63, read from there
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false));
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xf, 0xf, false));  // row_bcast:15, 31
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xf, 0xf, false));
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
+template <int NP>
+__device__ __forceinline__ floatx16 multiply(const uintx4 (&a)[NP], const Pair &b, floatx16 c) {
+    if constexpr (NP == 2) c = mfma(a[1], b.hi, c);
+    c = mfma(a[0], b.lo, c);
+    return mfma(a[0], b.hi, c);
+}
 
 // FULL: head_dim is DP; otherwise the dimensions past the last are zeros in LDS.  grid: a multiple of 8 workgroups
 template <int DP, bool F32, bool FULL>
-__global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
-    constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 3 : 1, BUFS = F32 ? 1 : 2, UNITS = 4 * DP;  // units: 8 numbers of a tile's keys or values
-    __shared__ uintx4 kv[BUFS][2][NP][UNITS];
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
+    constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 2 : 1, UNITS = 4 * DP, EACH = DP / 32;  // units: 8 numbers of a tile's keys or values
+    __shared__ uintx4 kv[2][2][NP][UNITS];
+    __shared__ float scales[2][4];  // of a tile's two blocks: keys' factors, values' powers of two
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     const int D = FULL ? DP : p.D;
     // workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps
     const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD, vid = (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD;
-    if (vid >= total || blockIdx.x / EDDLHIP_NUM_XCD >= per) return;
+    if (vid >= total) return;
     const int split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
     const Sequence q = sequence_of(p, seq);
     const int rows = q.fresh * p.group;
@@ -523,9 +603,10 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
     // K's lane order: row col of the product is token `k_token` of the tile
     const int a8 = col >> 3, k_token = 16 * (a8 >> 1) + 8 * ((col >> 2) & 1) + 4 * (a8 & 1) + (col & 3);
     const int k_unit = (k_token >> 4) * 2 * DP + half * 16 + (k_token & 15);
+    const int values = wave >> 1, block = wave & 1;  // what this wavefront brings of a tile
 
     if constexpr (!FULL) {
-        for (int i = tid; i < BUFS * 2 * NP * UNITS; i += 256) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
+        for (int i = tid; i < 2 * 2 * NP * UNITS; i += 256) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
     }
 
     for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * CHUNK_ROWS < rows; tile += p.q_tiles) {
@@ -537,173 +618,193 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
         const bool works = row_lo < row_hi;
         const Range range = works ? range_of(p, q, row_lo, row_hi) : Range{0, 0, 0, 0};
 
-        const int row = works ? min(row_lo + col, row_hi - 1) : 0, token = row / p.group, head = kv_head * p.group + row % p.group;
-        const int pos = q.length - q.fresh + token;
-        uintx4 qp[KS][3];
+        // ---- the tiles' way into LDS
+        bool bad = false;  // of the block that is on its way
+        int page_lane = 0, page_from = -1;
+        Raw<F32> raw[EACH];
+        auto fetch = [&](int j0) __attribute__((always_inline)) {
+            const int b = (j0 >> 4) + block;
+            if (page_from < 0 || b >= page_from + 64) {
+                page_from = b;
+                page_lane = pages[min((b + lane) << 4, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
+            }
+            bad = false;
+            const size_t base = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
+            const void *src = values ? p.V : p.K;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const float *src = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D + 16 * ks + 8 * half;
-            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-            if (FULL || 16 * ks < D) {
-                if (p.vec) {
-                    const floatx4 u = *reinterpret_cast<const floatx4 *>(src), v = *reinterpret_cast<const floatx4 *>(src + 4);
+            for (int i = 0; i < EACH; i++)
+                if (FULL || 64 * i + lane < 2 * D) raw[i].load(src, base + (size_t)(64 * i + lane) * 8);
+        };
+        auto place = [&](int j0, int buf) __attribute__((always_inline)) {
+            const int from = j0 + 16 * block;
+            if (from + 16 > q.length) {  // nothing behind the last token counts
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        x[j] = u[j] * p.scale;
-                        x[4 + j] = v[j] * p.scale;
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = src[j] * p.scale;
+                for (int i = 0; i < EACH; i++) {
+                    const int u = 64 * i + lane;
+                    if (values) raw[i].keep(q.length - (from + (u >= D ? 8 : 0)));
+                    else raw[i].keep(from + (u & 15) < q.length ? 8 : 0);
                 }
             }
-            const Parts s = split8(x);
+            unsigned top = 0;
 #pragma unroll
-            for (int n = 0; n < 3; n++) qp[ks][n] = s.p[n];
-            __builtin_amdgcn_sched_barrier(0);
+            for (int i = 0; i < EACH; i++)
+                if (FULL || 64 * i + lane < 2 * D) top = max(top, raw[i].largest());
+            const Scale scale = scale_of(wave_max(top));
+            if (lane == 0) scales[buf][wave] = bad ? __builtin_nanf("") : values ? scale.power : scale.down;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) {
+                const int u = 64 * i + lane, at = block * 2 * DP + u + (!FULL && values && u >= D ? DP - D : 0);
+                if (FULL || u < 2 * D) {
+                    float x[8];
+                    raw[i].numbers(x);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) x[j] *= scale.up;
+                    if constexpr (F32) {
+                        const Pair r = pair8(x);
+                        kv[buf][values][0][at] = r.hi;
+                        kv[buf][values][NP - 1][at] = r.lo;
+                    } else {
+                        kv[buf][values][0][at] = uintx4{round_half(x[0], x[1]), round_half(x[2], x[3]), round_half(x[4], x[5]), round_half(x[6], x[7])};
+                    }
+                }
+            }
+        };
+        if (lo < hi) fetch(lo);
+
+        // ---- queries
+        const int row = works ? min(row_lo + col, row_hi - 1) : 0, token = row / p.group, head = kv_head * p.group + row % p.group;
+        const int pos = q.length - q.fresh + token;
+        Pair qp[KS];
+        float q_down;
+        {
+            float x[KS][8], top = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float *src = p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D + 16 * ks + 8 * half;
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[ks][j] = 0.0f;
+                if (FULL || 16 * ks < D) {
+                    if (p.vec) {
+                        const floatx4 u = *reinterpret_cast<const floatx4 *>(src), v = *reinterpret_cast<const floatx4 *>(src + 4);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            x[ks][j] = u[j];
+                            x[ks][4 + j] = v[j];
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) x[ks][j] = src[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[ks][j]));
+            }
+            const Scale scale = scale_of(__builtin_bit_cast(unsigned, fmaxf(top, __shfl_xor(top, 32))));
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) x[ks][j] *= p.scale < 0.0f ? -scale.up : scale.up;
+                qp[ks] = pair8(x[ks]);
+            }
+            q_down = scale.down * fabsf(p.scale);  // (factors are positive: a block's largest score is that of its largest product)
         }
         floatx16 o[DT];
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
-        float m = NEG_INF, l = 0.0f;
-        bool bad = q.bad;
+        float m = NEG_INF, l = 0.0f, power = NEG_INF;  // power: the outputs' doublings, those of the largest values so far
         const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
 
-        // ---- the tiles' way into LDS
-        int page_lane = 0, page_from = -1;
-        size_t base0 = 0, base1 = 0;
-        auto find = [&](int j0) __attribute__((always_inline)) {
-            const int b = j0 >> 4;
-            if (page_from < 0 || b + 1 >= page_from + 64) {
-                page_from = b;
-                page_lane = pages[min((b + lane) << 4, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
+        __syncthreads();  // (the tile of rows before has read its last operands; zeros are in place)
+        if (lo < hi) {
+            place(lo, 0);
+            if (lo + TILE_KV < hi) fetch(lo + TILE_KV);
+        }
+        __syncthreads();
+        for (int j0 = lo, buf = 0; j0 < hi; j0 += TILE_KV, buf ^= 1) {
+            if (j0 + TILE_KV < hi) {
+                place(j0 + TILE_KV, buf ^ 1);
+                if (j0 + 2 * TILE_KV < hi) fetch(j0 + 2 * TILE_KV);
             }
-            base0 = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
-            base1 = block_base(p, __builtin_amdgcn_readlane(page_lane, b + 1 - page_from), b + 1, kv_head, bad);
-        };
-        constexpr int RAW = F32 ? (8 * DP + 255) / 256 : 1;
-        Raw<true> raw[RAW];
-        auto fetch = [&](int j0, int buf) __attribute__((always_inline)) {
-            find(j0);
-            if constexpr (F32) {
+            if (j0 < range.hi && j0 + TILE_KV > range.lo) {  // (some of this wavefront's rows see the tile)
+                floatx16 s;
 #pragma unroll
-                for (int i = 0; i < RAW; i++) {
-                    const int u = tid + 256 * i, values = u >= 4 * D, in = u - values * 4 * D, b = in >= 2 * D;
-                    if (FULL || u < 8 * D) raw[i].load(values ? p.V : p.K, (b ? base1 : base0) + (size_t)(in - b * 2 * D) * 8);
+                for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uintx4 k[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; n++) k[n] = kv[buf][0][n][k_unit + 32 * ks];
+                    s = multiply<NP>(k, qp[ks], s);
                 }
-            } else {  // (a wavefront copies one block's keys or values: 2 D units side by side)
-                const int values = wave >> 1, b = wave & 1;
-                const char *src = (const char *)(values ? p.V : p.K) + (b ? base1 : base0) * 2;
-                auto copy = [&](int from, int to, int units) __attribute__((always_inline)) {
-                    if (FULL || lane < units)
-                        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(src + (from + lane) * 16),
-                                                         (__attribute__((address_space(3))) void *)&kv[buf][values][0][b * 2 * DP + to], 16, 0, 0);
-                };
-                if (FULL || !values) {
+                // (a factor of 0 would make NaN of what is masked)
+                const float f[2] = {fmaxf(scales[buf][0] * q_down, 0x1p-126f), fmaxf(scales[buf][1] * q_down, 0x1p-126f)};
+                const float poison = (scales[buf][0] - scales[buf][0]) + (scales[buf][1] - scales[buf][1]);  // 0, or NaN (the maximum above drops it)
+                const float powers[2] = {scales[buf][2], scales[buf][3]};
+                if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
 #pragma unroll
-                    for (int i = 0; i < DP / 32; i++) copy(64 * i, 64 * i, 2 * D - 64 * i);
-                } else {  // (two runs of D units)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int i = 0; i < (DP + 63) / 64; i++) copy(h * D + 64 * i, h * DP + 64 * i, D - 64 * i);
+                    for (int r = 0; r < 16; r++) {
+                        const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
+                        s[r] = j >= see_lo && j < see_hi ? s[r] : NEG_INF;
+                    }
                 }
-            }
-        };
-        auto place = [&](int j0) __attribute__((always_inline)) {  // (fp32: from the registers, in parts)
-            if constexpr (F32) {
+                float top = NEG_INF;
 #pragma unroll
-                for (int i = 0; i < RAW; i++) {
-                    const int u = tid + 256 * i, values = u >= 4 * D, in = u - values * 4 * D, b = in >= 2 * D;
-                    if (FULL || u < 8 * D) {
-                        if (values && j0 + TILE_KV > q.length) raw[i].keep(q.length - (j0 + 16 * b + (in - b * 2 * D >= D ? 8 : 0)));
-                        const float x[8] = {raw[i].lo[0], raw[i].lo[1], raw[i].lo[2], raw[i].lo[3], raw[i].hi[0], raw[i].hi[1], raw[i].hi[2], raw[i].hi[3]};
-                        const Parts s = split8(x);
+                for (int b = 0; b < 2; b++) {
+                    float t = s[8 * b];
 #pragma unroll
-                        for (int n = 0; n < NP; n++) kv[0][values][n][b * 2 * DP + (in - b * 2 * D) + (values && in - b * 2 * D >= D ? DP - D : 0)] = s.p[n];
+                    for (int r = 1; r < 8; r++) t = fmaxf(t, s[8 * b + r]);
+                    top = fmaxf(top, t * f[b]);
+                }
+                top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+                const float most = fmaxf(fmaxf(powers[0], powers[1]), power);
+                if (__any(top > m) || most > power) {
+                    const float keep = m == NEG_INF ? 0.0f : power2(m - top), turn = keep * power2(power - most);
+                    l *= keep;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) o[dt][r] *= turn;
+                    m = top;
+                    power = most;
+                }
+                const float from = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const float c = powers[b] - power + 14.0f, shift = c - from + poison;
+                    float w[8], sum = 0.0f;
+#pragma unroll
+                    for (int r = 0; r < 8; r++) {
+                        w[r] = power2(__builtin_fmaf(s[8 * b + r], f[b], shift));
+                        sum += w[r];
+                    }
+                    if (c < -20.0f) {  // (values of another size than those before: their weights leave fp32's range earlier than the sum's)
+                        sum = 0.0f;
+#pragma unroll
+                        for (int r = 0; r < 8; r++) sum += power2(__builtin_fmaf(s[8 * b + r], f[b], -from));
+                        l += sum;
+                    } else {
+                        l = __builtin_fmaf(sum, power2(-c), l);
+                    }
+                    const Pair ws = pair8(w);
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++) {
+                        uintx4 v[NP];
+#pragma unroll
+                        for (int n = 0; n < NP; n++) v[n] = kv[buf][1][n][(b * 2 + half) * DP + 32 * dt + col];
+                        o[dt] = multiply<NP>(v, ws, o[dt]);
                     }
                 }
             }
-        };
-        __syncthreads();  // (the tile of rows before has read its last operands)
-        if (lo < hi) fetch(lo, 0);
-        for (int j0 = lo, buf = 0; j0 < hi; j0 += TILE_KV, buf = BUFS - 1 - buf) {
-            if constexpr (F32) {
-                if (j0 > lo) __syncthreads();
-                place(j0);
-                __syncthreads();
-                if (j0 + TILE_KV < hi) fetch(j0 + TILE_KV, 0);
-            } else {
-                __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's part of the tile is in LDS
-                __syncthreads();
-                if (j0 + TILE_KV < hi) fetch(j0 + TILE_KV, 1 - buf);
-            }
-            if (j0 >= range.hi || j0 + TILE_KV <= range.lo) continue;  // (none of this wavefront's rows sees the tile)
-            floatx16 large, small;
-#pragma unroll
-            for (int r = 0; r < 16; r++) large[r] = small[r] = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                uintx4 k[NP];
-#pragma unroll
-                for (int n = 0; n < NP; n++) k[n] = kv[buf][0][n][k_unit + 32 * ks];
-                multiply<NP>(k, qp[ks], large, small);
-            }
-            float s[16];
-#pragma unroll
-            for (int r = 0; r < 16; r++) s[r] = large[r] + small[r];
-            if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
-                    s[r] = j >= see_lo && j < see_hi ? s[r] : NEG_INF;
-                }
-            }
-            float top = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top, s[r]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            top = fmaxf(top, m);
-            if (__any(top > m)) {
-                const float keep = m == NEG_INF ? 0.0f : power2(m - top);
-                l *= keep;
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                    for (int r = 0; r < 16; r++) o[dt][r] *= keep;
-                m = top;
-            }
-            const float from = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[r] = power2(s[r] - from);
-                l += s[r];
-            }
-            const bool tail = !F32 && j0 + TILE_KV > q.length;
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const float w[8] = {s[8 * b], s[8 * b + 1], s[8 * b + 2], s[8 * b + 3], s[8 * b + 4], s[8 * b + 5], s[8 * b + 6], s[8 * b + 7]};
-                const Parts ws = split8(w);
-#pragma unroll
-                for (int dt = 0; dt < DT; dt++) {
-                    uintx4 v[NP];
-#pragma unroll
-                    for (int n = 0; n < NP; n++) v[n] = kv[buf][1][n][(b * 2 + half) * DP + 32 * dt + col];
-                    if constexpr (!F32) {
-                        if (tail) {
-                            Raw<false> x;
-                            x.v = v[0];
-                            x.keep(q.length - (j0 + 16 * b + 8 * half));
-                            v[0] = x.v;
-                        }
-                    }
-                    multiply<NP>(v, ws.p, o[dt], o[dt]);
-                }
-            }
+            __syncthreads();
         }
         l += __shfl_xor(l, 32);
+        const int doublings = power == NEG_INF ? 0 : (int)power - 14;
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[dt][r] = __builtin_amdgcn_ldexpf(o[dt][r], doublings);
 
         // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one
         float worst = l - l;
@@ -711,8 +812,8 @@ __global__ __launch_bounds__(256, (F32 ? DP <= 64 : DP <= 128) ? 2 : 1) void att
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int r = 0; r < 16; r++) worst += o[dt][r] - o[dt][r];
-        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi)) || bad;
-        again = again && row_lo + col < row_hi;
+        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi));
+        again = (again || q.bad) && row_lo + col < row_hi;
         unsigned long long todo = __ballot(again);
         todo = (todo | (todo >> 32)) & 0xffffffffull;
         const bool redo = (todo >> col) & 1;
@@ -877,6 +978,7 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     EH_REQUIRE(rows <= MAX_TOKENS && (long long)rows * q_heads <= 1LL << 30, "paged_attention: %d rows of %d heads are out of range", rows, q_heads);
     EH_REQUIRE(ldq >= (long long)q_heads * head_dim && ldo >= (long long)q_heads * head_dim, "paged_attention: rows of %lld and %lld floats do not hold %d heads of %d",
                ldq, ldo, q_heads, head_dim);
+    EH_REQUIRE(std::isfinite(scale), "paged_attention: the scale is not finite");
     EH_REQUIRE(max_new >= 0 && max_length >= 0 && window >= 0, "paged_attention: negative max_new, max_length or window");
     if (rows == 0 || seqs == 0) return 0;
     EH_REQUIRE(Q && O && k_pages && v_pages && table && offsets && lengths, "paged_attention: NULL tensor");

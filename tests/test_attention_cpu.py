@@ -24,7 +24,7 @@ ATTEND = dict(dev=0, Q=P, ldq=256, O=2 * P, ldo=256, rows=4, k=P, v=P, kind=0, p
 @pytest.mark.parametrize("change, text", [
     (dict(kind=2), "unknown cache type"), (dict(dim=40), "multiple of 16"), (dict(dim=272), "multiple of 16"), (dict(dim=0), "multiple of 16"),
     (dict(q_heads=5), "do not share"), (dict(kv_heads=0), "do not share"), (dict(page=24), "power of two"), (dict(page=8), "power of two"), (dict(pages=0), "pool of 0"),
-    (dict(width=0), "table of 0"), (dict(width=1 << 27), "table of 134217728"), (dict(rows=1 << 29), "out of range"), (dict(ldq=255), "do not hold"), (dict(ldo=100), "do not hold"), (dict(max_new=-1), "negative"), (dict(window=-1), "negative"),
+    (dict(width=0), "table of 0"), (dict(width=1 << 27), "table of 134217728"), (dict(rows=1 << 29), "out of range"), (dict(ldq=255), "do not hold"), (dict(ldo=100), "do not hold"), (dict(max_new=-1), "negative"), (dict(scale=float("nan")), "not finite"), (dict(scale=float("inf")), "not finite"), (dict(window=-1), "negative"),
     (dict(rows=-1), "-1 rows"), (dict(seqs=70000), "at most 65535"), (dict(Q=None), "NULL"), (dict(lengths=None), "NULL"), (dict(k=P + 8), "aligned")])
 def test_paged_attention_refusals(lib, change, text):
     _refused(lib, lib.eddlhip_paged_attention(*dict(ATTEND, **change).values()), text)

@@ -108,6 +108,51 @@ def test_attention_large_scores(hip):
     _near(_attend(hip, pool, q, 4, scale=0.5), want, tol)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("new", [2, 130])
+def test_attention_values_and_keys_of_all_sizes(hip, dtype, new):
+    """Values and keys of 1e-30 and 1e30, and blocks of tokens whose values differ by a factor of 1e25: the largest values carry the result,
+    the sums of the weights are those of all tokens."""
+    rng = np.random.default_rng(21)
+    length = new + 150
+    for size in (1e-30, 1e-10, 1.0, 1e30):
+        for what in ("k", "v", "both"):
+            pool = Pool(rng, [new], [length], 1, 64, 16, dtype)
+            j = np.arange(length)
+            for name in ("k", "v"):
+                if what in (name, "both"):
+                    pool.put(0, j, name, pool.get(0, j, name) * np.float32(size))
+            q = rng.standard_normal((new, 2 * 64), dtype=np.float32)
+            scale = 0.125 / (size if what != "v" and size > 1 else 1.0)
+            want, tol = attention(q, pool, 2, scale, True, 0)
+            got = _attend(hip, pool, q, 2, scale=scale)
+            _near(got, want, tol, (size, what))
+            assert np.linalg.norm((got - want) / size ** (what != "k")) <= 32 * EPS * np.linalg.norm(want / size ** (what != "k"))
+    for order in ((1e-15, 1e10), (1e10, 1e-15), (1e-15, 1.0, 0.0, 1e10, 1e-5)):
+        pool = Pool(rng, [new], [length], 1, 64, 16, dtype)
+        for n, size in enumerate(order):
+            j = np.arange(length * n // len(order), length * (n + 1) // len(order))
+            pool.put(0, j, "v", pool.get(0, j, "v") * np.float32(size))
+        q = rng.standard_normal((new, 2 * 64), dtype=np.float32)
+        want, tol = attention(q, pool, 2, 0.125, False, 0)
+        _near(_attend(hip, pool, q, 2, causal=False), want, tol, order)
+        # the first tokens alone: with a window of the last rows' neighbours none of the large values counts
+        want, tol = attention(q, pool, 2, 0.125, True, 20)
+        _near(_attend(hip, pool, q, 2, causal=True, window=20), want, tol + 2.0 ** -38 * np.abs(want).max(), order)
+
+
+def test_attention_negative_and_zero_scale(hip):
+    rng = np.random.default_rng(22)
+    for dtype in ("float32", "bfloat16"):
+        for new in (2, 60):
+            pool = Pool(rng, [new], [new + 40], 1, 64, 16, dtype)
+            q = rng.standard_normal((new, 2 * 64), dtype=np.float32)
+            for scale in (-0.3, 0.0):
+                want, _ = attention(q, pool, 2, scale, True, 0)
+                tol = attention(q, pool, 2, 0.3, True, 0)[1]
+                _near(_attend(hip, pool, q, 2, scale=scale), want, tol)
+
+
 def test_attention_rows_that_see_nothing_are_zero(hip):
     """Rows before place 0 (a sequence with more rows than tokens) and sequences of no tokens see nothing."""
     rng = np.random.default_rng(2)
