@@ -85,7 +85,12 @@ struct Raw;
 template <>
 struct Raw<false> {
     uintx4 v;
-    __device__ __forceinline__ void load(const void *base, size_t at) { v = *reinterpret_cast<const uintx4 *>((const unsigned short *)base + at); }
+    // ONCE: with the streaming hint, where no other wavefront reads the number
+    template <bool ONCE = false>
+    __device__ __forceinline__ void load(const void *base, size_t at) {
+        const uintx4 *src = reinterpret_cast<const uintx4 *>((const unsigned short *)base + at);
+        v = ONCE ? __builtin_nontemporal_load(src) : *src;
+    }
     // tokens from `count` of the eight on are zeros
     __device__ __forceinline__ void keep(int count) {
 #pragma unroll
@@ -108,10 +113,11 @@ struct Raw<false> {
 template <>
 struct Raw<true> {
     floatx4 lo, hi;
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const void *base, size_t at) {
         const floatx4 *src = reinterpret_cast<const floatx4 *>((const float *)base + at);
-        lo = src[0];
-        hi = src[1];
+        lo = ONCE ? __builtin_nontemporal_load(src) : src[0];
+        hi = ONCE ? __builtin_nontemporal_load(src + 1) : src[1];
     }
     __device__ __forceinline__ void keep(int count) {
 #pragma unroll
@@ -155,6 +161,15 @@ __device__ __forceinline__ float element(const AttendParams &p, const void *base
     return f32 ? ((const float *)base)[at] : __builtin_bit_cast(float, (unsigned)((const unsigned short *)base)[at] << 16);
 }
 
+// Parts of a divided length are written past the caches of an XCD and read so by the workgroup that joins them.
+__device__ __forceinline__ void put_part(float *dst, float a, float b) {
+    const float2 x = make_float2(a, b);
+    __hip_atomic_store((unsigned long long *)dst, __builtin_bit_cast(unsigned long long, x), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_part(const float *src) {
+    return __builtin_bit_cast(float2, __hip_atomic_load((const unsigned long long *)src, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
 // Where a row's result goes: the output, or its partial result.
 __device__ __forceinline__ void store_scale(const AttendParams &p, float m, float l, float &factor) {
     // (no visible token: m = -inf, l = 0, o = 0; visible ones that are all -inf: l > 0 and o = NaN, as the formula)
@@ -163,7 +178,7 @@ __device__ __forceinline__ void store_scale(const AttendParams &p, float m, floa
 
 // One row over the tokens [lo, hi), a wavefront together, one token at a time: lanes hold the dimensions lane, lane + 64, ...
 template <bool F32>
-__device__ void attend_row_again(const AttendParams &p, const Sequence &q, int seq, int kv_head, int token, int head, int lo, int hi, int split, bool bad) {
+__device__ void attend_row_again(const AttendParams &p, const Sequence &q, int seq, int kv_head, int token, int head, int lo, int hi, int split, int splits, bool bad) {
     const int lane = threadIdx.x & 63, pos = q.length - q.fresh + token;
     if (p.causal) hi = min(hi, pos + 1);
     if (p.window > 0) lo = max(lo, pos - p.window + 1);
@@ -190,11 +205,11 @@ __device__ void attend_row_again(const AttendParams &p, const Sequence &q, int s
     }
     if (bad) l = __builtin_nanf("");
     const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
-    if (p.splits > 1) {
+    if (splits > 1) {
         const size_t slot = (size_t)split * p.rows * p.q_heads + at;
-        if (lane == 0) p.part_s[slot] = make_float2(m, l);
+        if (lane == 0) put_part((float *)(p.part_s + slot), m, l);
         for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < p.D) p.part_o[slot * p.D + lane + 64 * i] = o[i];
+            if (lane + 64 * i < p.D) __hip_atomic_store(p.part_o + slot * p.D + lane + 64 * i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else {
         float factor;
         store_scale(p, m, l, factor);
@@ -226,6 +241,101 @@ __device__ __forceinline__ int part_at(int steps, int n, int parts) {
     return n * each + min(n, more);
 }
 
+// ------------------------------------------------------------------------------------------------ divided lengths
+// Few rows in up to 64 parts: workgroups that share rows count themselves in when their parts have reached the memory that all XCDs see;
+// the one that completes the count joins the parts, in groups that the shape alone fixes.  Nobody waits for another, and the
+// bits do not depend on who comes last.  A launch less: one token over 4096 28.6 -> 20.7 us.
+// Many rows, or more parts, are joined by a launch of their own, which the whole device works on (4 x 196 rows of 8 heads in 6 parts: 9 us
+// where the last workgroups took 19).  Rows that the launch did not count on (beyond q_tiles) are not divided.
+constexpr int MAX_COUNTS = 1024;  // divided launches have no more row tiles: two workgroups a tile fill the device
+static __device__ unsigned part_counts[MAX_COUNTS];
+
+constexpr int JOIN_HERE = 64;  // most parts that are joined so
+constexpr int JOIN_THREADS = 256;
+// `sums`: LDS of rows x parts; `red`: LDS of JOIN_THREADS.
+__device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence &q, int kv_head, int row_lo, int row_hi, float2 *sums, floatx4 *red, unsigned count,
+                                           int *last) {
+    const int tid = threadIdx.x, n = row_hi - row_lo, parts = p.splits, quads = p.D >> 2;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        const unsigned before = __hip_atomic_fetch_add(&part_counts[count], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        *last = before == (unsigned)parts - 1;
+        if (before == (unsigned)parts - 1) __hip_atomic_store(&part_counts[count], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // as the next launch expects it
+    }
+    __syncthreads();
+    if (!*last) return;
+    const size_t total = (size_t)p.rows * p.q_heads;
+    auto at_row = [&](int r) __attribute__((always_inline)) {
+        const int row = row_lo + r, token = row / p.group;
+        return (size_t)(q.row0 + token) * p.q_heads + kv_head * p.group + row % p.group;
+    };
+    for (int i = tid; i < n * parts; i += JOIN_THREADS) {
+        const int r = i / parts, s = i - r * parts;
+        sums[i] = get_part((const float *)(p.part_s + s * total + at_row(r)));
+    }
+    __syncthreads();
+    // four dimensions of a row a thread, or several threads where there are few
+    const int items = n * quads, lanes = items > JOIN_THREADS / 2 ? 1 : JOIN_THREADS / items;
+    for (int i0 = 0; i0 < items; i0 += JOIN_THREADS) {
+        const int i = lanes > 1 ? tid % items : i0 + tid, lane = lanes > 1 ? tid / items : 0, r = i / quads, d = 4 * (i - r * quads);
+        const bool works = i < items && lane < lanes;
+        float m = NEG_INF, l = 0.0f;
+        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (works) {
+            const float2 *ms = sums + r * parts;
+#pragma unroll 8
+            for (int s = 0; s < parts; s++) m = fmaxf(m, ms[s].x);
+            const float *src = p.part_o + at_row(r) * p.D + d;
+            constexpr int AHEAD = 16;
+            for (int s0 = lane; s0 < parts; s0 += AHEAD * lanes) {
+                float2 a[AHEAD], b[AHEAD];
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) {
+                    const int s = min(s0 + k * lanes, parts - 1);
+                    a[k] = get_part(src + s * total * p.D);
+                    b[k] = get_part(src + s * total * p.D + 2);
+                }
+#pragma unroll
+                for (int k = 0; k < AHEAD; k++) {
+                    const int s = s0 + k * lanes;
+                    if (s < parts) {
+                        const float2 x = ms[s];
+                        const float w = x.x == NEG_INF && x.y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(x.x - m);
+                        l += w * x.y;
+                        o += floatx4{a[k].x, a[k].y, b[k].x, b[k].y} * w;
+                    }
+                }
+            }
+        }
+        if (lanes > 1) {
+            __syncthreads();  // (all have read the sums)
+            red[tid] = o;
+            ((float *)sums)[tid] = l;
+            __syncthreads();
+            if (works && lane == 0)
+                for (int k = 1; k < lanes; k++) {
+                    o += red[k * items + i];
+                    l += ((float *)sums)[k * items + i];
+                }
+        }
+        if (works && lane == 0) {
+            float factor;
+            store_scale(p, m, l, factor);
+            if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
+            const int row = row_lo + r, token = row / p.group;
+            float *dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)(kv_head * p.group + row % p.group) * p.D + d;
+            o *= factor;
+            if (p.vec) {
+                *reinterpret_cast<floatx4 *>(dst) = o;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) dst[k] = o[k];
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 NQ rows of a sequence and key head (single tokens, short drafts): bound by the cache's bytes.  A workgroup takes a part of the
 // tokens, its four wavefronts take steps of 32 tokens in turn, operands straight from the cache into registers: every byte is read
@@ -235,6 +345,9 @@ __device__ __forceinline__ int part_at(int steps, int n, int parts) {
 // instead of 31 of 32, and the registers at half.  The wavefronts' sums meet in LDS once.
 // Rows of the product K Q^T: row 4g + i of tile t is token 8g + 4t + i of the step, so that lane group g holds tokens 8g .. 8g + 7.
 constexpr int FEW_WAVES = 4;
+// Workgroups of a CU (wavefronts of a SIMD): what the registers of a step's keys, values and outputs allow without spills.
+constexpr int few_groups(int dp, bool f32, int nq) { return dp > 128 || (f32 && dp > 96) || (f32 && dp > 64 && nq > 1) ? 1 : 2; }
+constexpr int FEW_SPLITS = 512;  // most parts of a length for up to 16 rows, half of it for up to 32
 
 __device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -268,13 +381,25 @@ struct Operand<true> {
     }
 };
 
+// The rows of a tile of keys: a load's or, in the odd lane groups of a bf16 cache, the other's.
+__device__ __forceinline__ Raw<false> tile_rows(const Raw<false> &a, const Raw<false> &b, bool exchanged) {
+    Raw<false> r;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r.v[i] = exchanged ? b.v[i] : a.v[i];
+    return r;
+}
+__device__ __forceinline__ const Raw<true> &tile_rows(const Raw<true> &a, const Raw<true> &, bool) { return a; }
+
 // FULL: head_dim is DP; otherwise DP - 64 < head_dim < DP: dimensions past the last are zeros of the queries, which meet the last 8
 // dimensions of the keys again, and outputs that nobody reads.  grid (q_tiles * splits, kv_heads, seqs)
 template <int DP, bool F32, int NQ, bool FULL>
-__global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ > 1) ? 1 : 2) void attend_few_kernel(const AttendParams p) {
+__global__ __launch_bounds__(64 * FEW_WAVES, few_groups(DP, F32, NQ)) void attend_few_kernel(const AttendParams p) {
     constexpr int KS = DP / 32, DT = DP / 16, W = FEW_WAVES, COLS = 16 * NQ, PITCH = DP + 4;
     constexpr int Q_BYTES = 3 * KS * NQ * 64 * 16, O_BYTES = W * COLS * PITCH * 4;
-    __shared__ __attribute__((aligned(16))) char lds[Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES];
+    constexpr int S_BYTES = COLS * JOIN_HERE * 8, MOST = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
+    __shared__ __attribute__((aligned(16))) char lds[S_BYTES > MOST ? S_BYTES : MOST];
+    __shared__ floatx4 red[JOIN_THREADS];
+    __shared__ int last;
     __shared__ float sums[W][COLS][2];
     __shared__ unsigned redo_columns;
     uintx4(*q_parts)[KS][NQ][64] = reinterpret_cast<uintx4(*)[KS][NQ][64]>(lds);
@@ -282,16 +407,19 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
     const int D = FULL ? DP : p.D;
-    const int split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
+    const int own_split = blockIdx.x % p.splits, kv_head = blockIdx.y, seq = blockIdx.z;
     const Sequence q = sequence_of(p, seq);
     const int rows = q.fresh * p.group;
     const int *pages = p.table + (size_t)seq * p.width;
 
     for (int tile = blockIdx.x / p.splits; tile * COLS < rows; tile += p.q_tiles) {
+        const bool counted = tile < p.q_tiles;
+        if (!counted && own_split != 0) break;
+        const int split = counted ? own_split : 0, splits = counted ? p.splits : 1;
         const int row_lo = tile * COLS, row_hi = min(rows, row_lo + COLS);
         const Range range = range_of(p, q, row_lo, row_hi);
         const int steps_all = max(0, (range.hi - range.lo + TILE_KV - 1) / TILE_KV);
-        const int step_lo = part_at(steps_all, split, p.splits), step_hi = part_at(steps_all, split + 1, p.splits);
+        const int step_lo = part_at(steps_all, split, splits), step_hi = part_at(steps_all, split + 1, splits);
         const int lo = range.lo + step_lo * TILE_KV, hi = min(range.hi, range.lo + step_hi * TILE_KV);
         __syncthreads();  // (the tile before has been stored)
 
@@ -310,20 +438,24 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
             base[0] = block_base(p, __builtin_amdgcn_readlane(page_lane, at), b, kv_head, bad);
             base[1] = block_base(p, __builtin_amdgcn_readlane(page_lane, at + 1), b + 1, kv_head, bad);
         };
+        // (bf16: lanes g and g ^ 1 read the same 8 dimensions, one the rows of tile 0 and one those of tile 1, so that a load covers whole lines;
+        // the next load brings the other 8 dimensions with the tiles exchanged.  fp32 rows fill their lines by themselves.)
         auto load_keys = [&]() __attribute__((always_inline)) {
             const size_t from = (col >> 3 ? base[1] : base[0]);
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int token = (8 * (col >> 2) + 4 * t + (col & 3)) & 15;
+            for (int n = 0; n < 2; n++) {
+                const int token = (8 * (col >> 2) + 4 * (F32 ? n : (g ^ n) & 1) + (col & 3)) & 15;
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-                    k[t][ks].load(p.K, from + token * 8 + (FULL ? 4 * ks + g : min(4 * ks + g, (D >> 3) - 1)) * 128);
+                for (int ks = 0; ks < KS; ks++) {
+                    const int chunk = 4 * ks + (F32 ? g : (g & 2) + n);
+                    k[n][ks].template load<true>(p.K, from + token * 8 + (FULL ? chunk : min(chunk, (D >> 3) - 1)) * 128);
+                }
             }
         };
         auto load_values = [&]() __attribute__((always_inline)) {
             const size_t from = (g & 2 ? base[1] : base[0]) + (size_t)(g & 1) * 8 * D;
 #pragma unroll
-            for (int dt = 0; dt < DT; dt++) v[dt].load(p.V, from + (FULL ? 16 * dt + col : min(16 * dt + col, D - 1)) * 8);
+            for (int dt = 0; dt < DT; dt++) v[dt].template load<true>(p.V, from + (FULL ? 16 * dt + col : min(16 * dt + col, D - 1)) * 8);
         };
         const int its = (step_hi - step_lo - wave + W - 1) / W;  // steps of this wavefront
         if (its > 0 && hi > lo) {
@@ -384,12 +516,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
                 for (int t = 0; t < 2; t++) large[nq][t] = small[nq][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const Operand<F32> a0(k[0][ks]), a1(k[1][ks]);
+                // rows of tile 0 with dimensions 8 (4 ks + g) .., rows of tile 1 with the same or (bf16) those of lane g ^ 1
+                const Operand<F32> a0(tile_rows(k[0][ks], k[1][ks], g & 1)), a1(tile_rows(k[1][ks], k[0][ks], g & 1));
+                const int other = F32 ? lane : lane ^ 16;
 #pragma unroll
                 for (int nq = 0; nq < NQ; nq++) {
-                    const uintx4 b0 = q_parts[0][ks][nq][lane], b1 = q_parts[1][ks][nq][lane], b2 = q_parts[2][ks][nq][lane];
-                    a0.multiply(b0, b1, b2, large[nq][0], small[nq][0]);
-                    a1.multiply(b0, b1, b2, large[nq][1], small[nq][1]);
+                    a0.multiply(q_parts[0][ks][nq][lane], q_parts[1][ks][nq][lane], q_parts[2][ks][nq][lane], large[nq][0], small[nq][0]);
+                    a1.multiply(q_parts[0][ks][nq][other], q_parts[1][ks][nq][other], q_parts[2][ks][nq][other], large[nq][1], small[nq][1]);
                 }
                 __builtin_amdgcn_sched_barrier(0);  // (one operand's parts at a time: registers)
             }
@@ -481,9 +614,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
                     atomicOr(&redo_columns, 1u << c);
                 }
                 const size_t at = (size_t)(q.row0 + token) * p.q_heads + head, slot = (size_t)split * p.rows * p.q_heads + at;
-                if (p.splits > 1) {
+                if (splits > JOIN_HERE) {
                     if (d == 0) p.part_s[slot] = make_float2(top, sum);
                     *reinterpret_cast<floatx4 *>(p.part_o + slot * D + d) = x;
+                } else if (splits > 1) {
+                    if (d == 0) put_part((float *)(p.part_s + slot), top, sum);
+                    put_part(p.part_o + slot * D + d, x[0], x[1]);
+                    put_part(p.part_o + slot * D + d + 2, x[2], x[3]);
                 } else {
                     float factor;
                     store_scale(p, top, sum, factor);
@@ -503,8 +640,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
         const bool any_bad = q.bad;
         for (unsigned todo = redo_columns; todo != 0; todo &= todo - 1) {
             const int c = __builtin_ctz(todo), r = row_lo + c;
-            if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, any_bad);
+            if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, splits, any_bad);
         }
+        if (splits > 1 && splits <= JOIN_HERE)
+            join_parts(p, q, kv_head, row_lo, row_hi, reinterpret_cast<float2 *>(lds), red, (seq * p.kv_heads + kv_head) * p.q_tiles + tile, &last);
     }
 }
 
@@ -523,6 +662,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, DP > 128 || (F32 && DP > 64 && NQ >
 // two tiles, one filled while the other is used, one barrier a tile.  The cache's order is the operands' order: every LDS
 // access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
 constexpr int CHUNK_ROWS = 128;
+constexpr int CHUNK_SPLITS = 16;  // most parts of a length: their sums fit where two tiles of 64 dimensions were
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
@@ -596,7 +736,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
     // workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps
     const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD, vid = (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD;
     if (vid >= total) return;
-    const int split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
+    const int own_split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
     const Sequence q = sequence_of(p, seq);
     const int rows = q.fresh * p.group;
     const int *pages = p.table + (size_t)seq * p.width;
@@ -610,9 +750,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
     }
 
     for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * CHUNK_ROWS < rows; tile += p.q_tiles) {
+        const bool counted = tile < p.q_tiles;
+        if (!counted && own_split != 0) break;
+        const int split = counted ? own_split : 0, splits = counted ? p.splits : 1;
         const Range all = range_of(p, q, tile * CHUNK_ROWS, min(rows, (tile + 1) * CHUNK_ROWS));
         const int steps_all = max(0, (all.hi - all.lo + TILE_KV - 1) / TILE_KV);
-        const int step_lo = part_at(steps_all, split, p.splits), step_hi = part_at(steps_all, split + 1, p.splits);
+        const int step_lo = part_at(steps_all, split, splits), step_hi = part_at(steps_all, split + 1, splits);
         const int lo = all.lo + step_lo * TILE_KV, hi = min(all.hi, all.lo + step_hi * TILE_KV);
         const int row_lo = min(rows, tile * CHUNK_ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
         const bool works = row_lo < row_hi;
@@ -819,21 +962,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
         const bool redo = (todo >> col) & 1;
         for (unsigned long long t = todo; t != 0; t &= t - 1) {
             const int r = row_lo + __builtin_ctzll(t);
-            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, q.bad);
+            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, splits, q.bad);
         }
 
         if (row_lo + col < row_hi && !redo) {
             const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
             const size_t slot = (size_t)split * p.rows * p.q_heads + at;
             float factor = 1.0f, *dst;
-            if (p.splits > 1) {
+            if (splits > 1) {
                 if (half == 0) p.part_s[slot] = make_float2(m, l);
                 dst = p.part_o + slot * D;
             } else {
                 store_scale(p, m, l, factor);
                 dst = p.O + (size_t)(q.row0 + token) * p.ldo + (size_t)head * D;
             }
-            const bool whole = p.splits > 1 || p.vec;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
@@ -841,7 +983,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
                     const int d = 32 * dt + 8 * g + 4 * half;
                     if (FULL || d < D) {
                         const floatx4 x = {o[dt][4 * g] * factor, o[dt][4 * g + 1] * factor, o[dt][4 * g + 2] * factor, o[dt][4 * g + 3] * factor};
-                        if (whole) {
+                        if (splits > 1 || p.vec) {
                             *reinterpret_cast<floatx4 *>(dst + d) = x;
                         } else {
 #pragma unroll
@@ -853,94 +995,52 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
     }
 }
 
-// Joins the few parts of a row, a wavefront a row: every lane reads all weights and four dimensions of every part.
-constexpr int JOIN_FEW = 16;
-__global__ __launch_bounds__(256) void attend_join_few_kernel(const AttendParams p) {
-    const int lane = threadIdx.x & 63, d = 4 * lane;
-    const long long total = (long long)p.rows * p.q_heads;
-    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
-    for (long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < total; at += (long long)gridDim.x * 4) {
-        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
-        if (row < first || row >= end) continue;
-        float m = NEG_INF, l = 0.0f;
-        for (int s = 0; s < p.splits; s++) m = fmaxf(m, p.part_s[(size_t)s * total + at].x);
-        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-        for (int s = 0; s < p.splits; s++) {
-            const float2 ms = p.part_s[(size_t)s * total + at];
-            const float w = ms.x == NEG_INF && ms.y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(ms.x - m);
-            l += w * ms.y;
-            if (d < p.D) o += *reinterpret_cast<const floatx4 *>(p.part_o + ((size_t)s * total + at) * p.D + d) * w;
-        }
-        float factor;
-        store_scale(p, m, l, factor);
-        if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
-        float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + d;
-        if (d < p.D) {
-            if (p.vec) {
-                *reinterpret_cast<floatx4 *>(dst) = o * factor;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
-            }
-        }
-    }
-}
-
-// Joins the many parts of a row, a workgroup a row: the weights of all parts first, then four dimensions and every (1024 / head_dim)th part a
-// thread, then those together, in an order that the shape alone fixes.
-constexpr int MAX_SPLITS = 512;
+// Joins parts in a launch of their own, a row in 16, 32 or 64 lanes of a wavefront: all parts' sums first, eight parts' outputs on their way at a
+// time; added in the order of the tokens.
+template <int LANES>
 __global__ __launch_bounds__(256) void attend_join_kernel(const AttendParams p) {
-    __shared__ float weights[MAX_SPLITS], red[8];
-    __shared__ floatx4 sums[256];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, quads = p.D >> 2, lanes = 256 / quads;
-    const long long total = (long long)p.rows * p.q_heads;
-    const int first = max(p.offsets[0], 0), end = min(p.offsets[p.seqs], p.rows);
-    for (long long at = blockIdx.x; at < total; at += gridDim.x) {
-        const int row = (int)(at / p.q_heads), head = (int)(at - (long long)row * p.q_heads);
-        if (row < first || row >= end) continue;
-        float2 ms[MAX_SPLITS / 256];
-        float m = NEG_INF, l = 0.0f;
+    const int sub = threadIdx.x % LANES, d = 4 * sub;
+    const long long total = (long long)p.rows * p.q_heads, at = (long long)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    if (at >= total) return;
+    const int row = (int)((unsigned)at / (unsigned)p.q_heads), head = (int)at - row * p.q_heads;
+    if (row < max(p.offsets[0], 0) || row >= p.offsets[p.seqs]) return;
+    constexpr int AHEAD = 8;
+    float m = NEG_INF, l = 0.0f;
+    floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const float *src = p.part_o + at * p.D + min(d, p.D - 4);
+    for (int s0 = 0; s0 < p.splits; s0 += AHEAD) {  // (a running maximum over groups of parts)
+        float2 ms[AHEAD];
+        floatx4 x[AHEAD];
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 256; i++) {
-            const int s = tid + 256 * i;
-            ms[i] = s < p.splits ? p.part_s[(size_t)s * total + at] : make_float2(NEG_INF, 0.0f);
-            m = fmaxf(m, ms[i].x);
-        }
-        for (int step = 32; step > 0; step >>= 1) m = fmaxf(m, __shfl_xor(m, step));
-        __syncthreads();  // (the row before has been read)
-        if (lane == 0) red[wave] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        for (int k = 0; k < AHEAD; k++) ms[k] = p.part_s[min(s0 + k, p.splits - 1) * total + at];
 #pragma unroll
-        for (int i = 0; i < MAX_SPLITS / 256; i++) {
-            const int s = tid + 256 * i;
-            const float w = ms[i].x == NEG_INF && ms[i].y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(ms[i].x - m);
-            l += w * ms[i].y;
-            if (s < p.splits) weights[s] = w;
-        }
-        for (int step = 32; step > 0; step >>= 1) l += __shfl_xor(l, step);
-        if (lane == 0) red[4 + wave] = l;
-        __syncthreads();
-        l = (red[4] + red[5]) + (red[6] + red[7]);
-        const int part = tid / quads, d = 4 * (tid - part * quads);
-        floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (part < lanes) {
-            const float *src = p.part_o + (size_t)at * p.D + d;
-            const size_t step = (size_t)total * p.D;
-#pragma unroll 4
-            for (int s = part; s < p.splits; s += lanes) o += *reinterpret_cast<const floatx4 *>(src + s * step) * weights[s];
-            sums[tid] = o;
-        }
-        __syncthreads();
-        if (part == 0) {
-            for (int n = 1; n < lanes; n++) o += sums[n * quads + tid];
-            float factor;
-            store_scale(p, m, l, factor);
-            if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
-            float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + d;
+        for (int k = 0; k < AHEAD; k++) x[k] = *reinterpret_cast<const floatx4 *>(src + min(s0 + k, p.splits - 1) * total * p.D);
+        float top = m;
 #pragma unroll
-            for (int i = 0; i < 4; i++) dst[i] = o[i] * factor;
+        for (int k = 0; k < AHEAD; k++) top = fmaxf(top, ms[k].x);
+        const float keep = m == NEG_INF ? (top == NEG_INF ? 1.0f : 0.0f) : power2(m - top);
+        l = m == NEG_INF && top != NEG_INF ? (l == l ? 0.0f : l) : l * keep;
+        o *= keep;
+        m = top;
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++)
+            if (s0 + k < p.splits) {
+                const float w = ms[k].x == NEG_INF && ms[k].y == 0.0f ? 0.0f : m == NEG_INF ? 1.0f : power2(ms[k].x - m);
+                l += w * ms[k].y;
+                o += x[k] * w;
+            }
+    }
+    float factor;
+    store_scale(p, m, l, factor);
+    if (m == NEG_INF && l != 0.0f) factor = __builtin_nanf("");
+    if (d < p.D) {
+        float *dst = p.O + (size_t)row * p.ldo + (size_t)head * p.D + d;
+        o *= factor;
+        if (p.vec) {
+            *reinterpret_cast<floatx4 *>(dst) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) dst[i] = o[i];
         }
     }
 }
@@ -962,6 +1062,19 @@ void launch_chunk(const AttendParams &p, bool f32, int total, hipStream_t st) {
 }
 
 }  // namespace
+
+namespace eddlhip {
+
+int attention_setup_device(int dev) {
+    void *ptr = nullptr;
+    EH_TRY_HIP(hipGetSymbolAddress(&ptr, HIP_SYMBOL(part_counts)));
+    EH_TRY_HIP(hipMemset(ptr, 0, sizeof(part_counts)));  // (also after a shutdown that cut launches short)
+    EH_TRY_HIP(hipDeviceSynchronize());
+    (void)dev;
+    return 0;
+}
+
+}  // namespace eddlhip
 
 extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, long long ldo, int rows, const void *k_pages, const void *v_pages,
                                        int cache_type, int pages, int page_size, int q_heads, int kv_heads, int head_dim, const int *table, int table_width,
@@ -1012,11 +1125,12 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : CHUNK_ROWS;
     const long long tiles = (tile_rows + per_tile - 1) / per_tile;
     p.q_tiles = (int)tiles;
-    const long long groups = tiles * kv_heads * seqs, want = (nq ? 3LL : 2LL) * state(dev).num_cu;
+    const long long groups = tiles * kv_heads * seqs, want = (nq ? few_groups(head_dim, cache_type == EDDLHIP_CACHE_F32, nq) : 2LL) * state(dev).num_cu;
     long long seen = max_length > 0 ? max_length : 1;
     if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
-    p.splits = (int)std::max(1LL, std::min({want / groups, steps / 8, (long long)MAX_SPLITS}));
+    p.splits = (int)std::max(1LL, std::min({want / groups, steps / 8, (long long)(nq ? FEW_SPLITS / nq : CHUNK_SPLITS)}));
+    EH_REQUIRE(p.splits == 1 || !nq || groups <= MAX_COUNTS, "paged_attention: %lld tiles of rows in parts", groups);  // (want / 2 at most)
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
@@ -1045,9 +1159,11 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     else if (head_dim <= 192) sized(std::integral_constant<int, 192>());
     else sized(std::integral_constant<int, 256>());
     EH_CHECK_LAUNCH();
-    if (p.splits > 1) {
-        if (p.splits <= JOIN_FEW) hipLaunchKernelGGL(attend_join_few_kernel, dim3(eh_blocks((size_t)rows * q_heads, 4, 65536)), dim3(256), 0, st, p);
-        else hipLaunchKernelGGL(attend_join_kernel, dim3(eh_blocks((size_t)rows * q_heads, 1, 65536)), dim3(256), 0, st, p);
+    if (p.splits > (nq ? JOIN_HERE : 1)) {
+        const long long joined = (long long)rows * q_heads;
+        if (head_dim <= 64) hipLaunchKernelGGL(attend_join_kernel<16>, dim3((unsigned)((joined + 15) / 16)), dim3(256), 0, st, p);
+        else if (head_dim <= 128) hipLaunchKernelGGL(attend_join_kernel<32>, dim3((unsigned)((joined + 7) / 8)), dim3(256), 0, st, p);
+        else hipLaunchKernelGGL(attend_join_kernel<64>, dim3((unsigned)((joined + 3) / 4)), dim3(256), 0, st, p);
         EH_CHECK_LAUNCH();
     }
     return 0;

@@ -48,6 +48,8 @@ int dense_split(int dev, const float *A, const float *B, float *C, int m, int k,
 // Per-device set-up of the convolution code (address of its fixed scratch array, kernel occupancies);
 // use_device calls it once, when it initialises the device.
 int conv_setup_device(int dev);
+// The same of the attention: clears the counts of divided lengths.
+int attention_setup_device(int dev);
 
 }  // namespace eddlhip
 
