@@ -51,7 +51,7 @@ struct AttendParams {
     float *part_o;   // [splits][rows * q_heads][D]
     float2 *part_s;  // [splits][rows * q_heads] maximum and sum
     long long ldq, ldo;
-    int rows, q_heads, kv_heads, group, D, pages, page_shift, width, seqs, causal, window, splits, q_tiles, vec;
+    int rows, q_heads, kv_heads, group, D, pages, page_shift, width, seqs, causal, window, splits, q_tiles, vec, grouped;
     float scale;  // with log2(e)
 };
 
@@ -251,8 +251,8 @@ constexpr int MAX_COUNTS = 1024;  // divided launches have no more row tiles: tw
 static __device__ unsigned part_counts[MAX_COUNTS];
 
 constexpr int JOIN_HERE = 64;  // most parts that are joined so
-constexpr int JOIN_THREADS = 256;
-// `sums`: LDS of rows x parts; `red`: LDS of JOIN_THREADS.
+// `sums`: LDS of rows x parts; `red`: LDS of THREADS.
+template <int THREADS>
 __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence &q, int kv_head, int row_lo, int row_hi, float2 *sums, floatx4 *red, unsigned count,
                                            int *last) {
     const int tid = threadIdx.x, n = row_hi - row_lo, parts = p.splits, quads = p.D >> 2;
@@ -270,14 +270,14 @@ __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence
         const int row = row_lo + r, token = row / p.group;
         return (size_t)(q.row0 + token) * p.q_heads + kv_head * p.group + row % p.group;
     };
-    for (int i = tid; i < n * parts; i += JOIN_THREADS) {
+    for (int i = tid; i < n * parts; i += THREADS) {
         const int r = i / parts, s = i - r * parts;
         sums[i] = get_part((const float *)(p.part_s + s * total + at_row(r)));
     }
     __syncthreads();
     // four dimensions of a row a thread, or several threads where there are few
-    const int items = n * quads, lanes = items > JOIN_THREADS / 2 ? 1 : JOIN_THREADS / items;
-    for (int i0 = 0; i0 < items; i0 += JOIN_THREADS) {
+    const int items = n * quads, lanes = items > THREADS / 2 ? 1 : THREADS / items;
+    for (int i0 = 0; i0 < items; i0 += THREADS) {
         const int i = lanes > 1 ? tid % items : i0 + tid, lane = lanes > 1 ? tid / items : 0, r = i / quads, d = 4 * (i - r * quads);
         const bool works = i < items && lane < lanes;
         float m = NEG_INF, l = 0.0f;
@@ -344,9 +344,12 @@ __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence
 // computed, 16 (32) KB a wavefront.  The 16x16x32 instruction keeps the queries that are not there at 15 of 16 columns
 // instead of 31 of 32, and the registers at half.  The wavefronts' sums meet in LDS once.
 // Rows of the product K Q^T: row 4g + i of tile t is token 8g + 4t + i of the step, so that lane group g holds tokens 8g .. 8g + 7.
-constexpr int FEW_WAVES = 4;
-// Workgroups of a CU (wavefronts of a SIMD): what the registers of a step's keys, values and outputs allow without spills.
-constexpr int few_groups(int dp, bool f32, int nq) { return dp > 128 || (f32 && dp > 96) || (f32 && dp > 64 && nq > 1) ? 1 : 2; }
+// Wavefronts of a SIMD, as the registers of a step's keys, values and outputs allow without spills, and wavefronts of a workgroup: all that a
+// CU holds where that is 8 (fewer parts to join, and a part lasts as long as possible: 1 token over 131072, heads of 128 in bf16, 95 us,
+// with two workgroups of 4 100 us).
+constexpr int few_per_simd(int dp, bool f32, int nq) { return dp > 128 || (f32 && dp > 96) || (f32 && dp > 64 && nq > 1) ? 1 : !f32 && dp <= 64 && nq == 1 ? 3 : 2; }
+constexpr int few_waves(int dp, bool f32, int nq) { return few_per_simd(dp, f32, nq) == 2 && !f32 ? 8 : 4; }
+constexpr int few_groups(int dp, bool f32, int nq) { return 4 * few_per_simd(dp, f32, nq) / few_waves(dp, f32, nq); }  // workgroups of a CU
 constexpr int FEW_SPLITS = 512;  // most parts of a length for up to 16 rows, half of it for up to 32
 
 __device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
@@ -393,12 +396,12 @@ __device__ __forceinline__ const Raw<true> &tile_rows(const Raw<true> &a, const 
 // FULL: head_dim is DP; otherwise DP - 64 < head_dim < DP: dimensions past the last are zeros of the queries, which meet the last 8
 // dimensions of the keys again, and outputs that nobody reads.  grid (q_tiles * splits, kv_heads, seqs)
 template <int DP, bool F32, int NQ, bool FULL>
-__global__ __launch_bounds__(64 * FEW_WAVES, few_groups(DP, F32, NQ)) void attend_few_kernel(const AttendParams p) {
-    constexpr int KS = DP / 32, DT = DP / 16, W = FEW_WAVES, COLS = 16 * NQ, PITCH = DP + 4;
+__global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, NQ)) void attend_few_kernel(const AttendParams p) {
+    constexpr int KS = DP / 32, DT = DP / 16, W = few_waves(DP, F32, NQ), COLS = 16 * NQ, PITCH = DP + 4;
     constexpr int Q_BYTES = 3 * KS * NQ * 64 * 16, O_BYTES = W * COLS * PITCH * 4;
     constexpr int S_BYTES = COLS * JOIN_HERE * 8, MOST = Q_BYTES > O_BYTES ? Q_BYTES : O_BYTES;
     __shared__ __attribute__((aligned(16))) char lds[S_BYTES > MOST ? S_BYTES : MOST];
-    __shared__ floatx4 red[JOIN_THREADS];
+    __shared__ floatx4 red[64 * W];
     __shared__ int last;
     __shared__ float sums[W][COLS][2];
     __shared__ unsigned redo_columns;
@@ -643,7 +646,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES, few_groups(DP, F32, NQ)) void atten
             if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, splits, any_bad);
         }
         if (splits > 1 && splits <= JOIN_HERE)
-            join_parts(p, q, kv_head, row_lo, row_hi, reinterpret_cast<float2 *>(lds), red, (seq * p.kv_heads + kv_head) * p.q_tiles + tile, &last);
+            join_parts<64 * W>(p, q, kv_head, row_lo, row_hi, reinterpret_cast<float2 *>(lds), red, (seq * p.kv_heads + kv_head) * p.q_tiles + tile, &last);
     }
 }
 
@@ -718,6 +721,13 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) {  // in lane 63, read 
     v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xf, 0xf, false));
     return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
+// The larger of a lane's and that of lane ^ 32.  (As assembly: of the builtin's two results with equal operands the compiler keeps one.  The
+// instruction wants two wait states behind the operands' last vector instruction.)
+__device__ __forceinline__ float larger_half(float x) {
+    float y = x;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+    return fmaxf(x, y);
+}
 template <int NP>
 __device__ __forceinline__ floatx16 multiply(const uintx4 (&a)[NP], const Pair &b, floatx16 c) {
     if constexpr (NP == 2) c = mfma(a[1], b.hi, c);
@@ -733,8 +743,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
     __shared__ float scales[2][4];  // of a tile's two blocks: keys' factors, values' powers of two
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
     const int D = FULL ? DP : p.D;
-    // workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps
-    const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD, vid = (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD;
+    // Workgroups that share an XCD get consecutive work: tiles and parts of one key head, whose keys and values its L2 keeps (2048 tokens over
+    // 8192 549 us, dealt round 595).  Not where sequences are ragged: an XCD would get the long ones (7 of 4 to 301 new tokens 48 us, dealt round 36).
+    const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
+    const int vid = p.grouped ? (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD : blockIdx.x;
     if (vid >= total) return;
     const int own_split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
     const Sequence q = sequence_of(p, seq);
@@ -866,10 +878,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
         }
         __syncthreads();
         for (int j0 = lo, buf = 0; j0 < hi; j0 += TILE_KV, buf ^= 1) {
-            if (j0 + TILE_KV < hi) {
-                place(j0 + TILE_KV, buf ^ 1);
-                if (j0 + 2 * TILE_KV < hi) fetch(j0 + 2 * TILE_KV);
-            }
             if (j0 < range.hi && j0 + TILE_KV > range.lo) {  // (some of this wavefront's rows see the tile)
                 floatx16 s;
 #pragma unroll
@@ -900,7 +908,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
                     for (int r = 1; r < 8; r++) t = fmaxf(t, s[8 * b + r]);
                     top = fmaxf(top, t * f[b]);
                 }
-                top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
+                top = fmaxf(larger_half(top), m);
                 const float most = fmaxf(fmaxf(powers[0], powers[1]), power);
                 if (__any(top > m) || most > power) {
                     const float keep = m == NEG_INF ? 0.0f : power2(m - top), turn = keep * power2(power - most);
@@ -939,6 +947,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
                         o[dt] = multiply<NP>(v, ws, o[dt]);
                     }
                 }
+            }
+            if (j0 + TILE_KV < hi) {
+                place(j0 + TILE_KV, buf ^ 1);
+                if (j0 + 2 * TILE_KV < hi) fetch(j0 + 2 * TILE_KV);
             }
             __syncthreads();
         }
@@ -1051,7 +1063,7 @@ void launch_few(const AttendParams &p, bool f32, int nq, dim3 grid, hipStream_t 
     constexpr int MOST = DP <= 128 ? 2 : 1;
     static const kernel kernels[2][2] = {{attend_few_kernel<DP, false, 1, FULL>, attend_few_kernel<DP, false, MOST, FULL>},
                                          {attend_few_kernel<DP, true, 1, FULL>, attend_few_kernel<DP, true, MOST, FULL>}};
-    hipLaunchKernelGGL(kernels[f32][nq - 1], grid, dim3(64 * FEW_WAVES), 0, st, p);
+    hipLaunchKernelGGL(kernels[f32][nq - 1], grid, dim3(64 * few_waves(DP, f32, nq)), 0, st, p);
 }
 
 template <int DP, bool FULL>
@@ -1125,12 +1137,14 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : CHUNK_ROWS;
     const long long tiles = (tile_rows + per_tile - 1) / per_tile;
     p.q_tiles = (int)tiles;
-    const long long groups = tiles * kv_heads * seqs, want = (nq ? few_groups(head_dim, cache_type == EDDLHIP_CACHE_F32, nq) : 2LL) * state(dev).num_cu;
+    // (sequences of fewer new tokens than max_new have fewer tiles, all together no more than their rows fill and one begun tile each)
+    const long long groups = tiles * kv_heads * seqs, filled = kv_heads * std::min(tiles * seqs, ((long long)rows * p.group) / per_tile + seqs), want = (nq ? few_groups(head_dim, cache_type == EDDLHIP_CACHE_F32, nq) : 2LL) * state(dev).num_cu;
     long long seen = max_length > 0 ? max_length : 1;
     if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
-    p.splits = (int)std::max(1LL, std::min({want / groups, steps / 8, (long long)(nq ? FEW_SPLITS / nq : CHUNK_SPLITS)}));
-    EH_REQUIRE(p.splits == 1 || !nq || groups <= MAX_COUNTS, "paged_attention: %lld tiles of rows in parts", groups);  // (want / 2 at most)
+    p.splits = (int)std::max(1LL, std::min({want / filled, steps / (nq ? 8 : 4), (long long)(nq ? FEW_SPLITS / nq : CHUNK_SPLITS)}));
+    if (nq && groups > MAX_COUNTS) p.splits = 1;
+    p.grouped = filled == groups;
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
