@@ -553,18 +553,20 @@ class Backend:
         ``gate`` [groups, columns] (or one row for all), ``mod``, ``shift`` [groups, columns] belong to ``group_rows`` rows side by side (all, unless
         given).  R, S, H may be None."""
         x, ldx, shape = _rows(X, "norm_residual")
-        (r, ldr, rs), (s, lds, ss), (h, ldh, hs) = (_rows(t, "norm_residual") if t is not None else (None, 0, shape) for t in (R, S, H))
-        if group_rows is None:
-            group_rows = max(shape[0], 1)
-        groups = -(-shape[0] // group_rows) if group_rows > 0 else 0
+        r, ldr, rs = _rows(R, "norm_residual") if R is not None else (None, 0, shape)
+        s, lds, ss = _rows(S, "norm_residual") if S is not None else (None, 0, shape)
+        h, ldh, hs = _rows(H, "norm_residual") if H is not None else (None, 0, shape)
         if not rs == ss == hs == shape:
             raise ValueError("norm_residual shapes x %s, residual %s, sum %s, normed %s" % (shape, rs, ss, hs))
+        if group_rows is None:
+            group_rows = shape[0] or 1
+        cols, grouped = shape[1], (-(-shape[0] // group_rows) if group_rows > 0 else 0) * shape[1]
         for t in (post[1], post[2], pre[1], pre[2]):
-            if t is not None and (t.size != shape[1] or t.dtype != "float32"):
-                raise ValueError("norm_residual: weights %s %s for %d columns" % (t.dtype, t.shape, shape[1]))
+            if t is not None and (t.size != cols or t.dtype != "float32"):
+                raise ValueError("norm_residual: weights %s %s for %d columns" % (t.dtype, t.shape, cols))
         for t in (gate, mod, shift):
-            if t is not None and (t.dtype != "float32" or t.size != max(groups, 1) * shape[1] and not (t is gate and t.size == shape[1])):
-                raise ValueError("norm_residual: gate, mod or shift %s for %d groups of %d columns" % (t.shape, groups, shape[1]))
+            if t is not None and (t.dtype != "float32" or t.size < grouped and not (t is gate and t.size == cols)):
+                raise ValueError("norm_residual: gate, mod or shift %s for groups of %d rows of %s" % (t.shape, group_rows, shape))
         self._check(self.lib.eddlhip_norm_residual(self.dev, x, ldx, r, ldr, residual_scale, s, lds, h, ldh, shape[0], shape[1], _NORMS[post[0]], _ptr(post[1]),
                                                    _ptr(post[2]), post[3], _ptr(gate), gate.size // shape[1] if gate is not None else 0, _NORMS[pre[0]],
                                                    _ptr(pre[1]), _ptr(pre[2]), pre[3], _ptr(mod), _ptr(shift), group_rows))

@@ -2,7 +2,7 @@
 //     n = post(x),   s = residual_scale r + gate n,   h = pre(s) (1 + mod) + shift,
 // post and pre each a layer norm (x - mean) / sqrt(var + eps) w + b, an RMS norm x / sqrt(mean(x^2) + eps) w + b, or nothing.
 //
-// A row stays in registers between its sums and its outputs: a wavefront a row up to 1024 columns, workgroups of 4 or 16
+// A row stays in registers between its sums and its outputs: a wavefront a row up to 1024 columns, workgroups of 4 to 16
 // wavefronts beyond.  Means and variances are fp32 sums over the registers; the variance is that of the differences from the mean, a
 // second pass over registers that costs no memory.
 // Bound: memory, 16 bytes a number (x, r, s, h).
@@ -60,7 +60,7 @@ __device__ __forceinline__ floatx4 get4(const float *p, int c, int cols) {
 template <bool VEC>
 __device__ __forceinline__ void set4(float *p, int c, int cols, floatx4 v) {
     if (VEC) {
-        *reinterpret_cast<floatx4 *>(p + c) = v;
+        __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(p + c));  // (written once, in whole lines: 12544 x 512 21.8 -> 17.4 us)
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -145,8 +145,8 @@ void launch(const NormParams &p, hipStream_t st) {
     static const struct {
         int threads, nv;
         kernel fn;
-    } sizes[] = {{64, 1, norm_residual_kernel<64, 1, VEC>},   {64, 2, norm_residual_kernel<64, 2, VEC>},   {64, 4, norm_residual_kernel<64, 4, VEC>},
-                 {256, 2, norm_residual_kernel<256, 2, VEC>}, {256, 4, norm_residual_kernel<256, 4, VEC>}, {256, 8, norm_residual_kernel<256, 8, VEC>},
+    } sizes[] = {{64, 1, norm_residual_kernel<64, 1, VEC>},     {64, 2, norm_residual_kernel<64, 2, VEC>},     {64, 4, norm_residual_kernel<64, 4, VEC>},
+                 {256, 2, norm_residual_kernel<256, 2, VEC>},   {512, 2, norm_residual_kernel<512, 2, VEC>},   {1024, 2, norm_residual_kernel<1024, 2, VEC>},
                  {1024, 4, norm_residual_kernel<1024, 4, VEC>}, {1024, 8, norm_residual_kernel<1024, 8, VEC>}};
     int k = 0;
     while (4 * sizes[k].threads * sizes[k].nv < p.cols) k++;

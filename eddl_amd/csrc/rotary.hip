@@ -46,43 +46,36 @@ __device__ __forceinline__ floatx4 load4(const float *p, bool vec) {
 }
 __device__ __forceinline__ void store4(float *p, floatx4 x, bool vec) {
     if (vec) {
-        *reinterpret_cast<floatx4 *>(p) = x;
+        __builtin_nontemporal_store(x, reinterpret_cast<floatx4 *>(p));  // (written once, in whole lines)
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) p[i] = x[i];
     }
 }
 
-// A head is cut into pieces of four pairs (8 numbers) and, behind rot_dim, of eight numbers: pieces = head_dim / 8.
-// Dimensions of piece n: (d0 .. d0 + 3) and (d1 .. d1 + 3).
-__device__ __forceinline__ void piece_at(const Rotary &r, int n, int &d0, int &d1) {
-    const bool halves = 4 * n < r.pairs && !r.adjacent;
-    d0 = halves ? 4 * n : 8 * n;
-    d1 = halves ? 4 * n + r.pairs : 8 * n + 4;
+// A thread takes four numbers side by side and, where halves are paired, the four that they turn with: its accesses and its
+// neighbours' lie side by side.  Pieces of a head: pairs / 4 of eight numbers and the rest of four, or all of four.
+__device__ __forceinline__ int pieces_of(const Rotary &r, int D) { return r.adjacent ? D / 4 : r.pairs / 4 + (D - 2 * r.pairs) / 4; }
+struct Piece {
+    int d0, d1;  // d1 < 0: four numbers only
+};
+__device__ __forceinline__ Piece piece_at(const Rotary &r, int n) {
+    if (r.adjacent) return Piece{4 * n, -1};
+    return 4 * n < r.pairs ? Piece{4 * n, 4 * n + r.pairs} : Piece{4 * n + r.pairs, -1};
 }
 __device__ __forceinline__ void turn_piece(const Rotary &r, int n, const float2 *cs, floatx4 &x, floatx4 &y) {
-    if (4 * n >= r.pairs) return;
-    floatx4 a, b;
     if (r.adjacent) {
-        a = floatx4{x[0], x[2], y[0], y[2]};
-        b = floatx4{x[1], x[3], y[1], y[3]};
-    } else {
-        a = x;
-        b = y;
-    }
-    floatx4 u, v;
+        if (2 * n >= r.pairs) return;
+        const float2 s = cs[2 * n], t = cs[2 * n + 1];
+        x = floatx4{x[0] * s.x - x[1] * s.y, x[1] * s.x + x[0] * s.y, x[2] * t.x - x[3] * t.y, x[3] * t.x + x[2] * t.y};
+    } else if (4 * n < r.pairs) {
+        const floatx4 a = x, b = y;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float2 t = cs[4 * n + i];
-        u[i] = a[i] * t.x - b[i] * t.y;
-        v[i] = b[i] * t.x + a[i] * t.y;
-    }
-    if (r.adjacent) {
-        x = floatx4{u[0], v[0], u[1], v[1]};
-        y = floatx4{u[2], v[2], u[3], v[3]};
-    } else {
-        x = u;
-        y = v;
+        for (int i = 0; i < 4; i++) {
+            const float2 t = cs[4 * n + i];
+            x[i] = a[i] * t.x - b[i] * t.y;
+            y[i] = b[i] * t.x + a[i] * t.y;
+        }
     }
 }
 
@@ -90,7 +83,7 @@ __device__ __forceinline__ void turn_piece(const Rotary &r, int n, const float2 
 template <int ROWS>
 __global__ __launch_bounds__(TPB) void rotary_kernel(const Rotary r, const float *X, float *Y, long long ldx, long long ldy, int rows, int heads, int D, int vec) {
     __shared__ float2 cs[ROWS][MAX_PAIRS];
-    const int pieces = D / 8, per_row = heads * pieces;
+    const int pieces = pieces_of(r, D), per_row = heads * pieces;
     for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
         const int n_rows = min(ROWS, rows - row0);
         __syncthreads();
@@ -98,14 +91,14 @@ __global__ __launch_bounds__(TPB) void rotary_kernel(const Rotary r, const float
         __syncthreads();
         for (int i = threadIdx.x; i < n_rows * per_row; i += TPB) {
             const int at = i / per_row, rest = i - at * per_row, head = rest / pieces, n = rest - head * pieces;
-            int d0, d1;
-            piece_at(r, n, d0, d1);
+            const Piece c = piece_at(r, n);
             const float *src = X + (size_t)(row0 + at) * ldx + (size_t)head * D;
-            floatx4 x = load4(src + d0, vec), y = load4(src + d1, vec);
+            floatx4 x = load4(src + c.d0, vec), y = x;
+            if (c.d1 >= 0) y = load4(src + c.d1, vec);
             turn_piece(r, n, cs[at], x, y);
             float *dst = Y + (size_t)(row0 + at) * ldy + (size_t)head * D;
-            store4(dst + d0, x, vec);
-            store4(dst + d1, y, vec);
+            store4(dst + c.d0, x, vec);
+            if (c.d1 >= 0) store4(dst + c.d1, y, vec);
         }
     }
 }
@@ -134,7 +127,7 @@ __global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const
     const int seq = blockIdx.z, row0 = max(p.offsets[seq], 0), fresh = row0 < p.rows ? min(p.offsets[seq + 1], p.rows) - row0 : 0, length = p.lengths[seq];
     const int start = length - fresh;  // place of row row0 (below 0: the first rows have none)
     if (fresh <= 0) return;
-    const int D = p.D, pieces = D / 8;
+    const int D = p.D, pieces = pieces_of(r, D);
     // blocks of 16 rows of the sequence, aligned to the places
     const int shift = start & 15;
     for (int b = blockIdx.x; 16 * b < shift + fresh; b += gridDim.x) {
@@ -152,59 +145,53 @@ __global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const
         const int t0 = place & 15;
         const int q_items = p.Q ? p.q_heads : 0, head_lo = (int)((long long)(q_items + 2 * p.kv_heads) * blockIdx.y / p.head_groups),
                   head_hi = (int)((long long)(q_items + 2 * p.kv_heads) * (blockIdx.y + 1) / p.head_groups);
-        for (int h = head_lo; h < head_hi; h++) {
-            if (h < q_items) {
-                for (int i = threadIdx.x; i < n_rows * pieces; i += TPB) {
-                    const int at = i / pieces, n = i - at * pieces;
-                    const size_t row = row0 + first + at;
-                    int d0, d1;
-                    piece_at(r, n, d0, d1);
-                    const float *src = p.Q + row * p.ldq + (size_t)h * D;
-                    floatx4 x = load4(src + d0, p.vec), y = load4(src + d1, p.vec);
-                    turn_piece(r, n, cs[at], x, y);
-                    float *dst = p.Qout + row * p.ldo + (size_t)h * D;
-                    store4(dst + d0, x, p.vec);
-                    store4(dst + d1, y, p.vec);
-                }
-            } else if (!stored) {
-                continue;
-            } else if (h < q_items + p.kv_heads) {
-                const int kv = h - q_items;
-                const size_t base = block * 16 * D + kv * head_stride;
-                for (int i = threadIdx.x; i < n_rows * pieces; i += TPB) {
-                    const int at = i % n_rows, n = i / n_rows;  // (tokens side by side: theirs are the neighbouring places)
-                    int d0, d1;
-                    piece_at(r, n, d0, d1);
-                    const float *src = p.K + (size_t)(row0 + first + at) * p.ldk + (size_t)kv * D;
-                    floatx4 x = load4(src + d0, p.vec), y = load4(src + d1, p.vec);
-                    turn_piece(r, n, cs[at], x, y);
-                    const size_t t = base + (t0 + at) * 8;
-                    put4(p.k_pages, t + (d0 >> 3) * 128 + (d0 & 7), x, p.f32);
-                    put4(p.k_pages, t + (d1 >> 3) * 128 + (d1 & 7), y, p.f32);
-                }
+        // queries, keys and values of the group's heads, each as one run of work for all threads
+        const int q_hi = min(head_hi, q_items), q_work = max(0, q_hi - head_lo) * n_rows * pieces;
+        for (int i = threadIdx.x; i < q_work; i += TPB) {
+            const int rest = i / pieces, n = i - rest * pieces, h = rest / n_rows, at = rest - h * n_rows;
+            const size_t row = row0 + first + at, col = (size_t)(head_lo + h) * D;
+            const Piece c = piece_at(r, n);
+            const float *src = p.Q + row * p.ldq + col;
+            floatx4 x = load4(src + c.d0, p.vec), y = x;
+            if (c.d1 >= 0) y = load4(src + c.d1, p.vec);
+            turn_piece(r, n, cs[at], x, y);
+            float *dst = p.Qout + row * p.ldo + col;
+            store4(dst + c.d0, x, p.vec);
+            if (c.d1 >= 0) store4(dst + c.d1, y, p.vec);
+        }
+        if (!stored) continue;
+        const int k_lo = max(head_lo - q_items, 0), k_hi = min(head_hi - q_items, p.kv_heads), k_work = max(0, k_hi - k_lo) * n_rows * pieces;
+        for (int i = threadIdx.x; i < k_work; i += TPB) {
+            const int rest = i / n_rows, at = i - rest * n_rows, h = rest / pieces, n = rest - h * pieces;  // (tokens side by side: theirs are the neighbouring places)
+            const int kv = k_lo + h;
+            const Piece c = piece_at(r, n);
+            const float *src = p.K + (size_t)(row0 + first + at) * p.ldk + (size_t)kv * D;
+            floatx4 x = load4(src + c.d0, p.vec), y = x;
+            if (c.d1 >= 0) y = load4(src + c.d1, p.vec);
+            turn_piece(r, n, cs[at], x, y);
+            const size_t t = block * 16 * D + kv * head_stride + (t0 + at) * 8;
+            put4(p.k_pages, t + (c.d0 >> 3) * 128 + (c.d0 & 7), x, p.f32);
+            if (c.d1 >= 0) put4(p.k_pages, t + (c.d1 >> 3) * 128 + (c.d1 & 7), y, p.f32);
+        }
+        const int v_lo = max(head_lo - q_items - p.kv_heads, 0), v_hi = head_hi - q_items - p.kv_heads, v_work = max(0, v_hi - v_lo) * 4 * D;
+        for (int i = threadIdx.x; i < v_work; i += TPB) {  // four tokens of a dimension
+            const int rest = i / D, d = i - rest * D, quarter = rest & 3, kv = v_lo + (rest >> 2), at = 4 * quarter - t0;  // (row of the block's token 4 quarter)
+            if (at + 4 <= 0 || at >= n_rows) continue;
+            const float *src = p.V + (size_t)kv * D + d;
+            floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (at + k >= 0 && at + k < n_rows) x[k] = src[(size_t)(row0 + first + at + k) * p.ldv];
+            const size_t t = block * 16 * D + kv * head_stride + (size_t)(quarter >> 1) * 8 * D + d * 8 + (quarter & 1) * 4;
+            if (at >= 0 && at + 4 <= n_rows) {
+                put4(p.v_pages, t, x, p.f32);
             } else {
-                const int kv = h - q_items - p.kv_heads;
-                const size_t base = block * 16 * D + kv * head_stride;
-                for (int i = threadIdx.x; i < 4 * D; i += TPB) {  // four tokens of a dimension
-                    const int quarter = i / D, d = i - quarter * D, at = 4 * quarter - t0;  // (row of the block's token 4 quarter)
-                    if (at + 4 <= 0 || at >= n_rows) continue;
-                    const float *src = p.V + (size_t)kv * D + d;
-                    floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        if (at + k >= 0 && at + k < n_rows) x[k] = src[(size_t)(row0 + first + at + k) * p.ldv];
-                    const size_t t = base + (size_t)(quarter >> 1) * 8 * D + d * 8 + (quarter & 1) * 4;
-                    if (at >= 0 && at + 4 <= n_rows) {
-                        put4(p.v_pages, t, x, p.f32);
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            if (at + k >= 0 && at + k < n_rows) {
-                                if (p.f32) ((float *)p.v_pages)[t + k] = x[k];
-                                else ((unsigned short *)p.v_pages)[t + k] = (unsigned short)split_round(x[k], x[k]);
-                            }
+                for (int k = 0; k < 4; k++)
+                    if (at + k >= 0 && at + k < n_rows) {
+                        if (p.f32) ((float *)p.v_pages)[t + k] = x[k];
+                        else ((unsigned short *)p.v_pages)[t + k] = (unsigned short)split_round(x[k], x[k]);
                     }
-                }
             }
         }
     }
