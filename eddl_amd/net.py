@@ -6,7 +6,8 @@ and each layer's unfused forward is the one call its reference counterpart makes
 (LConv::forward -> Conv2D, LBatchNorm::forward -> BatchNormForward in inference mode,
 LActivation -> ReLu/Sigmoid/FullSoftmax, LMaxPool -> MPool2D, LAveragePool -> AvgPool2D,
 LResize -> scale, LConcat -> concat, LAdd -> fill_+inc, LSum -> add, LPad -> pad,
-LDense -> mult2D + sum2D_rowwise, LReshape -> shared storage).
+LDense -> mult2D + sum2D_rowwise, LReshape -> shared storage).  Norms over the last axis and attention over a
+paged cache are layers of this package's own.
 
 ``Net.build(backend, fuse=True)`` additionally runs a fusion pass in the spirit of the
 reference's FPGA model transformation (src/apis/fpga.cpp:173-331,656+): chains
@@ -209,6 +210,41 @@ def Dense(parent, ndim, use_bias=True, name=""):
     return l
 
 
+# ---------------------------------------------------------------------------- attention blocks (no counterpart in the reference's path)
+def _norm(kind, parent, affine, epsilon, name):
+    l = Layer("norm", [parent], parent.out_shape, name or "%s_norm%d" % (kind, Layer._count.get("norm", 0) + 1), norm=kind, affine=affine, epsilon=float(epsilon))
+    if affine:
+        l.params["w"] = np.ones(parent.out_shape[-1], np.float32)
+        if kind == "layer":
+            l.params["b"] = np.zeros(parent.out_shape[-1], np.float32)
+    return l
+
+
+def LayerNormalization(parent, affine=True, epsilon=1e-5, name=""):
+    """(x - mean) / sqrt(variance + epsilon) w + b over the last axis.  In a fused plan a norm, the Add of two layers behind it and
+    a norm behind that become one launch (``eddlhip_norm_residual``), and so do an Add and the norm behind it."""
+    return _norm("layer", parent, affine, epsilon, name)
+
+
+def RMSNormalization(parent, affine=True, epsilon=1e-6, name=""):
+    """x / sqrt(mean(x^2) + epsilon) w over the last axis; fused like ``LayerNormalization``."""
+    return _norm("rms", parent, affine, epsilon, name)
+
+
+def PagedAttention(parent, heads, cache, batch, rotary=None, positions=None, causal=True, window=0, scale=None, name=""):
+    """Attention of new tokens over a paged cache.  ``parent``: [batch, tokens, (heads + 2 kv_heads) * head_dim], queries, keys and values
+    side by side as one Dense layer brings them; the output is [batch, tokens, heads * head_dim].  Each forward writes the tokens' keys
+    (turned by ``rotary``, with ``positions`` [batch * tokens, axes]) and values into ``cache`` and attends over what it then holds.
+    ``cache``, ``batch`` and ``rotary`` are those of ``eddl_amd.attention``; the program sets ``batch.lengths`` and ``positions``
+    (device tensors) before a forward or the replay of a captured plan."""
+    width = (int(heads) + 2 * cache.kv_heads) * cache.head_dim
+    if len(parent.out_shape) != 3 or parent.out_shape[2] != width or int(heads) % cache.kv_heads:
+        msg("PagedAttention needs [batch, tokens, %d] for %d query heads and %d key heads of %d, not %s"
+            % (width, heads, cache.kv_heads, cache.head_dim, parent.out_shape), "PagedAttention")
+    return Layer("attention", [parent], parent.out_shape[:2] + [int(heads) * cache.head_dim], name, heads=int(heads), cache=cache, batch=batch, rotary=rotary,
+                 positions=positions, causal=bool(causal), window=int(window), scale=scale)
+
+
 # ---------------------------------------------------------------------------- the net
 class Op:
     """One launch group of the built plan.  ``flops``/``bytes`` are the algorithmic figures
@@ -376,6 +412,9 @@ class Net:
             if l.kind == "dense":
                 self._emit_dense(l, fuse, absorbed, sole_child)
                 continue
+            if l.kind == "norm" or (fuse and l.kind == "sum" and any(c.kind == "norm" for c in l.children)):
+                self._emit_norm(l, fuse, absorbed, sole_child)
+                continue
             self._emit_plain(l)
         for o in self.lout:
             if id(o) not in self.out:
@@ -542,6 +581,46 @@ class Net:
         layers = [l] if last is l else [l, last]
         self.ops.append(Op("dense", name, run, 2 * rows * in_dim * ndim, 4 * (rows * in_dim + in_dim * ndim + rows * ndim), layers))
 
+    def _emit_norm(self, l, fuse, absorbed, sole_child):
+        """A norm, or in a fused plan norm -> sum -> norm, norm -> sum and sum -> norm: one launch, every step the separate layer's."""
+        hip = self.backend
+        post, total, other = (l, None, None) if l.kind == "norm" else (None, l, l.parents[0])
+        src = l.parents[0] if post is not None else l.parents[1]
+        if fuse and post is not None:
+            c = sole_child(l)
+            if c is not None and c.kind == "sum":
+                o = c.parents[1] if c.parents[0] is l else c.parents[0]
+                if id(o) in self.out and o is not l:
+                    total, other = c, o
+        pre = None
+        if total is not None and fuse:
+            pre = next((c for c in total.children if c.kind == "norm"), None)
+        if total is None:  # one norm by itself
+            post, pre = None, l
+        members = [m for m in (post, total, pre) if m is not None]
+        absorbed.update(id(m) for m in members if m is not l)
+        rows, cols = int(np.prod(l.out_shape[:-1])), l.out_shape[-1]
+
+        def output(layer, needed):
+            if layer is None or not needed:
+                return None
+            self.out[id(layer)] = hip.empty(layer.out_shape)
+            return self.out[id(layer)].reshape((rows, cols))
+
+        S = output(total, total is not None and (pre is None or len(total.children) > 1 or total in self.lout))
+        H = output(pre, True)
+        X = self.out[id(src)].reshape((rows, cols))
+        R = self.out[id(other)].reshape((rows, cols)) if other is not None else None
+
+        def params(n):
+            if n is None:
+                return (None, None, None, 0.0)
+            dp = self.dparams[id(n)]
+            return (n.attrs["norm"], dp.get("w"), dp.get("b"), n.attrs["epsilon"])
+        a, b = params(post), params(pre)
+        count = 1 + (R is not None) + (S is not None) + (H is not None)
+        self.ops.append(Op("norm", "+".join(m.name for m in members), lambda: hip.norm_residual(X, R, S, H, post=a, pre=b), 0, 4 * count * rows * cols, members))
+
     def _emit_plain(self, l):
         hip = self.backend
         k = l.kind
@@ -589,6 +668,16 @@ class Net:
                 for t in ins:
                     hip.inc(t, O)
             nbytes = 4 * n_out * (1 + 3 * len(ins))
+        elif k == "attention":
+            at = l.attrs
+            cache, batch, heads = at["cache"], at["batch"], at["heads"]
+            rows, q, kv = l.out_shape[0] * l.out_shape[1], heads * cache.head_dim, cache.kv_heads * cache.head_dim
+            qkv, O2, turned = ins[0].reshape((rows, q + 2 * kv)), O.reshape((rows, q)), hip.empty((rows, q))
+
+            def run():
+                hip.paged_append(qkv.columns(0, q), qkv.columns(q, q + kv), qkv.columns(q + kv, q + 2 * kv), turned, cache, batch, at["rotary"], at["positions"])
+                hip.paged_attention(turned, O2, cache, batch, at["scale"], at["causal"], at["window"])
+            nbytes = 4 * (n_out + rows * (q + 2 * kv))  # (what the cache holds grows)
         elif k == "pad":
             hip.fill_(O, l.attrs["constant"])  # the border is written once, here; forward copies the interior
             n_in = int(np.prod(l.parents[0].out_shape))

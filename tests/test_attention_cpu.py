@@ -148,3 +148,16 @@ def test_reference_layout_is_a_permutation():
         assert sorted(seen) == list(range(pool.pages * 16 * 2 * 32))
     x = np.array([1.0, 1.00390625, 1.01171875, -3.14159, np.inf], np.float32)
     assert bf16_value(bf16_bits(x)).tolist() == [1.0, 1.0, 1.015625, -3.140625, np.inf]
+
+
+def test_paged_attention_layer_checks_its_parent():
+    from eddl_amd import net as L
+    from eddl_amd.attention import PagedCache
+    cache = PagedCache(None, 4, 16, 2, 64, storage=(_Tensor((4, 2, 1, 8, 16, 8)), _Tensor((4, 2, 1, 2, 64, 8))))
+    ok = L.PagedAttention(L.Input([7, 8 * 64], 3), 4, cache, None)
+    assert ok.out_shape == [3, 7, 256]
+    for shape, heads in (([7, 8 * 64], 5), ([7, 500], 4), ([8 * 64], 4), ([7, 7 * 64], 3)):
+        with pytest.raises(RuntimeError):
+            L.PagedAttention(L.Input(shape, 3), heads, cache, None)
+    n = L.LayerNormalization(L.Input([7, 24], 3))
+    assert sorted(n.params) == ["b", "w"] and n.params["w"].shape == (24,) and not L.RMSNormalization(n, affine=False).params

@@ -628,3 +628,89 @@ def test_a_block_of_video_frames(hip, dtype):
         tol = (2e-5 if dtype == "float32" else 2e-3)
         assert np.abs(X.numpy() - want_s).max() <= tol * np.abs(want_s).max()
         assert np.abs(H.numpy() - want_h).max() <= tol * np.abs(want_h).max()
+
+
+def test_net_of_attention_blocks(hip):
+    """Layers: norm, dense, paged attention, dense, norm, Add, norm, dense, ReLU, dense, Add, norm.  The fused plan, the layer walk and a captured
+    plan give the same bits, frame after frame, and the network in 64 bits within 2e-5 of its largest output (some tens of EPS a stage)."""
+    from eddl_amd import net as L
+    from eddl_amd.attention import PagedBatch, PagedCache, RotaryPlan
+    rng = np.random.default_rng(17)
+    videos, tokens, heads, kv, dim, frames = 2, 9, 4, 2, 16, 3
+    cols, width = heads * dim, -(-frames * tokens // 16)
+    plan = RotaryPlan.sections(dim, (2, 3, 3))
+    table = rng.permutation(videos * width).reshape(videos, width)
+
+    def build(fuse):
+        cache = PagedCache(hip, videos * width, 16, kv, dim)
+        batch = PagedBatch(hip.array(table, "int32"), hip.array(np.arange(videos + 1) * tokens, "int32"), hip.empty((videos,), "int32"), tokens, frames * tokens)
+        pos = hip.empty((videos * tokens, 3))
+        x = L.Input([tokens, cols], videos)
+        a = L.PagedAttention(L.Dense(L.RMSNormalization(x), (heads + 2 * kv) * dim, use_bias=False), heads, cache, batch, plan, pos, causal=False)
+        s = L.Add(x, L.RMSNormalization(L.Dense(a, cols)))
+        h = L.Dense(L.ReLu(L.Dense(L.LayerNormalization(s), 2 * cols)), cols)
+        n = L.Net([x], [L.LayerNormalization(L.Add(s, h), affine=False)])
+        r = np.random.default_rng(18)
+        for l in n.layers:
+            for k, v in l.params.items():
+                scale = 1 / np.sqrt(v.shape[0]) if k == "W" else 0.1
+                l.params[k] = ((1.0 if k == "w" else 0.0) + scale * r.standard_normal(v.shape)).astype(np.float32)
+        return n.build(hip, fuse=fuse), batch, pos
+
+    (fused, b0, p0), (walk, b1, p1) = build(True), build(False)
+    assert sorted(op.kind for op in fused.ops) == ["attention"] + ["dense"] * 4 + ["norm"] * 3
+    assert sum(op.kind in ("norm", "sum") for op in walk.ops) == 6
+    graph, want_k, want_v = None, [], []
+    P = {(l.kind, i): {k: v.astype(np.float64) for k, v in l.params.items()} for i, l in enumerate(fused.layers)}
+    norms, denses = ([P[k] for k in P if k[0] == kind] for kind in ("norm", "dense"))
+    for f in range(frames):
+        x = rng.standard_normal((videos, tokens, cols), dtype=np.float32)
+        yy, xx = np.divmod(np.tile(np.arange(tokens), videos), 3)
+        pos = np.stack([np.full(videos * tokens, f), yy, xx], 1).astype(np.float32)
+        for b, p in ((b0, p0), (b1, p1)):
+            b.lengths.copy_from(np.full(videos, (f + 1) * tokens))
+            p.copy_from(pos)
+        got = fused.predict(x)[0]
+        assert np.array_equal(walk.predict(x)[0], got)
+        if graph is None:
+            graph = fused.capture()
+        fused.input_tensor().copy_from(x)
+        fused.run_graph()
+        assert np.array_equal(fused.output_of(fused.lout[0]).numpy(), got)
+        # in 64 bits
+        rows = x.reshape(-1, cols).astype(np.float64)
+        rms = lambda t, w: t / np.sqrt((t * t).mean(1, keepdims=True) + 1e-6) * w
+        lay = lambda t: (t - t.mean(1, keepdims=True)) / np.sqrt(((t - t.mean(1, keepdims=True)) ** 2).mean(1, keepdims=True) + 1e-5)
+        qkv = rms(rows, norms[0]["w"]) @ denses[0]["W"]
+        qk = turned(qkv[:, :cols + kv * dim], pos, heads + kv, dim, plan.axis, plan.freq, False)
+        want_k.append(qk[:, cols:].reshape(videos, tokens, kv, dim))
+        want_v.append(qkv[:, cols + kv * dim:].reshape(videos, tokens, kv, dim))
+        K, V, q = np.concatenate(want_k, 1), np.concatenate(want_v, 1), qk[:, :cols].reshape(videos, tokens, heads, dim)
+        att = np.zeros((videos, tokens, heads, dim))
+        for s in range(videos):
+            for hd in range(heads):
+                w = np.exp(q[s, :, hd] @ K[s, :, hd * kv // heads].T * dim ** -0.5)
+                att[s, :, hd] = w / w.sum(1, keepdims=True) @ V[s, :, hd * kv // heads]
+        s = rows + rms(att.reshape(-1, cols) @ denses[1]["W"] + denses[1]["bias"], norms[1]["w"])
+        h = np.maximum((lay(s) * norms[2]["w"] + norms[2]["b"]) @ denses[2]["W"] + denses[2]["bias"], 0) @ denses[3]["W"] + denses[3]["bias"]
+        want = lay(s + h)
+        assert np.abs(got.reshape(-1, cols) - want).max() <= 2e-5 * np.abs(want).max()
+
+
+@pytest.mark.parametrize("fuse", [True, False])
+def test_norms_in_nets_keep_what_others_read(hip, fuse):
+    """A sum that a norm and another layer read, a norm that two layers read, and a norm of a network's input as output."""
+    from eddl_amd import net as L
+    rng = np.random.default_rng(19)
+    x, y = L.Input([5, 24], 2), L.Input([5, 24], 2)
+    s = L.Add(x, y)
+    n1, r = L.LayerNormalization(s), L.ReLu(s)
+    n2 = L.RMSNormalization(n1)
+    net = L.Net([x, y], [L.Add(n1, r), n2, L.RMSNormalization(x, affine=False)]).build(hip, fuse=fuse)
+    a, b = (rng.standard_normal((2, 5, 24), dtype=np.float32) for _ in range(2))
+    got = net.predict([a, b])
+    t = (a.astype(np.float64) + b).reshape(10, 24)
+    n = (t - t.mean(1, keepdims=True)) / np.sqrt(t.var(1, keepdims=True) + 1e-5)
+    rms = lambda v: v / np.sqrt((v * v).mean(1, keepdims=True) + 1e-6)
+    for g, w in zip(got, (n + np.maximum(t, 0), rms(n), rms(a.reshape(10, 24).astype(np.float64)))):
+        assert np.abs(g.reshape(10, 24) - w).max() <= 160 * EPS * 2 * np.abs(w).max()
