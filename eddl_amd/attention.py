@@ -24,14 +24,14 @@ class PagedCache:
         if storage is None:
             self.keys, self.values = backend.empty(k_shape, dtype), backend.empty(v_shape, dtype)
             for t in (self.keys, self.values):  # (zeros in either type)
-                backend._check(backend.lib.eddlhip_fill(backend.dev, t.ptr, t.nbytes // 4, 0.0))
+                backend._check(backend.lib.eddlhip_fill(backend.dev, t.address, t.nbytes // 4, 0.0))
         else:
             self.keys, self.values = storage
             if tuple(self.keys.shape) != k_shape or tuple(self.values.shape) != v_shape or self.keys.dtype != dtype or self.values.dtype != dtype:
                 raise ValueError("a cache of %d pages of %d tokens, %d heads of %d holds keys %s and values %s of %s, not %s %s and %s %s"
                                  % (pages, page_size, kv_heads, head_dim, k_shape, v_shape, dtype, self.keys.dtype, self.keys.shape, self.values.dtype,
                                     self.values.shape))
-        self.arguments = (self.keys.ptr, self.values.ptr, _CACHE_TYPES[dtype], self.pages, self.page_size)
+        self.arguments = (self.keys.address, self.values.address, _CACHE_TYPES[dtype], self.pages, self.page_size)
 
 
 class PagedBatch:
@@ -44,7 +44,7 @@ class PagedBatch:
             raise ValueError("a batch is int32 table [sequences, width], offsets [sequences + 1], lengths [sequences], not %s %s %s" % (table.shape, offsets.shape, lengths.shape))
         self.table, self.offsets, self.lengths = table, offsets, lengths
         self.max_new, self.max_length = int(max_new), int(max_length)
-        self.arguments = (table.ptr, table.shape[1], offsets.ptr, lengths.ptr, table.shape[0])
+        self.arguments = (table.address, table.shape[1], offsets.address, lengths.address, table.shape[0])
 
 
 class RotaryPlan:

@@ -20,19 +20,22 @@ _TYPES = {"float32": (4, np.float32), "int32": (4, np.int32), "bfloat16": (2, np
 
 
 class DeviceTensor:
-    """A tensor in HBM owned by this object (freed when collected): float32, or, where an operator asks for them, int32 and bfloat16."""
+    """A float32 tensor in HBM owned by this object (freed when collected)."""
     dtype = "float32"
 
-    def __init__(self, backend, shape, dtype="float32"):
+    def __init__(self, backend, shape):
+        self._describe(backend, shape)
+        self.ptr = backend._malloc(self.nbytes)
+
+    def _describe(self, backend, shape):
         self.backend = backend
         self.shape = tuple(int(d) for d in shape)
         self.size = int(np.prod(self.shape)) if len(self.shape) else 1
-        if dtype not in _TYPES:
-            raise ValueError("no tensors of type %s: %s" % (dtype, ", ".join(_TYPES)))
-        if dtype != "float32":
-            self.dtype = dtype
-        self.nbytes = self.size * _TYPES[dtype][0]
-        self.ptr = backend._malloc(self.nbytes)
+        self.nbytes = self.size * _TYPES[self.dtype][0]
+
+    @property
+    def address(self):
+        return self.ptr
 
     def __del__(self):
         try:
@@ -44,33 +47,30 @@ class DeviceTensor:
 
     def numpy(self):
         out = np.empty(self.shape, _TYPES[self.dtype][1])
-        self.backend._check(self.backend.lib.eddlhip_memcpy_d2h(self.backend.dev, out.ctypes.data, self.ptr, self.nbytes))
+        self.backend._check(self.backend.lib.eddlhip_memcpy_d2h(self.backend.dev, out.ctypes.data, self.address, self.nbytes))
         return out
 
     def copy_from(self, host):
         host = np.ascontiguousarray(host, dtype=_TYPES[self.dtype][1])
         if host.size != self.size:
             raise ValueError("size mismatch: %s vs %s" % (host.shape, self.shape))
-        self.backend._check(self.backend.lib.eddlhip_memcpy_h2d(self.backend.dev, self.ptr, host.ctypes.data, self.nbytes))
+        self.backend._check(self.backend.lib.eddlhip_memcpy_h2d(self.backend.dev, self.address, host.ctypes.data, self.nbytes))
         return self
 
     def reshape(self, shape):
         """A view with another shape sharing the storage (the reference's reshape_)."""
-        view = object.__new__(DeviceTensor)
+        view = object.__new__(_View)
         view.backend, view.ptr, view.nbytes, view.size = self.backend, self.ptr, self.nbytes, self.size
         view.shape = tuple(int(d) for d in shape)
         if int(np.prod(view.shape)) != self.size:
             raise ValueError("reshape changes the size")
         view._base = self  # keeps the owner alive
-        if self.dtype != "float32":
-            view.dtype = self.dtype
-        view.__class__ = _View
         return view
 
     def columns(self, start, stop):
-        """Columns ``start`` .. ``stop - 1`` of a float32 matrix [rows, columns], for the operators that take rows of any distance."""
-        if len(self.shape) != 2 or self.dtype != "float32" or not 0 <= start < stop <= self.shape[1]:
-            raise ValueError("columns %d to %d of a %s tensor of shape %s" % (start, stop, self.dtype, self.shape))
+        """Columns ``start`` .. ``stop - 1`` of a matrix [rows, columns], for the operators that take rows of any distance."""
+        if len(self.shape) != 2 or not 0 <= start < stop <= self.shape[1]:
+            raise ValueError("columns %d to %d of a tensor of shape %s" % (start, stop, self.shape))
         return Columns(self, start, stop)
 
 
@@ -79,9 +79,39 @@ class _View(DeviceTensor):
         pass
 
 
-class _Foreign(DeviceTensor):
-    def __del__(self):  # storage belongs to the object that lent it
-        pass
+class TypedTensor(DeviceTensor):
+    """A tensor of int32 or bfloat16 numbers, for the operators that ask for them; the others take float32 tensors only, and find no ``ptr`` here."""
+
+    def __init__(self, backend, shape, dtype, owner=None, address=None):
+        if dtype not in _TYPES or dtype == "float32":
+            raise ValueError("no tensors of type %s: %s" % (dtype, ", ".join(_TYPES)))
+        self.dtype = dtype
+        self._describe(backend, shape)
+        self._owner, self._address = owner, backend._malloc(self.nbytes) if owner is None else address
+
+    @property
+    def address(self):
+        return self._address
+
+    @property
+    def ptr(self):
+        raise TypeError("this operator takes float32 tensors, not %s" % self.dtype)
+
+    def __del__(self):
+        try:
+            if self._owner is None and self._address:
+                self.backend._free(self._address)
+                self._address = None
+        except Exception:
+            pass
+
+    def reshape(self, shape):
+        if int(np.prod(shape)) != self.size:
+            raise ValueError("reshape changes the size")
+        return TypedTensor(self.backend, shape, self.dtype, self, self._address)
+
+    def columns(self, start, stop):
+        raise TypeError("columns are those of float32 matrices, not %s" % self.dtype)
 
 
 class Columns:
@@ -284,7 +314,7 @@ class Backend:
         return r.value, w.value, c.value
 
     def empty(self, shape, dtype="float32"):
-        return DeviceTensor(self, shape, dtype)
+        return DeviceTensor(self, shape) if dtype == "float32" else TypedTensor(self, shape, dtype)
 
     def wrap(self, owner, dtype=None):
         """Device memory that another library holds (an object with ``__cuda_array_interface__``, contiguous) as a tensor, without a copy; keeps
@@ -299,15 +329,18 @@ class Backend:
             if d > 1 and step != expect:
                 raise ValueError("the memory of a wrapped tensor is contiguous: shape %s, strides %s" % (shape, steps))
             expect *= d
-        t = object.__new__(_Foreign)
-        t.backend, t.shape, t.dtype, t._owner, t.ptr = self, shape, kind, owner, spec["data"][0]
-        t.size = int(np.prod(shape)) if shape else 1
-        t.nbytes = t.size * _TYPES[kind][0]
+        if kind != "float32":
+            return TypedTensor(self, shape, kind, owner, spec["data"][0])
+        t = object.__new__(_View)
+        t._describe(self, shape)
+        t._base, t.ptr = owner, spec["data"][0]
         return t
 
     def array(self, host, dtype="float32"):
+        if dtype not in _TYPES:
+            raise ValueError("no tensors of type %s: %s" % (dtype, ", ".join(_TYPES)))
         host = np.ascontiguousarray(host, dtype=_TYPES[dtype][1])
-        return DeviceTensor(self, host.shape, dtype).copy_from(host)
+        return self.empty(host.shape, dtype).copy_from(host)
 
     def full(self, shape, v):
         t = DeviceTensor(self, shape)

@@ -1,21 +1,20 @@
-// Attention of new tokens over a paged cache, in fp32 accuracy on the bf16 matrix instructions.
+// Attention of new tokens over a paged cache, in fp32 accuracy on the 16-bit matrix instructions.
 //
 // Row i of a sequence's `new` query rows stands at position p = length - new + i.  With the visible tokens j (j < length; causal:
 // j <= p; window: j > p - window)
 //     s_j = scale q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),   m = max_j s_j,   and o = 0 where nothing is visible.
 // One pass over the tokens with running maximum, sum and output; all three in fp32.  The exponentials are powers of two: log2(e)
-// goes into the queries together with the scale.
+// goes into the scores together with the scale.
 //
-// The two products run on v_mfma_f32_32x32x16_bf16.  Every fp32 operand (queries, weights, an fp32 cache) is the sum of three bf16
-// numbers (split_parts.h); a bf16 cache is its own single part.  An fp32 cache takes the six largest of nine products, a bf16
-// cache three, whose sum is the product of a bf16 and an fp32 number without any rounding but the accumulator's.  Parts of
-// numbers below 2^-110 lose bits: absolute errors of 2^-133, nothing beside a softmax's other terms.
+// Two kernels: attend_few_kernel for up to 32 rows (a token's query heads of one key head are rows side by side), which is bound by the
+// cache's bytes, and attend_chunk_kernel for more, which is bound by the matrix instruction.  A long sequence with few rows is
+// divided over workgroups, whose parts are joined.
 //
-// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a query is a column: lane l holds the scores of query
-// l % 32 in registers, the maximum and the sum of a query are those of two lanes (one shuffle), the rescaling of the output is
-// one factor a lane.  And S^T is the second product's operand as it stands: a lane needs eight consecutive tokens of its query, which
-// it has when row r = 8a + 4h + i of the first product is token 16 (a / 2) + 8h + 4 (a % 2) + i.  The rows of K are read in that
-// order; no score ever moves between lanes.
+// Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T, so that a query is a column: a lane holds scores of one query in
+// registers, the maximum of a query is that of two or four lanes, the rescaling of the output is one factor a lane.  And S^T is the
+// second product's operand as it stands: a lane needs eight consecutive tokens of its query, which it has when the rows of K are read
+// in the right order (with 32 rows, row 8a + 4h + i of the product is token 16 (a / 2) + 8h + 4 (a % 2) + i; with 16, row 4g + i of
+// tile t is token 8g + 4t + i).  No score ever moves between lanes.
 //
 // The cache is kept in the order in which these operands are read (eddlhip.h): a lane's operand is 16 (32) bytes side by side, and
 // the lanes' operands are side by side too.
@@ -338,11 +337,17 @@ __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence
 
 // ------------------------------------------------------------------------------------------------ few rows
 // Up to 16 NQ rows of a sequence and key head (single tokens, short drafts): bound by the cache's bytes.  A workgroup takes a part of the
-// tokens, its four wavefronts take steps of 32 tokens in turn, operands straight from the cache into registers: every byte is read
+// tokens, its four or eight wavefronts take steps of 32 tokens in turn, operands straight from the cache into registers: every byte is read
 // once, by one wavefront, so LDS would only add a trip.  Keys of the next step are asked for as soon as the products have
 // used this step's, values likewise, into the same registers: a step's loads are on their way while the other half of a step is
 // computed, 16 (32) KB a wavefront.  The 16x16x32 instruction keeps the queries that are not there at 15 of 16 columns
 // instead of 31 of 32, and the registers at half.  The wavefronts' sums meet in LDS once.
+// The matrix instruction has time to spare, so every fp32 operand (queries, weights, an fp32 cache) is the sum of three bf16 numbers
+// (split_parts.h), six products for an fp32 cache and three for a bf16 one, whose sum has no rounding but the accumulator's; no
+// exponents are kept.  (Parts of numbers below 2^-110 lose bits: absolute errors of 2^-133.)
+// Measured: 1 token over 131072, 8 key heads of 128 in bf16 (537 MB): 94 us, 5.7 TB/s, where a plain read stream reaches 6.9 - 7.1;
+// 32 over 4096 (fp32, 1.07 GB) 186 us, 5.8 TB/s.  Without the streaming hint 104 us; a second step in flight gains nothing, more
+// workgroups than the device holds at a time lose 4 to 15 %.
 // Rows of the product K Q^T: row 4g + i of tile t is token 8g + 4t + i of the step, so that lane group g holds tokens 8g .. 8g + 7.
 // Wavefronts of a SIMD, as the registers of a step's keys, values and outputs allow without spills, and wavefronts of a workgroup: all that a
 // CU holds where that is 8 (fewer parts to join, and a part lasts as long as possible: 1 token over 131072, heads of 128 in bf16, 95 us,
@@ -664,8 +669,11 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
 // Tiles: a wavefront brings the keys or the values of 16 tokens, their numbers go through its registers (the largest, the pairs) into LDS;
 // two tiles, one filled while the other is used, one barrier a tile.  The cache's order is the operands' order: every LDS
 // access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
+// Measured: 2048 tokens over 8192, 32 and 8 heads of 128, bf16 cache: 545 us, 440 TFLOP/s, 880 on the matrix instructions (42 % of the cycles
+// busy; the vector instructions fill 57 % and the two do not overlap: a version that computed the next tile's scores beside the
+// weights in one block, with the scheduler's groups, spilled and took 890).  As three bf16 parts with tiles loaded straight into LDS 621 us.
 constexpr int CHUNK_ROWS = 128;
-constexpr int CHUNK_SPLITS = 16;  // most parts of a length: their sums fit where two tiles of 64 dimensions were
+constexpr int CHUNK_SPLITS = 64;  // most parts of a length
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
@@ -1107,6 +1115,7 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     EH_REQUIRE(max_new >= 0 && max_length >= 0 && window >= 0, "paged_attention: negative max_new, max_length or window");
     if (rows == 0 || seqs == 0) return 0;
     EH_REQUIRE(Q && O && k_pages && v_pages && table && offsets && lengths, "paged_attention: NULL tensor");
+    EH_REQUIRE(!eh_rows_overlap(Q, ldq, (long long)q_heads * head_dim, O, ldo, (long long)q_heads * head_dim, rows), "paged_attention: the output lies on the queries");
     EH_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "paged_attention: the cache is not aligned to 16 bytes");
     EH_TRY(use_device(dev));
     AttendParams p;

@@ -78,6 +78,16 @@ int attention_setup_device(int dev);
 #define EH_NOT_CAPTURING(dev, what)                                                                                   \
     EH_REQUIRE(!eddlhip::state(dev).capturing, "%s is not possible between eddlhip_graph_begin and eddlhip_graph_end", what)
 
+// Whether rows of `width_a` floats, `ld_a` apart, share memory with rows of `width_b` floats (both `rows` of them); columns of one wider tensor do not.
+static inline bool eh_rows_overlap(const float *a, long long ld_a, long long width_a, const float *b, long long ld_b, long long width_b, long long rows) {
+    if (!a || !b || rows <= 0) return false;
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)b, a1 = a0 + 4 * ((rows - 1) * ld_a + width_a), b1 = b0 + 4 * ((rows - 1) * ld_b + width_b);
+    if (a1 <= b0 || b1 <= a0) return false;
+    if (ld_a != ld_b) return true;
+    const long long pitch = 4 * ld_a, off = (((long long)b0 - (long long)a0) % pitch + pitch) % pitch;  // of b's rows in a's
+    return off < 4 * width_a || off + 4 * width_b > pitch;
+}
+
 static inline unsigned eh_blocks(size_t work, unsigned per_block, unsigned cap = 1u << 20) {
     size_t b = (work + per_block - 1) / per_block;
     if (b < 1) b = 1;

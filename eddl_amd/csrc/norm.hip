@@ -176,7 +176,10 @@ extern "C" int eddlhip_norm_residual(int dev, const float *X, long long ldx, con
         EH_REQUIRE(out != X || (out == S ? lds : ldh) == ldx, "norm_residual: in place, but with rows of another length");
         EH_REQUIRE(!out || out != R || (out == S ? lds : ldh) == ldr, "norm_residual: in place, but with rows of another length");
     }
-    EH_REQUIRE(!S || S != H, "norm_residual: the sum and the norm of it share their rows");
+    for (const float *out : {S, H})
+        for (const float *in : {X, R})
+            EH_REQUIRE(out == in || !eh_rows_overlap(out, out == S ? lds : ldh, cols, in, in == X ? ldx : ldr, cols, rows), "norm_residual: an output lies on a part of an input");
+    EH_REQUIRE(!eh_rows_overlap(S, lds, cols, H, ldh, cols, rows), "norm_residual: the sum and the norm of it share their rows");
     EH_TRY(use_device(dev));
     NormParams p;
     p.X = X;

@@ -232,6 +232,7 @@ int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long l
                "rotary_axes: rows of %lld and %lld floats do not hold %d heads of %d", ldx, ldy, heads, head_dim);
     if (rows == 0) return 0;
     EH_REQUIRE(X && Y, "rotary_axes: NULL tensor");
+    EH_REQUIRE(X == Y || !eh_rows_overlap(X, ldx, (long long)heads * head_dim, Y, ldy, (long long)heads * head_dim, rows), "rotary_axes: the output lies on a part of the input");
     EH_REQUIRE(X != Y || ldx == ldy, "rotary_axes: in place, but rows of %lld and %lld floats", ldx, ldy);
     EH_TRY(use_device(dev));
     const int vec = aligned16(X, ldx) && aligned16(Y, ldy);
@@ -263,6 +264,9 @@ int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, lo
     if (rows == 0 || seqs == 0) return 0;
     EH_REQUIRE(K && V && k_pages && v_pages && table && offsets && lengths, "paged_append: NULL tensor");
     EH_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "paged_append: the cache is not aligned to 16 bytes");
+    const long long q_width = (long long)q_heads * head_dim, kv_width = (long long)kv_heads * head_dim;
+    EH_REQUIRE((Q == Qout || !eh_rows_overlap(Q, ldq, q_width, Qout, ldo, q_width, rows)) && !eh_rows_overlap(K, ldk, kv_width, Qout, ldo, q_width, rows) &&
+                   !eh_rows_overlap(V, ldv, kv_width, Qout, ldo, q_width, rows), "paged_append: the turned queries lie on a part of what is read");
     EH_REQUIRE(Q != Qout || ldq == ldo, "paged_append: queries in place, but rows of %lld and %lld floats", ldq, ldo);
     EH_TRY(use_device(dev));
     AppendParams p;

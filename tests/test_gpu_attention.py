@@ -91,6 +91,24 @@ def test_attention_of_long_chunks(hip, dtype, dim, heads, kv_heads):
     _check(hip, rng, [200], [333], heads, kv_heads, dim, 64, dtype, True, 50)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_in_many_parts(hip, dtype, dim):
+    """One key head and one sequence of 40000 tokens: more parts than the last workgroup joins; and chunks in parts over it."""
+    rng = np.random.default_rng(dim)
+    _check(hip, rng, [1], [40000], 3, 1, dim, 256, dtype, True, 0)
+    _check(hip, rng, [40], [3000], 1, 1, dim, 64, dtype, True, 0)
+    _check(hip, rng, [20, 3], [3000, 700], 2, 1, dim, 64, dtype, False, 0)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_attention_of_chunks_of_all_lengths(hip, dtype):
+    """Long and short chunks, and sequences without new tokens, in one call: tiles that are not there."""
+    rng = np.random.default_rng(23)
+    _check(hip, rng, [200, 3, 0, 5, 60, 1, 129], [210, 300, 40, 5, 333, 1, 200], 4, 2, 64, 32, dtype, True, 0)
+    _check(hip, rng, [1, 140, 2], [90, 200, 400], 2, 2, 96, 32, dtype, False, 70)
+
+
 def test_attention_beyond_the_bounds(hip):
     """max_new and max_length too small size the launch too small, never the result."""
     rng = np.random.default_rng(0)
@@ -295,7 +313,7 @@ def test_attention_pages_past_4_gib_elements(hip):
     for i, p in enumerate(pool.table[0]):
         for t, x in ((cache.keys, pool.k), (cache.values, pool.v)):
             bits = np.ascontiguousarray(bf16_bits(x[p * per:(p + 1) * per]))
-            hip._check(hip.lib.eddlhip_memcpy_h2d(hip.dev, t.ptr + 2 * per * int(table[0, i]), bits.ctypes.data, bits.nbytes))
+            hip._check(hip.lib.eddlhip_memcpy_h2d(hip.dev, t.address + 2 * per * int(table[0, i]), bits.ctypes.data, bits.nbytes))
     q = rng.standard_normal((3, kv * dim), dtype=np.float32)
     want, tol = attention(q, pool, kv, dim ** -0.5, True, 0)
     batch = PagedBatch(hip.array(table, "int32"), hip.array(pool.offsets, "int32"), hip.array(np.array([300]), "int32"), 3, 300)
@@ -547,6 +565,34 @@ def test_recorded_steps_follow_the_batch(hip):
             assert same, i
             assert all(np.array_equal(x.numpy(), y.numpy()) for x, y in ((cache.keys, other.keys), (cache.values, other.values)))
         del graph
+
+
+def test_graphs_that_share_the_workspace(hip):
+    """Two recorded calls whose parts lie in the same workspace, replayed in turn with an eager third between them, several times."""
+    rng = np.random.default_rng(24)
+    calls = []
+    for news, lengths, heads, kv, dim, dtype in (([1, 1], [3000, 700], 4, 2, 128, "bfloat16"), ([1], [40000], 3, 1, 64, "bfloat16"), ([40], [2500], 2, 1, 64, "float32")):
+        pool = Pool(rng, news, lengths, kv, dim, 64, dtype)
+        cache, batch = pool.on(hip)
+        Q = hip.array(rng.standard_normal((pool.rows, heads * dim)))
+        O = hip.empty(Q.shape)
+        run = lambda Q=Q, O=O, cache=cache, batch=batch: hip.paged_attention(Q, O, cache, batch)
+        run()
+        calls.append((run, O, O.numpy()))
+    for run, _, _ in calls:  # (the workspace has its size)
+        run()
+    graphs = [hip.record(run) for run, _, _ in calls[:2]]
+    for _ in range(4):
+        for _, O, _ in calls:
+            hip.fill_(O, -7.0)
+        graphs[0].launch()
+        calls[2][0]()
+        graphs[1].launch()
+        graphs[0].launch()
+        for _, O, want in calls:
+            same = np.array_equal(O.numpy(), want)
+            assert same
+    del graphs
 
 
 def test_on_a_stream_of_the_callers(hip):
