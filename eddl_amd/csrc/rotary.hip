@@ -173,24 +173,25 @@ __global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const
             put4(p.k_pages, t + (c.d0 >> 3) * 128 + (c.d0 & 7), x, p.f32);
             if (c.d1 >= 0) put4(p.k_pages, t + (c.d1 >> 3) * 128 + (c.d1 & 7), y, p.f32);
         }
-        const int v_lo = max(head_lo - q_items - p.kv_heads, 0), v_hi = head_hi - q_items - p.kv_heads, v_work = max(0, v_hi - v_lo) * 4 * D;
-        for (int i = threadIdx.x; i < v_work; i += TPB) {  // four tokens of a dimension
-            const int rest = i / D, d = i - rest * D, quarter = rest & 3, kv = v_lo + (rest >> 2), at = 4 * quarter - t0;  // (row of the block's token 4 quarter)
-            if (at + 4 <= 0 || at >= n_rows) continue;
-            const float *src = p.V + (size_t)kv * D + d;
-            floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int v_lo = max(head_lo - q_items - p.kv_heads, 0), v_hi = head_hi - q_items - p.kv_heads, v_work = max(0, v_hi - v_lo) * 2 * D;
+        for (int i = threadIdx.x; i < v_work; i += TPB) {  // eight tokens of a dimension: theirs are the places side by side
+            const int rest = i / D, d = i - rest * D, half = rest & 1, kv = v_lo + (rest >> 1), at = 8 * half - t0;  // (row of the half's first token)
+            if (at + 8 <= 0 || at >= n_rows) continue;
+            const float *src = p.V + (long long)(row0 + first + at) * p.ldv + (long long)kv * D + d;
+            float x[8];
+            const size_t t = block * 16 * D + kv * head_stride + (size_t)half * 8 * D + d * 8;
+            if (at >= 0 && at + 8 <= n_rows) {
 #pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (at + k >= 0 && at + k < n_rows) x[k] = src[(size_t)(row0 + first + at + k) * p.ldv];
-            const size_t t = block * 16 * D + kv * head_stride + (size_t)(quarter >> 1) * 8 * D + d * 8 + (quarter & 1) * 4;
-            if (at >= 0 && at + 4 <= n_rows) {
-                put4(p.v_pages, t, x, p.f32);
+                for (int k = 0; k < 8; k++) x[k] = src[k * p.ldv];
+                put4(p.v_pages, t, floatx4{x[0], x[1], x[2], x[3]}, p.f32);
+                put4(p.v_pages, t + 4, floatx4{x[4], x[5], x[6], x[7]}, p.f32);
             } else {
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int k = 0; k < 8; k++)
                     if (at + k >= 0 && at + k < n_rows) {
-                        if (p.f32) ((float *)p.v_pages)[t + k] = x[k];
-                        else ((unsigned short *)p.v_pages)[t + k] = (unsigned short)split_round(x[k], x[k]);
+                        const float v = src[k * p.ldv];
+                        if (p.f32) ((float *)p.v_pages)[t + k] = v;
+                        else ((unsigned short *)p.v_pages)[t + k] = (unsigned short)split_round(v, v);
                     }
             }
         }
