@@ -5,7 +5,8 @@
 // A row stays in registers between its sums and its outputs: a wavefront a row up to 1024 columns, workgroups of 4 to 16
 // wavefronts beyond.  Means and variances are fp32 sums over the registers; the variance is that of the differences from the mean, a
 // second pass over registers that costs no memory.
-// Bound: memory, 16 bytes a number (x, r, s, h).
+// Bound: memory, 16 bytes a number (x, r, s, h).  12544 x 2048 with two RMS norms, gate, shift and scale: 94 us, 4.4 TB/s; 50000 x 1000 with two layer
+// norms 159 us, 5.0 TB/s; 12544 x 512 17.5 us, 5.9 TB/s (partly from the last-level cache).
 #include <math.h>
 
 #include <algorithm>
@@ -72,6 +73,17 @@ __device__ __forceinline__ void set4(float *p, int c, int cols, floatx4 v) {
 template <int THREADS, int NV, bool VEC>
 __device__ __forceinline__ void normed(const Norm &n, floatx4 (&x)[NV], int t, int cols, float *red) {
     if (n.kind == EDDLHIP_NORM_NONE) return;
+    // (short rows: weight and bias are on their way while the sums are formed)
+    constexpr bool AHEAD = THREADS == 64 && NV <= 2;
+    floatx4 w[AHEAD ? NV : 1], b[AHEAD ? NV : 1];
+    if constexpr (AHEAD) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = 4 * (i * THREADS + t);
+            if (c < cols && n.w) w[i] = get4<VEC>(n.w, c, cols);
+            if (c < cols && n.b) b[i] = get4<VEC>(n.b, c, cols);
+        }
+    }
     float mean = 0.0f;
     if (n.kind == EDDLHIP_NORM_LAYER) {
         float sum = 0.0f;
@@ -95,8 +107,13 @@ __device__ __forceinline__ void normed(const Norm &n, floatx4 (&x)[NV], int t, i
         const int c = 4 * (i * THREADS + t);
         if (c < cols) {
             x[i] *= scale;
-            if (n.w) x[i] *= get4<VEC>(n.w, c, cols);
-            if (n.b) x[i] += get4<VEC>(n.b, c, cols);
+            if constexpr (AHEAD) {
+                if (n.w) x[i] *= w[i];
+                if (n.b) x[i] += b[i];
+            } else {
+                if (n.w) x[i] *= get4<VEC>(n.w, c, cols);
+                if (n.b) x[i] += get4<VEC>(n.b, c, cols);
+            }
         }
     }
 }
