@@ -245,7 +245,7 @@ __device__ __forceinline__ int part_at(int steps, int n, int parts) {
 // the one that completes the count joins the parts, in groups that the shape alone fixes.  Nobody waits for another, and the
 // bits do not depend on who comes last.  A launch less: one token over 4096 28.6 -> 20.7 us.
 // Many rows, or more parts, are joined by a launch of their own, which the whole device works on (4 x 196 rows of 8 heads in 6 parts: 9 us
-// where the last workgroups took 19).  Rows that the launch did not count on (beyond q_tiles) are not divided.
+// where the last workgroups took 19).  Where the last workgroup joins, rows that the launch did not count on (beyond q_tiles) are not divided.
 constexpr int MAX_COUNTS = 1024;  // divided launches have no more row tiles: two workgroups a tile fill the device
 static __device__ unsigned part_counts[MAX_COUNTS];
 
@@ -421,7 +421,7 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
     const int *pages = p.table + (size_t)seq * p.width;
 
     for (int tile = blockIdx.x / p.splits; tile * COLS < rows; tile += p.q_tiles) {
-        const bool counted = tile < p.q_tiles;
+        const bool counted = tile < p.q_tiles || p.splits > JOIN_HERE;  // (a launch joins the parts of all rows)
         if (!counted && own_split != 0) break;
         const int split = counted ? own_split : 0, splits = counted ? p.splits : 1;
         const int row_lo = tile * COLS, row_hi = min(rows, row_lo + COLS);
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
 }
 
 // ------------------------------------------------------------------------------------------------ many rows
-// A workgroup takes 128 rows, 32 a wavefront, and walks through its part of the tokens 32 at a time, which all four wavefronts read
+// A workgroup takes 128 or 256 rows, 32 a wavefront, and walks through its part of the tokens 32 at a time, which all its wavefronts read
 // from LDS.  Bound by the matrix instruction, so its operands are pairs of fp16 numbers here and not three bf16 numbers:
 // x 2^e = hi + lo, hi = fp16(x 2^e), lo = fp16(x 2^e - hi), with e such that the largest number of a row of queries, or of 16 tokens'
 // keys or values of a head, lies in 2^14 .. 2^15.  Each half brings 11 bits and its sign: a pair is off by at most 2^-23 of x, or, where
@@ -666,13 +666,14 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
 // factors, and the blocks' exponents of values into the weights: a weight is exp2(s - m + c) with c = 14 + (the block's exponent) - (the largest so
 // far), the output carries the largest, a whole number of doublings like m.  (14: weights of 2^-28 still have eleven bits in hi.)
 // A block whose largest number is infinite takes a NaN as its factor, so that its rows are computed again.
-// Tiles: a wavefront brings the keys or the values of 16 tokens, their numbers go through its registers (the largest, the pairs) into LDS;
+// Tiles: each of the first four wavefronts brings the keys or the values of 16 tokens, their numbers go through its registers (the largest, the pairs) into LDS;
 // two tiles, one filled while the other is used, one barrier a tile.  The cache's order is the operands' order: every LDS
 // access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
-// Measured: 2048 tokens over 8192, 32 and 8 heads of 128, bf16 cache: 545 us, 440 TFLOP/s, 880 on the matrix instructions (42 % of the cycles
-// busy; the vector instructions fill 57 % and the two do not overlap: a version that computed the next tile's scores beside the
+// Eight wavefronts (two on each SIMD, one of which brings tiles) halve that work for a row: 2048 tokens over 8192, 32 and 8 heads of 128, bf16
+// 561 -> 516 us, 4 x 1000 over 2000, heads of 64 102 -> 86; but a ragged batch has more empty rows in tiles of 256 (35 -> 44 us).
+// Measured: 2048 tokens over 8192, 32 and 8 heads of 128, bf16 cache: 516 us, 466 TFLOP/s, 930 on the matrix instructions (with four
+// wavefronts 42 % of the cycles busy; the vector instructions fill 57 % and the two do not overlap: a version that computed the next tile's scores beside the
 // weights in one block, with the scheduler's groups, spilled and took 890).  As three bf16 parts with tiles loaded straight into LDS 621 us.
-constexpr int CHUNK_ROWS = 128;
 constexpr int CHUNK_SPLITS = 64;  // most parts of a length
 
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
@@ -744,9 +745,9 @@ __device__ __forceinline__ floatx16 multiply(const uintx4 (&a)[NP], const Pair &
 }
 
 // FULL: head_dim is DP; otherwise the dimensions past the last are zeros in LDS.  grid: a multiple of 8 workgroups
-template <int DP, bool F32, bool FULL>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
-    constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 2 : 1, UNITS = 4 * DP, EACH = DP / 32;  // units: 8 numbers of a tile's keys or values
+template <int DP, bool F32, bool FULL, int W>
+__global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
+    constexpr int KS = DP / 16, DT = DP / 32, NP = F32 ? 2 : 1, UNITS = 4 * DP, EACH = DP / 32, ROWS = 32 * W;  // units: 8 numbers of a tile's keys or values
     __shared__ uintx4 kv[2][2][NP][UNITS];
     __shared__ float scales[2][4];  // of a tile's two blocks: keys' factors, values' powers of two
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, half = lane >> 5;
@@ -756,28 +757,26 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
     const int per = (total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
     const int vid = p.grouped ? (blockIdx.x % EDDLHIP_NUM_XCD) * per + blockIdx.x / EDDLHIP_NUM_XCD : blockIdx.x;
     if (vid >= total) return;
-    const int own_split = vid % p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
+    const int split = vid % p.splits, splits = p.splits, rest = vid / p.splits, of_head = rest / p.q_tiles, kv_head = of_head % p.kv_heads, seq = of_head / p.kv_heads;
     const Sequence q = sequence_of(p, seq);
     const int rows = q.fresh * p.group;
     const int *pages = p.table + (size_t)seq * p.width;
     // K's lane order: row col of the product is token `k_token` of the tile
     const int a8 = col >> 3, k_token = 16 * (a8 >> 1) + 8 * ((col >> 2) & 1) + 4 * (a8 & 1) + (col & 3);
     const int k_unit = (k_token >> 4) * 2 * DP + half * 16 + (k_token & 15);
-    const int values = wave >> 1, block = wave & 1;  // what this wavefront brings of a tile
+    const int values = wave >> 1 & 1, block = wave & 1;  // what this wavefront brings of a tile (the first four do)
+    const bool brings = W == 4 || wave < 4;
 
     if constexpr (!FULL) {
-        for (int i = tid; i < 2 * 2 * NP * UNITS; i += 256) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
+        for (int i = tid; i < 2 * 2 * NP * UNITS; i += 64 * W) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
     }
 
-    for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * CHUNK_ROWS < rows; tile += p.q_tiles) {
-        const bool counted = tile < p.q_tiles;
-        if (!counted && own_split != 0) break;
-        const int split = counted ? own_split : 0, splits = counted ? p.splits : 1;
-        const Range all = range_of(p, q, tile * CHUNK_ROWS, min(rows, (tile + 1) * CHUNK_ROWS));
+    for (int tile = p.q_tiles - 1 - rest % p.q_tiles; tile * ROWS < rows; tile += p.q_tiles) {
+        const Range all = range_of(p, q, tile * ROWS, min(rows, (tile + 1) * ROWS));
         const int steps_all = max(0, (all.hi - all.lo + TILE_KV - 1) / TILE_KV);
         const int step_lo = part_at(steps_all, split, splits), step_hi = part_at(steps_all, split + 1, splits);
         const int lo = all.lo + step_lo * TILE_KV, hi = min(all.hi, all.lo + step_hi * TILE_KV);
-        const int row_lo = min(rows, tile * CHUNK_ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
+        const int row_lo = min(rows, tile * ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
         const bool works = row_lo < row_hi;
         const Range range = works ? range_of(p, q, row_lo, row_hi) : Range{0, 0, 0, 0};
 
@@ -832,7 +831,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
                 }
             }
         };
-        if (lo < hi) fetch(lo);
+        if (brings && lo < hi) fetch(lo);
 
         // ---- queries
         const int row = works ? min(row_lo + col, row_hi - 1) : 0, token = row / p.group, head = kv_head * p.group + row % p.group;
@@ -880,7 +879,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
         const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
 
         __syncthreads();  // (the tile of rows before has read its last operands; zeros are in place)
-        if (lo < hi) {
+        if (brings && lo < hi) {
             place(lo, 0);
             if (lo + TILE_KV < hi) fetch(lo + TILE_KV);
         }
@@ -956,7 +955,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void attend_chunk_kernel(co
                     }
                 }
             }
-            if (j0 + TILE_KV < hi) {
+            if (brings && j0 + TILE_KV < hi) {
                 place(j0 + TILE_KV, buf ^ 1);
                 if (j0 + 2 * TILE_KV < hi) fetch(j0 + 2 * TILE_KV);
             }
@@ -1075,10 +1074,13 @@ void launch_few(const AttendParams &p, bool f32, int nq, dim3 grid, hipStream_t 
 }
 
 template <int DP, bool FULL>
-void launch_chunk(const AttendParams &p, bool f32, int total, hipStream_t st) {
+void launch_chunk(const AttendParams &p, bool f32, int waves, int total, hipStream_t st) {
+    typedef void (*kernel)(AttendParams, int);
+    constexpr int MOST = DP <= 128 ? 8 : 4;
+    static const kernel kernels[2][2] = {{attend_chunk_kernel<DP, false, FULL, 4>, attend_chunk_kernel<DP, false, FULL, MOST>},
+                                         {attend_chunk_kernel<DP, true, FULL, 4>, attend_chunk_kernel<DP, true, FULL, MOST>}};
     const dim3 grid((total + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD);
-    if (f32) hipLaunchKernelGGL((attend_chunk_kernel<DP, true, FULL>), grid, dim3(256), 0, st, p, total);
-    else hipLaunchKernelGGL((attend_chunk_kernel<DP, false, FULL>), grid, dim3(256), 0, st, p, total);
+    hipLaunchKernelGGL(kernels[f32][waves == 8], grid, dim3(64 * waves), 0, st, p, total);
 }
 
 }  // namespace
@@ -1143,17 +1145,20 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     p.scale = scale * 1.44269504088896340736f;
     // The launch goes by the bounds max_new and max_length; what is beyond them is still computed, by the same wavefronts.
     const long long fresh = std::min(max_new > 0 ? max_new : 1, rows), tile_rows = fresh * p.group;
-    const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0, per_tile = nq ? 16 * nq : CHUNK_ROWS;
+    const int nq = tile_rows <= 16 ? 1 : tile_rows <= 32 ? (head_dim <= 128 ? 2 : 1) : 0;
+    // (the rows fill the tiles of all sequences, but for one begun tile each)
+    const bool even = ((long long)rows * p.group) / 128 + seqs >= (tile_rows + 127) / 128 * seqs;
+    const int waves = head_dim <= 128 && tile_rows > 128 && even ? 8 : 4, per_tile = nq ? 16 * nq : 32 * waves;
     const long long tiles = (tile_rows + per_tile - 1) / per_tile;
     p.q_tiles = (int)tiles;
     // (sequences of fewer new tokens than max_new have fewer tiles, all together no more than their rows fill and one begun tile each)
-    const long long groups = tiles * kv_heads * seqs, filled = kv_heads * std::min(tiles * seqs, ((long long)rows * p.group) / per_tile + seqs), want = (nq ? few_groups(head_dim, cache_type == EDDLHIP_CACHE_F32, nq) : 2LL) * state(dev).num_cu;
+    const long long groups = tiles * kv_heads * seqs, filled = kv_heads * std::min(tiles * seqs, ((long long)rows * p.group) / per_tile + seqs), want = (nq ? few_groups(head_dim, cache_type == EDDLHIP_CACHE_F32, nq) : 8LL / waves) * state(dev).num_cu;
     long long seen = max_length > 0 ? max_length : 1;
     if (window > 0) seen = std::min<long long>(seen, (long long)window + fresh);
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
     p.splits = (int)std::max(1LL, std::min({want / filled, steps / (nq ? 8 : 4), (long long)(nq ? FEW_SPLITS / nq : CHUNK_SPLITS)}));
     if (nq && groups > MAX_COUNTS) p.splits = 1;
-    p.grouped = filled == groups;
+    p.grouped = even;
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
@@ -1170,7 +1175,7 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     const int total = (int)(groups * p.splits);
     auto launch = [&](auto size, auto full) {
         if (nq) launch_few<size(), full()>(p, f32, nq, grid, st);
-        else launch_chunk<size(), full()>(p, f32, total, st);
+        else launch_chunk<size(), full()>(p, f32, waves, total, st);
     };
     auto sized = [&](auto size) {
         if (head_dim == size()) launch(size, std::true_type());

@@ -5,7 +5,7 @@
 // A row stays in registers between its sums and its outputs: a wavefront a row up to 1024 columns, workgroups of 4 to 16
 // wavefronts beyond.  Means and variances are fp32 sums over the registers; the variance is that of the differences from the mean, a
 // second pass over registers that costs no memory.
-// Bound: memory, 16 bytes a number (x, r, s, h).  12544 x 2048 with two RMS norms, gate, shift and scale: 94 us, 4.4 TB/s; 50000 x 1000 with two layer
+// Bound: memory, 16 bytes a number (x, r, s, h).  12544 x 2048 with two RMS norms, gate, shift and scale: 91 us, 4.5 TB/s; 50000 x 1000 with two layer
 // norms 159 us, 5.0 TB/s; 12544 x 512 17.5 us, 5.9 TB/s (partly from the last-level cache).
 #include <math.h>
 

@@ -115,6 +115,12 @@ def test_attention_beyond_the_bounds(hip):
     for dtype in ("float32", "bfloat16"):
         _check(hip, rng, [200, 3], [250, 300], 4, 2, 64, 32, dtype, True, 0, max_new=1, max_length=1)
         _check(hip, rng, [3, 4], [250, 30], 4, 2, 64, 32, dtype, True, 0, max_new=900, max_length=100000)
+        # tiles of many rows beyond those that the launch has, undivided beside divided ones
+        _check(hip, rng, [300, 10], [1500, 700], 4, 2, 64, 32, dtype, True, 0, max_new=150)
+        _check(hip, rng, [300, 300], [900, 300], 2, 2, 80, 32, dtype, False, 100, max_new=40)
+        # the same of few rows, in parts that the last workgroup or a launch joins
+        _check(hip, rng, [50, 1], [1100, 600], 2, 2, 64, 32, dtype, True, 0, max_new=2)
+        _check(hip, rng, [20], [41000], 1, 1, 64, 256, dtype, True, 0, max_new=1)
 
 
 def test_attention_large_scores(hip):
