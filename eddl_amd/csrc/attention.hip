@@ -707,14 +707,15 @@ __device__ __forceinline__ Pair pair8(const float (&x)[8]) {
     }
     return r;
 }
-// Factor 2^(14 - exponent) of numbers whose largest magnitude is given by its bits, its inverse, and that as a power of two.
+// Factor 2^(14 - exponent) of numbers whose largest magnitude is given by its bits, its inverse, and that as a power of two.  Numbers below 2^-112
+// take the exponent of 2^-112, and so do blocks of zeros (tokens behind the last one among them): their power is the lowest and never raises another's.
 struct Scale {
     float up, down, power;
 };
 __device__ __forceinline__ Scale scale_of(unsigned bits) {
     unsigned e = bits >> 23;
     const bool whole = e < 255u;
-    e = bits == 0u ? 141u : max(e, 15u);
+    e = max(e, 15u);
     Scale s;
     s.up = whole ? __builtin_bit_cast(float, (268u - e) << 23) : 1.0f;
     s.down = whole ? __builtin_bit_cast(float, (e - 14u) << 23) : __builtin_nanf("");
