@@ -19,10 +19,11 @@
 // The cache is kept in the order in which these operands are read (eddlhip.h): a lane's operand is 16 (32) bytes side by side, and
 // the lanes' operands are side by side too.
 //
-// Infinities and NaN: what is not visible has no influence.  Masked scores are replaced, values behind the last token are
-// replaced by zeros; a NaN or infinity in a visible or masked place of a tile otherwise reaches the sums as NaN (0 * inf, or the parts
-// of an infinity), and rows whose sums are not finite are computed again one token at a time (attend_row_again), with what
-// the formula gives.
+// What is not visible has no influence beyond fp32 rounding.  Masked scores are replaced, values that no row of a tile sees are
+// replaced by zeros.  Other numbers share exponents with their neighbours in the kernel of many rows: rows that lose bits by that are computed
+// again in fp32 (attend_rows_fp32).  A NaN or infinity in a visible or masked place of a tile otherwise reaches the sums as NaN (0 * inf, or the
+// parts of an infinity), and rows whose sums are not finite are computed again one token at a time (attend_row_again), with
+// what the formula gives.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -221,6 +222,7 @@ __device__ void attend_row_again(const AttendParams &p, const Sequence &q, int s
 // The tokens that any row of a tile sees, and the bounds that all of them share.
 struct Range {
     int lo, hi;            // tokens of the tile's rows (lo on a boundary of TILE_KV)
+    int first;             // the first of them, where it is
     int all_lo, all_hi;    // every row sees [all_lo, all_hi)
 };
 __device__ __forceinline__ Range range_of(const AttendParams &p, const Sequence &q, int row_lo, int row_hi) {
@@ -228,9 +230,9 @@ __device__ __forceinline__ Range range_of(const AttendParams &p, const Sequence 
     Range r;
     r.hi = p.causal ? min(q.length, last + 1) : q.length;
     r.all_hi = p.causal ? min(q.length, first + 1) : q.length;
-    r.lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    r.first = p.window > 0 ? max(0, first - p.window + 1) : 0;
     r.all_lo = p.window > 0 ? max(0, last - p.window + 1) : 0;
-    r.lo &= ~(TILE_KV - 1);
+    r.lo = r.first & ~(TILE_KV - 1);
     return r;
 }
 
@@ -661,11 +663,12 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
 // x 2^e = hi + lo, hi = fp16(x 2^e), lo = fp16(x 2^e - hi), with e such that the largest number of a row of queries, or of 16 tokens'
 // keys or values of a head, lies in 2^14 .. 2^15.  Each half brings 11 bits and its sign: a pair is off by at most 2^-23 of x, or, where
 // lo runs out of fp16's range, by 2^-25 of 2^-14 of the largest number, 2^-39.  A bf16 number is its own hi down to 2^-31 of the largest.
-// Two pairs take three products (lo lo is below 2^-24 of the whole), a pair and a bf16 number two, where the bf16 parts take six and
+// Two pairs take three products (lo lo is left out), a pair and a bf16 number two, where the bf16 parts take six and
 // three; and a pair costs 4 instructions for two numbers where three parts cost 11.  The rows' and blocks' exponents go into the scores as
 // factors, and the blocks' exponents of values into the weights: a weight is exp2(s - m + c) with c = 14 + (the block's exponent) - (the largest so
 // far), the output carries the largest, a whole number of doublings like m.  (14: weights of 2^-28 still have eleven bits in hi.)
-// A block whose largest number is infinite takes a NaN as its factor, so that its rows are computed again.
+// A block whose largest number is infinite takes a NaN as its factor, so that its rows are computed again.  (lo lo: each lo is 2^-11 of its number at
+// most, their product 2^-22 of the whole; of numbers whose bits are even by chance 2^-25, with either sign.)
 // Tiles: each of the first four wavefronts brings the keys or the values of 16 tokens, their numbers go through its registers (the largest, the pairs) into LDS;
 // two tiles, one filled while the other is used, one barrier a tile.  The cache's order is the operands' order: every LDS
 // access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
@@ -745,6 +748,86 @@ __device__ __forceinline__ floatx16 multiply(const uintx4 (&a)[NP], const Pair &
     return mfma(a[0], b.hi, c);
 }
 
+// Where shared exponents end.  A number that is small beside the largest of its row or block is off by 2^-39 of that largest one:
+//   scores  by D f 2^-9 doublings at most, f their factor.  Up to f D = 2^-10 (products of the largest numbers of 2^20) that is 2^-19, and 2^-24 as
+//           the errors of many numbers add up;
+//   values  by 2^-39 of the largest value that the wavefront met, for every token (weights below 2^-28 have no more bits than that).  Where the
+//           largest sum of the row is 2^-12 of it or more, that is 2^-27 of the sum a token and, as errors add up, 2^-23 for thousands.
+// Rows beyond (a hidden token, or one without weight, is thousands of times larger than what the row's result consists of) are computed
+// again by attend_rows_fp32, 32 together.
+constexpr float SCORES_SPREAD = 0x1p-10f, LEAST_POWER = -126.0f;
+constexpr int VALUES_SPREAD = 12;
+
+// The rows of a wavefront over [lo, hi) on the fp32 matrix instruction, operands straight from memory: no exponents are shared and nothing is split, so a
+// row has the errors of the formula in fp32 whatever stands beside it.  The instruction takes two dimensions (tokens) where the fp16
+// one takes sixteen, and nothing is asked for ahead: 2048 tokens over 8192 (bf16) with all rows again 3550 us, without 506.
+template <int DT, bool F32, bool FULL>
+__device__ __forceinline__ void attend_rows_fp32(const AttendParams &p, const Sequence &q, const int *pages, int kv_head, const float *q_row, const Range &range, int lo, int hi,
+                                                 int see_lo, int see_hi, int k_token, floatx16 (&o)[DT], float &m, float &l) {
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, D = FULL ? 32 * DT : p.D;
+#pragma unroll
+    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
+    m = NEG_INF;
+    l = 0.0f;
+    const int to = min(hi, range.hi);
+#pragma unroll 1
+    for (int j0 = max(lo, range.lo); j0 < to; j0 += TILE_KV) {
+        bool bad[2] = {false, false};
+        size_t base[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) base[b] = block_base(p, pages[min(j0 + 16 * b, to - 1) >> p.page_shift], (j0 >> 4) + b, kv_head, bad[b]);
+        floatx16 s;
+#pragma unroll
+        for (int r = 0; r < 16; r++) s[r] = 0.0f;
+        const size_t k_from = (k_token >> 4 ? base[1] : base[0]) + (k_token & 15) * 8 + half * 128;
+#pragma unroll 1
+        for (int ks = 0; 16 * ks < D; ks++) {
+            Raw<F32> raw;
+            float k[8], x[8];
+            raw.load(p.K, k_from + ks * 256);
+            raw.numbers(k);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = q_row[16 * ks + 8 * half + i] * p.scale;
+#pragma unroll
+            for (int i = 0; i < 8; i++) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i], x[i], s, 0, 0, 0);
+        }
+        float top = m;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int j = j0 + 16 * (r >> 3) + 8 * half + (r & 7);
+            s[r] = j >= see_lo && j < see_hi && j < to ? (bad[r >> 3] ? __builtin_nanf("") : s[r]) : NEG_INF;
+            top = fmaxf(top, s[r]);
+        }
+        top = larger_half(top);
+        const float keep = m == NEG_INF ? 0.0f : power2(m - top), from = top == NEG_INF ? 0.0f : top;
+        l *= keep;
+        m = top;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[r] = power2(s[r] - from);
+            l += s[r];
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            o[dt] *= keep;
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                Raw<F32> raw;
+                float v[8];
+                raw.load(p.V, base[b] + (size_t)half * 8 * D + (FULL ? 32 * dt + col : min(32 * dt + col, D - 1)) * 8);
+                raw.keep(j0 + 16 * b + 16 <= range.first ? 0 : to - (j0 + 16 * b + 8 * half));
+                raw.numbers(v);
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[i], s[8 * b + i], o[dt], 0, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    l += __shfl_xor(l, 32);
+}
+
 // FULL: head_dim is DP; otherwise the dimensions past the last are zeros in LDS.  grid: a multiple of 8 workgroups
 template <int DP, bool F32, bool FULL, int W>
 __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_chunk_kernel(const AttendParams p, const int total) {
@@ -766,7 +849,6 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
     const int a8 = col >> 3, k_token = 16 * (a8 >> 1) + 8 * ((col >> 2) & 1) + 4 * (a8 & 1) + (col & 3);
     const int k_unit = (k_token >> 4) * 2 * DP + half * 16 + (k_token & 15);
     const int values = wave >> 1 & 1, block = wave & 1;  // what this wavefront brings of a tile (the first four do)
-    const bool brings = W == 4 || wave < 4;
 
     if constexpr (!FULL) {
         for (int i = tid; i < 2 * 2 * NP * UNITS; i += 64 * W) kv[0][0][0][i] = uintx4{0u, 0u, 0u, 0u};
@@ -779,7 +861,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
         const int lo = all.lo + step_lo * TILE_KV, hi = min(all.hi, all.lo + step_hi * TILE_KV);
         const int row_lo = min(rows, tile * ROWS + 32 * wave), row_hi = min(rows, row_lo + 32);
         const bool works = row_lo < row_hi;
-        const Range range = works ? range_of(p, q, row_lo, row_hi) : Range{0, 0, 0, 0};
+        const Range range = works ? range_of(p, q, row_lo, row_hi) : Range{0, 0, 0, 0, 0};
 
         // ---- the tiles' way into LDS
         bool bad = false;  // of the block that is on its way
@@ -799,13 +881,13 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
                 if (FULL || 64 * i + lane < 2 * D) raw[i].load(src, base + (size_t)(64 * i + lane) * 8);
         };
         auto place = [&](int j0, int buf) __attribute__((always_inline)) {
-            const int from = j0 + 16 * block;
-            if (from + 16 > q.length) {  // nothing behind the last token counts
+            const int from = j0 + 16 * block, end = from + 16 <= all.first ? 0 : all.hi;
+            if (from + 16 > end) {  // what none of the tile's rows sees takes no part in the block's exponent
 #pragma unroll
                 for (int i = 0; i < EACH; i++) {
                     const int u = 64 * i + lane;
-                    if (values) raw[i].keep(q.length - (from + (u >= D ? 8 : 0)));
-                    else raw[i].keep(from + (u & 15) < q.length ? 8 : 0);
+                    if (values) raw[i].keep(end - (from + (u >= D ? 8 : 0)));
+                    else raw[i].keep(from + (u & 15) < end ? 8 : 0);
                 }
             }
             unsigned top = 0;
@@ -832,7 +914,8 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
                 }
             }
         };
-        if (brings && lo < hi) fetch(lo);
+        const int brings_to = W == 4 || wave < 4 ? hi : lo;  // (the first four wavefronts bring tiles; a bound, and no condition, keeps the loop's outputs in one place)
+        if (lo < brings_to) fetch(lo);
 
         // ---- queries
         const int row = works ? min(row_lo + col, row_hi - 1) : 0, token = row / p.group, head = kv_head * p.group + row % p.group;
@@ -877,12 +960,13 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
 #pragma unroll
             for (int r = 0; r < 16; r++) o[dt][r] = 0.0f;
         float m = NEG_INF, l = 0.0f, power = NEG_INF;  // power: the outputs' doublings, those of the largest values so far
+        float f_most = 0.0f;                           // the largest factor of the row's scores
         const int see_lo = p.window > 0 ? pos - p.window + 1 : 0, see_hi = p.causal ? min(q.length, pos + 1) : q.length;
 
         __syncthreads();  // (the tile of rows before has read its last operands; zeros are in place)
-        if (brings && lo < hi) {
+        if (lo < brings_to) {
             place(lo, 0);
-            if (lo + TILE_KV < hi) fetch(lo + TILE_KV);
+            if (lo + TILE_KV < brings_to) fetch(lo + TILE_KV);
         }
         __syncthreads();
         for (int j0 = lo, buf = 0; j0 < hi; j0 += TILE_KV, buf ^= 1) {
@@ -901,6 +985,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
                 const float f[2] = {fmaxf(scales[buf][0] * q_down, 0x1p-126f), fmaxf(scales[buf][1] * q_down, 0x1p-126f)};
                 const float poison = (scales[buf][0] - scales[buf][0]) + (scales[buf][1] - scales[buf][1]);  // 0, or NaN (the maximum above drops it)
                 const float powers[2] = {scales[buf][2], scales[buf][3]};
+                f_most = fmaxf(f_most, fmaxf(f[0], f[1]));
                 if (j0 < range.all_lo || j0 + TILE_KV > range.all_hi) {
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
@@ -956,9 +1041,9 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
                     }
                 }
             }
-            if (brings && j0 + TILE_KV < hi) {
+            if (j0 + TILE_KV < brings_to) {
                 place(j0 + TILE_KV, buf ^ 1);
-                if (j0 + 2 * TILE_KV < hi) fetch(j0 + 2 * TILE_KV);
+                if (j0 + 2 * TILE_KV < brings_to) fetch(j0 + 2 * TILE_KV);
             }
             __syncthreads();
         }
@@ -969,13 +1054,32 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
 #pragma unroll
             for (int r = 0; r < 16; r++) o[dt][r] = __builtin_amdgcn_ldexpf(o[dt][r], doublings);
 
+        // ---- rows whose numbers differ too much in size for shared exponents, and those that the next step concerns, in fp32
+        const bool sees = max(lo, see_lo) < min(hi, see_hi);
+        auto not_finite = [&]() __attribute__((always_inline)) {
+            float worst = l - l;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) worst += o[dt][r] - o[dt][r];
+            return worst != 0.0f || (m == NEG_INF && sees);
+        };
+        bool again = not_finite();
+        {
+            float most = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) most = fmaxf(most, fabsf(o[dt][r]));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            const bool lost = f_most * (float)D > SCORES_SPREAD || (power > LEAST_POWER && most < __builtin_amdgcn_ldexpf(1.0f, (int)power + 14 - VALUES_SPREAD));
+            if (__any((lost && sees) || again) && works && !q.bad) {
+                attend_rows_fp32<DT, F32, FULL>(p, q, pages, kv_head, p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D, range, lo, hi, see_lo, see_hi, k_token, o, m, l);
+                again = not_finite();
+            }
+        }
+
         // ---- rows whose sums are not finite, and rows that see tokens but no score above -inf, one by one
-        float worst = l - l;
-#pragma unroll
-        for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) worst += o[dt][r] - o[dt][r];
-        bool again = worst != 0.0f || (m == NEG_INF && max(lo, see_lo) < min(hi, see_hi));
         again = (again || q.bad) && row_lo + col < row_hi;
         unsigned long long todo = __ballot(again);
         todo = (todo | (todo >> 32)) & 0xffffffffull;

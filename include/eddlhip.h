@@ -527,9 +527,13 @@ int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, lo
 /* Attention of the new tokens over the cache: query head h of a row at place p reads key head h / (q_heads / kv_heads),
  *     s_j = scale q . k_j,   o = sum_j softmax(s)_j v_j   over the visible tokens
  * j < length, with causal != 0 also j <= p, with window > 0 also j > p - window.  A row that sees nothing is 0.  What is not
- * visible has no influence, infinities and NaN included; among visible tokens they come out as the formula brings them.
- * Both products have the accuracy of fp32 (sums of bf16 products, as the split form of the convolutions), softmax
- * and sums are fp32.  The cache's length may be divided over workgroups, whose parts are joined in the order of the tokens: the
+ * visible has no influence, infinities and NaN included, except that it may move a result by a rounding of fp32; among visible tokens
+ * they come out as the formula brings them.  Softmax and sums are fp32, both products have the accuracy of fp32: errors are those of
+ * fp32 arithmetic beside the largest number of a row's head, whatever the sizes of the numbers.  (Sequences of up to 32 rows a key
+ * head: sums of bf16 products, as the split form of the convolutions.  More: products of pairs of fp16 numbers that share an
+ * exponent with 16 tokens.  Where a row's scores or result are thousands of times smaller than numbers that it shares exponents with,
+ * 32 rows together are computed again on the fp32 matrix instruction, in about six times the time; rows that an infinity or NaN
+ * in their tile reaches are computed one token at a time, which takes hundreds.)  The cache's length may be divided over workgroups, whose parts are joined in the order of the tokens: the
  * same call gives the same bits, calls of other bounds (max_new, max_length, seqs) may differ by rounding.
  * A sequence longer than its row of the table, or that reads a page outside the pool, comes out as NaN, in all of its rows that
  * would have read there.  O must not overlap Q or the cache.  Workspace: the parts of a divided length. */

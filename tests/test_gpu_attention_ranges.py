@@ -58,3 +58,64 @@ def test_keys_that_are_zero(hip, dtype):
         _scaled(pool, 0, np.arange(64, 80), "k", 0.0)
         q = rng.standard_normal((40, 2 * 64), dtype=np.float32)
         check_rows(_attend(hip, pool, q, 2, scale=0.125 / size), q, pool, 2, 0.125 / size, True, 0, size)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["v", "k", "both"])
+@pytest.mark.parametrize("factor", [1e4, 1e6, 1e8, 1e12, 1e25])
+def test_large_numbers_in_hidden_places(hip, dtype, name, factor):
+    """Finite keys and values that a row does not see - later tokens, tokens before its window - beside small ones that it sees."""
+    rng = np.random.default_rng(4)
+    for new, length, window in ((150, 240, 0), (150, 240, 40), (7, 240, 40), (40, 200, 0)):
+        pool = Pool(rng, [new], [length], 2, 64, 32, dtype)
+        places = np.array([3, length - new + 5, length - new // 2, length - 2])
+        for n in ("k", "v"):
+            if name in (n, "both"):
+                _scaled(pool, 0, places, n, factor)
+        q = rng.standard_normal((new, 4 * 64), dtype=np.float32)
+        check_rows(_attend(hip, pool, q, 4, True, window), q, pool, 4, 0.125, True, window, (name, factor, new, window))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("dim", [64, 80, 128, 256])
+@pytest.mark.parametrize("new", [2, 130])
+def test_tokens_of_very_different_sizes(hip, dtype, dim, new):
+    """Tokens in stretches whose values differ by up to 1e25, seen by some rows, by all, or through a window; every row against its own size."""
+    rng = np.random.default_rng(5)
+    length = new + 150
+    for order in ((1e-15, 1e10), (1e10, 1e-15), (1e-15, 1.0, 0.0, 1e10, 1e-5), (1.0, 1e6), (1e7, 1.0, 1e7)):
+        pool = Pool(rng, [new], [length], 1, dim, 16, dtype)
+        for n, size in enumerate(order):
+            _scaled(pool, 0, np.arange(length * n // len(order), length * (n + 1) // len(order)), "v", size)
+        q = rng.standard_normal((new, 2 * dim), dtype=np.float32)
+        for causal, window in ((False, 0), (True, 0), (True, 20)):
+            check_rows(_attend(hip, pool, q, 2, causal, window), q, pool, 2, dim ** -0.5, causal, window, (order, causal, window))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("large", [1e6, 1e9, 1e15])
+def test_visible_tokens_without_weight(hip, dtype, large):
+    """Large values whose scores are so low that they have no weight, and large keys among small ones that carry the result."""
+    rng = np.random.default_rng(6)
+    for new in (2, 60, 200):
+        length = new + 90
+        pool = Pool(rng, [new], [length], 1, 64, 32, dtype)
+        q = np.abs(rng.standard_normal((new, 2 * 64), dtype=np.float32)) + np.float32(0.5)
+        heavy = np.arange(0, length, 23)
+        pool.put(0, heavy, "k", np.full((len(heavy), 1, 64), -300.0, np.float32))
+        _scaled(pool, 0, heavy, "v", large)
+        check_rows(_attend(hip, pool, q, 2, causal=False), q, pool, 2, 0.125, False, 0, (new, "values"))
+        pool.put(0, heavy, "k", np.full((len(heavy), 1, 64), -large, np.float32))
+        check_rows(_attend(hip, pool, q, 2, causal=False), q, pool, 2, 0.125, False, 0, (new, "keys"))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tokens_of_very_different_sizes_in_parts(hip, dtype):
+    """The same where a length is divided over workgroups, and beyond the bounds that sized the launch."""
+    rng = np.random.default_rng(7)
+    for new, length, dim in ((40, 2500, 64), (130, 3000, 128), (300, 1500, 96)):
+        pool = Pool(rng, [new, 1], [length, 33], 1, dim, 64, dtype)
+        _scaled(pool, 0, np.arange(length), "v", np.where(np.arange(length) % 700 < 350, 1e9, 1.0)[:, None, None])
+        q = rng.standard_normal((new + 1, dim), dtype=np.float32)
+        for causal, window in ((True, 0), (True, 200)):
+            check_rows(_attend(hip, pool, q, 1, causal, window), q, pool, 1, dim ** -0.5, causal, window, (new, causal, window))
