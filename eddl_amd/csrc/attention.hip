@@ -29,6 +29,7 @@
 #include <type_traits>
 
 #include "common.h"
+#include "sequence_rows.h"
 #include "split_parts.h"
 
 using namespace eddlhip;
@@ -62,8 +63,9 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence_of(const AttendParams &p, int s) {
     Sequence q;
-    q.row0 = max(p.offsets[s], 0);
-    q.fresh = q.row0 < p.rows ? max(0, min(p.offsets[s + 1], p.rows) - q.row0) : 0;
+    const SequenceRows r = sequence_rows(p.offsets[s], p.offsets[s + 1], p.rows);
+    q.row0 = r.row0;
+    q.fresh = r.fresh;
     q.length = p.lengths[s];
     q.bad = q.length < 0 || (long long)q.length > ((long long)p.width << p.page_shift);
     if (q.bad) q.length = 0;

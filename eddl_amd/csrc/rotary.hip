@@ -15,6 +15,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "sequence_rows.h"
 #include "split_parts.h"
 
 using namespace eddlhip;
@@ -125,9 +126,11 @@ __device__ __forceinline__ void put4(void *base, size_t at, floatx4 x, int f32) 
 // grid (blocks of 16 places, looping; head_groups; seqs)
 __global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const AppendParams p) {
     __shared__ float2 cs[16][MAX_PAIRS];
-    const int seq = blockIdx.z, row0 = max(p.offsets[seq], 0), fresh = row0 < p.rows ? min(p.offsets[seq + 1], p.rows) - row0 : 0, length = p.lengths[seq];
+    const int seq = blockIdx.z, length = max(p.lengths[seq], 0);
+    const SequenceRows own = sequence_rows(p.offsets[seq], p.offsets[seq + 1], p.rows);
+    const int row0 = own.row0, fresh = own.fresh;
     const int start = length - fresh;  // place of row row0 (below 0: the first rows have none)
-    if (fresh <= 0) return;
+    if (fresh == 0) return;
     const int D = p.D, pieces = pieces_of(r, D);
     // blocks of 16 rows of the sequence, aligned to the places
     const int shift = start & 15;

@@ -119,3 +119,35 @@ def test_tokens_of_very_different_sizes_in_parts(hip, dtype):
         q = rng.standard_normal((new + 1, dim), dtype=np.float32)
         for causal, window in ((True, 0), (True, 200)):
             check_rows(_attend(hip, pool, q, 1, causal, window), q, pool, 1, dim ** -0.5, causal, window, (new, causal, window))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_offsets_that_are_no_offsets(hip, dtype):
+    """Offsets out of order or at the ends of an int: sequences without rows, and no access outside the buffers (sequence_rows.h, which
+    test_sequence_rows_cpu.py checks over all of them)."""
+    from eddl_amd.attention import PagedBatch
+    rng = np.random.default_rng(8)
+    low, high = -2 ** 31, 2 ** 31 - 1
+    for new in (5, 100):
+        pool = Pool(rng, [new, 3], [new + 20, 40], 1, 64, 16, dtype, fill=0.0)
+        cache, batch = pool.on(hip)
+        q = rng.standard_normal((new + 3, 2 * 64), dtype=np.float32)
+        Q, KV = hip.array(q), hip.array(rng.standard_normal((new + 3, 64)))
+        # a row ends before it begins, far before it begins, begins behind the batch, begins before it (those rows are the sequence's first new + 3)
+        for offsets, filled in (((4, low, low), 0), ((4, -1, 2), 2), ((high, high, low), 0), ((new + 3, low, 0), 0), ((low, 0, new + 3), new + 3), ((0, high, high), new + 3)):
+            b = PagedBatch(batch.table, hip.array(np.array(offsets, np.int64), "int32"), batch.lengths, new, new + 20)
+            O, T = hip.full(q.shape, -7.0), hip.full(q.shape, -7.0)
+            hip.paged_attention(Q, O, cache, b)
+            written = np.any(O.numpy() != -7.0, axis=1)
+            assert written[:filled].all() and not written[filled:].any(), offsets
+            keys = cache.keys.numpy()
+            hip.paged_append(Q, KV, KV, T, cache, b)
+            written = np.any(T.numpy() != -7.0, axis=1)
+            assert written[:filled].all() and not written[filled:].any(), offsets
+            assert filled or np.array_equal(cache.keys.numpy(), keys), offsets
+        lengths = hip.array(np.array([low, high]), "int32")
+        b = PagedBatch(batch.table, batch.offsets, lengths, new, new + 20)
+        hip.paged_append(Q, KV, KV, T, cache, b)
+        assert np.array_equal(T.numpy(), q)
+        hip.paged_attention(Q, O, cache, b)
+        assert np.isnan(O.numpy()).all()
