@@ -72,7 +72,8 @@ __device__ __forceinline__ Sequence sequence_of(const AttendParams &p, int s) {
     return q;
 }
 
-// Element offset of 16 tokens of a key head; a page that is not in the pool gives `bad` and the place of page 0.
+// Element offset of 16 tokens of a key head; a page that is not in the pool gives `bad` and the place of page 0.  (16 tokens that a tile's rows have
+// behind their windows are asked for there too, whatever the table holds: a program may have released their page.  Their numbers do not count.)
 __device__ __forceinline__ size_t block_base(const AttendParams &p, int page, int block16, int head, bool &bad) {
     if ((unsigned)page >= (unsigned)p.pages) {
         bad = true;
@@ -447,7 +448,7 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
                 page_lane = pages[min(j, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
             }
             const int b = (lo >> 4) + (wave + W * it) * 2, at = 2 * (it - page_it);
-            base[0] = block_base(p, __builtin_amdgcn_readlane(page_lane, at), b, kv_head, bad);
+            base[0] = block_base(p, 16 * b + 16 <= range.first ? 0 : __builtin_amdgcn_readlane(page_lane, at), b, kv_head, bad);
             base[1] = block_base(p, __builtin_amdgcn_readlane(page_lane, at + 1), b + 1, kv_head, bad);
         };
         // (bf16: lanes g and g ^ 1 read the same 8 dimensions, one the rows of tile 0 and one those of tile 1, so that a load covers whole lines;
@@ -543,9 +544,10 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
                 load_keys();
             }
             __builtin_amdgcn_sched_barrier(0);
-            if (j0 + TILE_KV > q.length) {
+            const bool early = j0 + 16 <= range.first;  // (nobody sees the first 16: page 0 stands in for theirs)
+            if (j0 + TILE_KV > q.length || early) {
 #pragma unroll
-                for (int dt = 0; dt < DT; dt++) v[dt].keep(q.length - (j0 + 8 * g));
+                for (int dt = 0; dt < DT; dt++) v[dt].keep(early && g < 2 ? 0 : q.length - (j0 + 8 * g));
             }
             Parts ws[NQ];
 #pragma unroll
@@ -779,7 +781,8 @@ __device__ __forceinline__ void attend_rows_fp32(const AttendParams &p, const Se
         bool bad[2] = {false, false};
         size_t base[2];
 #pragma unroll
-        for (int b = 0; b < 2; b++) base[b] = block_base(p, pages[min(j0 + 16 * b, to - 1) >> p.page_shift], (j0 >> 4) + b, kv_head, bad[b]);
+        for (int b = 0; b < 2; b++)
+            base[b] = block_base(p, j0 + 16 * b + 16 <= range.first ? 0 : pages[min(j0 + 16 * b, to - 1) >> p.page_shift], (j0 >> 4) + b, kv_head, bad[b]);
         floatx16 s;
 #pragma unroll
         for (int r = 0; r < 16; r++) s[r] = 0.0f;
@@ -876,7 +879,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
                 page_lane = pages[min((b + lane) << 4, hi - 1) >> p.page_shift];  // (behind the last token: its page again, whose values do not count)
             }
             bad = false;
-            const size_t base = block_base(p, __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
+            const size_t base = block_base(p, 16 * b + 16 <= all.first ? 0 : __builtin_amdgcn_readlane(page_lane, b - page_from), b, kv_head, bad);
             const void *src = values ? p.V : p.K;
 #pragma unroll
             for (int i = 0; i < EACH; i++)

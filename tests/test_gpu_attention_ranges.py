@@ -151,3 +151,23 @@ def test_offsets_that_are_no_offsets(hip, dtype):
         assert np.array_equal(T.numpy(), q)
         hip.paged_attention(Q, O, cache, b)
         assert np.isnan(O.numpy()).all()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_released_pages_before_the_windows(hip, dtype, page):
+    """Pages before the windows of all rows, released by the program: the same bits as with the pages in place, for windows that begin at
+    every place of a page, rows of one and of many tokens and divided lengths."""
+    rng = np.random.default_rng(9)
+    for new, length, heads, dim in ((1, 300, 2, 64), (20, 300, 1, 80), (100, 300, 1, 64), (1, 3000, 4, 128), (40, 2600, 1, 64), (140, 700, 1, 96)):
+        pool = Pool(rng, [new], [length], 1, dim, page, dtype)
+        q = rng.standard_normal((new, heads * dim), dtype=np.float32)
+        for window in (range(50, 83) if length == 300 else (700, 715, 716, 717)):
+            pool_table = pool.table.copy()
+            first = max(0, length - new - window + 1)
+            want = _attend(hip, pool, q, heads, True, window)
+            pool.table[0, :first // page] = -1
+            got = _attend(hip, pool, q, heads, True, window)
+            pool.table[:] = pool_table
+            assert np.array_equal(got, want), (new, length, window)
+        check_rows(want, q, pool, heads, dim ** -0.5, True, window, (new, length, window))
