@@ -205,6 +205,7 @@ __device__ void attend_row_again(const AttendParams &p, const Sequence &q, int s
             if (d < p.D) o[i] = (m == NEG_INF ? 0.0f : o[i] * keep) + w * element(p, p.V, base + ((j >> 3) & 1) * 8 * p.D + d * 8 + (j & 7), F32);
         }
         m = top;
+        if (bad || m != m) break;  // (the row is NaN, whatever comes)
     }
     if (bad) l = __builtin_nanf("");
     const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
