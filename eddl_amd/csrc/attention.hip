@@ -252,6 +252,8 @@ __device__ __forceinline__ int part_at(int steps, int n, int parts) {
 // bits do not depend on who comes last.  A launch less: one token over 4096 28.6 -> 20.7 us.
 // Many rows, or more parts, are joined by a launch of their own, which the whole device works on (4 x 196 rows of 8 heads in 6 parts: 9 us
 // where the last workgroups took 19).  Where the last workgroup joins, rows that the launch did not count on (beyond q_tiles) are not divided.
+// (One array for all launches on the device, zeros between them: they come one after another, on one stream, and eddlhip_set_stream
+// waits for the old one's.)
 constexpr int MAX_COUNTS = 1024;  // divided launches have no more row tiles: two workgroups a tile fill the device
 static __device__ unsigned part_counts[MAX_COUNTS];
 

@@ -25,6 +25,7 @@ struct DeviceState {
     bool capturing = false;
     hipStream_t capture_stream = nullptr;  // created on first use (non-blocking, default priority)
     hipStream_t stream_before_capture = nullptr;
+    bool program_captures = false;  // `stream` was being captured by the program when it was set
 };
 
 DeviceState &state(int dev);

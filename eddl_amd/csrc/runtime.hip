@@ -144,10 +144,22 @@ int eddlhip_device_name(int dev, char *buf, size_t buflen) {
     return 0;
 }
 
+// What earlier calls have put on the old stream ends first: calls share the workspace, and counts in device memory that a launch leaves as it
+// found them.  The host waits for the device, because nothing can be asked of the old stream: the program may have destroyed it.  Not
+// where the program captures one of the two streams itself; then it sees to the order.
 int eddlhip_set_stream(int dev, void *hip_stream) {
     EH_TRY(use_device(dev));
     EH_NOT_CAPTURING(dev, "eddlhip_set_stream");
-    state(dev).stream = (hipStream_t)hip_stream;
+    DeviceState &s = state(dev);
+    const hipStream_t to = (hipStream_t)hip_stream;
+    if (to == s.stream) return 0;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const bool failed = hipStreamIsCapturing(to, &status) != hipSuccess;  // (the null stream beside a capture)
+    if (failed) (void)hipGetLastError();
+    const bool captured = failed || status != hipStreamCaptureStatusNone;
+    if (!captured && !s.program_captures) EH_TRY_HIP(hipDeviceSynchronize());
+    s.program_captures = captured && to != nullptr;
+    s.stream = to;
     return 0;
 }
 

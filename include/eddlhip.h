@@ -53,6 +53,11 @@ int eddlhip_device_count(int *count);
 int eddlhip_init(int dev);
 int eddlhip_shutdown(int dev);
 int eddlhip_device_name(int dev, char *buf, size_t buflen);
+/* The stream of the device's calls from now on (NULL: the null stream).  A change of stream waits for the
+ * device, because calls share the workspace and counters and must not overlap, whatever their streams; the old stream may have been
+ * destroyed.  A program that captures the new stream into a graph of its own (and not by eddlhip_graph_begin) is not made to wait,
+ * and neither is its next change of stream: it sees to that order itself, and that such a graph's replays do not overlap with
+ * the library's calls on the device. */
 int eddlhip_set_stream(int dev, void *hip_stream);
 int eddlhip_synchronize(int dev);
 int eddlhip_malloc(int dev, size_t bytes, void **dev_ptr);

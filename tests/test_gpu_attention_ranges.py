@@ -1,4 +1,6 @@
 """Attention over keys and values of very different sizes: every row against its own bound (attention_bound.py)."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -171,3 +173,67 @@ def test_released_pages_before_the_windows(hip, dtype, page):
             pool.table[:] = pool_table
             assert np.array_equal(got, want), (new, length, window)
         check_rows(want, q, pool, heads, dim ** -0.5, True, window, (new, length, window))
+
+
+# ------------------------------------------------------------------------------------------------- streams
+def _streams(hip, n):
+    streams = [ctypes.c_void_p() for _ in range(n)]
+    for s in streams:
+        assert hip.lib.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0  # (non-blocking: nothing but eddlhip_set_stream orders them)
+    return streams
+
+
+def test_calls_on_changing_streams_come_one_after_another(hip):
+    """Calls on two streams in turn, without a synchronization between them, each reading what the one before wrote, divided lengths among
+    them, whose counts and parts lie in memory that all calls share; a stream that is destroyed before the next one is set."""
+    rng = np.random.default_rng(10)
+    calls = []
+    for new, length, dim in ((1, 30000, 64), (2, 2000, 64), (1, 7000, 64)):  # (different numbers of parts)
+        pool = Pool(rng, [new], [length], 1, dim, 64, "float32")
+        cache, batch = pool.on(hip)
+        Q = hip.array(rng.standard_normal((new, 4 * dim)))
+        O = hip.empty(Q.shape)
+        hip.paged_attention(Q, O, cache, batch)
+        calls.append((Q, O, O.numpy(), cache, batch))
+    a, b = hip.array(rng.standard_normal((20000, 512))), hip.empty((20000, 512))
+    hip.norm_residual(a, None, None, b, pre=("rms", None, None, 1e-6))
+    once = b.numpy()
+    hip.norm_residual(b, None, None, b, pre=("layer", None, None, 1e-6))
+    twice = b.numpy()
+    streams = _streams(hip, 2)
+    try:
+        for turn in range(12):
+            for _, O, _, _, _ in calls:
+                hip.fill_(O, -7.0)
+            hip._check(hip.lib.eddlhip_set_stream(hip.dev, streams[0]))
+            hip.norm_residual(a, None, None, b, pre=("rms", None, None, 1e-6))
+            for n, (Q, O, _, cache, batch) in enumerate(calls):
+                hip._check(hip.lib.eddlhip_set_stream(hip.dev, streams[n % 2]))
+                hip.paged_attention(Q, O, cache, batch)
+            hip._check(hip.lib.eddlhip_set_stream(hip.dev, streams[1]))
+            hip.norm_residual(b, None, None, b, pre=("layer", None, None, 1e-6))
+            hip._check(hip.lib.eddlhip_set_stream(hip.dev, None))
+            for _, O, want, _, _ in calls:
+                assert np.array_equal(O.numpy(), want), turn
+            assert np.array_equal(b.numpy(), twice), turn
+        hip._check(hip.lib.eddlhip_set_stream(hip.dev, streams[0]))
+        hip.norm_residual(a, None, None, b, pre=("rms", None, None, 1e-6))
+        hip.synchronize()
+        assert hip.lib.hipStreamDestroy(streams.pop(0)) == 0
+    finally:
+        hip._check(hip.lib.eddlhip_set_stream(hip.dev, None))
+        for s in streams:
+            hip.lib.hipStreamDestroy(s)
+    assert np.array_equal(b.numpy(), once)
+
+
+def test_setting_a_stream_while_a_graph_is_recorded_is_refused(hip):
+    stream, t = _streams(hip, 1)[0], hip.empty((64,))
+    hip._check(hip.lib.eddlhip_graph_begin(hip.dev))
+    hip.fill_(t, 1.0)
+    refused = hip.lib.eddlhip_set_stream(hip.dev, stream)
+    graph = ctypes.c_void_p()
+    hip._check(hip.lib.eddlhip_graph_end(hip.dev, ctypes.byref(graph)))
+    hip._check(hip.lib.eddlhip_graph_destroy(hip.dev, graph))
+    assert refused == -1
+    hip.lib.hipStreamDestroy(stream)
