@@ -86,8 +86,8 @@ template <int ROWS>
 __global__ __launch_bounds__(TPB) void rotary_kernel(const Rotary r, const float *X, float *Y, long long ldx, long long ldy, int rows, int heads, int D, int vec) {
     __shared__ float2 cs[ROWS][MAX_PAIRS];
     const int pieces = pieces_of(r, D), per_row = heads * pieces;
-    for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
-        const int n_rows = min(ROWS, rows - row0);
+    for (long long first = (long long)blockIdx.x * ROWS; first < rows; first += (long long)gridDim.x * ROWS) {  // (64 bits: the step beyond the last of 2^31 - 1 rows)
+        const int row0 = (int)first, n_rows = min(ROWS, rows - row0);
         __syncthreads();
         for (int i = threadIdx.x; i < n_rows * r.pairs; i += TPB) cs[i / r.pairs][i % r.pairs] = turn(r, row0 + i / r.pairs, i % r.pairs);
         __syncthreads();
@@ -134,8 +134,8 @@ __global__ __launch_bounds__(TPB) void paged_append_kernel(const Rotary r, const
     const int D = p.D, pieces = pieces_of(r, D);
     // blocks of 16 rows of the sequence, aligned to the places
     const int shift = start & 15;
-    for (int b = blockIdx.x; 16 * b < shift + fresh; b += gridDim.x) {
-        const int first = max(0, 16 * b - shift), n_rows = min(fresh, 16 * b - shift + 16) - first;  // of the sequence's rows
+    for (long long from = 16LL * blockIdx.x - shift; from < fresh; from += 16LL * gridDim.x) {
+        const int first = (int)max(0LL, from), n_rows = (int)min((long long)fresh, from + 16) - first;  // of the sequence's rows
         // the block's place in the cache; nothing is written where there is none
         const int place = start + first;
         int page = -1;
@@ -242,7 +242,7 @@ int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long l
     EH_TRY(use_device(dev));
     const int vec = aligned16(X, ldx) && aligned16(Y, ldy);
     if (rows >= 4 * 4 * state(dev).num_cu)
-        hipLaunchKernelGGL(rotary_kernel<4>, dim3(std::min((rows + 3) / 4, 1 << 20)), dim3(TPB), 0, state(dev).stream, r, X, Y, ldx, ldy, rows, heads, head_dim, vec);
+        hipLaunchKernelGGL(rotary_kernel<4>, dim3(std::min((rows - 1) / 4 + 1, 1 << 20)), dim3(TPB), 0, state(dev).stream, r, X, Y, ldx, ldy, rows, heads, head_dim, vec);
     else
         hipLaunchKernelGGL(rotary_kernel<1>, dim3(std::min(rows, 1 << 20)), dim3(TPB), 0, state(dev).stream, r, X, Y, ldx, ldy, rows, heads, head_dim, vec);
     EH_CHECK_LAUNCH();
@@ -298,7 +298,7 @@ int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, lo
     p.f32 = cache_type == EDDLHIP_CACHE_F32;
     p.vec = aligned16(K, ldk) && aligned16(V, ldv) && (Q == nullptr || (aligned16(Q, ldq) && aligned16(Qout, ldo)));
     // The launch goes by the bound max_new; sequences with more new tokens loop.
-    const int fresh = std::min(max_new > 0 ? max_new : 1, rows), blocks = (fresh + 14) / 16 + 1;
+    const int fresh = std::min(max_new > 0 ? max_new : 1, rows), blocks = (int)((fresh + 14LL) / 16) + 1;
     const long long items = (Q ? q_heads : 0) + 2LL * kv_heads, there = (long long)blocks * seqs;
     p.head_groups = (int)std::max(1LL, std::min({items, (8LL * state(dev).num_cu + there - 1) / there, 65535LL}));
     hipLaunchKernelGGL(paged_append_kernel, dim3(blocks, p.head_groups, seqs), dim3(TPB), 0, state(dev).stream, r, p);

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from attention_bound import check_rows
-from attention_ref import Pool
+from attention_ref import EPS, Pool
 
 pytestmark = pytest.mark.gpu
 
@@ -237,3 +237,20 @@ def test_setting_a_stream_while_a_graph_is_recorded_is_refused(hip):
     hip._check(hip.lib.eddlhip_graph_destroy(hip.dev, graph))
     assert refused == -1
     hip.lib.hipStreamDestroy(stream)
+
+
+# ------------------------------------------------------------------------------------------------- sizes at the end of an int
+def test_rotary_of_as_many_rows_as_an_int_counts(hip):
+    """2^31 - 1 rows of one head of 8, in place: the loops' steps and the launch's size stay in range, and the last rows are turned."""
+    from eddl_amd.attention import RotaryPlan
+    rows = 2 ** 31 - 1
+    X, P = hip.empty((rows, 8)), hip.empty((rows, 1))
+    hip.fill_(X, 1.0)
+    hip.fill_(P, 0.5)
+    hip.rotary_axes(X, X, RotaryPlan(8, [0] * 4, [1.0, 2.0, 3.0, 4.0]), P)
+    angle = 0.5 * np.array([1.0, 2.0, 3.0, 4.0])
+    want = np.concatenate([np.cos(angle) - np.sin(angle), np.cos(angle) + np.sin(angle)])
+    got = np.empty((64, 8), np.float32)
+    for row in (0, 2 ** 22 - 32, 2 ** 22 * 100, 2 ** 30, 2 ** 31 - 2 ** 22 - 64, rows - 64):
+        hip._check(hip.lib.eddlhip_memcpy_d2h(hip.dev, got.ctypes.data, X.ptr + 32 * row, got.nbytes))
+        assert np.abs(got - want).max() <= 8 * EPS * np.sqrt(2), row
