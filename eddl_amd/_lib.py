@@ -21,6 +21,7 @@ PROTOTYPES = {
     "eddlhip_init": [c_int],
     "eddlhip_shutdown": [c_int],
     "eddlhip_device_name": [c_int, ctypes.c_char_p, c_size_t],
+    "eddlhip_pointer_device": [P, intp],
     "eddlhip_set_stream": [c_int, c_void_p],
     "eddlhip_synchronize": [c_int],
     "eddlhip_malloc": [c_int, c_size_t, ctypes.POINTER(c_void_p)],

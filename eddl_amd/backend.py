@@ -318,8 +318,20 @@ class Backend:
 
     def wrap(self, owner, dtype=None):
         """Device memory that another library holds (an object with ``__cuda_array_interface__``, contiguous) as a tensor, without a copy; keeps
-        ``owner`` alive.  ``dtype`` says what the memory holds where the interface has no name for it ("bfloat16")."""
+        ``owner`` alive.  ``dtype`` says what the memory holds where the interface has no name for it ("bfloat16").
+
+        The operators read and write it on this backend's stream: the caller sees to it that other libraries' work on the memory has ended
+        by then, or is ordered before and behind it; where the interface names the null stream (1), the call waits for that.  Refused are memory of
+        another device, read-only or masked memory (a tensor may be any operator's output), and an interface that names another stream, on which the
+        memory may still be written."""
         spec = owner.__cuda_array_interface__
+        if spec["data"][1] or spec.get("mask") is not None:
+            raise ValueError("a wrapped tensor may be written: not read-only or masked memory")
+        lib, device = _lib.load(), ctypes.c_int(-1)
+        if spec.get("stream") is not None and (spec["stream"] != 1 or lib.hipStreamSynchronize(None) != 0):  # (of the runtime that the library runs on)
+            raise ValueError("the memory may still be written on stream %s: synchronize it, and pass an object that names none" % spec["stream"])
+        if lib.eddlhip_pointer_device(spec["data"][0], ctypes.byref(device)) == 0 and device.value not in (-1, self.dev):
+            raise ValueError("the memory lies on device %d, not on device %d" % (device.value, self.dev))
         kind = dtype or {"<f4": "float32", "<i4": "int32"}.get(spec["typestr"])
         shape = tuple(int(d) for d in spec["shape"])
         if kind not in _TYPES or _TYPES[kind][0] != int(spec["typestr"][2:]):

@@ -144,6 +144,15 @@ int eddlhip_device_name(int dev, char *buf, size_t buflen) {
     return 0;
 }
 
+int eddlhip_pointer_device(const void *ptr, int *device) {
+    EH_REQUIRE(device != nullptr, "device is NULL");
+    *device = -1;
+    hipPointerAttribute_t a;
+    if (ptr != nullptr && hipPointerGetAttributes(&a, ptr) != hipSuccess) (void)hipGetLastError();
+    else if (ptr != nullptr && a.type == hipMemoryTypeDevice) *device = a.device;
+    return 0;
+}
+
 // What earlier calls have put on the old stream ends first: calls share the workspace, and counts in device memory that a launch leaves as it
 // found them.  The host waits for the device, because nothing can be asked of the old stream: the program may have destroyed it.  Not
 // where the program captures one of the two streams itself; then it sees to the order.

@@ -53,6 +53,8 @@ int eddlhip_device_count(int *count);
 int eddlhip_init(int dev);
 int eddlhip_shutdown(int dev);
 int eddlhip_device_name(int dev, char *buf, size_t buflen);
+/* The device whose memory `ptr` points into, or -1 where it is none that this library's runtime knows.  No counterpart in the reference. */
+int eddlhip_pointer_device(const void *ptr, int *device);
 /* The stream of the device's calls from now on (NULL: the null stream).  A change of stream waits for the
  * device, because calls share the workspace and counters and must not overlap, whatever their streams; the old stream may have been
  * destroyed.  A program that captures the new stream into a graph of its own (and not by eddlhip_graph_begin) is not made to wait,

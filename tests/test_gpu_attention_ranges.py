@@ -254,3 +254,11 @@ def test_rotary_of_as_many_rows_as_an_int_counts(hip):
     for row in (0, 2 ** 22 - 32, 2 ** 22 * 100, 2 ** 30, 2 ** 31 - 2 ** 22 - 64, rows - 64):
         hip._check(hip.lib.eddlhip_memcpy_d2h(hip.dev, got.ctypes.data, X.ptr + 32 * row, got.nbytes))
         assert np.abs(got - want).max() <= 8 * EPS * np.sqrt(2), row
+
+
+def test_the_device_of_a_pointer(hip):
+    t, device = hip.empty((64, 64)), ctypes.c_int(7)
+    for ptr, want in ((t.ptr, hip.dev), (t.ptr + 100, hip.dev), (np.zeros(64).ctypes.data, -1), (None, -1)):
+        assert hip.lib.eddlhip_pointer_device(ptr, ctypes.byref(device)) == 0 and device.value == want
+    assert hip.lib.eddlhip_pointer_device(t.ptr, None) == -1
+    hip.fill_(t, 1.0)  # (the question about other memory leaves no error behind)
