@@ -19,6 +19,16 @@ class EddlHipError(RuntimeError):
 _TYPES = {"float32": (4, np.float32), "int32": (4, np.int32), "bfloat16": (2, np.uint16)}
 
 
+def _host(a, dtype):
+    """``a`` as a contiguous array of the numpy type of ``dtype``; numbers that the type does not hold are refused where it is not float32."""
+    a, kind = np.asarray(a), _TYPES[dtype][1]
+    if dtype == "bfloat16" and a.size and a.dtype != np.uint16:
+        raise ValueError("bfloat16 numbers travel as their 16 bits, uint16, not as %s" % a.dtype)
+    if dtype == "int32" and a.size and (a.dtype.kind not in "iub" or a.min() < -2 ** 31 or a.max() >= 2 ** 31):
+        raise ValueError("no int32 numbers: %s of %s" % (a.dtype, a.shape))
+    return np.ascontiguousarray(a, dtype=kind)
+
+
 class DeviceTensor:
     """A float32 tensor in HBM owned by this object (freed when collected)."""
     dtype = "float32"
@@ -51,7 +61,7 @@ class DeviceTensor:
         return out
 
     def copy_from(self, host):
-        host = np.ascontiguousarray(host, dtype=_TYPES[self.dtype][1])
+        host = _host(host, self.dtype)
         if host.size != self.size:
             raise ValueError("size mismatch: %s vs %s" % (host.shape, self.shape))
         self.backend._check(self.backend.lib.eddlhip_memcpy_h2d(self.backend.dev, self.address, host.ctypes.data, self.nbytes))
@@ -351,7 +361,7 @@ class Backend:
     def array(self, host, dtype="float32"):
         if dtype not in _TYPES:
             raise ValueError("no tensors of type %s: %s" % (dtype, ", ".join(_TYPES)))
-        host = np.ascontiguousarray(host, dtype=_TYPES[dtype][1])
+        host = _host(host, dtype)
         return self.empty(host.shape, dtype).copy_from(host)
 
     def full(self, shape, v):

@@ -54,3 +54,28 @@ def test_memory_of_another_device_is_refused_and_the_null_stream_waited_for(hip,
     library.failure = 1
     with pytest.raises(ValueError, match="stream 1"):
         hip.wrap(Lent(stream=1))
+
+
+def test_host_numbers_that_a_type_does_not_hold_are_refused(hip, monkeypatch):
+    """Nothing is cast into other numbers on its way to an int32 or bfloat16 tensor; float32 tensors take every number, as before."""
+    import numpy as np
+    from eddl_amd import backend
+    sent = []
+    hip.empty = lambda shape, dtype="float32": type("Tensor", (), {"copy_from": lambda self, host: sent.append((host.dtype, host.tolist()))})()
+    for host, dtype in (([1, 2], "bfloat16"), (np.array([0.5, 1.5]), "bfloat16"), (np.array([0.5], np.float32), "bfloat16"), (np.array([1], np.int16), "bfloat16"),
+                        (np.array([1.0]), "int32"), ([0.5], "int32"), (np.array([2 ** 31]), "int32"), (np.array([-2 ** 31 - 1]), "int32"), (np.array([2 ** 32], np.uint64), "int32")):
+        with pytest.raises(ValueError):
+            hip.array(host, dtype)
+        tensor = object.__new__(backend.TypedTensor)
+        tensor.dtype, tensor.size = dtype, 1
+        with pytest.raises(ValueError):
+            tensor.copy_from(host)
+    assert sent == []
+    hip.array(np.array([0x3F80, 0xFFFF], np.uint16), "bfloat16")
+    hip.array([-2 ** 31, 2 ** 31 - 1], "int32")
+    hip.array(np.zeros((2, 0)), "int32")
+    hip.array(np.array([True, False]), "int32")
+    hip.array([1, 2], "float32")
+    hip.array(np.array([0.1]))
+    assert sent == [(np.uint16, [0x3F80, 0xFFFF]), (np.int32, [-2 ** 31, 2 ** 31 - 1]), (np.int32, [[], []]), (np.int32, [1, 0]), (np.float32, [1.0, 2.0]),
+                    (np.float32, [float(np.float32(0.1))])]
