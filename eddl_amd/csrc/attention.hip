@@ -1232,6 +1232,9 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     EH_REQUIRE(Q && O && k_pages && v_pages && table && offsets && lengths, "paged_attention: NULL tensor");
     EH_REQUIRE(!eh_rows_overlap(Q, ldq, (long long)q_heads * head_dim, O, ldo, (long long)q_heads * head_dim, rows), "paged_attention: the output lies on the queries");
     EH_REQUIRE((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "paged_attention: the cache is not aligned to 16 bytes");
+    for (const void *cache : {k_pages, v_pages})
+        EH_REQUIRE(!eh_rows_meet(O, ldo, (long long)q_heads * head_dim, rows, cache, (size_t)pages * page_size * kv_heads * head_dim * (cache_type == EDDLHIP_CACHE_F32 ? 4 : 2)),
+                   "paged_attention: the output shares memory with the cache");
     EH_TRY(use_device(dev));
     AttendParams p;
     p.Q = Q;

@@ -89,6 +89,15 @@ static inline bool eh_rows_overlap(const float *a, long long ld_a, long long wid
     return off < 4 * width_a || off + 4 * width_b > pitch;
 }
 
+// Whether rows of `width` floats, `ld` apart, share memory with `bytes` side by side from `base` on; a stretch between two rows does not.
+static inline bool eh_rows_meet(const float *a, long long ld, long long width, long long rows, const void *base, size_t bytes) {
+    if (!a || !base || rows <= 0 || bytes == 0) return false;
+    const uintptr_t a0 = (uintptr_t)a, b0 = (uintptr_t)base, a1 = a0 + 4 * ((rows - 1) * ld + width), b1 = b0 + bytes;
+    if (a1 <= b0 || b1 <= a0) return false;
+    const unsigned long long pitch = 4 * ld, off = b0 >= a0 ? (b0 - a0) % pitch : 0;
+    return b0 < a0 || off < 4ull * width || off + bytes > pitch;
+}
+
 static inline unsigned eh_blocks(size_t work, unsigned per_block, unsigned cap = 1u << 20) {
     size_t b = (work + per_block - 1) / per_block;
     if (b < 1) b = 1;

@@ -209,6 +209,14 @@ extern "C" int eddlhip_norm_residual(int dev, const float *X, long long ldx, con
         for (const float *in : {X, R})
             EH_REQUIRE(out == in || !eh_rows_overlap(out, out == S ? lds : ldh, cols, in, in == X ? ldx : ldr, cols, rows), "norm_residual: an output lies on a part of an input");
     EH_REQUIRE(!eh_rows_overlap(S, lds, cols, H, ldh, cols, rows), "norm_residual: the sum and the norm of it share their rows");
+    const struct {
+        const float *at;
+        size_t floats;
+    } read[] = {{post_w, (size_t)cols}, {post_b, (size_t)cols},  {pre_w, (size_t)cols}, {pre_b, (size_t)cols},
+                {gate, (size_t)(gate_groups == 1 ? 1 : groups) * cols}, {mod, (size_t)groups * cols}, {shift, (size_t)groups * cols}};
+    for (const auto &r : read)
+        EH_REQUIRE(!eh_rows_meet(S, lds, cols, rows, r.at, r.floats * sizeof(float)) && !eh_rows_meet(H, ldh, cols, rows, r.at, r.floats * sizeof(float)),
+                   "norm_residual: an output lies on a weight, bias, gate, mod or shift");
     EH_TRY(use_device(dev));
     NormParams p;
     p.X = X;

@@ -239,6 +239,7 @@ int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long l
     EH_REQUIRE(X && Y, "rotary_axes: NULL tensor");
     EH_REQUIRE(X == Y || !eh_rows_overlap(X, ldx, (long long)heads * head_dim, Y, ldy, (long long)heads * head_dim, rows), "rotary_axes: the output lies on a part of the input");
     EH_REQUIRE(X != Y || ldx == ldy, "rotary_axes: in place, but rows of %lld and %lld floats", ldx, ldy);
+    EH_REQUIRE(rot_dim == 0 || !eh_rows_meet(Y, ldy, (long long)heads * head_dim, rows, positions, (size_t)rows * axes * sizeof(float)), "rotary_axes: the output lies on the positions");
     EH_TRY(use_device(dev));
     const int vec = aligned16(X, ldx) && aligned16(Y, ldy);
     if (rows >= 4 * 4 * state(dev).num_cu)
@@ -273,6 +274,12 @@ int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, lo
     EH_REQUIRE((Q == Qout || !eh_rows_overlap(Q, ldq, q_width, Qout, ldo, q_width, rows)) && !eh_rows_overlap(K, ldk, kv_width, Qout, ldo, q_width, rows) &&
                    !eh_rows_overlap(V, ldv, kv_width, Qout, ldo, q_width, rows), "paged_append: the turned queries lie on a part of what is read");
     EH_REQUIRE(Q != Qout || ldq == ldo, "paged_append: queries in place, but rows of %lld and %lld floats", ldq, ldo);
+    EH_REQUIRE(rot_dim == 0 || !eh_rows_meet(Qout, ldo, q_width, rows, positions, (size_t)rows * axes * sizeof(float)), "paged_append: the turned queries lie on the positions");
+    const size_t cache_bytes = (size_t)pages * page_size * kv_heads * head_dim * (cache_type == EDDLHIP_CACHE_F32 ? 4 : 2);
+    for (const void *cache : {(const void *)k_pages, (const void *)v_pages})
+        EH_REQUIRE(!eh_rows_meet(Q, ldq, q_width, rows, cache, cache_bytes) && !eh_rows_meet(Qout, ldo, q_width, rows, cache, cache_bytes) &&
+                       !eh_rows_meet(K, ldk, kv_width, rows, cache, cache_bytes) && !eh_rows_meet(V, ldv, kv_width, rows, cache, cache_bytes),
+                   "paged_append: rows share memory with the cache");
     EH_TRY(use_device(dev));
     AppendParams p;
     p.Q = Q;

@@ -516,7 +516,7 @@ int eddlhip_dense_fwd(int dev, const float *A, const float *W, const float *bias
  * dimensions of every head (a multiple of 8, up to head_dim and 256) turns by the angle a = positions[row][host_axis[n]] * host_freq[n]:
  *     y_i = x_i cos a - x_j sin a,  y_j = x_j cos a + x_i sin a,
  * (i, j) = (n, n + rot_dim / 2), or (2n, 2n + 1) when `adjacent` != 0.  The other dimensions are copied.  Angles are formed in
- * 64 bits.  host_axis (0 .. axes - 1) and host_freq are host arrays of rot_dim / 2 entries, read during the call.  Y may be X (ldx == ldy).
+ * 64 bits.  host_axis (0 .. axes - 1) and host_freq are host arrays of rot_dim / 2 entries, read during the call.  Y may be X (ldx == ldy), but not lie on the positions.
  * Negative frequencies turn back.  head_dim is a multiple of 8. */
 int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long long ldy, int rows, int heads, int head_dim,
                         const float *positions, int rot_dim, int adjacent, int axes, const int *host_axis, const double *host_freq);
@@ -524,7 +524,7 @@ int eddlhip_rotary_axes(int dev, const float *X, long long ldx, float *Y, long l
 /* The new tokens' keys (turned as above; rot_dim == 0: as they are) and values to their places in the cache, and the turned
  * queries to Qout (Q and Qout NULL: no queries; Qout may be Q).  A bf16 cache rounds to nearest even.  A token without a place - before
  * place 0, behind the table's row, on a page that is not in the pool - is not written; eddlhip_paged_attention reports its
- * sequence.  No page may be written by two sequences of a call. */
+ * sequence.  No page may be written by two sequences of a call, and no row lie in the cache. */
 int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, long long ldo, const float *K, long long ldk,
                          const float *V, long long ldv, int rows, int q_heads, int kv_heads, int head_dim,
                          const float *positions, int rot_dim, int adjacent, int axes, const int *host_axis, const double *host_freq,
@@ -555,7 +555,8 @@ int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, lo
  * post and pre are EDDLHIP_NORM_NONE, _LAYER ((x - mean) / sqrt(variance + eps) w + b) or _RMS (x / sqrt(mean(x^2) + eps) w + b)
  * over the columns; w and b [cols] may be NULL.  gate [gate_groups][cols] belongs to groups of group_rows rows side by side (an image's
  * tokens), or to all rows with gate_groups == 1; NULL: 1.  mod and shift [groups][cols], NULL: 0, with groups = ceil(rows / group_rows).
- * R NULL: no residual.  S or H may be NULL where nobody needs them.  S or H may be X or R (rows of the same distance), not each other.
+ * R NULL: no residual.  S or H may be NULL where nobody needs them.  S or H may be X or R (rows of the same distance), not each other, and
+ * lie on nothing else that is read.
  * Up to 32768 columns. */
 #define EDDLHIP_NORM_NONE 0
 #define EDDLHIP_NORM_LAYER 1
