@@ -262,3 +262,47 @@ def test_the_device_of_a_pointer(hip):
         assert hip.lib.eddlhip_pointer_device(ptr, ctypes.byref(device)) == 0 and device.value == want
     assert hip.lib.eddlhip_pointer_device(t.ptr, None) == -1
     hip.fill_(t, 1.0)  # (the question about other memory leaves no error behind)
+
+
+# ------------------------------------------------------------------------------------------------- rotary positions' accuracy
+def _turned_in_fp32(x, angle):
+    """Halves [rows, 2, pairs] turned with correctly rounded sines, products and sums rounded to fp32."""
+    c, s = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+    return np.concatenate([x[:, 0] * c - x[:, 1] * s, x[:, 1] * c + x[:, 0] * s], 1)
+
+
+def test_turned_pairs_are_as_exact_as_with_rounded_sines(hip):
+    """The argument of the sine is rounded by 2^-29 of a turn in the mean square (0.26 of the error that correctly rounded sines and the products
+    leave, 4.2e-8 of the pair), and a sine of one step's error where half a step is the least adds 0.5 of it: 1.15 times that error together."""
+    from eddl_amd.attention import RotaryPlan
+    rng = np.random.default_rng(11)
+    rows, pairs = 4000, 64
+    freq = 10000.0 ** -rng.uniform(0, 1, pairs)
+    x = rng.standard_normal((rows, 2, pairs), dtype=np.float32)
+    for positions in (np.floor(rng.uniform(0, 1e5, (rows, 1))), np.floor(rng.uniform(-1e6, 1e6, (rows, 1))), rng.uniform(-30, 30, (rows, 1))):
+        positions = positions.astype(np.float32)
+        Y = hip.empty((rows, 2 * pairs))
+        hip.rotary_axes(hip.array(x.reshape(rows, -1)), Y, RotaryPlan(2 * pairs, [0] * pairs, freq), hip.array(positions))
+        angle = positions.astype(np.longdouble) * freq
+        c, s, z = np.cos(angle), np.sin(angle), x.astype(np.longdouble)
+        want = np.concatenate([z[:, 0] * c - z[:, 1] * s, z[:, 1] * c + z[:, 0] * s], 1)
+        off, least = np.linalg.norm((Y.numpy() - want).astype(float)), np.linalg.norm((_turned_in_fp32(x, angle) - want).astype(float))
+        assert off <= 1.15 * least, (off, least)
+
+
+def test_quarters_of_a_turn(hip):
+    """Angles on and beside whole quarters, both ways round: the right quarter's signs, and on them the 0 and 1 of the angle in 64 bits (9 / 4 of a
+    turn, rounded three times, 2^-53 each: 7.5e-16 of a turn, 5e-15)."""
+    from eddl_amd.attention import RotaryPlan
+    quarters = np.arange(-9, 10)
+    turns = (quarters[:, None] / 4 + np.array([-0.125, -1e-3, 0.0, 1e-3, 0.125])[None, :]).reshape(-1, 1)
+    positions = turns.astype(np.float32)
+    x = np.tile(np.array([[1.0, 0, 0, 0, 0, 0, 0, 0]], np.float32), (len(turns), 1))  # (the first pair's first number; y = cos, sin)
+    Y = hip.empty(x.shape)
+    hip.rotary_axes(hip.array(x), Y, RotaryPlan(8, [0] * 4, [2 * np.pi] * 4), hip.array(positions))
+    got = Y.numpy()[:, [0, 4]]
+    angle = 2 * np.pi * positions[:, 0].astype(np.float64)
+    want = np.stack([np.cos(angle), np.sin(angle)], 1)
+    assert np.abs(got - want).max() <= 4 * EPS
+    whole = got.reshape(len(quarters), 5, 2)[:, 2]
+    assert np.abs(whole - np.array([[[1, 0], [0, 1], [-1, 0], [0, -1]][q % 4] for q in quarters])).max() <= 5e-15
