@@ -49,9 +49,9 @@ struct AttendParams {
     float *O;
     const void *K, *V;
     const int *table, *offsets, *lengths;
-    float *part_o;   // [splits][rows * q_heads][D]
-    float2 *part_s;  // [splits][rows * q_heads] maximum and sum
-    long long ldq, ldo;
+    float *part_o;   // [splits][part_rows][D]
+    float2 *part_s;  // [splits][part_rows] maximum and sum
+    long long ldq, ldo, part_rows;  // part_rows: rows * q_heads, or the rows of the launch's tiles where the last workgroup joins
     int rows, q_heads, kv_heads, group, D, pages, page_shift, width, seqs, causal, window, splits, q_tiles, vec, grouped;
     float scale;  // with log2(e)
 };
@@ -181,7 +181,7 @@ __device__ __forceinline__ void store_scale(const AttendParams &p, float m, floa
 
 // One row over the tokens [lo, hi), a wavefront together, one token at a time: lanes hold the dimensions lane, lane + 64, ...
 template <bool F32>
-__device__ void attend_row_again(const AttendParams &p, const Sequence &q, int seq, int kv_head, int token, int head, int lo, int hi, int split, int splits, bool bad) {
+__device__ void attend_row_again(const AttendParams &p, const Sequence &q, int seq, int kv_head, int token, int head, int lo, int hi, size_t slot, int splits, bool bad) {
     const int lane = threadIdx.x & 63, pos = q.length - q.fresh + token;
     if (p.causal) hi = min(hi, pos + 1);
     if (p.window > 0) lo = max(lo, pos - p.window + 1);
@@ -208,9 +208,7 @@ __device__ void attend_row_again(const AttendParams &p, const Sequence &q, int s
         if (bad || m != m) break;  // (the row is NaN, whatever comes)
     }
     if (bad) l = __builtin_nanf("");
-    const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
     if (splits > 1) {
-        const size_t slot = (size_t)split * p.rows * p.q_heads + at;
         if (lane == 0) put_part((float *)(p.part_s + slot), m, l);
         for (int i = 0; i < 4; i++)
             if (lane + 64 * i < p.D) __hip_atomic_store(p.part_o + slot * p.D + lane + 64 * i, o[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -258,10 +256,11 @@ constexpr int MAX_COUNTS = 1024;  // divided launches have no more row tiles: tw
 static __device__ unsigned part_counts[MAX_COUNTS];
 
 constexpr int JOIN_HERE = 64;  // most parts that are joined so
+constexpr size_t MOST_PARTS = (size_t)1 << 30;  // bytes of the parts that a launch joins
 // `sums`: LDS of rows x parts; `red`: LDS of THREADS.
 template <int THREADS>
 __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence &q, int kv_head, int row_lo, int row_hi, float2 *sums, floatx4 *red, unsigned count,
-                                           int *last) {
+                                           size_t slot, int *last) {  // slot: the tile's first in a part
     const int tid = threadIdx.x, n = row_hi - row_lo, parts = p.splits, quads = p.D >> 2;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -272,14 +271,10 @@ __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence
     }
     __syncthreads();
     if (!*last) return;
-    const size_t total = (size_t)p.rows * p.q_heads;
-    auto at_row = [&](int r) __attribute__((always_inline)) {
-        const int row = row_lo + r, token = row / p.group;
-        return (size_t)(q.row0 + token) * p.q_heads + kv_head * p.group + row % p.group;
-    };
+    const size_t total = p.part_rows;
     for (int i = tid; i < n * parts; i += THREADS) {
         const int r = i / parts, s = i - r * parts;
-        sums[i] = get_part((const float *)(p.part_s + s * total + at_row(r)));
+        sums[i] = get_part((const float *)(p.part_s + s * total + slot + r));
     }
     __syncthreads();
     // four dimensions of a row a thread, or several threads where there are few
@@ -293,7 +288,7 @@ __device__ __forceinline__ void join_parts(const AttendParams &p, const Sequence
             const float2 *ms = sums + r * parts;
 #pragma unroll 8
             for (int s = 0; s < parts; s++) m = fmaxf(m, ms[s].x);
-            const float *src = p.part_o + at_row(r) * p.D + d;
+            const float *src = p.part_o + (slot + r) * p.D + d;
             constexpr int AHEAD = 16;
             for (int s0 = lane; s0 < parts; s0 += AHEAD * lanes) {
                 float2 a[AHEAD], b[AHEAD];
@@ -608,6 +603,12 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
         }
         __syncthreads();
 
+        const size_t first_slot = (size_t)((seq * p.kv_heads + kv_head) * p.q_tiles + tile) * COLS;  // (of a part that the last workgroup joins)
+        auto slot_of = [&](int c) __attribute__((always_inline)) {
+            const int row = row_lo + c, token = row / p.group;
+            return (size_t)split * p.part_rows + (splits > JOIN_HERE ? (size_t)(q.row0 + token) * p.q_heads + kv_head * p.group + row % p.group : first_slot + c);
+        };
+
         // ---- the wavefronts' sums together, four dimensions of a row a thread
         const int quads = D >> 2, items = (row_hi - row_lo) * quads;
         for (int i0 = 0; i0 < items; i0 += 64 * W) {
@@ -630,7 +631,7 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
                 if (worst != 0.0f || (top == NEG_INF && from < to)) {
                     atomicOr(&redo_columns, 1u << c);
                 }
-                const size_t at = (size_t)(q.row0 + token) * p.q_heads + head, slot = (size_t)split * p.rows * p.q_heads + at;
+                const size_t slot = slot_of(c);
                 if (splits > JOIN_HERE) {
                     if (d == 0) p.part_s[slot] = make_float2(top, sum);
                     *reinterpret_cast<floatx4 *>(p.part_o + slot * D + d) = x;
@@ -657,10 +658,10 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
         const bool any_bad = q.bad;
         for (unsigned todo = redo_columns; todo != 0; todo &= todo - 1) {
             const int c = __builtin_ctz(todo), r = row_lo + c;
-            if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, splits, any_bad);
+            if (c % W == wave) attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, slot_of(c), splits, any_bad);
         }
         if (splits > 1 && splits <= JOIN_HERE)
-            join_parts<64 * W>(p, q, kv_head, row_lo, row_hi, reinterpret_cast<float2 *>(lds), red, (seq * p.kv_heads + kv_head) * p.q_tiles + tile, &last);
+            join_parts<64 * W>(p, q, kv_head, row_lo, row_hi, reinterpret_cast<float2 *>(lds), red, (seq * p.kv_heads + kv_head) * p.q_tiles + tile, first_slot, &last);
     }
 }
 
@@ -1094,12 +1095,13 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
         const bool redo = (todo >> col) & 1;
         for (unsigned long long t = todo; t != 0; t &= t - 1) {
             const int r = row_lo + __builtin_ctzll(t);
-            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, kv_head * p.group + r % p.group, lo, hi, split, splits, q.bad);
+            const int head_r = kv_head * p.group + r % p.group;
+            attend_row_again<F32>(p, q, seq, kv_head, r / p.group, head_r, lo, hi, (size_t)split * p.part_rows + (size_t)(q.row0 + r / p.group) * p.q_heads + head_r, splits, q.bad);
         }
 
         if (row_lo + col < row_hi && !redo) {
             const size_t at = (size_t)(q.row0 + token) * p.q_heads + head;
-            const size_t slot = (size_t)split * p.rows * p.q_heads + at;
+            const size_t slot = (size_t)split * p.part_rows + at;
             float factor = 1.0f, *dst;
             if (splits > 1) {
                 if (half == 0) p.part_s[slot] = make_float2(m, l);
@@ -1274,11 +1276,17 @@ extern "C" int eddlhip_paged_attention(int dev, const float *Q, long long ldq, f
     const long long steps = (seen + TILE_KV - 1) / TILE_KV;
     p.splits = (int)std::max(1LL, std::min({want / filled, steps / (nq ? 8 : 4), (long long)(nq ? FEW_SPLITS / nq : CHUNK_SPLITS)}));
     if (nq && groups > MAX_COUNTS) p.splits = 1;
+    // Parts that a launch joins have a place for every row of the tensors: with many more rows than the batch has (room for other batches), fewer
+    // parts, or those that the last workgroup joins, whose places are those of the launch's tiles.  A full batch takes 100 MB at most.
+    p.part_rows = (long long)rows * q_heads;
+    const size_t part_bytes = (size_t)p.part_rows * (head_dim + 2) * sizeof(float);
+    if (p.splits > (nq ? JOIN_HERE : 1) && p.splits * part_bytes > MOST_PARTS) p.splits = nq ? JOIN_HERE : (int)std::max((size_t)1, MOST_PARTS / part_bytes);
+    if (nq && p.splits <= JOIN_HERE) p.part_rows = groups * per_tile;
     p.grouped = even;
     p.part_o = nullptr;
     p.part_s = nullptr;
     if (p.splits > 1) {
-        const size_t slots = (size_t)p.splits * rows * q_heads;
+        const size_t slots = (size_t)p.splits * p.part_rows;
         void *ws = nullptr;
         EH_TRY(get_workspace(dev, slots * (head_dim + 2) * sizeof(float), &ws));
         p.part_o = (float *)ws;

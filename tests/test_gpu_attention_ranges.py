@@ -306,3 +306,27 @@ def test_quarters_of_a_turn(hip):
     assert np.abs(got - want).max() <= 4 * EPS
     whole = got.reshape(len(quarters), 5, 2)[:, 2]
     assert np.abs(whole - np.array([[[1, 0], [0, 1], [-1, 0], [0, -1]][q % 4] for q in quarters])).max() <= 5e-15
+
+
+# ------------------------------------------------------------------------------------------------- memory
+@pytest.mark.parametrize("new, length", [(1, 40000), (2, 3000), (40, 3000)])
+def test_parts_of_a_padded_batch_take_the_room_of_its_rows(hip, new, length):
+    """Tensors of 120000 rows of which the batch has a few: the parts of a divided length do not take room for all of them in every part (30 GB
+    for 150 parts), and the result is right, at the front, in the middle and at the end of the tensors."""
+    from eddl_amd.attention import PagedBatch
+    rng = np.random.default_rng(12)
+    pool = Pool(rng, [new], [length], 1, 64, 64, "float32")
+    q = rng.standard_normal((new, 8 * 64), dtype=np.float32)
+    cache, batch = pool.on(hip)
+    rows = 120000
+    Q, O = hip.empty((rows, 8 * 64)), hip.empty((rows, 8 * 64))
+    hip.workspace_trim()
+    for at in (0, 70001, rows - new):
+        hip.fill_(O, -7.0)
+        hip._check(hip.lib.eddlhip_memcpy_h2d(hip.dev, Q.ptr + 4 * 8 * 64 * at, q.ctypes.data, q.nbytes))
+        b = PagedBatch(batch.table, hip.array([at, at + new], "int32"), batch.lengths, new, length)
+        hip.paged_attention(Q, O, cache, b)
+        got = O.numpy()
+        check_rows(got[at:at + new], q, pool, 8, 0.125, True, 0, (new, at))
+        assert np.all(got[:at] == -7.0) and np.all(got[at + new:] == -7.0)
+        assert hip.workspace_bytes() <= 2 ** 30 + 2 ** 20
