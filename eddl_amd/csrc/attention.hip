@@ -63,10 +63,13 @@ struct Sequence {
 };
 __device__ __forceinline__ Sequence sequence_of(const AttendParams &p, int s) {
     Sequence q;
-    const SequenceRows r = sequence_rows(p.offsets[s], p.offsets[s + 1], p.rows);
+    const int begin = p.offsets[s], end = p.offsets[s + 1];
+    int length = p.lengths[s];
+    asm volatile("" : "+s"(length));  // (asked for together with the offsets, not behind a branch on them: 1 token over 50 6.1 -> 5.9 us)
+    const SequenceRows r = sequence_rows(begin, end, p.rows);
     q.row0 = r.row0;
     q.fresh = r.fresh;
-    q.length = p.lengths[s];
+    q.length = length;
     q.bad = q.length < 0 || (long long)q.length > ((long long)p.width << p.page_shift);
     if (q.bad) q.length = 0;
     return q;
