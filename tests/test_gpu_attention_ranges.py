@@ -79,8 +79,8 @@ def test_large_numbers_in_hidden_places(hip, dtype, name, factor):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("dim", [64, 80, 128, 256])
-@pytest.mark.parametrize("new", [2, 130])
+@pytest.mark.parametrize("dim", [16, 48, 64, 80, 96, 112, 128, 192, 240, 256])
+@pytest.mark.parametrize("new", [2, 40, 130])
 def test_tokens_of_very_different_sizes(hip, dtype, dim, new):
     """Tokens in stretches whose values differ by up to 1e25, seen by some rows, by all, or through a window; every row against its own size."""
     rng = np.random.default_rng(5)
