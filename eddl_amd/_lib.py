@@ -120,7 +120,12 @@ def load_probe():
     return lib
 
 
+_loaded = {}  # path -> library with its prototypes set (150 us of work)
+
+
 def load():
+    if LIB_PATH in _loaded:
+        return _loaded[LIB_PATH]
     if not os.path.exists(LIB_PATH):
         raise ImportError(
             "%s is missing: build it with `python -m eddl_amd.build` (hipcc, gfx950). "
@@ -130,4 +135,5 @@ def load():
         fn = getattr(lib, name)  # AttributeError if the library lacks a declared symbol
         fn.argtypes = args
         fn.restype = _RESTYPE.get(name, c_int)
+    _loaded[LIB_PATH] = lib
     return lib

@@ -79,3 +79,8 @@ def test_host_numbers_that_a_type_does_not_hold_are_refused(hip, monkeypatch):
     hip.array(np.array([0.1]))
     assert sent == [(np.uint16, [0x3F80, 0xFFFF]), (np.int32, [-2 ** 31, 2 ** 31 - 1]), (np.int32, [[], []]), (np.int32, [1, 0]), (np.float32, [1.0, 2.0]),
                     (np.float32, [float(np.float32(0.1))])]
+
+
+def test_the_library_is_set_up_once():
+    from eddl_amd import _lib
+    assert _lib.load() is _lib.load()
