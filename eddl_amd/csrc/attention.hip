@@ -685,8 +685,8 @@ __global__ __launch_bounds__(64 * few_waves(DP, F32, NQ), few_per_simd(DP, F32, 
 // access is 16 bytes a lane of 16 lanes side by side.  The queries' pairs stay in registers.
 // Eight wavefronts (two on each SIMD, one of which brings tiles) halve that work for a row: 2048 tokens over 8192, 32 and 8 heads of 128, bf16
 // 561 -> 516 us, 4 x 1000 over 2000, heads of 64 102 -> 86; but a ragged batch has more empty rows in tiles of 256 (35 -> 44 us).
-// Measured: 2048 tokens over 8192, 32 and 8 heads of 128, bf16 cache: 516 us, 466 TFLOP/s, 930 on the matrix instructions (with four
-// wavefronts 42 % of the cycles busy; the vector instructions fill 57 % and the two do not overlap: a version that computed the next tile's scores beside the
+// Measured: 2048 tokens over 8192, 32 and 8 heads of 128, bf16 cache: 508 us, 473 TFLOP/s, 950 on the matrix instructions (48 % of the
+// cycles busy; the vector instructions fill 53 % and the two do not overlap: a version that computed the next tile's scores beside the
 // weights in one block, with the scheduler's groups, spilled and took 890).  As three bf16 parts with tiles loaded straight into LDS 621 us.
 constexpr int CHUNK_SPLITS = 64;  // most parts of a length
 

@@ -6,7 +6,8 @@
 // wavefronts beyond.  Means and variances are fp32 sums over the registers; the variance is that of the differences from the mean, a
 // second pass over registers that costs no memory.
 // Bound: memory, 16 bytes a number (x, r, s, h).  12544 x 2048 with two RMS norms, gate, shift and scale: 91 us, 4.5 TB/s; 50000 x 1000 with two layer
-// norms 159 us, 5.0 TB/s; 12544 x 512 17.5 us, 5.9 TB/s (partly from the last-level cache).
+// norms 159 us, 5.0 TB/s; 12544 x 512 17.5 us, 5.9 TB/s (partly from the last-level cache).  Rows that are no multiple of four columns (or not
+// aligned) are read 4 bytes at a time: 50000 x 1001 351 us.  Rows of 64 columns use 16 of a wavefront's lanes: 400000 x 64 223 us, 1.8 TB/s.
 #include <math.h>
 
 #include <algorithm>
