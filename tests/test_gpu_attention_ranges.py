@@ -227,6 +227,37 @@ def test_calls_on_changing_streams_come_one_after_another(hip):
     assert np.array_equal(b.numpy(), once)
 
 
+def test_a_stream_that_the_program_captures(hip):
+    """A program's own graph of the library's calls: setting its stream, and the next one, waits for nothing and leaves the capture whole."""
+    lib, stream = hip.lib, _streams(hip, 1)[0]
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((300, 256), dtype=np.float32)
+    X, H, other = hip.array(x), hip.full((300, 256), -7.0), hip.empty((300, 256))
+    norm = lambda X, H: hip.norm_residual(X, None, None, H, pre=("rms", None, None, 1e-6))
+    norm(X, other)
+    want = other.numpy()
+    hip.fill_(other, 0.0)
+    graph, program = ctypes.c_void_p(), ctypes.c_void_p()
+    assert lib.hipStreamBeginCapture(stream, 1) == 0  # (thread-local)
+    first = lib.eddlhip_set_stream(hip.dev, stream)
+    norm(X, H)
+    second = lib.eddlhip_set_stream(hip.dev, None)
+    assert lib.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0 and (first, second) == (0, 0)
+    assert np.all(H.numpy() == -7.0)
+    assert lib.hipGraphInstantiate(ctypes.byref(program), graph, None, None, ctypes.c_size_t(0)) == 0
+    for turn in range(3):
+        hip.fill_(H, float(turn))
+        X.copy_from(x * np.float32(2.0 ** turn))
+        assert lib.hipGraphLaunch(program, None) == 0
+        norm(X, other)
+        hip.synchronize()
+        assert np.array_equal(H.numpy(), other.numpy())
+    assert np.abs(other.numpy() - want).max() <= 1e-5 * np.abs(want).max()
+    lib.hipGraphExecDestroy(program)
+    lib.hipGraphDestroy(graph)
+    lib.hipStreamDestroy(stream)
+
+
 def test_setting_a_stream_while_a_graph_is_recorded_is_refused(hip):
     stream, t = _streams(hip, 1)[0], hip.empty((64,))
     hip._check(hip.lib.eddlhip_graph_begin(hip.dev))
