@@ -23,7 +23,8 @@
 // replaced by zeros.  Other numbers share exponents with their neighbours in the kernel of many rows: rows that lose bits by that are computed
 // again in fp32 (attend_rows_fp32).  A NaN or infinity in a visible or masked place of a tile otherwise reaches the sums as NaN (0 * inf, or the
 // parts of an infinity), and rows whose sums are not finite are computed again one token at a time (attend_row_again), with
-// what the formula gives.
+// what the formula gives - in the kernel of many rows only those that fp32 leaves with a finite sum of weights (2048 tokens over 8192
+// that all see a NaN: among the keys 3.7 ms, among the values 259).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -1087,7 +1088,7 @@ __global__ __launch_bounds__(64 * W, W == 8 || DP <= 128 ? 2 : 1) void attend_ch
             const bool lost = f_most * (float)D > SCORES_SPREAD || (power > LEAST_POWER && most < __builtin_amdgcn_ldexpf(1.0f, (int)power + 14 - VALUES_SPREAD));
             if (__any((lost && sees) || again) && works && !q.bad) {
                 attend_rows_fp32<DT, F32, FULL>(p, q, pages, kv_head, p.Q + (size_t)(q.row0 + token) * p.ldq + (size_t)head * D, range, lo, hi, see_lo, see_hi, k_token, o, m, l);
-                again = not_finite();
+                again = not_finite() && l == l;  // (a sum that is NaN is that of visible scores: so is the row)
             }
         }
 

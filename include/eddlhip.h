@@ -539,9 +539,10 @@ int eddlhip_paged_append(int dev, const float *Q, long long ldq, float *Qout, lo
  * fp32 arithmetic beside the largest number of a row's head, whatever the sizes of the numbers.  (Sequences of up to 32 rows a key
  * head: sums of bf16 products, as the split form of the convolutions.  More: products of pairs of fp16 numbers that share an
  * exponent with 16 tokens.  Where a row's scores or result are thousands of times smaller than numbers that it shares exponents with,
- * 32 rows together are computed again on the fp32 matrix instruction, in about six times the time; rows that an infinity or NaN
- * in their tile reaches are computed one token at a time, which takes hundreds.)  The cache's length may be divided over workgroups, whose parts are joined in the order of the tokens: the
- * same call gives the same bits, calls of other bounds (max_new, max_length, seqs) may differ by rounding.
+ * 32 rows together are computed again on the fp32 matrix instruction, in about six times the time, and so are rows of 32 that an
+ * infinity or NaN reaches; where it is a value's, they are computed one token at a time behind that, in hundreds of times the time.)
+ * The cache's length may be divided over workgroups, whose parts are joined in the order of the tokens: the same call gives
+ * the same bits, calls of other bounds (max_new, max_length, seqs) may differ by rounding.
  * A sequence longer than its row of the table, or that reads a page outside the pool, comes out as NaN, in all of its rows that
  * would have read there.  O must not overlap Q or the cache.  Workspace: the parts of a divided length. */
 int eddlhip_paged_attention(int dev, const float *Q, long long ldq, float *O, long long ldo, int rows,
