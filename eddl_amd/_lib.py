@@ -94,6 +94,10 @@ PROTOTYPES = {
                                + [c_float, c_int, c_int],
     "eddlhip_norm_residual": [c_int, P, c_longlong, P, c_longlong, c_float, P, c_longlong, P, c_longlong, c_int, c_int, c_int, P, P, c_float, P, c_int,
                               c_int, P, P, c_float, P, P, c_int],
+    "eddlhip_group_norm": [c_int, P, c_longlong, P, c_longlong] + [c_int] * 5 + [P, P, c_float, P, P, c_int],
+    "eddlhip_causal_conv": [c_int, P, c_longlong, P, P, P, c_longlong] + [c_int] * 5 + [P, c_int, P, P, P, P, c_int, c_int],
+    "eddlhip_selective_scan": [c_int, P, c_longlong, P, c_longlong, P, P, c_longlong, P, c_longlong, P, P, c_longlong, P, P, c_longlong] + [c_int] * 6
+                              + [P, c_int, P, P, P, P, c_int, c_int],
 }
 _RESTYPE = {"eddlhip_version": ctypes.c_char_p, "eddlhip_last_error": ctypes.c_char_p,
             "eddlhip_conv2d_last_kernel": ctypes.c_char_p}

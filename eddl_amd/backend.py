@@ -626,5 +626,72 @@ class Backend:
                                                    _ptr(post[2]), post[3], _ptr(gate), gate.size // shape[1] if gate is not None else 0, _NORMS[pre[0]],
                                                    _ptr(pre[1]), _ptr(pre[2]), pre[3], _ptr(mod), _ptr(shift), group_rows))
 
+    # ---- group norm and state space blocks (eddl_amd.state_space holds the batch that the last two take)
+    def group_norm(self, X, Y, groups, weight=None, bias=None, eps=1e-5, activation=None, mod=None, shift=None, image_rows=None):
+        """Y = act(n (1 + mod) + shift), n the norm of ``groups`` groups of channels over the pixels of an image, its ``weight`` and ``bias`` [channels].
+        ``X``, ``Y``: maps [images, channels, height, width], or rows of tokens [rows, channels], ``image_rows`` rows an image (all, unless
+        given); ``Y`` may be ``X``.  ``activation`` None, "relu" or "silu"; ``mod``, ``shift`` [images, channels] or None."""
+        if len(X.shape) == 4 and len(Y.shape) == 4 and image_rows is None:
+            if X.dtype != "float32" or X.shape != Y.shape:
+                raise ValueError("group_norm shapes %s -> %s" % (X.shape, Y.shape))
+            images, channels, pixels, last = X.shape[0], X.shape[1], X.shape[2] * X.shape[3], 0
+            x, ldx, y, ldy = X.ptr, channels, Y.ptr, channels
+        else:
+            (x, ldx, shape), (y, ldy, yshape) = _rows(X, "group_norm"), _rows(Y, "group_norm")
+            pixels, channels, last = shape[0] if image_rows is None else int(image_rows), shape[1], 1
+            if shape != yshape or pixels < 0 or (shape[0] % pixels if pixels else shape[0]):
+                raise ValueError("group_norm: rows %s -> %s in images of %s rows" % (shape, yshape, image_rows))
+            images, pixels = (shape[0] // pixels, pixels) if shape[0] else (0, 1)
+        for t, size in ((weight, channels), (bias, channels), (mod, images * channels), (shift, images * channels)):
+            if t is not None and (t.size != size or t.dtype != "float32"):
+                raise ValueError("group_norm: weight, bias, mod or shift %s %s for %d images of %d channels" % (t.dtype, t.shape, images, channels))
+        self._check(self.lib.eddlhip_group_norm(self.dev, x, ldx, y, ldy, images, channels, pixels, last, groups, _ptr(weight), _ptr(bias), eps, _ptr(mod), _ptr(shift),
+                                                _activation(activation)))
+
+    def causal_conv(self, X, W, bias, Y, batch, states=None, activation=None, reverse=False):
+        """The short convolution of every channel along the tokens of a ragged batch: ``X`` -> ``Y`` [rows, channels], ``W`` [channels, width],
+        ``bias`` [channels] or None, ``batch`` a StateBatch, ``states`` [slots, width - 1, channels] or None (every sequence begins with its new tokens)."""
+        (x, ldx, shape), (y, ldy, yshape) = _rows(X, "causal_conv"), _rows(Y, "causal_conv")
+        channels = shape[1]
+        if shape != yshape or len(W.shape) != 2 or W.shape[0] != channels or W.dtype != "float32" or bias is not None and (bias.size != channels or bias.dtype != "float32"):
+            raise ValueError("causal_conv shapes %s -> %s, weights %s, bias %s" % (shape, yshape, W.shape, getattr(bias, "shape", None)))
+        pool = _pool(states, batch, (W.shape[1] - 1, channels), "causal_conv")
+        self._check(self.lib.eddlhip_causal_conv(self.dev, x, ldx, W.ptr, _ptr(bias), y, ldy, shape[0], channels, W.shape[1], _activation(activation), int(bool(reverse)),
+                                                 *pool, *batch.arguments))
+
+    def selective_scan(self, X, dt, A, B, C, Y, batch, states=None, skip=None, gate=None, dt_bias=None, softplus=True, reverse=False):
+        """The selective scan along the tokens of a ragged batch: ``X``, ``dt``, ``Y`` and ``gate`` (or None) [rows, channels], ``A`` [channels, n], ``B`` and ``C``
+        [rows, groups * n], ``skip`` and ``dt_bias`` [channels] or None, ``batch`` a StateBatch, ``states`` [slots, channels, n] or None (every
+        sequence begins with its new tokens)."""
+        (x, ldx, shape), (d, lddt, dshape), (y, ldy, yshape) = _rows(X, "selective_scan"), _rows(dt, "selective_scan"), _rows(Y, "selective_scan")
+        (b, ldb, bshape), (c, ldc, cshape) = _rows(B, "selective_scan"), _rows(C, "selective_scan")
+        g, ldg, gshape = _rows(gate, "selective_scan") if gate is not None else (None, 0, shape)
+        rows, channels = shape
+        n = A.shape[1] if len(A.shape) == 2 and A.dtype == "float32" else 0
+        if not shape == dshape == yshape == gshape or bshape != cshape or bshape[0] != rows or A.shape[0] != channels or not n or bshape[1] % n:
+            raise ValueError("selective_scan shapes x %s, dt %s, gate %s -> %s, A %s, B %s, C %s" % (shape, dshape, gshape, yshape, A.shape, bshape, cshape))
+        for t in (skip, dt_bias):
+            if t is not None and (t.size != channels or t.dtype != "float32"):
+                raise ValueError("selective_scan: skip or dt_bias %s %s for %d channels" % (t.dtype, t.shape, channels))
+        pool = _pool(states, batch, (channels, n), "selective_scan")
+        self._check(self.lib.eddlhip_selective_scan(self.dev, x, ldx, d, lddt, A.ptr, b, ldb, c, ldc, _ptr(skip), g, ldg, _ptr(dt_bias), y, ldy, rows, channels, n,
+                                                    bshape[1] // n, int(bool(softplus)), int(bool(reverse)), *pool, *batch.arguments))
+
 
 _NORMS = {None: 0, "layer": 1, "rms": 2}
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+
+
+def _activation(name):
+    if name not in _ACTIVATIONS:
+        raise ValueError("no activation %r: None, \"relu\" or \"silu\"" % (name,))
+    return _ACTIVATIONS[name]
+
+
+def _pool(states, batch, each, what):
+    """(pointer, slots) of a pool of states of shape ``each``."""
+    if states is None:
+        return None, 0
+    if len(states.shape) != 3 or tuple(states.shape[1:]) != each or states.dtype != "float32" or batch.slots is None:
+        raise ValueError("%s: states are float32 [slots, %d, %d] with a batch that names lengths and slots, not %s %s" % (what, *each, states.dtype, states.shape))
+    return states.ptr, states.shape[0]

@@ -568,6 +568,53 @@ int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R
                           int pre_kind, const float *pre_w, const float *pre_b, float pre_eps, const float *mod, const float *shift,
                           int group_rows);
 
+/* ------------------------------------------------------------------ group norm and state space blocks
+ * What networks need whose blocks mix the tokens of an image or video by a state instead of attention (or beside it), and the group norm that
+ * image networks put between their convolutions.  No counterpart in the reference's forward path.  Inference only, fp32.
+ *
+ * Activations are EDDLHIP_ACT_NONE, _RELU (max(x, 0); NaN stays) or _SILU (x / (1 + e^-x)). */
+#define EDDLHIP_ACT_NONE 0
+#define EDDLHIP_ACT_RELU 1
+#define EDDLHIP_ACT_SILU 2
+
+/* The norm of groups of channels side by side, over all pixels of an image, and its activation:
+ *     n = (x - mean) / sqrt(variance + eps) w + b,   Y = act(n (1 + mod) + shift).
+ * channels_last == 0: maps X, Y [images][channels][pixels], ldx and ldy are not looked at.  Otherwise rows of tokens [images * pixels][channels] that lie
+ * ldx and ldy floats apart.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
+ * whose group holds an infinity or NaN is NaN in that group; images and groups do not reach one another. */
+int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last,
+                       int groups, const float *w, const float *b, float eps, const float *mod, const float *shift, int activation);
+
+/* Batches of the two operators below: int tensors on the device, read when the kernels run, so that a recorded graph follows them:
+ *     offsets [seqs + 1]          rows offsets[s] .. offsets[s + 1] - 1 are the new tokens of sequence s (maybe none)
+ *     lengths [seqs]              tokens of the sequence so far, the new ones included: a sequence with no more than the new ones begins with them
+ *     slots, out_slots [seqs]     where in the pool the state lies that the sequence continues, and where its state goes (the same ones as a rule; others
+ *                                 keep the state before the call, or start several sequences from one)
+ * A sequence that begins starts from zeros and its slot is not read.  One without new tokens neither reads nor writes a state.  A slot outside the pool: a sequence that
+ * continues it comes out as NaN in all that the state reaches; a state that goes there is not kept.  states NULL (pool 0): every sequence begins, no state is
+ * kept, and lengths and slots are not looked at.  What a call writes to a slot no other sequence of the call may read or write.
+ * Rows before offsets[0] and from offsets[seqs] on are neither read nor written, no access leaves the buffers whatever the tensors hold; the rows of
+ * sequences must not overlap.  max_new is the host's bound of a sequence's new tokens: it sizes the launch, and sequences beyond it come out right too, only
+ * slower.  reverse != 0: tokens are taken from the last new one to the first, in the state as well. */
+
+/* The short convolution of every channel along the tokens: Y[t][c] = act(bias[c] + sum_k W[c][k] x[t - width + 1 + k][c]), width 2 to 8.  Before the new tokens
+ * stand the inputs in the state, [pool][width - 1][channels], the oldest first; the state afterwards holds the last width - 1 inputs, as they are.
+ * bias may be NULL.  Y must not lie on X. */
+int eddlhip_causal_conv(int dev, const float *X, long long ldx, const float *W, const float *bias, float *Y, long long ldy, int rows, int channels,
+                        int width, int activation, int reverse, float *states, int pool, const int *offsets, const int *lengths,
+                        const int *slots, const int *out_slots, int seqs, int max_new);
+
+/* The selective scan: for every channel c a state of n numbers (1 to 64), for every token
+ *     d = dt + dt_bias[c], with softplus != 0 log(1 + e^d) of that,
+ *     h[c][i] = e^(d A[c][i]) h[c][i] + d x B[i],   Y = (sum_i C[i] h[c][i] + skip[c] x) silu(gate).
+ * X, dt, gate, Y [rows][channels]; B and C [rows][groups * n], a vector for each of `groups` equal parts of the channels; A [channels][n]; skip and dt_bias
+ * [channels] may be NULL (0), gate too (no factor).  The state is [pool][channels][n].  Y and the states lie on nothing else that is read.
+ * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  Sums and states are fp32. */
+int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
+                           const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,
+                           int rows, int channels, int n, int groups, int softplus, int reverse, float *states, int pool,
+                           const int *offsets, const int *lengths, const int *slots, const int *out_slots, int seqs, int max_new);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,382 @@
+"""Group norm, causal convolution and selective scan against their formulas in 64 bits."""
+import numpy as np
+import pytest
+
+from state_space_ref import EPS, causal_conv, group_norm, selective_scan
+
+pytestmark = pytest.mark.gpu
+
+TINY = 2.0 ** -120  # what numbers below the normal ones may lose
+
+
+def _check(got, want, err, what=""):
+    """Every number within its bound; where the formula gives none (or rows are of no sequence) ``got`` is not looked at."""
+    fine = np.isfinite(want)
+    off = np.abs(got.astype(np.float64) - want)[fine]
+    worst = float((off / (err[fine] + TINY)).max()) if off.size else 0.0
+    assert np.all(off <= err[fine] + TINY), (what, worst)
+    return worst
+
+
+# ------------------------------------------------------------------------------------------------- group norm
+SHAPES = [(1, 1, 1, 1, 1), (2, 4, 1, 1, 2), (1, 512, 7, 7, 32), (3, 6, 5, 1, 3), (2, 64, 33, 31, 8), (5, 30, 3, 4, 10), (1, 128, 64, 64, 1), (2, 66, 37, 37, 11), (4, 96, 14, 14, 32),
+          (1, 2, 300, 301, 1), (1, 1, 1024, 1024, 1), (2, 320, 16, 16, 32), (65, 32, 2, 2, 4), (1, 4096, 3, 3, 4), (1, 8, 257, 255, 2), (1, 24, 1, 700, 24), (1, 7, 1, 40000, 7)]
+
+
+@pytest.mark.parametrize("images, channels, height, width, groups", SHAPES)
+@pytest.mark.parametrize("kind", [None, "relu", "silu"])
+def test_group_norm(hip, images, channels, height, width, groups, kind):
+    rng = np.random.default_rng([images, channels, height, groups])
+    n = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    pixels = height * width
+    x = n(images, channels, pixels) * (0.5 + rng.random((1, channels, 1), dtype=np.float32)) + 0.5 * n(1, channels, 1)
+    full = kind != "relu"
+    w, b = (1 + 0.1 * n(channels), 0.1 * n(channels)) if full else (None, None)
+    mod, shift = (0.2 * n(images, channels), 0.2 * n(images, channels)) if kind == "silu" else (None, None)
+    want, err = group_norm(x, groups, w, b, 1e-5, mod, shift, kind)
+    d = lambda t: None if t is None else hip.array(t)
+    args = dict(weight=d(w), bias=d(b), eps=1e-5, activation=kind, mod=d(mod), shift=d(shift))
+    X = hip.array(x.reshape(images, channels, height, width))
+    Y = hip.full(X.shape, -7.0)
+    hip.group_norm(X, Y, groups, **args)
+    got = Y.numpy()
+    _check(got.reshape(x.shape), want, err, "maps")
+    hip.group_norm(X, X, groups, **args)
+    assert np.array_equal(X.numpy(), got)
+    # the same as rows of tokens, channels last, whole and as columns of a wider tensor, at even and odd distances
+    rows = np.ascontiguousarray(x.transpose(0, 2, 1)).reshape(images * pixels, channels)
+    R = hip.array(rows)
+    Y = hip.full(R.shape, -7.0)
+    hip.group_norm(R, Y, groups, image_rows=pixels, **args)
+    got = Y.numpy()
+    back = lambda t: t.reshape(images, pixels, channels).transpose(0, 2, 1)
+    _check(back(got), want, err, "rows")
+    hip.group_norm(R, R, groups, image_rows=pixels, **args)
+    assert np.array_equal(R.numpy(), got)
+    if rows.size > 1 << 20:
+        return
+    for before, behind in ((4, 8), (3, 2)):
+        wide = np.full((len(rows), channels + before + behind), -7.0, np.float32)
+        wide[:, before:before + channels] = rows
+        W, O = hip.array(wide), hip.full((len(rows), channels + behind), -7.0)
+        hip.group_norm(W.columns(before, before + channels), O.columns(behind, behind + channels), groups, image_rows=pixels, **args)
+        o = O.numpy()
+        _check(back(o[:, behind:]), want, err, ("columns", before, behind))
+        assert np.all(o[:, :behind] == -7.0)
+
+
+def test_group_norm_keeps_images_and_groups_apart(hip):
+    """Infinities and NaN reach their own group of their own image only; a group that is constant is its bias, far from 0 too."""
+    rng = np.random.default_rng(3)
+    for channels, pixels, groups in ((8, 100, 4), (64, 1500, 4), (6, 40000, 2)):
+        x = rng.standard_normal((3, channels, pixels), dtype=np.float32)
+        b = rng.standard_normal(channels, dtype=np.float32)
+        per = channels // groups
+        x[0, 0, 3], x[1, per, 7], x[2, channels - 1, pixels - 1] = np.inf, np.nan, -np.inf
+        x[1, :per] = 1e4
+        want, err = group_norm(np.where(np.isfinite(x), x, 0), groups, None, b, 1e-5, None, None, None)
+        for i, g in ((0, 0), (1, 1), (2, groups - 1)):
+            want[i, g * per:(g + 1) * per] = np.nan
+        X = hip.array(x.reshape(3, channels, pixels, 1))
+        hip.group_norm(X, X, groups, bias=hip.array(b))
+        got = X.numpy().reshape(x.shape)
+        _check(got, want, err)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        R = hip.array(x.transpose(0, 2, 1).reshape(-1, channels))
+        hip.group_norm(R, R, groups, bias=hip.array(b), image_rows=pixels)
+        got = R.numpy().reshape(3, pixels, channels).transpose(0, 2, 1)
+        _check(got, want, err)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+
+
+def test_group_norm_far_from_zero(hip):
+    """A mean a thousand times the spread: the variance is that of the differences, not a difference of squares."""
+    rng = np.random.default_rng(4)
+    for channels, side, groups in ((16, 10, 2), (4, 400, 2)):
+        x = (1000 + rng.standard_normal((2, channels, side * side))).astype(np.float32)
+        want, err = group_norm(x, groups, None, None, 1e-5, None, None, None)
+        X = hip.array(x.reshape(2, channels, side, side))
+        hip.group_norm(X, X, groups)
+        _check(X.numpy().reshape(x.shape), want, err)
+
+
+# ------------------------------------------------------------------------------------------------- batches
+class Ragged:
+    """Sequences of ``news`` new tokens with rows before and behind them that belong to none, and a pool whose slots are in no order."""
+
+    def __init__(self, rng, news, before=2, behind=3, kept=True, apart=True):
+        self.news = np.asarray(news)
+        self.offsets = (before + np.concatenate([[0], np.cumsum(self.news)])).astype(np.int32)
+        self.rows, seqs = int(self.offsets[-1]) + behind, len(news)
+        order = rng.permutation(2 * seqs + 1).astype(np.int32)
+        self.pool = 2 * seqs + 1
+        self.slots, self.out_slots = order[:seqs], order[seqs:2 * seqs] if apart else order[:seqs]
+        self.lengths = (self.news + np.where(np.arange(seqs) % 3 == 1, 0, rng.integers(1, 90, seqs))).astype(np.int32)
+        self.kept, self.apart = kept, apart
+
+    def on(self, hip, max_new=None):
+        from eddl_amd.state_space import StateBatch
+        i = lambda t: hip.array(t, "int32")
+        kept = dict(lengths=i(self.lengths), slots=i(self.slots), out_slots=i(self.out_slots) if self.apart else None) if self.kept else {}
+        return StateBatch(i(self.offsets), max(1, int(self.news.max(initial=0))) if max_new is None else max_new, **kept)
+
+    def reference(self, pool):
+        return dict(offsets=self.offsets, **(dict(pool=pool, lengths=self.lengths, slots=self.slots, out_slots=self.out_slots) if self.kept else {}))
+
+    def outside(self, y):
+        return np.concatenate([y[:self.offsets[0]], y[self.offsets[-1]:]])
+
+
+NEWS = [[1], [5], [0, 1, 2, 3], [1] * 9, [16, 17, 0, 15, 33], [130, 1, 64], [300], [129, 7, 0, 200, 128]]
+
+
+# ------------------------------------------------------------------------------------------------- causal convolution
+@pytest.mark.parametrize("width", [2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("channels", [1, 7, 64, 130, 260, 1028])
+def test_causal_conv(hip, width, channels):
+    rng = np.random.default_rng([width, channels])
+    n = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    for turn, news in enumerate(NEWS):
+        kind, reverse, bias = (None, "silu", "relu")[turn % 3], turn % 2 == 1, None if turn == 3 else n(channels)
+        batch = Ragged(rng, news, kept=turn % 4 != 2, apart=turn % 3 != 1)
+        x, w, pool = n(batch.rows, channels), n(channels, width), n(batch.pool, width - 1, channels)
+        want, err, after, = causal_conv(x, w, bias, kind=kind, reverse=reverse, **batch.reference(pool))
+        for at, ld in ((0, channels), (3, channels + 5), (4, channels + 8 - channels % 4)):  # whole tensors, and columns of wider ones
+            X, S = np.full((batch.rows, ld), 9.0, np.float32), hip.array(pool)
+            X[:, at:at + channels] = x
+            X, Y = hip.array(X), hip.full((batch.rows, ld), -7.0)
+            hip.causal_conv(X.columns(at, at + channels), hip.array(w), None if bias is None else hip.array(bias), Y.columns(0, channels), batch.on(hip, (None, 1, 1000)[turn % 3]),
+                            states=S if batch.kept else None, activation=kind, reverse=reverse)
+            y = Y.numpy()
+            _check(y[:, :channels], want, err, (news, at))
+            assert np.all(batch.outside(y) == -7.0) and np.all(y[:, channels:] == -7.0)
+            assert np.array_equal(S.numpy(), after if batch.kept else pool)
+
+
+def test_causal_conv_in_pieces(hip):
+    """A sequence in calls of a few tokens each, its state kept in one slot: the bits of one call."""
+    from eddl_amd.state_space import StateBatch
+    rng = np.random.default_rng(5)
+    n = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    tokens, channels, width = 70, 36, 4
+    x, w, b = n(tokens, channels), n(channels, width), n(channels)
+    i = lambda *t: hip.array(np.array(t), "int32")
+    W, b, Y = hip.array(w), hip.array(b), hip.empty((tokens, channels))
+    hip.causal_conv(hip.array(x), W, b, Y, StateBatch(i(0, tokens), tokens), activation="silu")
+    S, at, got = hip.full((2, width - 1, channels), np.nan), 0, []
+    for piece in (1, 1, 2, 16, 1, 30, 19):
+        P = hip.empty((piece, channels))
+        hip.causal_conv(hip.array(x[at:at + piece]), W, b, P, StateBatch(i(0, piece), piece, i(at + piece), i(1)), states=S, activation="silu")
+        got.append(P.numpy())
+        at += piece
+    assert at == tokens and np.array_equal(np.concatenate(got), Y.numpy())
+    assert np.array_equal(S.numpy()[1], x[-3:]) and np.all(np.isnan(S.numpy()[0]))
+
+
+# ------------------------------------------------------------------------------------------------- selective scan
+def _scan_case(rng, batch, channels, n, groups, softplus=True, gate=True, skip=True):
+    r = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    rows = batch.rows
+    steps = np.exp(rng.random(channels) * np.log(100) + np.log(0.001))
+    return dict(x=r(rows, channels), dt=0.5 * r(rows, channels) if softplus else (steps * np.exp(0.3 * r(rows, channels))).astype(np.float32),
+                dt_bias=(steps + np.log(-np.expm1(-steps))).astype(np.float32) if softplus else None,
+                A=(-np.arange(1, n + 1) * (0.8 + 0.4 * rng.random((channels, n)))).astype(np.float32), B=r(rows, groups * n), C=r(rows, groups * n),
+                skip=r(channels) if skip else None, gate=2 * r(rows, channels) if gate else None, softplus=softplus)
+
+
+def _scan(hip, case, batch, pool, reverse, max_new=None, at=0, wider=0):
+    """(output, pool afterwards) of the call on columns of tensors that are ``wider``."""
+    def columns(t):
+        if t is None:
+            return None
+        wide = np.full((len(t), t.shape[1] + wider), 9.0, np.float32)
+        wide[:, at:at + t.shape[1]] = t
+        return hip.array(wide).columns(at, at + t.shape[1])
+    d = lambda t: None if t is None else hip.array(t)
+    channels = case["x"].shape[1]
+    Y, S = hip.full((batch.rows, channels + wider), -7.0), hip.array(pool)
+    hip.selective_scan(columns(case["x"]), columns(case["dt"]), d(case["A"]), columns(case["B"]), columns(case["C"]), Y.columns(at, at + channels), batch.on(hip, max_new),
+                       states=S if batch.kept else None, skip=d(case["skip"]), gate=columns(case["gate"]), dt_bias=d(case["dt_bias"]), softplus=case["softplus"], reverse=reverse)
+    y = Y.numpy()
+    outside = np.concatenate([y[:, :at], y[:, at + channels:]], 1)
+    assert np.all(outside == -7.0)
+    return y[:, at:at + channels], S.numpy()
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 12, 16, 17, 24, 32, 48, 64])
+@pytest.mark.parametrize("channels, groups", [(1, 1), (6, 3), (64, 1), (130, 2), (264, 1)])
+def test_selective_scan(hip, n, channels, groups):
+    rng = np.random.default_rng([n, channels])
+    for turn, news in enumerate(NEWS):
+        batch = Ragged(rng, news, kept=turn % 4 != 2, apart=turn % 3 != 1)
+        case = _scan_case(rng, batch, channels, n, groups, softplus=turn % 3 != 0, gate=turn % 4 != 3, skip=turn % 5 != 4)
+        reverse, pool = turn % 2 == 1, rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+        want, err, after, after_err = selective_scan(reverse=reverse, **case, **batch.reference(pool))
+        for at, wider in ((0, 0), (3, 5), (4, 8)):
+            y, s = _scan(hip, case, batch, pool, reverse, (None, 1, 1000)[(turn + at) % 3], at, wider)
+            _check(y, want, err, (news, at))
+            assert np.all(batch.outside(y) == -7.0)
+            if batch.kept:
+                _check(s, after, after_err, (news, "state"))
+                untouched = np.ones(batch.pool, bool)
+                untouched[batch.out_slots[batch.news > 0]] = False
+                assert np.array_equal(s[untouched], pool[untouched])
+
+
+@pytest.mark.parametrize("channels, n, news", [(16, 16, [5000]), (5, 16, [3001, 40]), (64, 16, [2000]), (128, 4, [1500, 1000]), (40, 1, [4000]), (33, 64, [1025]), (600, 16, [700, 30, 2, 650]),
+                                               (1500, 8, [400] * 3)])
+def test_selective_scan_of_long_sequences(hip, channels, n, news):
+    rng = np.random.default_rng([channels, n])
+    batch = Ragged(rng, news, apart=False)
+    case = _scan_case(rng, batch, channels, n, 1)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    for reverse in (False, True):
+        want, err, after, after_err = selective_scan(reverse=reverse, **case, **batch.reference(pool))
+        y, s = _scan(hip, case, batch, pool, reverse)
+        _check(y, want, err)
+        _check(s, after, after_err)
+        assert np.all(batch.outside(y) == -7.0)
+        again, t = _scan(hip, case, batch, pool, reverse)
+        assert np.array_equal(y, again) and np.array_equal(s, t)
+
+
+def test_selective_scan_of_growing_and_of_constant_states(hip):
+    """A of 0 keeps what came, a positive one grows; steps of 0 leave the state as it is, steps of 40 wipe it."""
+    rng = np.random.default_rng(6)
+    for channels, n in ((20, 16), (64, 4), (3, 1)):
+        batch = Ragged(rng, [150, 20])
+        case = _scan_case(rng, batch, channels, n, 1, softplus=False)
+        case["A"][:, 0] = 0
+        case["A"][1, :] = 0.5
+        case["dt"][:, 2 % channels] = 0
+        case["dt"][10:60:7] = 40 / np.arange(1, channels + 1) ** 2
+        case["A"][case["A"] > 0.4] = 0.02
+        pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+        want, err, after, after_err = selective_scan(**case, **batch.reference(pool))
+        y, s = _scan(hip, case, batch, pool, False)
+        _check(y, want, err)
+        _check(s, after, after_err)
+
+
+def test_softplus_over_its_range(hip):
+    """One token whose state starts from zeros and whose A is 0: the output is d itself, within 14 EPS from steps of e^-80 to steps of 100."""
+    from eddl_amd.state_space import StateBatch
+    v = np.concatenate([np.linspace(-80, 100, 3000), np.linspace(-1, 1, 500), -np.logspace(-8, 1, 300), np.logspace(-8, 1, 200)]).astype(np.float32)
+    X, one = hip.full((1, len(v)), 1.0), hip.full((1, 1), 1.0)
+    Y = hip.empty(X.shape)
+    hip.selective_scan(X, hip.array(v[None]), hip.full((len(v), 1), 0.0), one, one, Y, StateBatch(hip.array(np.array([0, 1]), "int32"), 1))
+    want = np.logaddexp(v.astype(np.float64), 0)
+    off = np.abs(Y.numpy()[0] - want) / want
+    assert off.max() <= 14 * EPS, (off.max() / EPS, v[off.argmax()])
+
+
+def test_gate_over_its_range(hip):
+    from eddl_amd.state_space import StateBatch
+    v = np.concatenate([np.linspace(-80, 100, 3000), np.linspace(-1, 1, 500)]).astype(np.float32)
+    X, one = hip.full((1, len(v)), 1.0), hip.full((1, 1), 0.0)
+    Y = hip.empty(X.shape)
+    hip.selective_scan(X, X, hip.full((len(v), 1), 0.0), one, one, Y, StateBatch(hip.array(np.array([0, 1]), "int32"), 1), skip=hip.full((len(v),), 1.0), gate=hip.array(v[None]),
+                       softplus=False)
+    v = v.astype(np.float64)
+    want = v / (1 + np.exp(-v))
+    off = np.abs(Y.numpy()[0] - want) / np.maximum(np.abs(want), 2.0 ** -100)
+    assert off.max() <= 11 * EPS, off.max() / EPS
+
+
+@pytest.mark.parametrize("channels, n", [(20, 16), (64, 4), (7, 1), (130, 64)])
+def test_infinities_and_nan_stay_in_their_channel(hip, channels, n):
+    """An input that is not finite: from its token on the channel is infinite or NaN, before it and in other channels and sequences nothing changes by a bit.  A
+    NaN among B or C reaches the channels that share them.  Slots that a sequence does not continue are not read."""
+    rng = np.random.default_rng(7)
+    batch = Ragged(rng, [140, 33, 1])
+    case = _scan_case(rng, batch, channels, n, 1)
+    case["A"] = np.maximum(case["A"], -2)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    pool[batch.slots[1]] = np.nan  # (sequence 1 begins)
+    y, s = _scan(hip, case, batch, pool, False)
+    assert np.all(np.isfinite(y[batch.offsets[0]:batch.offsets[-1]]))
+    for value in (np.inf, np.nan):
+        bad = dict(case, x=case["x"].copy())
+        at = int(batch.offsets[0]) + 77
+        bad["x"][at, 2] = value
+        y2, s2 = _scan(hip, bad, batch, pool, False)
+        end = int(batch.offsets[1])
+        assert not np.any(np.isfinite(y2[at:end, 2])) and not np.any(np.isfinite(s2[batch.out_slots[0], 2]))
+        y2[at:end, 2], s2[batch.out_slots[0], 2] = y[at:end, 2], s[batch.out_slots[0], 2]
+        assert np.array_equal(y, y2) and np.array_equal(s, s2, equal_nan=True)
+    bad = dict(case, C=case["C"].copy())
+    bad["C"][at, n - 1] = np.nan
+    y2, s2 = _scan(hip, bad, batch, pool, False)
+    assert np.all(np.isnan(y2[at])) and np.array_equal(s, s2, equal_nan=True)
+    y2[at] = y[at]
+    assert np.array_equal(y, y2)
+
+
+def test_slots_outside_the_pool(hip):
+    """A sequence that continues a state outside the pool is NaN, one whose state goes there is right and not kept; nothing else changes.  Offsets that
+    run backwards or out of range are cut."""
+    rng = np.random.default_rng(8)
+    for channels, n in ((12, 16), (70, 3)):
+        for news in ([1, 1, 1, 1], [20, 200, 3, 150]):
+            batch = Ragged(rng, news)
+            batch.lengths[:] = batch.news + 5
+            case = _scan_case(rng, batch, channels, n, 1)
+            pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+            batch.slots[1], batch.out_slots[2], batch.out_slots[3] = batch.pool, -1, 1 << 30
+            want, err, after, after_err = selective_scan(**case, **batch.reference(pool))
+            y, s = _scan(hip, case, batch, pool, False)
+            _check(y, want, err)
+            _check(s, after, after_err)
+            lost = slice(int(batch.offsets[1]), int(batch.offsets[2]))
+            assert np.all(np.isnan(y[lost])) and np.all(np.isnan(s[batch.out_slots[1]])) and np.array_equal(np.isnan(s), np.isnan(after))
+            x, w, states = case["x"], rng.standard_normal((channels, 4), dtype=np.float32), rng.standard_normal((batch.pool, 3, channels), dtype=np.float32)
+            want, err, after = causal_conv(x, w, None, kind="silu", reverse=False, **batch.reference(states))
+            Y, S = hip.full(x.shape, -7.0), hip.array(states)
+            hip.causal_conv(hip.array(x), hip.array(w), None, Y, batch.on(hip), states=S, activation="silu")
+            y = Y.numpy()
+            _check(y, want, err)
+            first = int(batch.offsets[1])
+            assert np.all(np.isnan(y[first:first + min(news[1], 3)])) and np.array_equal(S.numpy(), after, equal_nan=True)
+            batch.offsets[:] = [-5, 7, 3, 1 << 30, -(1 << 31)]
+            batch.lengths[:] = 0
+            batch.out_slots[:] = -1
+            for reverse in (False, True):
+                want, err = selective_scan(reverse=reverse, **case, **batch.reference(pool))[:2]
+                y, s = _scan(hip, case, batch, pool, reverse)
+                # (sequences 0 and 2 share rows 3 .. 6, whose results are those of either)
+                _check(y[7:], want[7:], err[7:])
+                assert np.array_equal(s, pool)
+
+
+def test_single_tokens_continue_a_prompt(hip):
+    """A prompt, then token by token and in small pieces, against the whole sequence at once: both within the bounds."""
+    from eddl_amd.state_space import StateBatch
+    rng = np.random.default_rng(9)
+    for channels, n in ((48, 16), (20, 5), (256, 32)):
+        tokens, batch = 160, Ragged(rng, [160], before=0, behind=0, kept=False)
+        case = _scan_case(rng, batch, channels, n, 1)
+        want, err = selective_scan(offsets=[0, tokens], **case)[:2]
+        S = hip.full((3, channels, n), np.nan)
+        at = 0
+        i = lambda *t: hip.array(np.array(t), "int32")
+        d = lambda t: hip.array(t[at:at + piece])
+        for piece in (100, 1, 1, 1, 2, 7, 1, 17, 30):
+            Y = hip.empty((piece, channels))
+            hip.selective_scan(d(case["x"]), d(case["dt"]), hip.array(case["A"]), d(case["B"]), d(case["C"]), Y, StateBatch(i(0, piece), piece, i(at + piece), i(2)), states=S,
+                               skip=hip.array(case["skip"]), gate=d(case["gate"]), dt_bias=hip.array(case["dt_bias"]))
+            _check(Y.numpy(), want[at:at + piece], err[at:at + piece], at)
+            at += piece
+        assert at == tokens and np.all(np.isnan(S.numpy()[:2]))
+
+
+def test_empty_calls(hip):
+    from eddl_amd.state_space import StateBatch
+    none, E, V = StateBatch(hip.array(np.zeros(3), "int32") if False else hip.array(np.zeros(3, np.int32), "int32"), 1), hip.empty((0, 8)), hip.empty((0, 4))
+    hip.causal_conv(E, hip.full((8, 4), 1.0), None, E, none)
+    hip.selective_scan(E, E, hip.full((8, 4), 1.0), V, V, E, none)
+    hip.group_norm(E, E, 2)
+    hip.group_norm(hip.empty((0, 8, 3, 3)), hip.empty((0, 8, 3, 3)), 2)
+    X, Y, V = hip.full((5, 8), 1.0), hip.full((5, 8), -7.0), hip.full((5, 4), 1.0)
+    hip.causal_conv(X, hip.full((8, 4), 1.0), None, Y, none)
+    hip.selective_scan(X, X, hip.full((8, 4), 1.0), V, V, Y, none)
+    assert np.all(Y.numpy() == -7.0)
