@@ -6,7 +6,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SOURCES = ["runtime.hip", "elementwise.hip", "pool.hip", "conv.hip", "dense.hip", "generator.hip",
-           "attention.hip", "rotary.hip", "norm.hip", "group_norm.hip", "state_space.hip"]
+           "attention.hip", "rotary.hip", "norm.hip", "group_norm.hip", "causal_conv.hip", "selective_scan.hip"]
 LIB = os.path.join(HERE, "libeddlhip.so")
 # the benchmark's device probes: a library of their own beside the C ABI (include/eddlhip_probe.h)
 PROBE_SOURCES = ["probe.hip"]

@@ -1,0 +1,489 @@
+// The selective scan
+//     d = softplus(dt + dt_bias),   h[c][n] = e^(d A[c][n]) h[c][n] + d x B[n],   y = (sum_n C[n] h[c][n] + skip x) silu(gate),
+// token by token, over ragged batches of sequences whose states lie in slots of a pool.
+#include <algorithm>
+
+#include "common.h"
+#include "activation.h"
+#include "state_batch.h"
+
+using namespace eddlhip;
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+struct ScanParams {
+    const float *X, *dt, *gate, *B, *C, *A, *skip, *dt_bias;
+    float *Y, *states;
+    float *part_states, *part_factors;  // [sequence][part + 1][channel][NP], [sequence][part][channel][NP]
+    long long ldx, lddt, ldg, ldb, ldc, ldy;
+    int channels, n, per;  // channels that share B and C
+    int blocks, group_blocks, parts;
+    long long jobs;
+    bool softplus, vectors;  // B and C are read 16 bytes at a time
+    StateBatch batch;
+};
+
+// Sums over LANES lanes side by side, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float swapped(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float x) {
+    if constexpr (LANES >= 2) x += swapped<0xB1>(x);    // the neighbour
+    if constexpr (LANES >= 4) x += swapped<0x4E>(x);    // the other pair of four
+    if constexpr (LANES >= 8) x += swapped<0x141>(x);   // the other four of eight, mirrored
+    if constexpr (LANES >= 16) x += swapped<0x140>(x);  // the other eight of sixteen, mirrored
+    return x;
+}
+
+// The NL states of channel c from n0 on: as the sequence finds them, and on their way to the pool; the factors of the steps in powers of two.
+template <int NL>
+__device__ __forceinline__ void first_state(const ScanParams &p, const Sequence &q, int c, int n0, float (&h)[NL]) {
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        h[i] = 0.0f;
+        if (q.read >= 0 && n0 + i < p.n) h[i] = p.states[((long long)q.read * p.channels + c) * p.n + n0 + i];
+        if (q.read == -2) h[i] = __builtin_nanf("");
+    }
+}
+template <int NL>
+__device__ __forceinline__ void keep_state(const ScanParams &p, const Sequence &q, int c, int n0, const float (&h)[NL]) {
+    if (q.write < 0) return;
+#pragma unroll
+    for (int i = 0; i < NL; i++)
+        if (n0 + i < p.n) p.states[((long long)q.write * p.channels + c) * p.n + n0 + i] = h[i];
+}
+template <int NL>
+__device__ __forceinline__ void exponents(const ScanParams &p, int c, int n0, float (&a)[NL]) {
+#pragma unroll
+    for (int i = 0; i < NL; i++) a[i] = n0 + i < p.n ? p.A[(long long)c * p.n + n0 + i] * LOG2_E : 0.0f;
+}
+
+// Few tokens a sequence: LANES lanes a channel, NL states each; token after token from memory.
+template <int LANES, int NL>
+__global__ __launch_bounds__(256) void scan_tokens_kernel(const ScanParams p) {
+    const Sequence q = sequence(p.batch, blockIdx.y);
+    const int c = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES, n0 = lane * NL;
+    if (q.fresh == 0 || c >= p.channels) return;
+    float a[NL], h[NL];
+    exponents<NL>(p, c, n0, a);
+    first_state<NL>(p, q, c, n0, h);
+    const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.skip ? p.skip[c] : 0.0f;
+    const int v0 = c / p.per * p.n + n0;
+    for (int t = 0; t < q.fresh; t++) {
+        const long long row = q.row(t);
+        const float raw = p.dt[row * p.lddt + c] + bias, d = p.softplus ? softplus(raw) : raw, x = p.X[row * p.ldx + c], dx = d * x;
+        float y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const bool has = n0 + i < p.n;
+            const float b = has ? p.B[row * p.ldb + v0 + i] : 0.0f, cc = has ? p.C[row * p.ldc + v0 + i] : 0.0f;
+            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a[i]), h[i], dx * b);
+            y = __builtin_fmaf(cc, h[i], y);
+        }
+        y = lane_sum<LANES>(y);
+        if (lane == 0) {
+            if (p.skip) y = __builtin_fmaf(skip, x, y);
+            if (p.gate) y *= silu(p.gate[row * p.ldg + c]);
+            p.Y[row * p.ldy + c] = y;
+        }
+    }
+    keep_state<NL>(p, q, c, n0, h);
+}
+
+// Many tokens.  A workgroup of eight wavefronts takes a tile of tokens of some channels into LDS - steps d, products d x, vectors B and C - and
+// walks it with LANES lanes a channel, NL states each.  WT of the wavefronts divide the tile's tokens, the others its channels.  With WT > 1 a wavefront first
+// brings its tokens' state from zeros (keeping the factors e^(d A), the dearest part, in registers), then takes in what the wavefronts
+// before it brought, and walks its tokens again with the state that they begin with.
+constexpr int SCAN_THREADS = 512;
+template <int LANES, int NL, int WT>
+struct ScanTile {
+    static constexpr int TT = LANES == 4 ? 16 : 8;          // tokens of a wavefront
+    static constexpr int TOKENS = TT * WT;                  // of a tile
+    static constexpr int CHANNELS = 64 / LANES * (8 / WT);  // of a workgroup
+    static constexpr int NP = LANES * NL;                   // states, with those behind the last
+    static constexpr int STRIDE = TOKENS + 4;               // floats from a channel's steps to the next one's (neighbours' 16 bytes lie in banks of their own)
+    static constexpr int QUADS = TOKENS * CHANNELS / 4;     // numbers of four channels side by side
+    static constexpr int PER = (QUADS + SCAN_THREADS - 1) / SCAN_THREADS;
+    static constexpr int VECTORS = TOKENS * LANES;          // pieces of NL numbers of B or C
+    static constexpr int VPER = (VECTORS + SCAN_THREADS - 1) / SCAN_THREADS;
+};
+
+// PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups: PART 1 brings the state of every part from
+// zeros and the factor of what comes before it, PART 2 takes in the parts before its own and brings the outputs.
+template <int LANES, int NL, int WT, bool VEC, int PART>
+__global__ __launch_bounds__(SCAN_THREADS, 4) void scan_tile_kernel(const ScanParams p) {
+    using T = ScanTile<LANES, NL, WT>;
+    typedef float vec __attribute__((ext_vector_type(NL)));
+    constexpr int SETS = 64 * (8 / WT);  // lanes that walk the same tokens
+    __shared__ __attribute__((aligned(16))) float steps[T::CHANNELS * T::STRIDE], inputs[T::CHANNELS * T::STRIDE];  // d and d x, whose place the outputs take
+    __shared__ __attribute__((aligned(16))) vec vb[T::VECTORS], vc[PART == 1 ? 1 : T::VECTORS];
+    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? SCAN_THREADS : 1], factor[WT > 1 ? SCAN_THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
+
+    // Workgroups side by side in channels share lines of memory: they are put on one XCD.
+    const long long per_xcd = (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
+    for (long long id = blockIdx.x; id < per_xcd * EDDLHIP_NUM_XCD; id += gridDim.x) {
+    const long long job = id % EDDLHIP_NUM_XCD * per_xcd + id / EDDLHIP_NUM_XCD;
+    if (job >= p.jobs) continue;
+    const int block = (int)(job % p.blocks), group = block / p.group_blocks, part = (int)(job / p.blocks % p.parts), s = (int)(job / p.blocks / p.parts);
+    const Sequence q = sequence(p.batch, s);
+    const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + p.parts - 1) / p.parts;  // (of a part)
+    const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
+    if (tile0 == tile1) continue;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
+    const int c0 = group * p.per + block % p.group_blocks * T::CHANNELS, cend = (group + 1) * p.per;
+    const int ch = wc * (64 / LANES) + lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
+    const bool mine = c < cend;
+
+    float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a part)
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+        a[i] = h[i] = 0.0f;
+        through[i] = 1.0f;
+    }
+    if (mine) exponents<NL>(p, c, n0, a);
+    if (mine && wt == 0) {
+        float *states = PART ? p.part_states + ((long long)s * (p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
+        if (PART == 0) {
+            first_state<NL>(p, q, c, n0, h);
+        } else if (PART == 1) {
+            if (part == 0) {  // kept for the second launch, in which the slot may be written already
+                float kept[NL];
+                first_state<NL>(p, q, c, n0, kept);
+#pragma unroll
+                for (int i = 0; i < NL; i++) states[i] = kept[i];
+            }
+        } else {
+            const float *factors = p.part_factors + ((long long)s * p.parts * p.channels + c) * T::NP + n0;
+            const long long step = (long long)p.channels * T::NP;
+            const vec v = *reinterpret_cast<const vec *>(states);
+#pragma unroll
+            for (int i = 0; i < NL; i++) h[i] = v[i];
+            for (int j = 0; j < part; j++) {
+                const vec f = *reinterpret_cast<const vec *>(factors + j * step), b = *reinterpret_cast<const vec *>(states + (j + 1) * step);
+#pragma unroll
+                for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[i], h[i], b[i]);
+            }
+        }
+        if (WT > 1 && PART != 1) {
+            vec v;
+#pragma unroll
+            for (int i = 0; i < NL; i++) v[i] = h[i];
+            begin[set] = v;
+        }
+    }
+
+    // what a thread brings of a tile, one tile ahead
+    floatx4 x[T::PER], d[T::PER], g[T::PER], bias[T::PER], skip[T::PER];
+    vec b[T::VPER], cc[T::VPER];
+    constexpr int CQ = T::CHANNELS / 4;
+    const floatx4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto get4 = [&](const float *from, int at) {
+        if (VEC) return *reinterpret_cast<const floatx4 *>(from + at);
+        floatx4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = at + i < cend ? from[at + i] : 0.0f;
+        return v;
+    };
+#pragma unroll
+    for (int k = 0; k < T::PER; k++) {
+        const int e = tid + k * SCAN_THREADS, at = c0 + e % CQ * 4;
+        bias[k] = p.dt_bias && at < cend ? get4(p.dt_bias, at) : zeros;
+        skip[k] = p.skip && at < cend ? get4(p.skip, at) : zeros;
+    }
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int k = 0; k < T::PER; k++) {
+            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = c0 + e % CQ * 4;
+            x[k] = d[k] = g[k] = zeros;
+            if (e < T::QUADS && t < q.fresh && at < cend) {
+                const long long row = q.row(t);
+                x[k] = get4(p.X + row * p.ldx, at);
+                d[k] = get4(p.dt + row * p.lddt, at);
+                if (PART != 1 && p.gate) g[k] = get4(p.gate + row * p.ldg, at);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < T::VPER; k++) {
+            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / LANES, at = e % LANES * NL;
+#pragma unroll
+            for (int i = 0; i < NL; i++) b[k][i] = cc[k][i] = 0.0f;
+            if (e < T::VECTORS && t < q.fresh && at < p.n) {
+                const long long row = q.row(t);
+                const float *fb = p.B + row * p.ldb + (long long)group * p.n + at, *fc = p.C + row * p.ldc + (long long)group * p.n + at;
+                if (p.vectors) {
+                    b[k] = *reinterpret_cast<const vec *>(fb);
+                    if (PART != 1) cc[k] = *reinterpret_cast<const vec *>(fc);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NL; i++)
+                        if (at + i < p.n) {
+                            b[k][i] = fb[i];
+                            if (PART != 1) cc[k][i] = fc[i];
+                        }
+                }
+            }
+        }
+    };
+    // steps and inputs are 0 behind the sequence's last token and the last channel: the state stays
+    auto stage = [&](int tile) {
+#pragma unroll
+        for (int k = 0; k < T::PER; k++) {
+            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = e % CQ * 4;
+            if (e < T::QUADS) {
+                const bool in = t < q.fresh;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float raw = d[k][i] + bias[k][i], step = in && c0 + at + i < cend ? (p.softplus ? softplus(raw) : raw) : 0.0f;
+                    steps[(at + i) * T::STRIDE + e / CQ] = step;
+                    inputs[(at + i) * T::STRIDE + e / CQ] = step * x[k][i];
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < T::VPER; k++) {
+            const int e = tid + k * SCAN_THREADS;
+            if (e < T::VECTORS) {
+                vb[e] = b[k];
+                if (PART != 1) vc[e] = cc[k];
+            }
+        }
+    };
+
+    const float *my_steps = steps + ch * T::STRIDE + wt * T::TT;
+    float *my_inputs = inputs + ch * T::STRIDE + wt * T::TT;
+    const vec *my_b = vb + wt * T::TT * LANES + ln, *my_c = vc + (PART == 1 ? 0 : wt * T::TT * LANES + ln);
+
+    fetch(tile0);
+    for (int tile = tile0; tile < tile1; tile++) {
+        stage(tile);
+        floatx4 x0[T::PER], g0[T::PER];
+#pragma unroll
+        for (int k = 0; k < T::PER; k++) {
+            x0[k] = x[k];
+            g0[k] = g[k];
+        }
+        if (tile + 1 < tile1) fetch(tile + 1);
+        __syncthreads();
+        float kept[WT > 1 ? T::TT : 1][NL];
+        if constexpr (WT > 1) {
+            float local[NL], sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NL; i++) local[i] = 0.0f;
+#pragma unroll
+            for (int t = 0; t < T::TT; t += 4) {
+                const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const vec bv = my_b[(t + j) * LANES];
+                    sum += dv[j];
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        const float f = __builtin_amdgcn_exp2f(dv[j] * a[i]);
+                        kept[t + j][i] = f;
+                        local[i] = __builtin_fmaf(f, local[i], xv[j] * bv[i]);
+                    }
+                }
+            }
+            vec v, f;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                v[i] = local[i];
+                f[i] = __builtin_amdgcn_exp2f(sum * a[i]);
+            }
+            brought[wt * SETS + set] = v;
+            factor[wt * SETS + set] = f;
+            __syncthreads();
+            const int before = PART == 1 ? (wt == 0 ? WT : 0) : wt;
+            if (PART != 1) {
+                const vec v0 = begin[(tile - tile0 & 1) * SETS + set];
+#pragma unroll
+                for (int i = 0; i < NL; i++) h[i] = v0[i];
+            }
+            for (int w = 0; w < before; w++) {
+                const vec wf = factor[w * SETS + set], wb = brought[w * SETS + set];
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    h[i] = __builtin_fmaf(wf[i], h[i], wb[i]);
+                    if (PART == 1) through[i] *= wf[i];
+                }
+            }
+        }
+        if constexpr (PART != 1) {
+#pragma unroll
+            for (int t = 0; t < T::TT; t += 4) {
+                const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+                floatx4 y;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const vec bv = my_b[(t + j) * LANES], cv = my_c[(t + j) * LANES];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        const float f = WT > 1 ? kept[t + j][i] : __builtin_amdgcn_exp2f(dv[j] * a[i]);
+                        h[i] = __builtin_fmaf(f, h[i], xv[j] * bv[i]);
+                        sum = __builtin_fmaf(cv[i], h[i], sum);
+                    }
+                    y[j] = lane_sum<LANES>(sum);
+                }
+                if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
+            }
+            if (WT > 1 && wt == WT - 1) {
+                vec v;
+#pragma unroll
+                for (int i = 0; i < NL; i++) v[i] = h[i];
+                begin[(tile - tile0 + 1 & 1) * SETS + set] = v;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < T::PER; k++) {
+                const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = e % CQ * 4;
+                if (e < T::QUADS && t < q.fresh && c0 + at < cend) {
+                    floatx4 y;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        y[i] = inputs[(at + i) * T::STRIDE + e / CQ];
+                        if (p.skip) y[i] = __builtin_fmaf(skip[k][i], x0[k][i], y[i]);
+                        if (p.gate) y[i] *= silu(g0[k][i]);
+                    }
+                    float *to = p.Y + q.row(t) * p.ldy + c0 + at;
+                    if (VEC) {
+                        *reinterpret_cast<floatx4 *>(to) = y;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (c0 + at + i < cend) to[i] = y[i];
+                    }
+                }
+            }
+        }
+    }
+    if (PART == 1) {
+        if (mine && wt == 0) {
+            float *states = p.part_states + (((long long)s * (p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
+            float *factors = p.part_factors + (((long long)s * p.parts + part) * p.channels + c) * T::NP + n0;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                states[i] = h[i];
+                factors[i] = through[i];
+            }
+        }
+    } else if (mine && wt == WT - 1 && tile1 == tiles) {
+        keep_state<NL>(p, q, c, n0, h);
+    }
+    __syncthreads();  // (the next job's tiles)
+    }
+}
+
+constexpr int MOST_STATES = 64;
+constexpr int FEW_TOKENS = 8;  // up to here token after token from memory
+
+template <int LANES, int NL>
+int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
+    const hipStream_t st = state(dev).stream;
+    if (tokens <= FEW_TOKENS) {
+        hipLaunchKernelGGL((scan_tokens_kernel<LANES, NL>), dim3((unsigned)(((long long)p.channels * LANES + 255) / 256), seqs), dim3(256), 0, st, p);
+        EH_CHECK_LAUNCH();
+        return 0;
+    }
+    const int groups = p.channels / p.per, num_cu = state(dev).num_cu;
+    auto sized = [&](auto wt) {
+        using T = ScanTile<LANES, NL, decltype(wt)::value>;
+        p.group_blocks = (p.per + T::CHANNELS - 1) / T::CHANNELS;
+        p.blocks = groups * p.group_blocks;
+    };
+    auto launch = [&](auto fn) {
+        p.jobs = (long long)p.blocks * p.parts * seqs;
+        const long long most = 1 << 22;  // workgroups (a grid holds less than 2^32 threads); they walk what is beyond
+        hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(SCAN_THREADS), 0, st, p);
+        EH_CHECK_LAUNCH();
+        return 0;
+    };
+    p.parts = 1;
+    sized(std::integral_constant<int, 1>());
+    if ((long long)p.blocks * seqs >= 2LL * num_cu) return vec ? launch(scan_tile_kernel<LANES, NL, 1, true, 0>) : launch(scan_tile_kernel<LANES, NL, 1, false, 0>);
+    sized(std::integral_constant<int, 8>());
+    using T = ScanTile<LANES, NL, 8>;
+    const long long workgroups = (long long)p.blocks * seqs, tiles = (tokens + T::TOKENS - 1) / T::TOKENS;
+    if (workgroups * 2 <= num_cu && tiles >= 8) p.parts = (int)std::min<long long>({2LL * num_cu / workgroups, tiles / 4, 64});
+    if (p.parts == 1) return vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 0>) : launch(scan_tile_kernel<LANES, NL, 8, false, 0>);
+    const size_t each = (size_t)p.channels * T::NP * sizeof(float);
+    void *ws = nullptr;
+    EH_TRY(get_workspace(dev, each * seqs * (2 * (size_t)p.parts + 1), &ws));
+    p.part_states = (float *)ws;
+    p.part_factors = (float *)((char *)ws + each * seqs * (p.parts + 1));
+    EH_TRY(vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 1>) : launch(scan_tile_kernel<LANES, NL, 8, false, 1>));
+    return vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 2>) : launch(scan_tile_kernel<LANES, NL, 8, false, 2>);
+}
+
+}  // namespace
+
+extern "C" int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
+                                      const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,
+                                      int rows, int channels, int n, int groups, int softplus, int reverse, float *states, int pool, const int *offsets,
+                                      const int *lengths, const int *slots, const int *out_slots, int seqs, int max_new) {
+    EH_REQUIRE(channels > 0 && channels <= MOST_CHANNELS && n > 0 && n <= MOST_STATES, "selective_scan: %d channels (up to %d) of %d states (1 to %d)", channels, MOST_CHANNELS, n, MOST_STATES);
+    EH_REQUIRE(groups > 0 && channels % groups == 0, "selective_scan: %d channels in %d groups", channels, groups);
+    EH_REQUIRE(ldx >= channels && lddt >= channels && ldy >= channels && (!gate || ldg >= channels), "selective_scan: rows shorter than %d channels", channels);
+    EH_REQUIRE(ldb >= (long long)groups * n && ldc >= (long long)groups * n, "selective_scan: rows shorter than %d vectors of %d", groups, n);
+    EH_TRY(check_batch("selective_scan", rows, seqs, max_new, states, pool, offsets, lengths, slots, out_slots));
+    if (rows == 0 || seqs == 0) return 0;
+    EH_REQUIRE(X && dt && A && B && C && Y, "selective_scan: NULL tensor");
+    const size_t state_bytes = (size_t)pool * channels * n * 4;
+    const struct {
+        const float *at;
+        long long ld, width;
+    } inputs[] = {{X, ldx, channels}, {dt, lddt, channels}, {gate, ldg, channels}, {B, ldb, (long long)groups * n}, {C, ldc, (long long)groups * n}};
+    for (const auto &i : inputs) {
+        EH_REQUIRE(!eh_rows_overlap(i.at, i.ld, i.width, Y, ldy, channels, rows), "selective_scan: the output lies on an input");
+        EH_REQUIRE(!eh_rows_meet(i.at, i.ld, i.width, rows, states, state_bytes), "selective_scan: the states lie on an input");
+    }
+    const struct {
+        const void *at;
+        size_t bytes;
+    } others[] = {{states, state_bytes}, {A, (size_t)channels * n * 4}, {skip, (size_t)channels * 4}, {dt_bias, (size_t)channels * 4},
+                  {offsets, ((size_t)seqs + 1) * 4}, {lengths, (size_t)seqs * 4}, {slots, (size_t)seqs * 4}, {out_slots, (size_t)seqs * 4}};
+    for (const auto &o : others) {
+        EH_REQUIRE(!eh_rows_meet(Y, ldy, channels, rows, o.at, o.bytes), "selective_scan: the output lies on the states, weights or the batch");
+        EH_REQUIRE(&o == others || !eh_rows_meet((const float *)o.at, o.bytes / 4, o.bytes / 4, 1, states, state_bytes), "selective_scan: the states lie on the weights or the batch");
+    }
+    EH_TRY(use_device(dev));
+    ScanParams p;
+    p.X = X;
+    p.dt = dt;
+    p.gate = gate;
+    p.B = B;
+    p.C = C;
+    p.A = A;
+    p.skip = skip;
+    p.dt_bias = dt_bias;
+    p.Y = Y;
+    p.states = states;
+    p.ldx = ldx;
+    p.lddt = lddt;
+    p.ldg = ldg;
+    p.ldb = ldb;
+    p.ldc = ldc;
+    p.ldy = ldy;
+    p.channels = channels;
+    p.n = n;
+    p.per = channels / groups;
+    p.softplus = softplus != 0;
+    p.batch = StateBatch{offsets, lengths, slots, out_slots, rows, pool, reverse != 0};
+    // (a group's first channel, too, has to be aligned)
+    uintptr_t rows16 = 0, vectors16 = (uintptr_t)B | (uintptr_t)C;
+    for (const void *at : {(const void *)X, (const void *)dt, (const void *)gate, (const void *)Y, (const void *)skip, (const void *)dt_bias}) rows16 |= (uintptr_t)at;
+    const bool vec = (rows16 & 15) == 0 && p.per % 4 == 0 && ldx % 4 == 0 && lddt % 4 == 0 && ldy % 4 == 0 && (!gate || ldg % 4 == 0);
+    p.vectors = n == 1 || ((vectors16 & 15) == 0 && n % 4 == 0 && ldb % 4 == 0 && ldc % 4 == 0);
+    const int tokens = std::max(1, std::min(max_new, rows));
+    if (n == 1) return launch_scan<1, 1>(dev, p, seqs, tokens, vec);
+    if (n <= 4) return launch_scan<1, 4>(dev, p, seqs, tokens, vec);
+    if (n <= 8) return launch_scan<2, 4>(dev, p, seqs, tokens, vec);
+    if (n <= 16) return launch_scan<4, 4>(dev, p, seqs, tokens, vec);
+    if (n <= 32) return launch_scan<8, 4>(dev, p, seqs, tokens, vec);
+    return launch_scan<16, 4>(dev, p, seqs, tokens, vec);
+}
