@@ -2,6 +2,10 @@
 //     n = (x - mean) / sqrt(variance + eps) w + b,   y = act(n (1 + mod) + shift).
 // Maps [images][channels][pixels], where a group is one stretch of memory, or rows of tokens [images * pixels][channels], where it is a
 // piece of every row.
+//
+// Bound: memory, 8 bytes a number, if a group is read once.  A group of up to 32768 numbers stays in the registers of a workgroup between its
+// sums and its outputs (group_norm_kernel, WHOLE).  A larger one is divided: the first launch brings mean and squared differences of every part, the second
+// joins them and reads the numbers again.  The variance is that of differences from a mean, never a difference of squares.
 #include <math.h>
 
 #include <algorithm>
@@ -13,19 +17,38 @@ using namespace eddlhip;
 
 namespace {
 
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+enum { WHOLE, SUMS, APPLY };  // what a launch does
+
 struct GroupNormParams {
     const float *X, *w, *b, *mod, *shift;
     float *Y;
+    float2 *parts;  // mean and squared differences of every part
     long long ldx, ldy;
     int images, channels, pixels, groups, activation;
-    bool rows;
+    int per;              // channels of a group
+    int split;            // parts of a group
+    long long part;       // numbers of a part, or rows of one (short rows)
+    long long jobs;       // of the launch
+    int together;         // groups of a workgroup (short rows)
     float eps;
 };
 
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float x, float *red) {
+// Workgroups side by side share lines of memory where a group is a piece of a row: they are put on one XCD.
+__device__ __forceinline__ long long job_of(long long id, long long jobs) {
+    const long long each = (jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
+    return id % EDDLHIP_NUM_XCD * each + id / EDDLHIP_NUM_XCD;
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
     for (int step = 32; step > 0; step >>= 1) x += __shfl_xor(x, step);
+    return x;
+}
+template <int THREADS>
+__device__ __forceinline__ float block_sum(float x, float *red) {
+    x = wave_sum(x);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
     __syncthreads();
@@ -35,40 +58,329 @@ __device__ __forceinline__ float block_sum(float x, float *red) {
     return x;
 }
 
-// A workgroup a group of an image, three passes over memory.
-__global__ __launch_bounds__(256) void group_norm_kernel(const GroupNormParams p) {
-    __shared__ float red[4];
-    const int per = p.channels / p.groups;
-    const long long count = (long long)per * p.pixels;
-    for (long long job = blockIdx.x; job < (long long)p.images * p.groups; job += gridDim.x) {
-        const int image = (int)(job / p.groups), group = (int)(job % p.groups), c0 = group * per;
-        const long long row0 = (long long)image * p.pixels;
-        auto at = [&](long long e, long long ld, int &c) -> long long {
-            if (p.rows) {
-                c = c0 + (int)(e % per);
-                return (row0 + e / per) * ld + c;
-            }
-            c = c0 + (int)(e / p.pixels);
-            return ((long long)image * p.channels + c0) * p.pixels + e;
-        };
-        int c;
-        float sum = 0.0f, squares = 0.0f;
-        for (long long e = threadIdx.x; e < count; e += 256) sum += p.X[at(e, p.ldx, c)];
-        const float mean = block_sum<256>(sum, red) / (float)count;
-        for (long long e = threadIdx.x; e < count; e += 256) {
-            const float d = p.X[at(e, p.ldx, c)] - mean;
-            squares += d * d;
-        }
-        const float scale = 1.0f / sqrtf(block_sum<256>(squares, red) / (float)count + p.eps);
-        for (long long e = threadIdx.x; e < count; e += 256) {
-            float v = (p.X[at(e, p.ldx, c)] - mean) * scale;
-            if (p.w) v *= p.w[c];
-            if (p.b) v += p.b[c];
-            if (p.mod) v *= 1.0f + p.mod[(long long)image * p.channels + c];
-            if (p.shift) v += p.shift[(long long)image * p.channels + c];
-            p.Y[at(e, p.ldy, c)] = activated(v, p.activation);
-        }
+template <int UNIT>
+struct Unit {
+    float v[UNIT];
+};
+template <int UNIT>
+__device__ __forceinline__ Unit<UNIT> get(const float *from) {
+    Unit<UNIT> u;
+    if constexpr (UNIT == 4) {
+        const floatx4 v = *reinterpret_cast<const floatx4 *>(from);
+#pragma unroll
+        for (int i = 0; i < 4; i++) u.v[i] = v[i];
+    } else {
+        u.v[0] = *from;
     }
+    return u;
+}
+template <int UNIT>
+__device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
+    if constexpr (UNIT == 4) {
+        floatx4 v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = u.v[i];
+        __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(to));
+    } else {
+        *to = u.v[0];
+    }
+}
+
+// y = act((x - mean) slope + lift) for a channel of an image
+__device__ __forceinline__ void coefficients(const GroupNormParams &p, int image, int c, float scale, float &slope, float &lift) {
+    const long long at = (long long)image * p.channels + c;
+    const float more = p.mod ? 1.0f + p.mod[at] : 1.0f;
+    slope = scale * (p.w ? p.w[c] : 1.0f) * more;
+    lift = (p.b ? p.b[c] : 0.0f) * more + (p.shift ? p.shift[at] : 0.0f);
+}
+
+// Mean and squared differences of n more numbers taken into those of `count`.
+__device__ __forceinline__ void join(double &count, float &mean, float &squares, double n, float mean_n, float squares_n) {
+    const float delta = mean_n - mean, share = (float)(n / (count + n));
+    mean = __builtin_fmaf(delta, share, mean);
+    squares += squares_n + delta * delta * (float)count * share;
+    count += n;
+}
+// Those of all parts of a group of `total` numbers, parts of `part` each, by a wavefront; in all of its lanes.
+__device__ __forceinline__ void join_parts(const float2 *parts, int split, long long part, long long total, float &mean, float &squares) {
+    const int lane = threadIdx.x & 63;
+    float sum = 0.0f;
+    for (int k = lane; k < split; k += 64) sum += parts[k].x * ((float)min(part, total - k * part) / (float)total);
+    mean = wave_sum(sum);
+    sum = 0.0f;
+    for (int k = lane; k < split; k += 64) {
+        const float2 v = parts[k];
+        sum += v.y + (v.x - mean) * (v.x - mean) * (float)min(part, total - k * part);
+    }
+    squares = wave_sum(sum);
+}
+
+constexpr int COEFFICIENTS = 1024;  // channels of a group whose slope and lift lie in LDS
+
+// A workgroup a group of an image or a part of one.  UNIT numbers are read at a time; ROWS: the numbers are counted along the group's pieces of the rows.
+template <int THREADS, int NV, int UNIT, bool ROWS, int WHAT>
+__global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormParams p) {
+    __shared__ float red[THREADS / 64];
+    __shared__ float slopes[WHAT == SUMS ? 1 : COEFFICIENTS], lifts[WHAT == SUMS ? 1 : COEFFICIENTS];
+    constexpr int STEP = THREADS * UNIT, TILE = STEP * NV;
+    const long long count = (long long)p.per * p.pixels;
+    const int inner = ROWS ? p.per : p.pixels, step_hi = STEP / inner, step_lo = STEP % inner;  // (a number's row and channel, or channel and pixel)
+    for (long long id = blockIdx.x; id < (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD; id += gridDim.x) {
+        const long long job = job_of(id, p.jobs);
+        if (job >= p.jobs) continue;
+        const long long which = job / p.split, first = job % p.split * p.part, last = min(count, first + p.part);
+        const int image = (int)(which / p.groups), c0 = (int)(which % p.groups) * p.per;
+        const float *X = p.X + (ROWS ? (long long)image * p.pixels * p.ldx + c0 : ((long long)image * p.channels + c0) * p.pixels);
+        float *Y = p.Y + (ROWS ? (long long)image * p.pixels * p.ldy + c0 : ((long long)image * p.channels + c0) * p.pixels);
+        float mean = 0.0f, squares = 0.0f;
+        double seen = 0.0;
+        if (WHAT == APPLY) join_parts(p.parts + which * p.split, p.split, p.part, count, mean, squares);
+        auto prepare = [&]() {  // slopes and lifts of the group's channels
+            const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
+            if (p.per <= COEFFICIENTS) {
+                if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
+                for (int c = threadIdx.x; c < p.per; c += THREADS) coefficients(p, image, c0 + c, scale, slopes[c], lifts[c]);
+                __syncthreads();
+            }
+            return scale;
+        };
+        float scale = 0.0f;
+        if (WHAT == APPLY) scale = prepare();
+        for (long long at = first; at < last; at += TILE) {
+            const long long e0 = at + threadIdx.x * UNIT;
+            const int hi0 = (int)(e0 / inner), lo0 = (int)(e0 % inner);
+            Unit<UNIT> v[NV];
+            int hi = hi0, lo = lo0;
+            float sum = 0.0f;
+            auto advance = [&]() {
+                hi += step_hi;
+                lo += step_lo;
+                if (lo >= inner) {
+                    lo -= inner;
+                    hi++;
+                }
+            };
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const long long e = e0 + k * STEP;
+#pragma unroll
+                for (int i = 0; i < UNIT; i++) v[k].v[i] = 0.0f;
+                if (e < last) v[k] = get<UNIT>(X + (ROWS ? hi * p.ldx + lo : e));
+                if (ROWS) advance();
+            }
+            if (WHAT != APPLY) {
+#pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    if constexpr (UNIT == 4) sum += (v[k].v[0] + v[k].v[1]) + (v[k].v[2] + v[k].v[3]);
+                    else sum += v[k].v[0];
+                }
+                const float n = (float)min((long long)TILE, last - at), mean_n = block_sum<THREADS>(sum, red) / n;
+                float sq = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NV; k++)
+                    if (e0 + k * STEP < last) {
+#pragma unroll
+                        for (int i = 0; i < UNIT; i++) {
+                            const float d = v[k].v[i] - mean_n;
+                            sq = __builtin_fmaf(d, d, sq);
+                        }
+                    }
+                const float squares_n = block_sum<THREADS>(sq, red);
+                if (WHAT == SUMS) {
+                    join(seen, mean, squares, n, mean_n, squares_n);
+                } else {
+                    mean = mean_n;
+                    squares = squares_n;
+                    scale = prepare();
+                }
+            }
+            if (WHAT != SUMS) {
+                hi = hi0;
+                lo = lo0;
+                asm volatile("" : "+v"(hi), "+v"(lo));  // (counted again: the places of the first walk would take registers)
+#pragma unroll
+                for (int k = 0; k < NV; k++) {
+                    const long long e = e0 + k * STEP;
+                    if (e < last) {
+#pragma unroll
+                        for (int i = 0; i < UNIT; i++) {
+                            const int c = ROWS ? lo + i : hi + (UNIT == 4 && lo + i >= inner ? 1 : 0);
+                            float slope, lift;
+                            if (p.per <= COEFFICIENTS) {
+                                slope = slopes[c];
+                                lift = lifts[c];
+                            } else {
+                                coefficients(p, image, c0 + c, scale, slope, lift);
+                            }
+                            v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope, lift), p.activation);
+                        }
+                        set<UNIT>(Y + (ROWS ? hi * p.ldy + lo : e), v[k]);
+                    }
+                    advance();
+                }
+            }
+        }
+        if (WHAT == SUMS && threadIdx.x == 0) p.parts[job] = float2{mean, squares};
+    }
+}
+
+// Groups of few channels in rows: a workgroup takes several side by side, so that its pieces of the rows are long enough, and a thread stays in its columns.
+template <int NV, int UNIT, int WHAT>
+__global__ __launch_bounds__(256) void group_norm_rows_kernel(const GroupNormParams p) {
+    __shared__ float red[256], stat[64];
+    const int blocks = (p.groups + p.together - 1) / p.together;
+    for (long long id = blockIdx.x; id < (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD; id += gridDim.x) {
+        const long long job = job_of(id, p.jobs);
+        if (job >= p.jobs) continue;
+        const long long which = job / p.split;
+        const int piece = (int)(job % p.split), image = (int)(which / blocks), g0 = (int)(which % blocks) * p.together, here = min(p.together, p.groups - g0);
+        const int units = p.per / UNIT, wide = here * units, rows_at_once = 256 / wide;  // (of a group, of a row, rows of a step)
+        const int tr = threadIdx.x / wide, cu = threadIdx.x % wide, g = cu / units, c = g0 * p.per + cu * UNIT;
+        const bool mine = tr < rows_at_once;
+        const long long first = piece * p.part, last = min((long long)p.pixels, first + p.part), total = (long long)p.per * p.pixels;
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        // the sums of the groups over all threads, by the wavefronts in turn
+        auto group_sum = [&](float x) {
+            __syncthreads();
+            red[threadIdx.x] = x;
+            __syncthreads();
+            for (int j = wave; j < here; j += 4) {
+                float s = 0.0f;
+                for (int k = lane; k < rows_at_once * units; k += 64) s += red[k / units * wide + j * units + k % units];
+                s = wave_sum(s);
+                if (lane == 0) stat[j] = s;
+            }
+            __syncthreads();
+            return stat[mine ? g : 0];
+        };
+        float mean = 0.0f, squares = 0.0f, slope[UNIT], lift[UNIT];
+        double seen = 0.0;
+        auto prepare = [&]() {
+            const float scale = 1.0f / sqrtf(squares / (float)total + p.eps);
+#pragma unroll
+            for (int i = 0; i < UNIT; i++)
+                if (mine) coefficients(p, image, c + i, scale, slope[i], lift[i]);
+        };
+        if (WHAT == APPLY) {
+            __syncthreads();
+            for (int j = wave; j < here; j += 4) {
+                join_parts(p.parts + ((long long)image * p.groups + g0 + j) * p.split, p.split, p.part * p.per, total, mean, squares);
+                if (lane == 0) {
+                    red[j] = mean;
+                    stat[j] = squares;
+                }
+            }
+            __syncthreads();
+            mean = red[mine ? g : 0];
+            squares = stat[mine ? g : 0];
+            prepare();
+        }
+        for (long long at = first; at < last; at += (long long)rows_at_once * NV) {
+            const long long row0 = (long long)image * p.pixels + at + tr;
+            Unit<UNIT> v[NV];
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+#pragma unroll
+                for (int i = 0; i < UNIT; i++) v[k].v[i] = 0.0f;
+                if (mine && at + tr + k * rows_at_once < last) v[k] = get<UNIT>(p.X + (row0 + k * rows_at_once) * p.ldx + c);
+#pragma unroll
+                for (int i = 0; i < UNIT; i++) sum += v[k].v[i];
+            }
+            if (WHAT != APPLY) {
+                const double n = (double)min((long long)rows_at_once * NV, last - at) * p.per;
+                const float mean_n = group_sum(sum) / (float)n;
+                float sq = 0.0f;
+#pragma unroll
+                for (int k = 0; k < NV; k++)
+                    if (mine && at + tr + k * rows_at_once < last) {
+#pragma unroll
+                        for (int i = 0; i < UNIT; i++) {
+                            const float d = v[k].v[i] - mean_n;
+                            sq = __builtin_fmaf(d, d, sq);
+                        }
+                    }
+                const float squares_n = group_sum(sq);
+                if (WHAT == SUMS) {
+                    join(seen, mean, squares, n, mean_n, squares_n);
+                } else {
+                    mean = mean_n;
+                    squares = squares_n;
+                    prepare();
+                }
+            }
+            if (WHAT != SUMS) {
+#pragma unroll
+                for (int k = 0; k < NV; k++)
+                    if (mine && at + tr + k * rows_at_once < last) {
+#pragma unroll
+                        for (int i = 0; i < UNIT; i++) v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope[i], lift[i]), p.activation);
+                        set<UNIT>(p.Y + (row0 + k * rows_at_once) * p.ldy + c, v[k]);
+                    }
+            }
+        }
+        if (WHAT == SUMS && tr == 0 && cu % units == 0) p.parts[((long long)image * p.groups + g0 + g) * p.split + piece] = float2{mean, squares};
+    }
+}
+
+typedef void (*Kernel)(GroupNormParams);
+
+// A workgroup for every part of `groups` groups (or of groups taken together).
+int launch(int dev, GroupNormParams &p, Kernel fn, int threads, long long groups) {
+    p.jobs = groups * p.split;
+    const long long most = (1LL << 32) / threads - EDDLHIP_NUM_XCD;  // (a grid holds less than 2^32 threads; its workgroups walk what is beyond)
+    hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(threads), 0, state(dev).stream, p);
+    EH_CHECK_LAUNCH();
+    return 0;
+}
+
+// Sums and outputs of divided groups.
+int launch_divided(int dev, GroupNormParams &p, Kernel sums, Kernel apply, long long groups) {
+    void *ws = nullptr;
+    EH_TRY(get_workspace(dev, (size_t)p.images * p.groups * p.split * sizeof(float2), &ws));
+    p.parts = (float2 *)ws;
+    EH_TRY(launch(dev, p, sums, 256, groups));
+    return launch(dev, p, apply, 256, groups);
+}
+
+constexpr int MOST_PARTS = 256, WORKGROUPS = 4096;  // parts of a group; workgroups after which groups are not divided further
+
+template <int UNIT, bool ROWS>
+int launch_groups(int dev, GroupNormParams &p) {
+    static const struct {
+        int threads, nv;
+        Kernel fn;
+    } sizes[] = {{256, 1, group_norm_kernel<256, 1, UNIT, ROWS, WHOLE>},           {256, 4, group_norm_kernel<256, 4, UNIT, ROWS, WHOLE>},
+                 {256, 32 / UNIT, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, WHOLE>}, {512, 32 / UNIT, group_norm_kernel<512, 32 / UNIT, UNIT, ROWS, WHOLE>},
+                 {1024, 32 / UNIT, group_norm_kernel<1024, 32 / UNIT, UNIT, ROWS, WHOLE>}};
+    const long long count = (long long)p.per * p.pixels, groups = (long long)p.images * p.groups;
+    p.split = 1;
+    p.part = count;
+    for (const auto &s : sizes)
+        if (count <= (long long)s.threads * s.nv * UNIT) return launch(dev, p, s.fn, s.threads, groups);
+    constexpr int TILE = 256 * 32;
+    const long long tiles = (count + TILE - 1) / TILE, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
+    p.part = (tiles + parts - 1) / parts * TILE;
+    p.split = (int)((count + p.part - 1) / p.part);
+    return launch_divided(dev, p, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, SUMS>, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, APPLY>, groups);
+}
+
+constexpr int SHORT = 16;  // channels of a group: with fewer, 64 bytes of a row are taken together
+
+template <int UNIT>
+int launch_short(int dev, GroupNormParams &p) {
+    p.together = std::min(p.groups, (2 * SHORT + p.per - 1) / p.per);
+    const int at_once = 256 / (p.together * p.per / UNIT);  // rows
+    const long long groups = (long long)p.images * ((p.groups + p.together - 1) / p.together);
+    p.split = 1;
+    p.part = p.pixels;
+    if (p.pixels <= 4 * at_once) return launch(dev, p, group_norm_rows_kernel<4, UNIT, WHOLE>, 256, groups);
+    if (p.pixels <= 32 / UNIT * at_once) return launch(dev, p, group_norm_rows_kernel<32 / UNIT, UNIT, WHOLE>, 256, groups);
+    const int tile = 32 / UNIT * at_once;
+    const long long tiles = (p.pixels + tile - 1) / tile, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
+    p.part = (tiles + parts - 1) / parts * tile;
+    p.split = (int)((p.pixels + p.part - 1) / p.part);
+    return launch_divided(dev, p, group_norm_rows_kernel<32 / UNIT, UNIT, SUMS>, group_norm_rows_kernel<32 / UNIT, UNIT, APPLY>, groups);
 }
 
 }  // namespace
@@ -106,9 +418,16 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     p.pixels = pixels;
     p.groups = groups;
     p.activation = activation;
-    p.rows = channels_last != 0;
+    p.per = channels / groups;
+    p.parts = nullptr;
+    p.together = 1;
     p.eps = eps;
-    hipLaunchKernelGGL(group_norm_kernel, dim3(eh_blocks((size_t)images * groups, 1)), dim3(256), 0, state(dev).stream, p);
-    EH_CHECK_LAUNCH();
-    return 0;
+    const bool aligned = (((uintptr_t)X | (uintptr_t)Y) & 15) == 0;
+    if (!channels_last) {  // (a group begins at a multiple of 16 bytes, and four numbers meet two channels at most)
+        if (aligned && (long long)p.per * pixels % 4 == 0 && pixels >= 4) return launch_groups<4, false>(dev, p);
+        return launch_groups<1, false>(dev, p);
+    }
+    const bool vec = aligned && p.per % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0;
+    if (p.per < SHORT && groups > 1) return vec ? launch_short<4>(dev, p) : launch_short<1>(dev, p);
+    return vec ? launch_groups<4, true>(dev, p) : launch_groups<1, true>(dev, p);
 }
