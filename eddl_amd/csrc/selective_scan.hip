@@ -94,293 +94,322 @@ __global__ __launch_bounds__(256) void scan_tokens_kernel(const ScanParams p) {
     keep_state<NL>(p, q, c, n0, h);
 }
 
-// Many tokens.  A workgroup of eight wavefronts takes a tile of tokens of some channels into LDS - steps d, products d x, vectors B and C - and
-// walks it with LANES lanes a channel, NL states each.  WT of the wavefronts divide the tile's tokens, the others its channels.  With WT > 1 a wavefront first
-// brings its tokens' state from zeros (keeping the factors e^(d A), the dearest part, in registers), then takes in what the wavefronts
-// before it brought, and walks its tokens again with the state that they begin with.
-constexpr int SCAN_THREADS = 512;
-template <int LANES, int NL, int WT>
+// Many tokens.  A workgroup takes a tile of tokens of some channels into LDS - steps d, products d x, vectors B and C - and walks it with LANES lanes a
+// channel, NL states each.  WT of its WAVES wavefronts divide the tile's tokens, the others its channels.  With WT > 1 a wavefront first brings its tokens' state
+// from zeros, keeping factors e^(d A) and products d x B in registers, then takes in what the wavefronts before it brought, and walks its tokens
+// again with the state that they begin with.
+template <int LANES, int NL, int WAVES, int WT>
 struct ScanTile {
-    static constexpr int TT = LANES == 4 ? 16 : 8;          // tokens of a wavefront
-    static constexpr int TOKENS = TT * WT;                  // of a tile
-    static constexpr int CHANNELS = 64 / LANES * (8 / WT);  // of a workgroup
-    static constexpr int NP = LANES * NL;                   // states, with those behind the last
-    static constexpr int STRIDE = TOKENS + 4;               // floats from a channel's steps to the next one's (neighbours' 16 bytes lie in banks of their own)
-    static constexpr int QUADS = TOKENS * CHANNELS / 4;     // numbers of four channels side by side
-    static constexpr int PER = (QUADS + SCAN_THREADS - 1) / SCAN_THREADS;
-    static constexpr int VECTORS = TOKENS * LANES;          // pieces of NL numbers of B or C
-    static constexpr int VPER = (VECTORS + SCAN_THREADS - 1) / SCAN_THREADS;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int TT = LANES == 4 ? 16 : 8;                // tokens of a wavefront
+    static constexpr int TOKENS = TT * WT;                        // of a tile
+    static constexpr int CHANNELS = 64 / LANES * (WAVES / WT);    // of a workgroup
+    static constexpr int NP = LANES * NL;                         // states, with those behind the last
+    static constexpr int STRIDE = TOKENS + 4;                     // floats from a channel's steps to the next one's (neighbours' 16 bytes lie in banks of their own)
+    static constexpr int CQ = CHANNELS / 4;                       // a thread brings numbers of four channels side by side
+    static constexpr int QUADS = TOKENS * CQ;
+    static constexpr int PER = (QUADS + THREADS - 1) / THREADS;
+    static constexpr int VECTORS = TOKENS * LANES;                // pieces of NL numbers of B or C
+    static constexpr int VPER = (VECTORS + THREADS - 1) / THREADS;
 };
 
 // PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups: PART 1 brings the state of every part from
 // zeros and the factor of what comes before it, PART 2 takes in the parts before its own and brings the outputs.
-template <int LANES, int NL, int WT, bool VEC, int PART>
-__global__ __launch_bounds__(SCAN_THREADS, 4) void scan_tile_kernel(const ScanParams p) {
-    using T = ScanTile<LANES, NL, WT>;
+template <int LANES, int NL, int WAVES, int WT, bool VEC, int PART>
+__global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan_tile_kernel(const ScanParams p) {
+    using T = ScanTile<LANES, NL, WAVES, WT>;
     typedef float vec __attribute__((ext_vector_type(NL)));
-    constexpr int SETS = 64 * (8 / WT);  // lanes that walk the same tokens
+    constexpr int SETS = 64 * (WAVES / WT);  // lanes that walk the same tokens
     __shared__ __attribute__((aligned(16))) float steps[T::CHANNELS * T::STRIDE], inputs[T::CHANNELS * T::STRIDE];  // d and d x, whose place the outputs take
     __shared__ __attribute__((aligned(16))) vec vb[T::VECTORS], vc[PART == 1 ? 1 : T::VECTORS];
-    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? SCAN_THREADS : 1], factor[WT > 1 ? SCAN_THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
+    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? T::THREADS : 1], factor[WT > 1 ? T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
 
     // Workgroups side by side in channels share lines of memory: they are put on one XCD.
     const long long per_xcd = (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
     for (long long id = blockIdx.x; id < per_xcd * EDDLHIP_NUM_XCD; id += gridDim.x) {
-    const long long job = id % EDDLHIP_NUM_XCD * per_xcd + id / EDDLHIP_NUM_XCD;
-    if (job >= p.jobs) continue;
-    const int block = (int)(job % p.blocks), group = block / p.group_blocks, part = (int)(job / p.blocks % p.parts), s = (int)(job / p.blocks / p.parts);
-    const Sequence q = sequence(p.batch, s);
-    const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + p.parts - 1) / p.parts;  // (of a part)
-    const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
-    if (tile0 == tile1) continue;
+        const long long job = id % EDDLHIP_NUM_XCD * per_xcd + id / EDDLHIP_NUM_XCD;
+        if (job >= p.jobs) continue;
+        const int block = (int)(job % p.blocks), group = block / p.group_blocks, part = (int)(job / p.blocks % p.parts), s = (int)(job / p.blocks / p.parts);
+        const Sequence q = sequence(p.batch, s);
+        const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + p.parts - 1) / p.parts;  // (of a part)
+        const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
+        if (tile0 == tile1) continue;
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
-    const int c0 = group * p.per + block % p.group_blocks * T::CHANNELS, cend = (group + 1) * p.per;
-    const int ch = wc * (64 / LANES) + lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
-    const bool mine = c < cend;
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
+        const int c0 = group * p.per + block % p.group_blocks * T::CHANNELS, cend = (group + 1) * p.per;
+        const int ch = wc * (64 / LANES) + lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
+        const bool mine = c < cend;
 
-    float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a part)
+        float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a part)
 #pragma unroll
-    for (int i = 0; i < NL; i++) {
-        a[i] = h[i] = 0.0f;
-        through[i] = 1.0f;
-    }
-    if (mine) exponents<NL>(p, c, n0, a);
-    if (mine && wt == 0) {
-        float *states = PART ? p.part_states + ((long long)s * (p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
-        if (PART == 0) {
-            first_state<NL>(p, q, c, n0, h);
-        } else if (PART == 1) {
-            if (part == 0) {  // kept for the second launch, in which the slot may be written already
-                float kept[NL];
-                first_state<NL>(p, q, c, n0, kept);
-#pragma unroll
-                for (int i = 0; i < NL; i++) states[i] = kept[i];
-            }
-        } else {
-            const float *factors = p.part_factors + ((long long)s * p.parts * p.channels + c) * T::NP + n0;
-            const long long step = (long long)p.channels * T::NP;
-            const vec v = *reinterpret_cast<const vec *>(states);
-#pragma unroll
-            for (int i = 0; i < NL; i++) h[i] = v[i];
-            for (int j = 0; j < part; j++) {
-                const vec f = *reinterpret_cast<const vec *>(factors + j * step), b = *reinterpret_cast<const vec *>(states + (j + 1) * step);
-#pragma unroll
-                for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[i], h[i], b[i]);
-            }
+        for (int i = 0; i < NL; i++) {
+            a[i] = h[i] = 0.0f;
+            through[i] = 1.0f;
         }
-        if (WT > 1 && PART != 1) {
-            vec v;
+        if (mine) exponents<NL>(p, c, n0, a);
+        if (mine && wt == 0) {
+            float *states = PART ? p.part_states + ((long long)s * (p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
+            if (PART == 0) {
+                first_state<NL>(p, q, c, n0, h);
+            } else if (PART == 1) {
+                if (part == 0) {  // kept for the second launch, in which the slot may be written already
+                    float kept[NL];
+                    first_state<NL>(p, q, c, n0, kept);
 #pragma unroll
-            for (int i = 0; i < NL; i++) v[i] = h[i];
-            begin[set] = v;
-        }
-    }
-
-    // what a thread brings of a tile, one tile ahead
-    floatx4 x[T::PER], d[T::PER], g[T::PER], bias[T::PER], skip[T::PER];
-    vec b[T::VPER], cc[T::VPER];
-    constexpr int CQ = T::CHANNELS / 4;
-    const floatx4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto get4 = [&](const float *from, int at) {
-        if (VEC) return *reinterpret_cast<const floatx4 *>(from + at);
-        floatx4 v;
+                    for (int i = 0; i < NL; i++) states[i] = kept[i];
+                }
+            } else {
+                const float *factors = p.part_factors + ((long long)s * p.parts * p.channels + c) * T::NP + n0;
+                const long long step = (long long)p.channels * T::NP;
+                const vec v = *reinterpret_cast<const vec *>(states);
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = at + i < cend ? from[at + i] : 0.0f;
-        return v;
-    };
+                for (int i = 0; i < NL; i++) h[i] = v[i];
+                for (int j = 0; j < part; j++) {
+                    const vec f = *reinterpret_cast<const vec *>(factors + j * step), b = *reinterpret_cast<const vec *>(states + (j + 1) * step);
 #pragma unroll
-    for (int k = 0; k < T::PER; k++) {
-        const int e = tid + k * SCAN_THREADS, at = c0 + e % CQ * 4;
-        bias[k] = p.dt_bias && at < cend ? get4(p.dt_bias, at) : zeros;
-        skip[k] = p.skip && at < cend ? get4(p.skip, at) : zeros;
-    }
-    auto fetch = [&](int tile) {
-#pragma unroll
-        for (int k = 0; k < T::PER; k++) {
-            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = c0 + e % CQ * 4;
-            x[k] = d[k] = g[k] = zeros;
-            if (e < T::QUADS && t < q.fresh && at < cend) {
-                const long long row = q.row(t);
-                x[k] = get4(p.X + row * p.ldx, at);
-                d[k] = get4(p.dt + row * p.lddt, at);
-                if (PART != 1 && p.gate) g[k] = get4(p.gate + row * p.ldg, at);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < T::VPER; k++) {
-            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / LANES, at = e % LANES * NL;
-#pragma unroll
-            for (int i = 0; i < NL; i++) b[k][i] = cc[k][i] = 0.0f;
-            if (e < T::VECTORS && t < q.fresh && at < p.n) {
-                const long long row = q.row(t);
-                const float *fb = p.B + row * p.ldb + (long long)group * p.n + at, *fc = p.C + row * p.ldc + (long long)group * p.n + at;
-                if (p.vectors) {
-                    b[k] = *reinterpret_cast<const vec *>(fb);
-                    if (PART != 1) cc[k] = *reinterpret_cast<const vec *>(fc);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NL; i++)
-                        if (at + i < p.n) {
-                            b[k][i] = fb[i];
-                            if (PART != 1) cc[k][i] = fc[i];
-                        }
+                    for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[i], h[i], b[i]);
                 }
             }
-        }
-    };
-    // steps and inputs are 0 behind the sequence's last token and the last channel: the state stays
-    auto stage = [&](int tile) {
-#pragma unroll
-        for (int k = 0; k < T::PER; k++) {
-            const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = e % CQ * 4;
-            if (e < T::QUADS) {
-                const bool in = t < q.fresh;
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float raw = d[k][i] + bias[k][i], step = in && c0 + at + i < cend ? (p.softplus ? softplus(raw) : raw) : 0.0f;
-                    steps[(at + i) * T::STRIDE + e / CQ] = step;
-                    inputs[(at + i) * T::STRIDE + e / CQ] = step * x[k][i];
-                }
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < T::VPER; k++) {
-            const int e = tid + k * SCAN_THREADS;
-            if (e < T::VECTORS) {
-                vb[e] = b[k];
-                if (PART != 1) vc[e] = cc[k];
-            }
-        }
-    };
-
-    const float *my_steps = steps + ch * T::STRIDE + wt * T::TT;
-    float *my_inputs = inputs + ch * T::STRIDE + wt * T::TT;
-    const vec *my_b = vb + wt * T::TT * LANES + ln, *my_c = vc + (PART == 1 ? 0 : wt * T::TT * LANES + ln);
-
-    fetch(tile0);
-    for (int tile = tile0; tile < tile1; tile++) {
-        stage(tile);
-        floatx4 x0[T::PER], g0[T::PER];
-#pragma unroll
-        for (int k = 0; k < T::PER; k++) {
-            x0[k] = x[k];
-            g0[k] = g[k];
-        }
-        if (tile + 1 < tile1) fetch(tile + 1);
-        __syncthreads();
-        float kept[WT > 1 ? T::TT : 1][NL];
-        if constexpr (WT > 1) {
-            float local[NL], sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < NL; i++) local[i] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < T::TT; t += 4) {
-                const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const vec bv = my_b[(t + j) * LANES];
-                    sum += dv[j];
-#pragma unroll
-                    for (int i = 0; i < NL; i++) {
-                        const float f = __builtin_amdgcn_exp2f(dv[j] * a[i]);
-                        kept[t + j][i] = f;
-                        local[i] = __builtin_fmaf(f, local[i], xv[j] * bv[i]);
-                    }
-                }
-            }
-            vec v, f;
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                v[i] = local[i];
-                f[i] = __builtin_amdgcn_exp2f(sum * a[i]);
-            }
-            brought[wt * SETS + set] = v;
-            factor[wt * SETS + set] = f;
-            __syncthreads();
-            const int before = PART == 1 ? (wt == 0 ? WT : 0) : wt;
-            if (PART != 1) {
-                const vec v0 = begin[(tile - tile0 & 1) * SETS + set];
-#pragma unroll
-                for (int i = 0; i < NL; i++) h[i] = v0[i];
-            }
-            for (int w = 0; w < before; w++) {
-                const vec wf = factor[w * SETS + set], wb = brought[w * SETS + set];
-#pragma unroll
-                for (int i = 0; i < NL; i++) {
-                    h[i] = __builtin_fmaf(wf[i], h[i], wb[i]);
-                    if (PART == 1) through[i] *= wf[i];
-                }
-            }
-        }
-        if constexpr (PART != 1) {
-#pragma unroll
-            for (int t = 0; t < T::TT; t += 4) {
-                const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
-                floatx4 y;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const vec bv = my_b[(t + j) * LANES], cv = my_c[(t + j) * LANES];
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NL; i++) {
-                        const float f = WT > 1 ? kept[t + j][i] : __builtin_amdgcn_exp2f(dv[j] * a[i]);
-                        h[i] = __builtin_fmaf(f, h[i], xv[j] * bv[i]);
-                        sum = __builtin_fmaf(cv[i], h[i], sum);
-                    }
-                    y[j] = lane_sum<LANES>(sum);
-                }
-                if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
-            }
-            if (WT > 1 && wt == WT - 1) {
+            if (WT > 1 && PART != 1) {
                 vec v;
 #pragma unroll
                 for (int i = 0; i < NL; i++) v[i] = h[i];
-                begin[(tile - tile0 + 1 & 1) * SETS + set] = v;
+                begin[set] = v;
             }
-            __syncthreads();
+        }
+
+        // What a thread brings of a tile, one tile ahead.  Its places are pointers that go on by a tile's rows.
+        floatx4 x[T::PER], d[T::PER], g[T::PER];
+        vec b[T::VPER], cc[T::VPER];
+        const floatx4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int tq = tid / T::CQ, at = tid % T::CQ * 4, tv = tid / LANES, av = tid % LANES * NL;  // token and first channel, or state
+        const int dir = p.batch.reverse ? -1 : 1;
+        const long long row = q.row(tile0 * T::TOKENS + tq), vrow = q.row(tile0 * T::TOKENS + tv);
+        const float *px = p.X + row * p.ldx + c0 + at, *pd = p.dt + row * p.lddt + c0 + at, *pg = p.gate + row * p.ldg + c0 + at;
+        const float *pb = p.B + vrow * p.ldb + (long long)group * p.n + av, *pc = p.C + vrow * p.ldc + (long long)group * p.n + av;
+        float *py = p.Y + row * p.ldy + c0 + at;
+        const long long mx = dir * p.ldx, md = dir * p.lddt, mg = dir * p.ldg, my = dir * p.ldy, mb = dir * p.ldb, mc = dir * p.ldc;
+        constexpr int APART = T::THREADS / T::CQ, VAPART = T::THREADS / LANES;  // tokens between a thread's pieces
+        const bool has = c0 + at < cend, hasv = av < p.n;
+        auto get4 = [&](const float *from) {
+            if (VEC) return *reinterpret_cast<const floatx4 *>(from);
+            floatx4 v;
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = c0 + at + i < cend ? from[i] : 0.0f;
+            return v;
+        };
+        const floatx4 bias = p.dt_bias && has ? get4(p.dt_bias + c0 + at) : zeros, skip = p.skip && has ? get4(p.skip + c0 + at) : zeros;
+        auto fetch = [&](int tile) {
 #pragma unroll
             for (int k = 0; k < T::PER; k++) {
-                const int e = tid + k * SCAN_THREADS, t = tile * T::TOKENS + e / CQ, at = e % CQ * 4;
-                if (e < T::QUADS && t < q.fresh && c0 + at < cend) {
-                    floatx4 y;
+                x[k] = d[k] = g[k] = zeros;
+                if (has && tid + k * T::THREADS < T::QUADS && tile * T::TOKENS + tq + k * APART < q.fresh) {
+                    x[k] = get4(px + k * APART * mx);
+                    d[k] = get4(pd + k * APART * md);
+                    if (PART != 1 && p.gate) g[k] = get4(pg + k * APART * mg);
+                }
+            }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        y[i] = inputs[(at + i) * T::STRIDE + e / CQ];
-                        if (p.skip) y[i] = __builtin_fmaf(skip[k][i], x0[k][i], y[i]);
-                        if (p.gate) y[i] *= silu(g0[k][i]);
-                    }
-                    float *to = p.Y + q.row(t) * p.ldy + c0 + at;
-                    if (VEC) {
-                        *reinterpret_cast<floatx4 *>(to) = y;
+            for (int k = 0; k < T::VPER; k++) {
+#pragma unroll
+                for (int i = 0; i < NL; i++) b[k][i] = cc[k][i] = 0.0f;
+                if (hasv && tid + k * T::THREADS < T::VECTORS && tile * T::TOKENS + tv + k * VAPART < q.fresh) {
+                    const float *fb = pb + k * VAPART * mb, *fc = pc + k * VAPART * mc;
+                    if (p.vectors) {
+                        b[k] = *reinterpret_cast<const vec *>(fb);
+                        if (PART != 1) cc[k] = *reinterpret_cast<const vec *>(fc);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            if (c0 + at + i < cend) to[i] = y[i];
+                        for (int i = 0; i < NL; i++)
+                            if (av + i < p.n) {
+                                b[k][i] = fb[i];
+                                if (PART != 1) cc[k][i] = fc[i];
+                            }
                     }
                 }
             }
-        }
-    }
-    if (PART == 1) {
-        if (mine && wt == 0) {
-            float *states = p.part_states + (((long long)s * (p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
-            float *factors = p.part_factors + (((long long)s * p.parts + part) * p.channels + c) * T::NP + n0;
+            px += T::TOKENS * mx;
+            pd += T::TOKENS * md;
+            pg += T::TOKENS * mg;
+            pb += T::TOKENS * mb;
+            pc += T::TOKENS * mc;
+        };
+        // steps and inputs are 0 behind the sequence's last token and the last channel: the state stays
+        auto stage = [&](int tile) {
 #pragma unroll
-            for (int i = 0; i < NL; i++) {
-                states[i] = h[i];
-                factors[i] = through[i];
+            for (int k = 0; k < T::PER; k++) {
+                if (tid + k * T::THREADS < T::QUADS) {
+                    const bool in = tile * T::TOKENS + tq + k * APART < q.fresh;
+                    floatx4 step = d[k] + bias;
+                    if (p.softplus) {  // (four side by side: each is a chain of dependent instructions)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) step[i] = softplus(step[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        step[i] = in && c0 + at + i < cend ? step[i] : 0.0f;
+                        steps[(at + i) * T::STRIDE + tq + k * APART] = step[i];
+                        inputs[(at + i) * T::STRIDE + tq + k * APART] = step[i] * x[k][i];
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < T::VPER; k++)
+                if (tid + k * T::THREADS < T::VECTORS) {
+                    vb[tid + k * T::THREADS] = b[k];
+                    if (PART != 1) vc[tid + k * T::THREADS] = cc[k];
+                }
+        };
+
+        const float *my_steps = steps + ch * T::STRIDE + wt * T::TT;
+        float *my_inputs = inputs + ch * T::STRIDE + wt * T::TT;
+        const vec *my_b = vb + wt * T::TT * LANES + ln, *my_c = vc + (PART == 1 ? 0 : wt * T::TT * LANES + ln);
+
+        fetch(tile0);
+        for (int tile = tile0; tile < tile1; tile++) {
+            stage(tile);
+            floatx4 x0[T::PER], g0[T::PER];
+#pragma unroll
+            for (int k = 0; k < T::PER; k++) {
+                x0[k] = x[k];
+                g0[k] = g[k];
+            }
+            if (tile + 1 < tile1) fetch(tile + 1);
+            __syncthreads();
+            float kept[WT > 1 ? T::TT : 1][NL], put[WT > 1 && PART != 1 ? T::TT : 1][NL];  // factors and products of the tokens
+            if constexpr (WT > 1) {
+                float local[NL], sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NL; i++) local[i] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < T::TT; t += 4) {
+                    const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const vec bv = my_b[(t + j) * LANES];
+                        sum += dv[j];
+#pragma unroll
+                        for (int i = 0; i < NL; i++) {
+                            const float f = __builtin_amdgcn_exp2f(dv[j] * a[i]), u = xv[j] * bv[i];
+                            local[i] = __builtin_fmaf(f, local[i], u);
+                            kept[t + j][i] = f;
+                            if (PART != 1) put[t + j][i] = u;
+                        }
+                    }
+                }
+                vec v, f;
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    v[i] = local[i];
+                    f[i] = __builtin_amdgcn_exp2f(sum * a[i]);
+                }
+                brought[wt * SETS + set] = v;
+                factor[wt * SETS + set] = f;
+                __syncthreads();
+                const int before = __builtin_amdgcn_readfirstlane(PART == 1 ? (wt == 0 ? WT : 0) : wt);
+                const vec *all = brought + set, *all_f = factor + set;
+                if (PART != 1) {
+                    const vec v0 = begin[(tile - tile0 & 1) * SETS + set];
+#pragma unroll
+                    for (int i = 0; i < NL; i++) h[i] = v0[i];
+                }
+                auto take = [&](int w, auto count) {  // (reads in flight together)
+                    constexpr int N = decltype(count)::value;
+                    vec wf[N], wb[N];
+#pragma unroll
+                    for (int k = 0; k < N; k++) {
+                        wf[k] = all_f[(w + k) * SETS];
+                        wb[k] = all[(w + k) * SETS];
+                    }
+#pragma unroll
+                    for (int k = 0; k < N; k++)
+#pragma unroll
+                        for (int i = 0; i < NL; i++) {
+                            h[i] = __builtin_fmaf(wf[k][i], h[i], wb[k][i]);
+                            if (PART == 1) through[i] *= wf[k][i];
+                        }
+                };
+                int w = 0;
+                for (; w + 4 <= before; w += 4) take(w, std::integral_constant<int, 4>());
+                if (before & 2) take(w, std::integral_constant<int, 2>()), w += 2;
+                if (before & 1) take(w, std::integral_constant<int, 1>());
+            }
+            if constexpr (PART != 1) {
+#pragma unroll
+                for (int t = 0; t < T::TT; t += 4) {
+                    floatx4 dv, xv, y;
+                    if constexpr (WT == 1) {
+                        dv = *reinterpret_cast<const floatx4 *>(my_steps + t);
+                        xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        vec bv;
+                        if constexpr (WT == 1) bv = my_b[(t + j) * LANES];
+                        const vec cv = my_c[(t + j) * LANES];
+                        float sum = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < NL; i++) {
+                            if constexpr (WT == 1) h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dv[j] * a[i]), h[i], xv[j] * bv[i]);
+                            else h[i] = __builtin_fmaf(kept[t + j][i], h[i], put[t + j][i]);
+                            sum = i ? __builtin_fmaf(cv[i], h[i], sum) : cv[i] * h[i];
+                        }
+                        y[j] = lane_sum<LANES>(sum);
+                    }
+                    if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
+                }
+                if (WT > 1 && wt == WT - 1) {
+                    vec v;
+#pragma unroll
+                    for (int i = 0; i < NL; i++) v[i] = h[i];
+                    begin[(tile - tile0 + 1 & 1) * SETS + set] = v;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < T::PER; k++) {
+                    if (has && tid + k * T::THREADS < T::QUADS && tile * T::TOKENS + tq + k * APART < q.fresh) {
+                        floatx4 y;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            y[i] = inputs[(at + i) * T::STRIDE + tq + k * APART];
+                            y[i] = __builtin_fmaf(skip[i], x0[k][i], y[i]);
+                        }
+                        if (p.gate) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) y[i] *= silu(g0[k][i]);
+                        }
+                        float *to = py + k * APART * my;
+                        if (VEC) {
+                            *reinterpret_cast<floatx4 *>(to) = y;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                if (c0 + at + i < cend) to[i] = y[i];
+                        }
+                    }
+                }
+                py += T::TOKENS * my;
             }
         }
-    } else if (mine && wt == WT - 1 && tile1 == tiles) {
-        keep_state<NL>(p, q, c, n0, h);
-    }
-    __syncthreads();  // (the next job's tiles)
+        if (PART == 1) {
+            if (mine && wt == 0) {
+                float *states = p.part_states + (((long long)s * (p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
+                float *factors = p.part_factors + (((long long)s * p.parts + part) * p.channels + c) * T::NP + n0;
+#pragma unroll
+                for (int i = 0; i < NL; i++) {
+                    states[i] = h[i];
+                    factors[i] = through[i];
+                }
+            }
+        } else if (mine && wt == WT - 1 && tile1 == tiles) {
+            keep_state<NL>(p, q, c, n0, h);
+        }
+        __syncthreads();  // (the next job's tiles)
     }
 }
 
 constexpr int MOST_STATES = 64;
-constexpr int FEW_TOKENS = 8;  // up to here token after token from memory
+constexpr int FEW_TOKENS = 3;  // up to here token after token from memory (32 sequences of 2 tokens of 2048 channels 8.8 us, as tiles 10.9; of 8 19.0 and 12.1)
 
 template <int LANES, int NL>
 int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
@@ -390,34 +419,54 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
         EH_CHECK_LAUNCH();
         return 0;
     }
-    const int groups = p.channels / p.per, num_cu = state(dev).num_cu;
-    auto sized = [&](auto wt) {
-        using T = ScanTile<LANES, NL, decltype(wt)::value>;
-        p.group_blocks = (p.per + T::CHANNELS - 1) / T::CHANNELS;
-        p.blocks = groups * p.group_blocks;
-    };
-    auto launch = [&](auto fn) {
+    const int groups = p.channels / p.per;
+    const long long num_cu = state(dev).num_cu;
+    auto launch = [&](auto fn, int threads) {
         p.jobs = (long long)p.blocks * p.parts * seqs;
-        const long long most = 1 << 22;  // workgroups (a grid holds less than 2^32 threads); they walk what is beyond
-        hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(SCAN_THREADS), 0, st, p);
+        const long long most = (1LL << 32) / threads - EDDLHIP_NUM_XCD;  // workgroups (a grid holds less than 2^32 threads); they walk what is beyond
+        hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(threads), 0, st, p);
         EH_CHECK_LAUNCH();
         return 0;
     };
-    p.parts = 1;
-    sized(std::integral_constant<int, 1>());
-    if ((long long)p.blocks * seqs >= 2LL * num_cu) return vec ? launch(scan_tile_kernel<LANES, NL, 1, true, 0>) : launch(scan_tile_kernel<LANES, NL, 1, false, 0>);
-    sized(std::integral_constant<int, 8>());
-    using T = ScanTile<LANES, NL, 8>;
-    const long long workgroups = (long long)p.blocks * seqs, tiles = (tokens + T::TOKENS - 1) / T::TOKENS;
-    if (workgroups * 2 <= num_cu && tiles >= 8) p.parts = (int)std::min<long long>({2LL * num_cu / workgroups, tiles / 4, 64});
-    if (p.parts == 1) return vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 0>) : launch(scan_tile_kernel<LANES, NL, 8, false, 0>);
-    const size_t each = (size_t)p.channels * T::NP * sizeof(float);
-    void *ws = nullptr;
-    EH_TRY(get_workspace(dev, each * seqs * (2 * (size_t)p.parts + 1), &ws));
-    p.part_states = (float *)ws;
-    p.part_factors = (float *)((char *)ws + each * seqs * (p.parts + 1));
-    EH_TRY(vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 1>) : launch(scan_tile_kernel<LANES, NL, 8, false, 1>));
-    return vec ? launch(scan_tile_kernel<LANES, NL, 8, true, 2>) : launch(scan_tile_kernel<LANES, NL, 8, false, 2>);
+    // (workgroups of a call without parts)
+    auto sized = [&](auto tile) {
+        using T = decltype(tile);
+        p.parts = 1;
+        p.group_blocks = (p.per + T::CHANNELS - 1) / T::CHANNELS;
+        p.blocks = groups * p.group_blocks;
+        return (long long)p.blocks * seqs;
+    };
+    auto divided = [&](auto tile, auto first, auto second, int parts) {
+        using T = decltype(tile);
+        p.parts = parts;
+        const size_t each = (size_t)p.channels * T::NP * sizeof(float);
+        void *ws = nullptr;
+        EH_TRY(get_workspace(dev, each * seqs * (2 * (size_t)parts + 1), &ws));
+        p.part_states = (float *)ws;
+        p.part_factors = (float *)((char *)ws + each * seqs * (parts + 1));
+        EH_TRY(launch(first, T::THREADS));
+        return launch(second, T::THREADS);
+    };
+    // By the workgroups that there are, in multiples of the compute units: four wavefronts of different channels do the least work a token; where that leaves
+    // the device half empty, they divide the tokens of a quarter of the channels (512 tokens of 2048 channels, us: 16 sequences 107 against 128, 12 105 and 95, 4 84 and
+    // 36); where that would, too, eight do (2 sequences 28 and 22); and where those do not meet every unit, sequences are divided over workgroups.
+    using Alone = ScanTile<LANES, NL, 4, 1>;
+    using Four = ScanTile<LANES, NL, 4, 4>;
+    using Eight = ScanTile<LANES, NL, 8, 8>;
+    if (sized(Alone()) >= 2 * num_cu || tokens <= Alone::TOKENS)
+        return launch(vec ? scan_tile_kernel<LANES, NL, 4, 1, true, 0> : scan_tile_kernel<LANES, NL, 4, 1, false, 0>, Alone::THREADS);
+    const long long workgroups = sized(Four());  // (as many as of eight wavefronts, which have as many channels)
+    if (2 * workgroups >= 3 * num_cu) return launch(vec ? scan_tile_kernel<LANES, NL, 4, 4, true, 0> : scan_tile_kernel<LANES, NL, 4, 4, false, 0>, Four::THREADS);
+    const long long parts = num_cu / workgroups, tiles = (tokens + Eight::TOKENS - 1) / Eight::TOKENS;
+    if (parts < 2 || tiles < 4)
+        return launch(vec ? scan_tile_kernel<LANES, NL, 8, 8, true, 0> : scan_tile_kernel<LANES, NL, 8, 8, false, 0>, Eight::THREADS);
+    // (4096 tokens of 1024 channels: not divided 125 us, 4 parts of eight wavefronts 63, 8 of four 57; 1000 tokens 39, 24 and 25)
+    if (tiles >= 8 * parts)
+        return vec ? divided(Four(), scan_tile_kernel<LANES, NL, 4, 4, true, 1>, scan_tile_kernel<LANES, NL, 4, 4, true, 2>, (int)(2 * parts))
+                   : divided(Four(), scan_tile_kernel<LANES, NL, 4, 4, false, 1>, scan_tile_kernel<LANES, NL, 4, 4, false, 2>, (int)(2 * parts));
+    const int n = (int)std::min(parts, tiles);
+    return vec ? divided(Eight(), scan_tile_kernel<LANES, NL, 8, 8, true, 1>, scan_tile_kernel<LANES, NL, 8, 8, true, 2>, n)
+               : divided(Eight(), scan_tile_kernel<LANES, NL, 8, 8, false, 1>, scan_tile_kernel<LANES, NL, 8, 8, false, 2>, n);
 }
 
 }  // namespace

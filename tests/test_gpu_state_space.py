@@ -20,7 +20,8 @@ def _check(got, want, err, what=""):
 
 # ------------------------------------------------------------------------------------------------- group norm
 SHAPES = [(1, 1, 1, 1, 1), (2, 4, 1, 1, 2), (1, 512, 7, 7, 32), (3, 6, 5, 1, 3), (2, 64, 33, 31, 8), (5, 30, 3, 4, 10), (1, 128, 64, 64, 1), (2, 66, 37, 37, 11), (4, 96, 14, 14, 32),
-          (1, 2, 300, 301, 1), (1, 1, 1024, 1024, 1), (2, 320, 16, 16, 32), (65, 32, 2, 2, 4), (1, 4096, 3, 3, 4), (1, 8, 257, 255, 2), (1, 24, 1, 700, 24), (1, 7, 1, 40000, 7)]
+          (1, 2, 300, 301, 1), (1, 1, 1024, 1024, 1), (2, 320, 16, 16, 32), (65, 32, 2, 2, 4), (1, 4096, 3, 3, 4), (1, 8, 257, 255, 2), (1, 24, 1, 700, 24), (1, 7, 1, 40000, 7),
+          (1, 2400, 20, 20, 1), (3000, 4, 1, 1, 2), (2, 1026, 9, 7, 1), (1, 48, 130, 131, 2), (1, 33, 150, 150, 3), (1, 51, 120, 100, 3), (1, 16, 200, 200, 4), (2, 40, 90, 90, 1)]
 
 
 @pytest.mark.parametrize("images, channels, height, width, groups", SHAPES)
@@ -223,7 +224,7 @@ def test_selective_scan(hip, n, channels, groups):
                 assert np.array_equal(s[untouched], pool[untouched])
 
 
-@pytest.mark.parametrize("channels, n, news", [(16, 16, [5000]), (5, 16, [3001, 40]), (64, 16, [2000]), (128, 4, [1500, 1000]), (40, 1, [4000]), (33, 64, [1025]), (600, 16, [700, 30, 2, 650]),
+@pytest.mark.parametrize("channels, n, news", [(16, 16, [5000]), (5, 16, [3001, 40]), (64, 16, [2000]), (128, 4, [1500, 1000]), (40, 1, [4000]), (33, 64, [1025]), (600, 16, [700, 30, 2, 650]), (16, 16, [9000]), (24, 8, [2100, 1, 1030]),
                                                (1500, 8, [400] * 3)])
 def test_selective_scan_of_long_sequences(hip, channels, n, news):
     rng = np.random.default_rng([channels, n])
