@@ -12,12 +12,11 @@
 
 #include "common.h"
 #include "activation.h"
+#include "xcd.h"
 
 using namespace eddlhip;
 
 namespace {
-
-typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 enum { WHOLE, SUMS, APPLY };  // what a launch does
 
@@ -26,20 +25,16 @@ struct GroupNormParams {
     float *Y;
     float2 *parts;  // mean and squared differences of every part
     long long ldx, ldy;
-    int images, channels, pixels, groups, activation;
+    int images, channels, pixels, activation;
+    unsigned groups;
     int per;              // channels of a group
-    int split;            // parts of a group
+    unsigned split;       // parts of a group
+    unsigned blocks;      // groups taken together, of an image (short rows)
     long long part;       // numbers of a part, or rows of one (short rows)
     long long jobs;       // of the launch
     int together;         // groups of a workgroup (short rows)
     float eps;
 };
-
-// Workgroups side by side share lines of memory where a group is a piece of a row: they are put on one XCD.
-__device__ __forceinline__ long long job_of(long long id, long long jobs) {
-    const long long each = (jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
-    return id % EDDLHIP_NUM_XCD * each + id / EDDLHIP_NUM_XCD;
-}
 
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
@@ -64,26 +59,21 @@ struct Unit {
 };
 template <int UNIT>
 __device__ __forceinline__ Unit<UNIT> get(const float *from) {
+    typedef float vec __attribute__((ext_vector_type(UNIT)));
+    const vec v = *reinterpret_cast<const vec *>(from);
     Unit<UNIT> u;
-    if constexpr (UNIT == 4) {
-        const floatx4 v = *reinterpret_cast<const floatx4 *>(from);
 #pragma unroll
-        for (int i = 0; i < 4; i++) u.v[i] = v[i];
-    } else {
-        u.v[0] = *from;
-    }
+    for (int i = 0; i < UNIT; i++) u.v[i] = v[i];
     return u;
 }
 template <int UNIT>
 __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
-    if constexpr (UNIT == 4) {
-        floatx4 v;
+    typedef float vec __attribute__((ext_vector_type(UNIT)));
+    vec v;
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = u.v[i];
-        __builtin_nontemporal_store(v, reinterpret_cast<floatx4 *>(to));
-    } else {
-        *to = u.v[0];
-    }
+    for (int i = 0; i < UNIT; i++) v[i] = u.v[i];
+    if constexpr (UNIT == 4) __builtin_nontemporal_store(v, reinterpret_cast<vec *>(to));
+    else *reinterpret_cast<vec *>(to) = v;
 }
 
 // y = act((x - mean) slope + lift) for a channel of an image
@@ -115,47 +105,51 @@ __device__ __forceinline__ void join_parts(const float2 *parts, int split, long 
     squares = wave_sum(sum);
 }
 
-constexpr int COEFFICIENTS = 1024;  // channels of a group whose slope and lift lie in LDS
+constexpr int SHORT = 16;  // channels of a group in rows: with fewer, 64 bytes of a row are taken together
+
+constexpr int MOST_CHANNELS = 4096;  // of a group: their slopes and lifts lie in LDS
 
 // A workgroup a group of an image or a part of one.  UNIT numbers are read at a time; ROWS: the numbers are counted along the group's pieces of the rows.
 template <int THREADS, int NV, int UNIT, bool ROWS, int WHAT>
 __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormParams p) {
     __shared__ float red[THREADS / 64];
-    __shared__ float slopes[WHAT == SUMS ? 1 : COEFFICIENTS], lifts[WHAT == SUMS ? 1 : COEFFICIENTS];
+    extern __shared__ float slopes[];  // of the group's channels, and their lifts
+    float *lifts = slopes + p.per;
     constexpr int STEP = THREADS * UNIT, TILE = STEP * NV;
     const long long count = (long long)p.per * p.pixels;
-    const int inner = ROWS ? p.per : p.pixels, step_hi = STEP / inner, step_lo = STEP % inner;  // (a number's row and channel, or channel and pixel)
-    for (long long id = blockIdx.x; id < (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD; id += gridDim.x) {
-        const long long job = job_of(id, p.jobs);
+    const unsigned inner = ROWS ? p.per : p.pixels, step_hi = STEP / inner, step_lo = STEP % inner;  // (a number's row and channel, or channel and pixel)
+    const bool whole_units = p.pixels % UNIT == 0;
+    for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
+        long long job = xcd_job(id);  // (groups side by side share lines of memory where they are pieces of rows)
         if (job >= p.jobs) continue;
-        const long long which = job / p.split, first = job % p.split * p.part, last = min(count, first + p.part);
-        const int image = (int)(which / p.groups), c0 = (int)(which % p.groups) * p.per;
+        if (WHAT == APPLY) job = p.jobs - 1 - job;  // (what the sums read last is still in the last-level cache)
+        const unsigned which = (unsigned)job / p.split;  // (fewer than 2^31 jobs)
+        const long long first = (unsigned)job % p.split * p.part, last = min(count, first + p.part);
+        const int image = which / p.groups, c0 = (int)(which % p.groups) * p.per;
         const float *X = p.X + (ROWS ? (long long)image * p.pixels * p.ldx + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float *Y = p.Y + (ROWS ? (long long)image * p.pixels * p.ldy + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float mean = 0.0f, squares = 0.0f;
         double seen = 0.0;
-        if (WHAT == APPLY) join_parts(p.parts + which * p.split, p.split, p.part, count, mean, squares);
+        if (WHAT == APPLY) join_parts(p.parts + (long long)which * (int)p.split, (int)p.split, p.part, count, mean, squares);
         auto prepare = [&]() {  // slopes and lifts of the group's channels
             const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
-            if (p.per <= COEFFICIENTS) {
-                if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
-                for (int c = threadIdx.x; c < p.per; c += THREADS) coefficients(p, image, c0 + c, scale, slopes[c], lifts[c]);
-                __syncthreads();
-            }
-            return scale;
+            if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
+            for (int c = threadIdx.x; c < p.per; c += THREADS) coefficients(p, image, c0 + c, scale, slopes[c], lifts[c]);
+            __syncthreads();
         };
-        float scale = 0.0f;
-        if (WHAT == APPLY) scale = prepare();
+        if (WHAT == APPLY) prepare();
         for (long long at = first; at < last; at += TILE) {
             const long long e0 = at + threadIdx.x * UNIT;
-            const int hi0 = (int)(e0 / inner), lo0 = (int)(e0 % inner);
+            // (the tile's first number by the workgroup, the thread's in 32 bits)
+            const unsigned hi_at = WHAT == WHOLE ? 0 : (unsigned)(at / inner), lo_at = (WHAT == WHOLE ? 0 : (unsigned)(at % inner)) + threadIdx.x * UNIT;
+            const int hi0 = hi_at + lo_at / inner, lo0 = lo_at % inner;
             Unit<UNIT> v[NV];
             int hi = hi0, lo = lo0;
             float sum = 0.0f;
             auto advance = [&]() {
                 hi += step_hi;
                 lo += step_lo;
-                if (lo >= inner) {
+                if ((unsigned)lo >= inner) {
                     lo -= inner;
                     hi++;
                 }
@@ -166,12 +160,16 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
 #pragma unroll
                 for (int i = 0; i < UNIT; i++) v[k].v[i] = 0.0f;
                 if (e < last) v[k] = get<UNIT>(X + (ROWS ? hi * p.ldx + lo : e));
-                if (ROWS) advance();
+                if (ROWS) {
+                    advance();
+                    asm volatile("" : "+v"(hi), "+v"(lo));  // (one place that goes on: all of them at once take registers)
+                }
             }
             if (WHAT != APPLY) {
 #pragma unroll
                 for (int k = 0; k < NV; k++) {
                     if constexpr (UNIT == 4) sum += (v[k].v[0] + v[k].v[1]) + (v[k].v[2] + v[k].v[3]);
+                    else if constexpr (UNIT == 2) sum += v[k].v[0] + v[k].v[1];
                     else sum += v[k].v[0];
                 }
                 const float n = (float)min((long long)TILE, last - at), mean_n = block_sum<THREADS>(sum, red) / n;
@@ -191,32 +189,32 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 } else {
                     mean = mean_n;
                     squares = squares_n;
-                    scale = prepare();
+                    prepare();
                 }
             }
             if (WHAT != SUMS) {
                 hi = hi0;
                 lo = lo0;
-                asm volatile("" : "+v"(hi), "+v"(lo));  // (counted again: the places of the first walk would take registers)
 #pragma unroll
                 for (int k = 0; k < NV; k++) {
                     const long long e = e0 + k * STEP;
                     if (e < last) {
+                        // (numbers read together lie in one channel of a map where its pixels are a multiple of them)
+                        const bool alike = !ROWS && whole_units;
+                        float slope = slopes[ROWS ? lo : hi], lift = lifts[ROWS ? lo : hi];
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) {
-                            const int c = ROWS ? lo + i : hi + (UNIT == 4 && lo + i >= inner ? 1 : 0);
-                            float slope, lift;
-                            if (p.per <= COEFFICIENTS) {
+                            if (i && !alike) {
+                                const int c = ROWS ? lo + i : hi + ((unsigned)(lo + i) >= inner ? 1 : 0);
                                 slope = slopes[c];
                                 lift = lifts[c];
-                            } else {
-                                coefficients(p, image, c0 + c, scale, slope, lift);
                             }
                             v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope, lift), p.activation);
                         }
                         set<UNIT>(Y + (ROWS ? hi * p.ldy + lo : e), v[k]);
                     }
                     advance();
+                    if (ROWS) asm volatile("" : "+v"(hi), "+v"(lo));
                 }
             }
         }
@@ -224,34 +222,39 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
     }
 }
 
-// Groups of few channels in rows: a workgroup takes several side by side, so that its pieces of the rows are long enough, and a thread stays in its columns.
-template <int NV, int UNIT, int WHAT>
-__global__ __launch_bounds__(256) void group_norm_rows_kernel(const GroupNormParams p) {
-    __shared__ float red[256], stat[64];
-    const int blocks = (p.groups + p.together - 1) / p.together;
-    for (long long id = blockIdx.x; id < (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD; id += gridDim.x) {
-        const long long job = job_of(id, p.jobs);
+// Rows of tokens whose groups are not wide: a thread stays in its columns.  ONE: a workgroup a group; otherwise several groups side by side, whose
+// pieces of a row would be short.
+template <int THREADS, int NV, int UNIT, bool ONE, int WHAT>
+__global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNormParams p) {
+    __shared__ float red[ONE ? THREADS / 64 : THREADS], stat[ONE ? 1 : 2 * SHORT];
+    for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
+        long long job = xcd_job(id);
         if (job >= p.jobs) continue;
-        const long long which = job / p.split;
-        const int piece = (int)(job % p.split), image = (int)(which / blocks), g0 = (int)(which % blocks) * p.together, here = min(p.together, p.groups - g0);
-        const int units = p.per / UNIT, wide = here * units, rows_at_once = 256 / wide;  // (of a group, of a row, rows of a step)
-        const int tr = threadIdx.x / wide, cu = threadIdx.x % wide, g = cu / units, c = g0 * p.per + cu * UNIT;
+        if (WHAT == APPLY) job = p.jobs - 1 - job;
+        const unsigned which = (unsigned)job / p.split, piece = (unsigned)job % p.split;  // (fewer than 2^31 jobs)
+        const int image = which / p.blocks, g0 = (int)(which % p.blocks) * p.together, here = ONE ? 1 : min(p.together, (int)p.groups - g0);
+        const int units = p.per / UNIT, wide = here * units, rows_at_once = THREADS / wide;  // (of a group, of a row, rows of a step)
+        const int tr = threadIdx.x / wide, cu = threadIdx.x % wide, g = ONE ? 0 : cu / units, c = g0 * p.per + cu * UNIT;
         const bool mine = tr < rows_at_once;
         const long long first = piece * p.part, last = min((long long)p.pixels, first + p.part), total = (long long)p.per * p.pixels;
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-        // the sums of the groups over all threads, by the wavefronts in turn
+        // the sums of the groups over all threads; of several groups by the wavefronts in turn
         auto group_sum = [&](float x) {
-            __syncthreads();
-            red[threadIdx.x] = x;
-            __syncthreads();
-            for (int j = wave; j < here; j += 4) {
-                float s = 0.0f;
-                for (int k = lane; k < rows_at_once * units; k += 64) s += red[k / units * wide + j * units + k % units];
-                s = wave_sum(s);
-                if (lane == 0) stat[j] = s;
+            if constexpr (ONE) {
+                return block_sum<THREADS>(x, red);
+            } else {
+                __syncthreads();
+                red[threadIdx.x] = x;
+                __syncthreads();
+                for (int j = wave; j < here; j += THREADS / 64) {
+                    float s = 0.0f;
+                    for (int k = lane; k < rows_at_once * units; k += 64) s += red[k / units * wide + j * units + k % units];
+                    s = wave_sum(s);
+                    if (lane == 0) stat[j] = s;
+                }
+                __syncthreads();
+                return stat[mine ? g : 0];
             }
-            __syncthreads();
-            return stat[mine ? g : 0];
         };
         float mean = 0.0f, squares = 0.0f, slope[UNIT], lift[UNIT];
         double seen = 0.0;
@@ -262,30 +265,45 @@ __global__ __launch_bounds__(256) void group_norm_rows_kernel(const GroupNormPar
                 if (mine) coefficients(p, image, c + i, scale, slope[i], lift[i]);
         };
         if (WHAT == APPLY) {
-            __syncthreads();
-            for (int j = wave; j < here; j += 4) {
-                join_parts(p.parts + ((long long)image * p.groups + g0 + j) * p.split, p.split, p.part * p.per, total, mean, squares);
-                if (lane == 0) {
-                    red[j] = mean;
-                    stat[j] = squares;
+            const float2 *parts = p.parts + ((long long)image * (int)p.groups + g0) * (int)p.split;
+            if constexpr (ONE) {
+                join_parts(parts, (int)p.split, p.part * p.per, total, mean, squares);
+            } else {
+                __syncthreads();
+                for (int j = wave; j < here; j += THREADS / 64) {
+                    join_parts(parts + j * (int)p.split, (int)p.split, p.part * p.per, total, mean, squares);
+                    if (lane == 0) {
+                        red[j] = mean;
+                        stat[j] = squares;
+                    }
                 }
+                __syncthreads();
+                mean = red[mine ? g : 0];
+                squares = stat[mine ? g : 0];
             }
-            __syncthreads();
-            mean = red[mine ? g : 0];
-            squares = stat[mine ? g : 0];
             prepare();
         }
         for (long long at = first; at < last; at += (long long)rows_at_once * NV) {
+            const long long step_x = rows_at_once * p.ldx, step_y = rows_at_once * p.ldy;
             const long long row0 = (long long)image * p.pixels + at + tr;
+            const int left = mine ? (int)min((long long)rows_at_once * NV, last - at) - tr : 0;  // (rows of the tile from the thread's first one on)
+            const float *x = p.X + row0 * p.ldx + c;
+            float *y = p.Y + row0 * p.ldy + c;
             Unit<UNIT> v[NV];
             float sum = 0.0f;
 #pragma unroll
             for (int k = 0; k < NV; k++) {
 #pragma unroll
                 for (int i = 0; i < UNIT; i++) v[k].v[i] = 0.0f;
-                if (mine && at + tr + k * rows_at_once < last) v[k] = get<UNIT>(p.X + (row0 + k * rows_at_once) * p.ldx + c);
+                if (k * rows_at_once < left) v[k] = get<UNIT>(x);
+                x += step_x;
+                asm volatile("" : "+v"(x));  // (one place that goes on: all of them at once take two registers each)
+            }
 #pragma unroll
-                for (int i = 0; i < UNIT; i++) sum += v[k].v[i];
+            for (int k = 0; k < NV; k++) {
+                if constexpr (UNIT == 4) sum += (v[k].v[0] + v[k].v[1]) + (v[k].v[2] + v[k].v[3]);
+                else if constexpr (UNIT == 2) sum += v[k].v[0] + v[k].v[1];
+                else sum += v[k].v[0];
             }
             if (WHAT != APPLY) {
                 const double n = (double)min((long long)rows_at_once * NV, last - at) * p.per;
@@ -293,7 +311,7 @@ __global__ __launch_bounds__(256) void group_norm_rows_kernel(const GroupNormPar
                 float sq = 0.0f;
 #pragma unroll
                 for (int k = 0; k < NV; k++)
-                    if (mine && at + tr + k * rows_at_once < last) {
+                    if (k * rows_at_once < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) {
                             const float d = v[k].v[i] - mean_n;
@@ -311,76 +329,99 @@ __global__ __launch_bounds__(256) void group_norm_rows_kernel(const GroupNormPar
             }
             if (WHAT != SUMS) {
 #pragma unroll
-                for (int k = 0; k < NV; k++)
-                    if (mine && at + tr + k * rows_at_once < last) {
+                for (int k = 0; k < NV; k++) {
+                    if (k * rows_at_once < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope[i], lift[i]), p.activation);
-                        set<UNIT>(p.Y + (row0 + k * rows_at_once) * p.ldy + c, v[k]);
+                        set<UNIT>(y, v[k]);
                     }
+                    y += step_y;
+                    asm volatile("" : "+v"(y));
+                }
             }
         }
-        if (WHAT == SUMS && tr == 0 && cu % units == 0) p.parts[((long long)image * p.groups + g0 + g) * p.split + piece] = float2{mean, squares};
+        if (WHAT == SUMS && tr == 0 && cu % units == 0) p.parts[((long long)image * (int)p.groups + g0 + g) * (int)p.split + (int)piece] = float2{mean, squares};
     }
 }
 
 typedef void (*Kernel)(GroupNormParams);
 
 // A workgroup for every part of `groups` groups (or of groups taken together).
-int launch(int dev, GroupNormParams &p, Kernel fn, int threads, long long groups) {
+int launch(int dev, GroupNormParams &p, Kernel fn, int threads, long long groups, size_t lds) {
     p.jobs = groups * p.split;
-    const long long most = (1LL << 32) / threads - EDDLHIP_NUM_XCD;  // (a grid holds less than 2^32 threads; its workgroups walk what is beyond)
-    hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(threads), 0, state(dev).stream, p);
+    hipLaunchKernelGGL(fn, dim3(xcd_grid(p.jobs, threads)), dim3(threads), lds, state(dev).stream, p);
     EH_CHECK_LAUNCH();
     return 0;
 }
 
 // Sums and outputs of divided groups.
-int launch_divided(int dev, GroupNormParams &p, Kernel sums, Kernel apply, long long groups) {
+int launch_divided(int dev, GroupNormParams &p, Kernel sums, Kernel apply, long long groups, size_t lds) {
     void *ws = nullptr;
     EH_TRY(get_workspace(dev, (size_t)p.images * p.groups * p.split * sizeof(float2), &ws));
     p.parts = (float2 *)ws;
-    EH_TRY(launch(dev, p, sums, 256, groups));
-    return launch(dev, p, apply, 256, groups);
+    EH_TRY(launch(dev, p, sums, 256, groups, 0));
+    return launch(dev, p, apply, 256, groups, lds);
 }
 
 constexpr int MOST_PARTS = 256, WORKGROUPS = 4096;  // parts of a group; workgroups after which groups are not divided further
 
+// The kernels of a group of `count` numbers: the smallest workgroup that holds it in registers, up to 32 numbers a thread.
+struct Size {
+    int threads, numbers;  // of a thread
+    Kernel fn;
+};
 template <int UNIT, bool ROWS>
 int launch_groups(int dev, GroupNormParams &p) {
-    static const struct {
-        int threads, nv;
-        Kernel fn;
-    } sizes[] = {{256, 1, group_norm_kernel<256, 1, UNIT, ROWS, WHOLE>},           {256, 4, group_norm_kernel<256, 4, UNIT, ROWS, WHOLE>},
-                 {256, 32 / UNIT, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, WHOLE>}, {512, 32 / UNIT, group_norm_kernel<512, 32 / UNIT, UNIT, ROWS, WHOLE>},
-                 {1024, 32 / UNIT, group_norm_kernel<1024, 32 / UNIT, UNIT, ROWS, WHOLE>}};
+    constexpr int NV = 32 / UNIT;
+    static const Size sizes[] = {{256, 4, group_norm_kernel<256, 4 / UNIT, UNIT, ROWS, WHOLE>},   {256, 8, group_norm_kernel<256, 8 / UNIT, UNIT, ROWS, WHOLE>},
+                                 {256, 16, group_norm_kernel<256, 16 / UNIT, UNIT, ROWS, WHOLE>}, {256, 32, group_norm_kernel<256, NV, UNIT, ROWS, WHOLE>},
+                                 {512, 32, group_norm_kernel<512, NV, UNIT, ROWS, WHOLE>},        {1024, 32, group_norm_kernel<1024, NV, UNIT, ROWS, WHOLE>}};
     const long long count = (long long)p.per * p.pixels, groups = (long long)p.images * p.groups;
+    const size_t lds = 2 * p.per * sizeof(float);
     p.split = 1;
     p.part = count;
-    for (const auto &s : sizes)
-        if (count <= (long long)s.threads * s.nv * UNIT) return launch(dev, p, s.fn, s.threads, groups);
+    for (const Size &s : sizes)
+        if (count <= (long long)s.threads * s.numbers) return launch(dev, p, s.fn, s.threads, groups, lds);
     constexpr int TILE = 256 * 32;
     const long long tiles = (count + TILE - 1) / TILE, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
     p.part = (tiles + parts - 1) / parts * TILE;
-    p.split = (int)((count + p.part - 1) / p.part);
-    return launch_divided(dev, p, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, SUMS>, group_norm_kernel<256, 32 / UNIT, UNIT, ROWS, APPLY>, groups);
+    p.split = (unsigned)((count + p.part - 1) / p.part);
+    return launch_divided(dev, p, group_norm_kernel<256, NV, UNIT, ROWS, SUMS>, group_norm_kernel<256, NV, UNIT, ROWS, APPLY>, groups, lds);
 }
 
-constexpr int SHORT = 16;  // channels of a group: with fewer, 64 bytes of a row are taken together
-
-template <int UNIT>
-int launch_short(int dev, GroupNormParams &p) {
-    p.together = std::min(p.groups, (2 * SHORT + p.per - 1) / p.per);
-    const int at_once = 256 / (p.together * p.per / UNIT);  // rows
-    const long long groups = (long long)p.images * ((p.groups + p.together - 1) / p.together);
+template <int UNIT, bool ONE>
+int launch_rows(int dev, GroupNormParams &p) {
+    constexpr int NV = 32 / UNIT;
+    static const Size sizes[] = {{256, 4, group_norm_rows_kernel<256, 4 / UNIT, UNIT, ONE, WHOLE>},   {256, 8, group_norm_rows_kernel<256, 8 / UNIT, UNIT, ONE, WHOLE>},
+                                 {256, 16, group_norm_rows_kernel<256, 16 / UNIT, UNIT, ONE, WHOLE>}, {256, 24, group_norm_rows_kernel<256, 24 / UNIT, UNIT, ONE, WHOLE>},
+                                 {256, 32, group_norm_rows_kernel<256, NV, UNIT, ONE, WHOLE>},        {512, 32, group_norm_rows_kernel<512, NV, UNIT, ONE, WHOLE>},
+                                 {1024, 32, group_norm_rows_kernel<1024, NV, UNIT, ONE, WHOLE>}};
+    p.together = ONE ? 1 : std::min((int)p.groups, (2 * SHORT + p.per - 1) / p.per);
+    p.blocks = (p.groups + p.together - 1) / p.together;
+    const int wide = p.together * p.per / UNIT;  // units of a row
+    const long long groups = (long long)p.images * p.blocks;
     p.split = 1;
     p.part = p.pixels;
-    if (p.pixels <= 4 * at_once) return launch(dev, p, group_norm_rows_kernel<4, UNIT, WHOLE>, 256, groups);
-    if (p.pixels <= 32 / UNIT * at_once) return launch(dev, p, group_norm_rows_kernel<32 / UNIT, UNIT, WHOLE>, 256, groups);
-    const int tile = 32 / UNIT * at_once;
+    for (const Size &s : sizes)
+        if (p.pixels <= (long long)(s.threads / wide) * (s.numbers / UNIT)) return launch(dev, p, s.fn, s.threads, groups, 0);
+    const int tile = 256 / wide * NV;  // rows
     const long long tiles = (p.pixels + tile - 1) / tile, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
     p.part = (tiles + parts - 1) / parts * tile;
-    p.split = (int)((p.pixels + p.part - 1) / p.part);
-    return launch_divided(dev, p, group_norm_rows_kernel<32 / UNIT, UNIT, SUMS>, group_norm_rows_kernel<32 / UNIT, UNIT, APPLY>, groups);
+    p.split = (unsigned)((p.pixels + p.part - 1) / p.part);
+    return launch_divided(dev, p, group_norm_rows_kernel<256, NV, UNIT, ONE, SUMS>, group_norm_rows_kernel<256, NV, UNIT, ONE, APPLY>, groups, 0);
+}
+
+// Maps: a group begins at a multiple of UNIT numbers, which meet two channels at most.
+int launch_maps(int dev, GroupNormParams &p, int aligned) {
+    const long long count = (long long)p.per * p.pixels;
+    if (aligned == 4 && count % 4 == 0 && p.pixels >= 4) return launch_groups<4, false>(dev, p);
+    if (aligned >= 2 && count % 2 == 0 && p.pixels >= 2) return launch_groups<2, false>(dev, p);
+    return launch_groups<1, false>(dev, p);
+}
+template <int UNIT>
+int launch_tokens(int dev, GroupNormParams &p) {
+    if (p.per < SHORT && p.groups > 1) return launch_rows<UNIT, false>(dev, p);
+    return p.per / UNIT <= 32 ? launch_rows<UNIT, true>(dev, p) : launch_groups<UNIT, true>(dev, p);  // (an eighth of the threads idle at most)
 }
 
 }  // namespace
@@ -388,7 +429,7 @@ int launch_short(int dev, GroupNormParams &p) {
 extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last, int groups,
                                   const float *w, const float *b, float eps, const float *mod, const float *shift, int activation) {
     EH_REQUIRE(images >= 0 && channels > 0 && pixels > 0, "group_norm: %d images of %d channels of %d pixels", images, channels, pixels);
-    EH_REQUIRE(groups > 0 && channels % groups == 0, "group_norm: %d channels in %d groups", channels, groups);
+    EH_REQUIRE(groups > 0 && channels % groups == 0 && channels / groups <= MOST_CHANNELS, "group_norm: %d channels in %d groups (of up to %d)", channels, groups, MOST_CHANNELS);
     EH_REQUIRE((long long)images * pixels <= 0x7fffffffLL && (long long)images * channels <= 0x7fffffffLL, "group_norm: %d images of %d channels of %d pixels are out of range", images, channels, pixels);
     EH_REQUIRE(activation == EDDLHIP_ACT_NONE || activation == EDDLHIP_ACT_RELU || activation == EDDLHIP_ACT_SILU, "group_norm: unknown activation %d", activation);
     EH_REQUIRE(!channels_last || (ldx >= channels && ldy >= channels), "group_norm: rows shorter than %d channels", channels);
@@ -421,13 +462,13 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     p.per = channels / groups;
     p.parts = nullptr;
     p.together = 1;
+    p.blocks = groups;
     p.eps = eps;
-    const bool aligned = (((uintptr_t)X | (uintptr_t)Y) & 15) == 0;
-    if (!channels_last) {  // (a group begins at a multiple of 16 bytes, and four numbers meet two channels at most)
-        if (aligned && (long long)p.per * pixels % 4 == 0 && pixels >= 4) return launch_groups<4, false>(dev, p);
-        return launch_groups<1, false>(dev, p);
-    }
-    const bool vec = aligned && p.per % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0;
-    if (p.per < SHORT && groups > 1) return vec ? launch_short<4>(dev, p) : launch_short<1>(dev, p);
-    return vec ? launch_groups<4, true>(dev, p) : launch_groups<1, true>(dev, p);
+    // (numbers that may be read at a time)
+    const uintptr_t bits = (uintptr_t)X | (uintptr_t)Y;
+    const int aligned = bits % 16 == 0 ? 4 : bits % 8 == 0 ? 2 : 1;
+    if (!channels_last) return launch_maps(dev, p, aligned);
+    if (aligned == 4 && p.per % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0) return launch_tokens<4>(dev, p);
+    if (aligned >= 2 && p.per % 2 == 0 && ldx % 2 == 0 && ldy % 2 == 0) return launch_tokens<2>(dev, p);
+    return launch_tokens<1>(dev, p);
 }

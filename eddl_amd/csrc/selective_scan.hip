@@ -6,6 +6,7 @@
 #include "common.h"
 #include "activation.h"
 #include "state_batch.h"
+#include "xcd.h"
 
 using namespace eddlhip;
 
@@ -19,7 +20,7 @@ struct ScanParams {
     float *part_states, *part_factors;  // [sequence][part + 1][channel][NP], [sequence][part][channel][NP]
     long long ldx, lddt, ldg, ldb, ldc, ldy;
     int channels, n, per;  // channels that share B and C
-    int blocks, group_blocks, parts;
+    unsigned blocks, group_blocks, parts;
     long long jobs;
     bool softplus, vectors;  // B and C are read 16 bytes at a time
     StateBatch batch;
@@ -39,59 +40,84 @@ __device__ __forceinline__ float lane_sum(float x) {
     return x;
 }
 
-// The NL states of channel c from n0 on: as the sequence finds them, and on their way to the pool; the factors of the steps in powers of two.
-template <int NL>
-__device__ __forceinline__ void first_state(const ScanParams &p, const Sequence &q, int c, int n0, float (&h)[NL]) {
+// NL numbers from n0 of n on; 0 behind the last.  VEC: n is a multiple of NL and the place one of their size.
+template <int NL, bool VEC>
+__device__ __forceinline__ void get(const float *from, int n0, int n, float (&v)[NL]) {
+    typedef float vec __attribute__((ext_vector_type(NL)));
+    if constexpr (VEC) {
+        vec u;
 #pragma unroll
-    for (int i = 0; i < NL; i++) {
-        h[i] = 0.0f;
-        if (q.read >= 0 && n0 + i < p.n) h[i] = p.states[((long long)q.read * p.channels + c) * p.n + n0 + i];
-        if (q.read == -2) h[i] = __builtin_nanf("");
+        for (int i = 0; i < NL; i++) u[i] = 0.0f;
+        if (n0 < n) u = *reinterpret_cast<const vec *>(from + n0);
+#pragma unroll
+        for (int i = 0; i < NL; i++) v[i] = u[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NL; i++) v[i] = n0 + i < n ? from[n0 + i] : 0.0f;
     }
 }
-template <int NL>
-__device__ __forceinline__ void keep_state(const ScanParams &p, const Sequence &q, int c, int n0, const float (&h)[NL]) {
-    if (q.write < 0) return;
+// The NL states of channel c from n0 on: as the sequence finds them, and on their way to the pool; the factors of the steps in powers of two.
+template <int NL, bool VEC>
+__device__ __forceinline__ void first_state(const ScanParams &p, const Sequence &q, int c, int n0, float (&h)[NL]) {
 #pragma unroll
-    for (int i = 0; i < NL; i++)
-        if (n0 + i < p.n) p.states[((long long)q.write * p.channels + c) * p.n + n0 + i] = h[i];
+    for (int i = 0; i < NL; i++) h[i] = q.read == -2 ? __builtin_nanf("") : 0.0f;
+    if (q.read >= 0) get<NL, VEC>(p.states + ((long long)q.read * p.channels + c) * p.n, n0, p.n, h);
 }
-template <int NL>
-__device__ __forceinline__ void exponents(const ScanParams &p, int c, int n0, float (&a)[NL]) {
+template <int NL, bool VEC>
+__device__ __forceinline__ void keep_state(const ScanParams &p, const Sequence &q, int c, int n0, const float (&h)[NL]) {
+    typedef float vec __attribute__((ext_vector_type(NL)));
+    if (q.write < 0) return;
+    float *to = p.states + ((long long)q.write * p.channels + c) * p.n + n0;
+    if constexpr (VEC) {
+        vec u;
 #pragma unroll
-    for (int i = 0; i < NL; i++) a[i] = n0 + i < p.n ? p.A[(long long)c * p.n + n0 + i] * LOG2_E : 0.0f;
+        for (int i = 0; i < NL; i++) u[i] = h[i];
+        if (n0 < p.n) *reinterpret_cast<vec *>(to) = u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+            if (n0 + i < p.n) to[i] = h[i];
+    }
+}
+template <int NL, bool VEC>
+__device__ __forceinline__ void exponents(const ScanParams &p, int c, int n0, float (&a)[NL]) {
+    get<NL, VEC>(p.A + (long long)c * p.n, n0, p.n, a);
+#pragma unroll
+    for (int i = 0; i < NL; i++) a[i] *= LOG2_E;
 }
 
-// Few tokens a sequence: LANES lanes a channel, NL states each; token after token from memory.
-template <int LANES, int NL>
+// Few tokens a sequence: LANES lanes a channel, NL states each; token after token from memory.  VEC: vectors, states and A are read 16 bytes at a time.
+template <int LANES, int NL, bool VEC>
 __global__ __launch_bounds__(256) void scan_tokens_kernel(const ScanParams p) {
     const Sequence q = sequence(p.batch, blockIdx.y);
     const int c = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES, n0 = lane * NL;
     if (q.fresh == 0 || c >= p.channels) return;
     float a[NL], h[NL];
-    exponents<NL>(p, c, n0, a);
-    first_state<NL>(p, q, c, n0, h);
+    first_state<NL, VEC>(p, q, c, n0, h);
+    exponents<NL, VEC>(p, c, n0, a);
     const float bias = p.dt_bias ? p.dt_bias[c] : 0.0f, skip = p.skip ? p.skip[c] : 0.0f;
-    const int v0 = c / p.per * p.n + n0;
+    const int v0 = c / p.per * p.n;
     for (int t = 0; t < q.fresh; t++) {
         const long long row = q.row(t);
-        const float raw = p.dt[row * p.lddt + c] + bias, d = p.softplus ? softplus(raw) : raw, x = p.X[row * p.ldx + c], dx = d * x;
+        float b[NL], cc[NL];
+        get<NL, VEC>(p.B + row * p.ldb + v0, n0, p.n, b);
+        get<NL, VEC>(p.C + row * p.ldc + v0, n0, p.n, cc);
+        const float raw = p.dt[row * p.lddt + c] + bias, x = p.X[row * p.ldx + c], g = p.gate ? p.gate[row * p.ldg + c] : 0.0f;
+        const float d = p.softplus ? softplus(raw) : raw, dx = d * x;
         float y = 0.0f;
 #pragma unroll
         for (int i = 0; i < NL; i++) {
-            const bool has = n0 + i < p.n;
-            const float b = has ? p.B[row * p.ldb + v0 + i] : 0.0f, cc = has ? p.C[row * p.ldc + v0 + i] : 0.0f;
-            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a[i]), h[i], dx * b);
-            y = __builtin_fmaf(cc, h[i], y);
+            h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a[i]), h[i], dx * b[i]);
+            y = __builtin_fmaf(cc[i], h[i], y);
         }
         y = lane_sum<LANES>(y);
         if (lane == 0) {
-            if (p.skip) y = __builtin_fmaf(skip, x, y);
-            if (p.gate) y *= silu(p.gate[row * p.ldg + c]);
+            y = __builtin_fmaf(skip, x, y);
+            if (p.gate) y *= silu(g);
             p.Y[row * p.ldy + c] = y;
         }
     }
-    keep_state<NL>(p, q, c, n0, h);
+    keep_state<NL, VEC>(p, q, c, n0, h);
 }
 
 // Many tokens.  A workgroup takes a tile of tokens of some channels into LDS - steps d, products d x, vectors B and C - and walks it with LANES lanes a
@@ -124,19 +150,19 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
     __shared__ __attribute__((aligned(16))) vec vb[T::VECTORS], vc[PART == 1 ? 1 : T::VECTORS];
     __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? T::THREADS : 1], factor[WT > 1 ? T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
 
-    // Workgroups side by side in channels share lines of memory: they are put on one XCD.
-    const long long per_xcd = (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD;
-    for (long long id = blockIdx.x; id < per_xcd * EDDLHIP_NUM_XCD; id += gridDim.x) {
-        const long long job = id % EDDLHIP_NUM_XCD * per_xcd + id / EDDLHIP_NUM_XCD;
+    // (workgroups side by side in channels share lines of memory, and B and C)
+    for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
+        const long long job = xcd_job(id);
         if (job >= p.jobs) continue;
-        const int block = (int)(job % p.blocks), group = block / p.group_blocks, part = (int)(job / p.blocks % p.parts), s = (int)(job / p.blocks / p.parts);
+        const unsigned rest = (unsigned)job / p.blocks;  // (fewer than 2^31 jobs)
+        const int block = (unsigned)job % p.blocks, group = block / p.group_blocks, part = rest % p.parts, s = rest / p.parts;
         const Sequence q = sequence(p.batch, s);
-        const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + p.parts - 1) / p.parts;  // (of a part)
+        const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + (int)p.parts - 1) / (int)p.parts;  // (of a part)
         const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
         if (tile0 == tile1) continue;
 
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
-        const int c0 = group * p.per + block % p.group_blocks * T::CHANNELS, cend = (group + 1) * p.per;
+        const int c0 = group * p.per + (int)(block % p.group_blocks) * T::CHANNELS, cend = (group + 1) * p.per;
         const int ch = wc * (64 / LANES) + lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
         const bool mine = c < cend;
 
@@ -146,20 +172,20 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             a[i] = h[i] = 0.0f;
             through[i] = 1.0f;
         }
-        if (mine) exponents<NL>(p, c, n0, a);
+        if (mine) exponents<NL, false>(p, c, n0, a);
         if (mine && wt == 0) {
-            float *states = PART ? p.part_states + ((long long)s * (p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
+            float *states = PART ? p.part_states + ((long long)s * ((int)p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
             if (PART == 0) {
-                first_state<NL>(p, q, c, n0, h);
+                first_state<NL, false>(p, q, c, n0, h);
             } else if (PART == 1) {
                 if (part == 0) {  // kept for the second launch, in which the slot may be written already
                     float kept[NL];
-                    first_state<NL>(p, q, c, n0, kept);
+                    first_state<NL, false>(p, q, c, n0, kept);
 #pragma unroll
                     for (int i = 0; i < NL; i++) states[i] = kept[i];
                 }
             } else {
-                const float *factors = p.part_factors + ((long long)s * p.parts * p.channels + c) * T::NP + n0;
+                const float *factors = p.part_factors + ((long long)s * (int)p.parts * p.channels + c) * T::NP + n0;
                 const long long step = (long long)p.channels * T::NP;
                 const vec v = *reinterpret_cast<const vec *>(states);
 #pragma unroll
@@ -393,8 +419,8 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
         }
         if (PART == 1) {
             if (mine && wt == 0) {
-                float *states = p.part_states + (((long long)s * (p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
-                float *factors = p.part_factors + (((long long)s * p.parts + part) * p.channels + c) * T::NP + n0;
+                float *states = p.part_states + (((long long)s * ((int)p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
+                float *factors = p.part_factors + (((long long)s * (int)p.parts + part) * p.channels + c) * T::NP + n0;
 #pragma unroll
                 for (int i = 0; i < NL; i++) {
                     states[i] = h[i];
@@ -402,7 +428,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                 }
             }
         } else if (mine && wt == WT - 1 && tile1 == tiles) {
-            keep_state<NL>(p, q, c, n0, h);
+            keep_state<NL, false>(p, q, c, n0, h);
         }
         __syncthreads();  // (the next job's tiles)
     }
@@ -415,7 +441,8 @@ template <int LANES, int NL>
 int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
     const hipStream_t st = state(dev).stream;
     if (tokens <= FEW_TOKENS) {
-        hipLaunchKernelGGL((scan_tokens_kernel<LANES, NL>), dim3((unsigned)(((long long)p.channels * LANES + 255) / 256), seqs), dim3(256), 0, st, p);
+        const bool whole = p.vectors && (((uintptr_t)p.states | (uintptr_t)p.A) & 15) == 0;
+        hipLaunchKernelGGL((whole ? scan_tokens_kernel<LANES, NL, true> : scan_tokens_kernel<LANES, NL, false>), dim3((unsigned)(((long long)p.channels * LANES + 255) / 256), seqs), dim3(256), 0, st, p);
         EH_CHECK_LAUNCH();
         return 0;
     }
@@ -423,8 +450,8 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
     const long long num_cu = state(dev).num_cu;
     auto launch = [&](auto fn, int threads) {
         p.jobs = (long long)p.blocks * p.parts * seqs;
-        const long long most = (1LL << 32) / threads - EDDLHIP_NUM_XCD;  // workgroups (a grid holds less than 2^32 threads); they walk what is beyond
-        hipLaunchKernelGGL(fn, dim3((unsigned)std::min(most, (p.jobs + EDDLHIP_NUM_XCD - 1) / EDDLHIP_NUM_XCD * EDDLHIP_NUM_XCD)), dim3(threads), 0, st, p);
+        EH_REQUIRE(p.jobs < (1LL << 31), "selective_scan: %d sequences of %d channels in %d groups are out of range", seqs, p.channels, groups);
+        hipLaunchKernelGGL(fn, dim3(xcd_grid(p.jobs, threads)), dim3(threads), 0, st, p);
         EH_CHECK_LAUNCH();
         return 0;
     };

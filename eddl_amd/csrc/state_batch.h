@@ -29,7 +29,7 @@ __device__ __forceinline__ Sequence sequence(const StateBatch &b, int s) {
     return q;
 }
 
-constexpr int MOST_CHANNELS = 1 << 24, MOST_ROWS = 1 << 30;
+constexpr int MOST_CHANNELS = 1 << 20, MOST_ROWS = 1 << 30;
 
 // What both entry points ask of a batch; `name` opens the error's text.
 inline int check_batch(const char *name, int rows, int seqs, int max_new, const float *states, int pool, const int *offsets, const int *lengths, const int *slots, const int *out_slots) {

@@ -580,7 +580,7 @@ int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R
 /* The norm of groups of channels side by side, over all pixels of an image, and its activation:
  *     n = (x - mean) / sqrt(variance + eps) w + b,   Y = act(n (1 + mod) + shift).
  * channels_last == 0: maps X, Y [images][channels][pixels], ldx and ldy are not looked at.  Otherwise rows of tokens [images * pixels][channels] that lie
- * ldx and ldy floats apart.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
+ * ldx and ldy floats apart.  Up to 4096 channels a group.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
  * whose group holds an infinity or NaN is NaN in that group; images and groups do not reach one another. */
 int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last,
                        int groups, const float *w, const float *b, float eps, const float *mod, const float *shift, int activation);

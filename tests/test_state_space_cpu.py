@@ -28,7 +28,7 @@ NORM = dict(dev=99, X=P[0], ldx=64, Y=P[1], ldy=64, images=3, channels=64, pixel
 
 
 @pytest.mark.parametrize("change, text", [
-    (dict(), None), (dict(groups=7), "64 channels in 7 groups"), (dict(groups=0), "in 0 groups"), (dict(groups=-8), "groups"), (dict(channels=0), "0 channels"), (dict(pixels=0), "0 pixels"),
+    (dict(), None), (dict(groups=7), "64 channels in 7 groups"), (dict(groups=0), "in 0 groups"), (dict(groups=-8), "groups"), (dict(groups=1, channels=4097, ldx=5000, ldy=5000), "of up to 4096"), (dict(channels=0), "0 channels"), (dict(pixels=0), "0 pixels"),
     (dict(images=-1), "-1 images"), (dict(images=1 << 16, pixels=1 << 16), "out of range"), (dict(activation=3), "unknown activation 3"), (dict(activation=-1), "unknown activation"),
     (dict(ldx=63), "shorter"), (dict(ldy=63), "shorter"), (dict(ldx=1, ldy=1, last=0), None), (dict(X=None), "NULL"), (dict(Y=None), "NULL"), (dict(Y=P[0]), None),
     (dict(Y=P[0], ldy=80), "in place"), (dict(Y=P[0] + 16), "part of the input"), (dict(Y=P[0] + 64 * 4, ldx=128, ldy=128), None), (dict(Y=P[0] + 64 * 4, last=0), "part of the input"),
