@@ -33,6 +33,7 @@ struct GroupNormParams {
     long long part;       // numbers of a part, or rows of one (short rows)
     long long jobs;       // of the launch
     int together;         // groups of a workgroup (short rows)
+    bool lines;           // a workgroup writes whole lines of memory
     float eps;
 };
 
@@ -66,14 +67,21 @@ __device__ __forceinline__ Unit<UNIT> get(const float *from) {
     for (int i = 0; i < UNIT; i++) u.v[i] = v[i];
     return u;
 }
+// Whole lines of memory are written past the caches (rows of 32 channels a group 29 -> 24 us); of a piece of a line the L2 makes a whole one
+// (24 channels a group 27 -> 21).
 template <int UNIT>
-__device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
+__device__ __forceinline__ void set(float *to, const Unit<UNIT> &u, bool lines) {
     typedef float vec __attribute__((ext_vector_type(UNIT)));
     vec v;
 #pragma unroll
     for (int i = 0; i < UNIT; i++) v[i] = u.v[i];
-    if constexpr (UNIT == 4) __builtin_nontemporal_store(v, reinterpret_cast<vec *>(to));
-    else *reinterpret_cast<vec *>(to) = v;
+    if (UNIT == 4 && lines) {
+        asm volatile("");  // (or the compiler makes one store of the two, without the hint)
+        __builtin_nontemporal_store(v, reinterpret_cast<vec *>(to));
+        asm volatile("");
+    } else {
+        *reinterpret_cast<vec *>(to) = v;
+    }
 }
 
 // y = act((x - mean) slope + lift) for a channel of an image
@@ -123,23 +131,26 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
         long long job = xcd_job(id);  // (groups side by side share lines of memory where they are pieces of rows)
         if (job >= p.jobs) continue;
         if (WHAT == APPLY) job = p.jobs - 1 - job;  // (what the sums read last is still in the last-level cache)
-        const unsigned which = (unsigned)job / p.split;  // (fewer than 2^31 jobs)
-        const long long first = (unsigned)job % p.split * p.part, last = min(count, first + p.part);
+        // (fewer than 2^31 jobs; in rows the groups of a piece come one after another, since they share lines)
+        const unsigned piece = ROWS ? (unsigned)job / p.groups % p.split : (unsigned)job % p.split;
+        const unsigned which = ROWS ? (unsigned)job / p.groups / p.split * p.groups + (unsigned)job % p.groups : (unsigned)job / p.split;
+        const long long first = piece * p.part, last = min(count, first + p.part);
         const int image = which / p.groups, c0 = (int)(which % p.groups) * p.per;
         const float *X = p.X + (ROWS ? (long long)image * p.pixels * p.ldx + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float *Y = p.Y + (ROWS ? (long long)image * p.pixels * p.ldy + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float mean = 0.0f, squares = 0.0f;
         double seen = 0.0;
-        if (WHAT == APPLY) join_parts(p.parts + (long long)which * (int)p.split, (int)p.split, p.part, count, mean, squares);
         auto prepare = [&]() {  // slopes and lifts of the group's channels
             const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
             if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
             for (int c = threadIdx.x; c < p.per; c += THREADS) coefficients(p, image, c0 + c, scale, slopes[c], lifts[c]);
             __syncthreads();
         };
-        if (WHAT == APPLY) prepare();
         for (long long at = first; at < last; at += TILE) {
             const long long e0 = at + threadIdx.x * UNIT;
+            const int left = (int)(min((long long)TILE, last - at) - threadIdx.x * UNIT);  // (numbers of the tile from the thread's first one on)
+            const float *x = X + e0;
+            float *y = Y + e0;
             // (the tile's first number by the workgroup, the thread's in 32 bits)
             const unsigned hi_at = WHAT == WHOLE ? 0 : (unsigned)(at / inner), lo_at = (WHAT == WHOLE ? 0 : (unsigned)(at % inner)) + threadIdx.x * UNIT;
             const int hi0 = hi_at + lo_at / inner, lo0 = lo_at % inner;
@@ -156,14 +167,17 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
             };
 #pragma unroll
             for (int k = 0; k < NV; k++) {
-                const long long e = e0 + k * STEP;
 #pragma unroll
                 for (int i = 0; i < UNIT; i++) v[k].v[i] = 0.0f;
-                if (e < last) v[k] = get<UNIT>(X + (ROWS ? hi * p.ldx + lo : e));
+                if (k * STEP < left) v[k] = get<UNIT>(ROWS ? X + hi * p.ldx + lo : x + k * STEP);
                 if (ROWS) {
                     advance();
                     asm volatile("" : "+v"(hi), "+v"(lo));  // (one place that goes on: all of them at once take registers)
                 }
+            }
+            if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
+                join_parts(p.parts + (long long)which * (int)p.split, (int)p.split, p.part, count, mean, squares);
+                prepare();
             }
             if (WHAT != APPLY) {
 #pragma unroll
@@ -176,7 +190,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 float sq = 0.0f;
 #pragma unroll
                 for (int k = 0; k < NV; k++)
-                    if (e0 + k * STEP < last) {
+                    if (k * STEP < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) {
                             const float d = v[k].v[i] - mean_n;
@@ -197,8 +211,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 lo = lo0;
 #pragma unroll
                 for (int k = 0; k < NV; k++) {
-                    const long long e = e0 + k * STEP;
-                    if (e < last) {
+                    if (k * STEP < left) {
                         // (numbers read together lie in one channel of a map where its pixels are a multiple of them)
                         const bool alike = !ROWS && whole_units;
                         float slope = slopes[ROWS ? lo : hi], lift = lifts[ROWS ? lo : hi];
@@ -211,14 +224,14 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                             }
                             v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope, lift), p.activation);
                         }
-                        set<UNIT>(Y + (ROWS ? hi * p.ldy + lo : e), v[k]);
+                        set<UNIT>(ROWS ? Y + hi * p.ldy + lo : y + k * STEP, v[k], p.lines);
                     }
                     advance();
-                    if (ROWS) asm volatile("" : "+v"(hi), "+v"(lo));
+                    asm volatile("" : "+v"(hi), "+v"(lo));
                 }
             }
         }
-        if (WHAT == SUMS && threadIdx.x == 0) p.parts[job] = float2{mean, squares};
+        if (WHAT == SUMS && threadIdx.x == 0) p.parts[(long long)which * (int)p.split + (int)piece] = float2{mean, squares};
     }
 }
 
@@ -231,8 +244,8 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
         long long job = xcd_job(id);
         if (job >= p.jobs) continue;
         if (WHAT == APPLY) job = p.jobs - 1 - job;
-        const unsigned which = (unsigned)job / p.split, piece = (unsigned)job % p.split;  // (fewer than 2^31 jobs)
-        const int image = which / p.blocks, g0 = (int)(which % p.blocks) * p.together, here = ONE ? 1 : min(p.together, (int)p.groups - g0);
+        const unsigned which = (unsigned)job / p.blocks, piece = which % p.split;  // (fewer than 2^31 jobs; pieces of the same rows one after another)
+        const int image = which / p.split, g0 = (int)((unsigned)job % p.blocks) * p.together, here = ONE ? 1 : min(p.together, (int)p.groups - g0);
         const int units = p.per / UNIT, wide = here * units, rows_at_once = THREADS / wide;  // (of a group, of a row, rows of a step)
         const int tr = threadIdx.x / wide, cu = threadIdx.x % wide, g = ONE ? 0 : cu / units, c = g0 * p.per + cu * UNIT;
         const bool mine = tr < rows_at_once;
@@ -264,25 +277,6 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
             for (int i = 0; i < UNIT; i++)
                 if (mine) coefficients(p, image, c + i, scale, slope[i], lift[i]);
         };
-        if (WHAT == APPLY) {
-            const float2 *parts = p.parts + ((long long)image * (int)p.groups + g0) * (int)p.split;
-            if constexpr (ONE) {
-                join_parts(parts, (int)p.split, p.part * p.per, total, mean, squares);
-            } else {
-                __syncthreads();
-                for (int j = wave; j < here; j += THREADS / 64) {
-                    join_parts(parts + j * (int)p.split, (int)p.split, p.part * p.per, total, mean, squares);
-                    if (lane == 0) {
-                        red[j] = mean;
-                        stat[j] = squares;
-                    }
-                }
-                __syncthreads();
-                mean = red[mine ? g : 0];
-                squares = stat[mine ? g : 0];
-            }
-            prepare();
-        }
         for (long long at = first; at < last; at += (long long)rows_at_once * NV) {
             const long long step_x = rows_at_once * p.ldx, step_y = rows_at_once * p.ldy;
             const long long row0 = (long long)image * p.pixels + at + tr;
@@ -298,6 +292,25 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                 if (k * rows_at_once < left) v[k] = get<UNIT>(x);
                 x += step_x;
                 asm volatile("" : "+v"(x));  // (one place that goes on: all of them at once take two registers each)
+            }
+            if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
+                const float2 *parts = p.parts + ((long long)image * (int)p.groups + g0) * (int)p.split;
+                if constexpr (ONE) {
+                    join_parts(parts, (int)p.split, p.part * p.per, total, mean, squares);
+                } else {
+                    __syncthreads();
+                    for (int j = wave; j < here; j += THREADS / 64) {
+                        join_parts(parts + j * (int)p.split, (int)p.split, p.part * p.per, total, mean, squares);
+                        if (lane == 0) {
+                            red[j] = mean;
+                            stat[j] = squares;
+                        }
+                    }
+                    __syncthreads();
+                    mean = red[mine ? g : 0];
+                    squares = stat[mine ? g : 0];
+                }
+                prepare();
             }
 #pragma unroll
             for (int k = 0; k < NV; k++) {
@@ -333,7 +346,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                     if (k * rows_at_once < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope[i], lift[i]), p.activation);
-                        set<UNIT>(y, v[k]);
+                        set<UNIT>(y, v[k], p.lines);
                     }
                     y += step_y;
                     asm volatile("" : "+v"(y));
@@ -467,6 +480,7 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     // (numbers that may be read at a time)
     const uintptr_t bits = (uintptr_t)X | (uintptr_t)Y;
     const int aligned = bits % 16 == 0 ? 4 : bits % 8 == 0 ? 2 : 1;
+    p.lines = !channels_last || (p.per % 32 == 0 && ldy % 32 == 0 && (uintptr_t)Y % 128 == 0);
     if (!channels_last) return launch_maps(dev, p, aligned);
     if (aligned == 4 && p.per % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0) return launch_tokens<4>(dev, p);
     if (aligned >= 2 && p.per % 2 == 0 && ldx % 2 == 0 && ldy % 2 == 0) return launch_tokens<2>(dev, p);
