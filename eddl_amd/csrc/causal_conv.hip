@@ -41,7 +41,7 @@ __device__ __forceinline__ Unit<UNIT> get(const float *from) {
 }
 template <int UNIT>
 __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
-    if constexpr (UNIT == 4) *reinterpret_cast<floatx4 *>(to) = floatx4{u.v[0], u.v[1], u.v[2], u.v[3]};
+    if constexpr (UNIT == 4) __builtin_nontemporal_store(floatx4{u.v[0], u.v[1], u.v[2], u.v[3]}, reinterpret_cast<floatx4 *>(to));  // (4096 tokens of 4096 channels 38 -> 30 us)
     else *to = u.v[0];
 }
 

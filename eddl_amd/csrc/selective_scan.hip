@@ -120,35 +120,44 @@ __global__ __launch_bounds__(256) void scan_tokens_kernel(const ScanParams p) {
     keep_state<NL, VEC>(p, q, c, n0, h);
 }
 
-// Many tokens.  A workgroup takes a tile of tokens of some channels into LDS - steps d, products d x, vectors B and C - and walks it with LANES lanes a
-// channel, NL states each.  WT of its WAVES wavefronts divide the tile's tokens, the others its channels.  With WT > 1 a wavefront first brings its tokens' state
-// from zeros, keeping factors e^(d A) and products d x B in registers, then takes in what the wavefronts before it brought, and walks its tokens
-// again with the state that they begin with.
+// Many tokens.  A wavefront lays a tile of its tokens and channels out in LDS of its own - steps d, products d x, vectors B and C - and walks it with LANES
+// lanes a channel, NL states each; nothing but a wavefront's own order of instructions stands between the two.  WT of a workgroup's WAVES wavefronts divide
+// the tokens of the same channels: each first brings its tokens' state from zeros, keeping factors e^(d A) and products d x B in registers, then takes
+// in what the wavefronts before it brought, and walks its tokens again with the state that they begin with.  The others have channels of their own.
 template <int LANES, int NL, int WAVES, int WT>
 struct ScanTile {
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int TT = LANES == 4 ? 16 : 8;                // tokens of a wavefront
-    static constexpr int TOKENS = TT * WT;                        // of a tile
-    static constexpr int CHANNELS = 64 / LANES * (WAVES / WT);    // of a workgroup
-    static constexpr int NP = LANES * NL;                         // states, with those behind the last
-    static constexpr int STRIDE = TOKENS + 4;                     // floats from a channel's steps to the next one's (neighbours' 16 bytes lie in banks of their own)
-    static constexpr int CQ = CHANNELS / 4;                       // a thread brings numbers of four channels side by side
-    static constexpr int QUADS = TOKENS * CQ;
-    static constexpr int PER = (QUADS + THREADS - 1) / THREADS;
-    static constexpr int VECTORS = TOKENS * LANES;                // pieces of NL numbers of B or C
-    static constexpr int VPER = (VECTORS + THREADS - 1) / THREADS;
+    static constexpr int TT = LANES >= 4 ? 16 : 8;         // tokens of a wavefront
+    static constexpr int TOKENS = TT * WT;                 // of a workgroup at a time
+    static constexpr int CH = 64 / LANES;                  // channels of a wavefront
+    static constexpr int CHANNELS = CH * (WAVES / WT);     // of a workgroup
+    static constexpr int NP = LANES * NL;                  // states, with those behind the last
+    static constexpr int STRIDE = TT + 4;                  // floats from a channel's steps to the next one's (16 bytes of neighbours lie in banks of their own)
+    static constexpr int U = TT / LANES < 4 ? TT / LANES : 4;  // a lane brings numbers of U channels side by side
+    static constexpr int CQ = CH / U;
+    static constexpr int PER = TT * CQ / 64;
+    static constexpr int VECTORS = TT * LANES;             // pieces of NL numbers of B or C
+    static constexpr int VPER = (VECTORS + 63) / 64;
 };
+// What a wavefront's lanes wrote to LDS before is what they read behind: the hardware keeps the order, the compiler has to.
+__device__ __forceinline__ void in_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups: PART 1 brings the state of every part from
 // zeros and the factor of what comes before it, PART 2 takes in the parts before its own and brings the outputs.
 template <int LANES, int NL, int WAVES, int WT, bool VEC, int PART>
 __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan_tile_kernel(const ScanParams p) {
     using T = ScanTile<LANES, NL, WAVES, WT>;
+    constexpr int U = T::U;
     typedef float vec __attribute__((ext_vector_type(NL)));
+    typedef float unit __attribute__((ext_vector_type(U)));
     constexpr int SETS = 64 * (WAVES / WT);  // lanes that walk the same tokens
-    __shared__ __attribute__((aligned(16))) float steps[T::CHANNELS * T::STRIDE], inputs[T::CHANNELS * T::STRIDE];  // d and d x, whose place the outputs take
-    __shared__ __attribute__((aligned(16))) vec vb[T::VECTORS], vc[PART == 1 ? 1 : T::VECTORS];
-    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? T::THREADS : 1], factor[WT > 1 ? T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
+    __shared__ __attribute__((aligned(16))) float all_steps[WAVES][T::CH * T::STRIDE], all_inputs[WAVES][T::CH * T::STRIDE];  // d and d x, whose place the outputs take
+    __shared__ __attribute__((aligned(16))) vec all_b[WAVES][T::VECTORS], all_c[WAVES][PART == 1 ? 1 : T::VECTORS];
+    // (two of each: a wavefront may be a tile ahead of the slowest one)
+    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? 2 * T::THREADS : 1], factor[WT > 1 ? 2 * T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
 
     // (workgroups side by side in channels share lines of memory, and B and C)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
@@ -161,9 +170,9 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
         const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
         if (tile0 == tile1) continue;
 
-        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
-        const int c0 = group * p.per + (int)(block % p.group_blocks) * T::CHANNELS, cend = (group + 1) * p.per;
-        const int ch = wc * (64 / LANES) + lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
+        const int c0 = group * p.per + (int)(block % p.group_blocks) * T::CHANNELS + wc * T::CH, cend = (group + 1) * p.per;  // the wavefront's first channel
+        const int ch = lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
         const bool mine = c < cend;
 
         float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a part)
@@ -204,42 +213,46 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             }
         }
 
-        // What a thread brings of a tile, one tile ahead.  Its places are pointers that go on by a tile's rows.
-        floatx4 x[T::PER], d[T::PER], g[T::PER];
+        // What a lane brings of a tile, one tile ahead.  Its places are pointers that go on by a tile's rows.
+        unit x[T::PER], d[T::PER], g[T::PER];
         vec b[T::VPER], cc[T::VPER];
-        const floatx4 zeros = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int tq = tid / T::CQ, at = tid % T::CQ * 4, tv = tid / LANES, av = tid % LANES * NL;  // token and first channel, or state
-        const int dir = p.batch.reverse ? -1 : 1;
-        const long long row = q.row(tile0 * T::TOKENS + tq), vrow = q.row(tile0 * T::TOKENS + tv);
+        const int tq = lane / T::CQ, at = lane % T::CQ * U, tv = lane / LANES, av = lane % LANES * NL;  // token and first channel, or state
+        const int dir = p.batch.reverse ? -1 : 1, t0 = wt * T::TT;
+        const long long row = q.row(tile0 * T::TOKENS + t0 + tq), vrow = q.row(tile0 * T::TOKENS + t0 + tv);
         const float *px = p.X + row * p.ldx + c0 + at, *pd = p.dt + row * p.lddt + c0 + at, *pg = p.gate + row * p.ldg + c0 + at;
         const float *pb = p.B + vrow * p.ldb + (long long)group * p.n + av, *pc = p.C + vrow * p.ldc + (long long)group * p.n + av;
         float *py = p.Y + row * p.ldy + c0 + at;
         const long long mx = dir * p.ldx, md = dir * p.lddt, mg = dir * p.ldg, my = dir * p.ldy, mb = dir * p.ldb, mc = dir * p.ldc;
-        constexpr int APART = T::THREADS / T::CQ, VAPART = T::THREADS / LANES;  // tokens between a thread's pieces
+        constexpr int APART = 64 / T::CQ, VAPART = 64 / LANES;  // tokens between a lane's pieces
         const bool has = c0 + at < cend, hasv = av < p.n;
-        auto get4 = [&](const float *from) {
-            if (VEC) return *reinterpret_cast<const floatx4 *>(from);
-            floatx4 v;
+        auto get_unit = [&](const float *from) {
+            if (VEC) return *reinterpret_cast<const unit *>(from);
+            unit v;
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[i] = c0 + at + i < cend ? from[i] : 0.0f;
+            for (int i = 0; i < U; i++) v[i] = c0 + at + i < cend ? from[i] : 0.0f;
             return v;
         };
-        const floatx4 bias = p.dt_bias && has ? get4(p.dt_bias + c0 + at) : zeros, skip = p.skip && has ? get4(p.skip + c0 + at) : zeros;
+        unit zeros, bias, skip;
+#pragma unroll
+        for (int i = 0; i < U; i++) zeros[i] = 0.0f;
+        bias = p.dt_bias && has ? get_unit(p.dt_bias + c0 + at) : zeros;
+        skip = p.skip && has ? get_unit(p.skip + c0 + at) : zeros;
         auto fetch = [&](int tile) {
+            const int left = q.fresh - tile * T::TOKENS - t0;  // tokens from the wavefront's first one on
 #pragma unroll
             for (int k = 0; k < T::PER; k++) {
                 x[k] = d[k] = g[k] = zeros;
-                if (has && tid + k * T::THREADS < T::QUADS && tile * T::TOKENS + tq + k * APART < q.fresh) {
-                    x[k] = get4(px + k * APART * mx);
-                    d[k] = get4(pd + k * APART * md);
-                    if (PART != 1 && p.gate) g[k] = get4(pg + k * APART * mg);
+                if (has && tq + k * APART < left) {
+                    x[k] = get_unit(px + k * APART * mx);
+                    d[k] = get_unit(pd + k * APART * md);
+                    if (PART != 1 && p.gate) g[k] = get_unit(pg + k * APART * mg);
                 }
             }
 #pragma unroll
             for (int k = 0; k < T::VPER; k++) {
 #pragma unroll
                 for (int i = 0; i < NL; i++) b[k][i] = cc[k][i] = 0.0f;
-                if (hasv && tid + k * T::THREADS < T::VECTORS && tile * T::TOKENS + tv + k * VAPART < q.fresh) {
+                if (hasv && (T::VECTORS >= 64 || lane < T::VECTORS) && tv + k * VAPART < left) {
                     const float *fb = pb + k * VAPART * mb, *fc = pc + k * VAPART * mc;
                     if (p.vectors) {
                         b[k] = *reinterpret_cast<const vec *>(fb);
@@ -260,48 +273,50 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             pb += T::TOKENS * mb;
             pc += T::TOKENS * mc;
         };
+        float *steps = all_steps[wave], *inputs = all_inputs[wave];
+        vec *vb = all_b[wave], *vc = all_c[wave];
         // steps and inputs are 0 behind the sequence's last token and the last channel: the state stays
         auto stage = [&](int tile) {
+            const int left = q.fresh - tile * T::TOKENS - t0;
 #pragma unroll
             for (int k = 0; k < T::PER; k++) {
-                if (tid + k * T::THREADS < T::QUADS) {
-                    const bool in = tile * T::TOKENS + tq + k * APART < q.fresh;
-                    floatx4 step = d[k] + bias;
-                    if (p.softplus) {  // (four side by side: each is a chain of dependent instructions)
+                const bool in = tq + k * APART < left;
+                unit step = d[k] + bias;
+                if (p.softplus) {  // (side by side: each is a chain of dependent instructions)
 #pragma unroll
-                        for (int i = 0; i < 4; i++) step[i] = softplus(step[i]);
-                    }
+                    for (int i = 0; i < U; i++) step[i] = softplus(step[i]);
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        step[i] = in && c0 + at + i < cend ? step[i] : 0.0f;
-                        steps[(at + i) * T::STRIDE + tq + k * APART] = step[i];
-                        inputs[(at + i) * T::STRIDE + tq + k * APART] = step[i] * x[k][i];
-                    }
+                for (int i = 0; i < U; i++) {
+                    step[i] = in && c0 + at + i < cend ? step[i] : 0.0f;
+                    steps[(at + i) * T::STRIDE + tq + k * APART] = step[i];
+                    inputs[(at + i) * T::STRIDE + tq + k * APART] = step[i] * x[k][i];
                 }
             }
 #pragma unroll
             for (int k = 0; k < T::VPER; k++)
-                if (tid + k * T::THREADS < T::VECTORS) {
-                    vb[tid + k * T::THREADS] = b[k];
-                    if (PART != 1) vc[tid + k * T::THREADS] = cc[k];
+                if (T::VECTORS >= 64 || lane < T::VECTORS) {
+                    vb[lane + k * 64] = b[k];
+                    if (PART != 1) vc[lane + k * 64] = cc[k];
                 }
         };
 
-        const float *my_steps = steps + ch * T::STRIDE + wt * T::TT;
-        float *my_inputs = inputs + ch * T::STRIDE + wt * T::TT;
-        const vec *my_b = vb + wt * T::TT * LANES + ln, *my_c = vc + (PART == 1 ? 0 : wt * T::TT * LANES + ln);
+        const float *my_steps = steps + ch * T::STRIDE;
+        float *my_inputs = inputs + ch * T::STRIDE;
+        const vec *my_b = vb + ln, *my_c = vc + (PART == 1 ? 0 : ln);
 
         fetch(tile0);
         for (int tile = tile0; tile < tile1; tile++) {
+            in_order();
             stage(tile);
-            floatx4 x0[T::PER], g0[T::PER];
+            unit x0[T::PER], g0[T::PER];
 #pragma unroll
             for (int k = 0; k < T::PER; k++) {
                 x0[k] = x[k];
                 g0[k] = g[k];
             }
             if (tile + 1 < tile1) fetch(tile + 1);
-            __syncthreads();
+            in_order();
             float kept[WT > 1 ? T::TT : 1][NL], put[WT > 1 && PART != 1 ? T::TT : 1][NL];  // factors and products of the tokens
             if constexpr (WT > 1) {
                 float local[NL], sum = 0.0f;
@@ -329,13 +344,14 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                     v[i] = local[i];
                     f[i] = __builtin_amdgcn_exp2f(sum * a[i]);
                 }
-                brought[wt * SETS + set] = v;
-                factor[wt * SETS + set] = f;
+                const int half = tile - tile0 & 1;
+                vec *all = brought + half * T::THREADS + set, *all_f = factor + half * T::THREADS + set;
+                all[wt * SETS] = v;
+                all_f[wt * SETS] = f;
                 __syncthreads();
-                const int before = __builtin_amdgcn_readfirstlane(PART == 1 ? (wt == 0 ? WT : 0) : wt);
-                const vec *all = brought + set, *all_f = factor + set;
+                const int before = PART == 1 ? (wt == 0 ? WT : 0) : wt;
                 if (PART != 1) {
-                    const vec v0 = begin[(tile - tile0 & 1) * SETS + set];
+                    const vec v0 = begin[half * SETS + set];
 #pragma unroll
                     for (int i = 0; i < NL; i++) h[i] = v0[i];
                 }
@@ -390,26 +406,27 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                     for (int i = 0; i < NL; i++) v[i] = h[i];
                     begin[(tile - tile0 + 1 & 1) * SETS + set] = v;
                 }
-                __syncthreads();
+                in_order();
+                const int left = q.fresh - tile * T::TOKENS - t0;
 #pragma unroll
                 for (int k = 0; k < T::PER; k++) {
-                    if (has && tid + k * T::THREADS < T::QUADS && tile * T::TOKENS + tq + k * APART < q.fresh) {
-                        floatx4 y;
+                    if (has && tq + k * APART < left) {
+                        unit y;
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
+                        for (int i = 0; i < U; i++) {
                             y[i] = inputs[(at + i) * T::STRIDE + tq + k * APART];
                             y[i] = __builtin_fmaf(skip[i], x0[k][i], y[i]);
                         }
                         if (p.gate) {
 #pragma unroll
-                            for (int i = 0; i < 4; i++) y[i] *= silu(g0[k][i]);
+                            for (int i = 0; i < U; i++) y[i] *= silu(g0[k][i]);
                         }
                         float *to = py + k * APART * my;
                         if (VEC) {
-                            *reinterpret_cast<floatx4 *>(to) = y;
+                            *reinterpret_cast<unit *>(to) = y;
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
+                            for (int i = 0; i < U; i++)
                                 if (c0 + at + i < cend) to[i] = y[i];
                         }
                     }
@@ -430,7 +447,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
         } else if (mine && wt == WT - 1 && tile1 == tiles) {
             keep_state<NL, false>(p, q, c, n0, h);
         }
-        __syncthreads();  // (the next job's tiles)
+        __syncthreads();  // (the next job's states)
     }
 }
 
