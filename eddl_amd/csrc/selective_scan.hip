@@ -29,7 +29,7 @@ struct ScanParams {
 // Sums over LANES lanes side by side, in all of them.
 template <int CTRL>
 __device__ __forceinline__ float swapped(float x) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
 template <int LANES>
 __device__ __forceinline__ float lane_sum(float x) {
@@ -397,6 +397,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                             sum = i ? __builtin_fmaf(cv[i], h[i], sum) : cv[i] * h[i];
                         }
                         y[j] = lane_sum<LANES>(sum);
+                        asm volatile("" : "+v"(y[j]));  // (or the last addition goes into the branch below, apart from its swap)
                     }
                     if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
                 }

@@ -6,8 +6,8 @@ and each layer's unfused forward is the one call its reference counterpart makes
 (LConv::forward -> Conv2D, LBatchNorm::forward -> BatchNormForward in inference mode,
 LActivation -> ReLu/Sigmoid/FullSoftmax, LMaxPool -> MPool2D, LAveragePool -> AvgPool2D,
 LResize -> scale, LConcat -> concat, LAdd -> fill_+inc, LSum -> add, LPad -> pad,
-LDense -> mult2D + sum2D_rowwise, LReshape -> shared storage).  Norms over the last axis and attention over a
-paged cache are layers of this package's own.
+LDense -> mult2D + sum2D_rowwise, LReshape -> shared storage).  Norms over the last axis, attention over a
+paged cache, group norms and the state space layers are layers of this package's own.
 
 ``Net.build(backend, fuse=True)`` additionally runs a fusion pass in the spirit of the
 reference's FPGA model transformation (src/apis/fpga.cpp:173-331,656+): chains
@@ -245,6 +245,59 @@ def PagedAttention(parent, heads, cache, batch, rotary=None, positions=None, cau
                  positions=positions, causal=bool(causal), window=int(window), scale=scale)
 
 
+# ---------------------------------------------------------------------------- group norm and state space blocks
+def GroupNormalization(parent, groups, epsilon=1e-3, affine=True, activation=None, name=""):
+    """The norm of ``groups`` groups of channels over all pixels of an image, its weight and bias a channel, and an activation (None, "relu" or "silu").
+    ``parent``: maps [batch, channels, height, width], or tokens [batch, tokens, channels], channels last.  A fused plan takes a following ReLU along."""
+    shape, axis = parent.out_shape, 1 if len(parent.out_shape) == 4 else 2
+    if len(shape) not in (3, 4) or int(groups) < 1 or shape[axis] % int(groups):
+        msg("GroupNormalization needs [batch, channels, height, width] or [batch, tokens, channels] of channels in %s groups, not %s" % (groups, shape), "GroupNormalization")
+    if activation not in (None, "relu", "silu"):
+        msg("GroupNormalization knows no activation %s" % activation, "GroupNormalization")
+    l = Layer("group_norm", [parent], shape, name, groups=int(groups), epsilon=float(epsilon), affine=affine, activation=activation)
+    if affine:
+        l.params["w"], l.params["b"] = np.ones(shape[axis], np.float32), np.zeros(shape[axis], np.float32)
+    return l
+
+
+def CausalConvolution(parent, width, channels=None, use_bias=True, activation="silu", reverse=False, batch=None, states=None, name=""):
+    """The short convolution of every channel along the tokens.  ``parent``: [batch, tokens, columns], whose first ``channels`` columns (all, unless given) are
+    the inputs.  ``batch``: a StateBatch over the batch * tokens rows, with ``states`` [slots, width - 1, channels] or without; None: every entry of the
+    batch is a sequence that begins."""
+    shape = parent.out_shape
+    n = shape[-1] if channels is None else int(channels)
+    if len(shape) != 3 or not 1 <= n <= shape[2] or not 2 <= int(width) <= 8:
+        msg("CausalConvolution needs [batch, tokens, columns] with %s channels and a width of 2 to 8, not %s and %s" % (channels, shape, width), "CausalConvolution")
+    if states is not None and batch is None:
+        msg("states come with a batch", "CausalConvolution")
+    l = Layer("causal_conv", [parent], shape[:2] + [n], name, activation=activation, reverse=bool(reverse), batch=batch, states=states)
+    l.params["W"] = np.zeros((n, int(width)), np.float32)
+    if use_bias:
+        l.params["bias"] = np.zeros(n, np.float32)
+    return l
+
+
+def SelectiveScan(parent, dt, vectors, state, groups=1, gate=None, softplus=True, reverse=False, batch=None, states=None, name=""):
+    """The selective scan of ``parent`` [batch, tokens, channels] with time steps ``dt`` [batch, tokens, channels], a state of ``state`` numbers a channel, and
+    the last 2 * groups * state columns of ``vectors`` [batch, tokens, columns] as B and C; gated by the last columns of ``gate`` [batch, tokens, columns] where
+    there is one.  ``batch`` and ``states`` [slots, channels, state] as in ``CausalConvolution``.  Parameters: A [channels, state], the skip and the time
+    steps' bias."""
+    shape, n, need = parent.out_shape, int(state), 2 * int(groups) * int(state)
+    others = [vectors] + ([gate] if gate is not None else [])
+    if len(shape) != 3 or dt.out_shape != shape or not 1 <= n <= 64 or int(groups) < 1 or shape[2] % int(groups) or any(o.out_shape[:2] != shape[:2] or len(o.out_shape) != 3 for o in others) \
+            or vectors.out_shape[2] < need or (gate is not None and gate.out_shape[2] < shape[2]):
+        msg("SelectiveScan needs [batch, tokens, channels], time steps of the same shape, %d columns of vectors and as many of a gate as channels, not %s"
+            % (need, [l.out_shape for l in (parent, dt, *others)]), "SelectiveScan")
+    if states is not None and batch is None:
+        msg("states come with a batch", "SelectiveScan")
+    l = Layer("selective_scan", [parent, dt, vectors] + ([gate] if gate is not None else []), shape, name, state=n, groups=int(groups), softplus=bool(softplus), reverse=bool(reverse),
+              batch=batch, states=states)
+    l.params["A"] = np.repeat(-np.arange(1, n + 1, dtype=np.float32)[None], shape[2], 0)
+    l.params["skip"] = np.ones(shape[2], np.float32)
+    l.params["dt_bias"] = np.zeros(shape[2], np.float32)
+    return l
+
+
 # ---------------------------------------------------------------------------- the net
 class Op:
     """One launch group of the built plan.  ``flops``/``bytes`` are the algorithmic figures
@@ -414,6 +467,9 @@ class Net:
                 continue
             if l.kind == "norm" or (fuse and l.kind == "sum" and any(c.kind == "norm" for c in l.children)):
                 self._emit_norm(l, fuse, absorbed, sole_child)
+                continue
+            if l.kind == "group_norm":
+                self._emit_group_norm(l, fuse, absorbed, sole_child)
                 continue
             self._emit_plain(l)
         for o in self.lout:
@@ -621,6 +677,33 @@ class Net:
         count = 1 + (R is not None) + (S is not None) + (H is not None)
         self.ops.append(Op("norm", "+".join(m.name for m in members), lambda: hip.norm_residual(X, R, S, H, post=a, pre=b), 0, 4 * count * rows * cols, members))
 
+    def _emit_group_norm(self, l, fuse, absorbed, sole_child):
+        """One launch (two where a group is large); a fused plan takes a following ReLU along."""
+        hip, at = self.backend, l.attrs
+        last, activation = l, at["activation"]
+        c = sole_child(l)
+        if fuse and activation is None and c is not None and c.kind == "relu":
+            last, activation = c, "relu"
+            absorbed.add(id(c))
+        X, O, dp = self.out[id(l.parents[0])], hip.empty(last.out_shape), self.dparams[id(l)]
+        self.out[id(last)] = O
+        tokens = None
+        if len(l.out_shape) == 3:  # tokens, channels last
+            rows, tokens = (l.out_shape[0] * l.out_shape[1], l.out_shape[2]), l.out_shape[1]
+            X, O = X.reshape(rows), O.reshape(rows)
+        members = [l] if last is l else [l, last]
+        self.ops.append(Op("group_norm", "+".join(m.name for m in members),
+                           lambda: hip.group_norm(X, O, at["groups"], dp.get("w"), dp.get("b"), at["epsilon"], activation, image_rows=tokens),
+                           0, 8 * int(np.prod(l.out_shape)), members))
+
+    def _sequences(self, l):
+        """The batch of a layer along tokens: its own, or every entry of the batch a sequence that begins."""
+        if l.attrs["batch"] is not None:
+            return l.attrs["batch"]
+        from .state_space import StateBatch
+        n, tokens = l.out_shape[:2]
+        return StateBatch(self.backend.array(np.arange(n + 1) * tokens, "int32"), tokens)
+
     def _emit_plain(self, l):
         hip = self.backend
         k = l.kind
@@ -678,6 +761,18 @@ class Net:
                 hip.paged_append(qkv.columns(0, q), qkv.columns(q, q + kv), qkv.columns(q + kv, q + 2 * kv), turned, cache, batch, at["rotary"], at["positions"])
                 hip.paged_attention(turned, O2, cache, batch, at["scale"], at["causal"], at["window"])
             nbytes = 4 * (n_out + rows * (q + 2 * kv))  # (what the cache holds grows)
+        elif k in ("causal_conv", "selective_scan"):
+            at, dp, batch, channels = l.attrs, self.dparams[id(l)], self._sequences(l), l.out_shape[2]
+            two = [t.reshape((l.out_shape[0] * l.out_shape[1], t.shape[2])) for t in ins + [O]]
+            if k == "causal_conv":
+                run = lambda: hip.causal_conv(two[0].columns(0, channels), dp["W"], dp.get("bias"), two[1], batch, at["states"], at["activation"], at["reverse"])
+                nbytes = 8 * n_out
+            else:
+                half, wide = at["groups"] * at["state"], two[2].shape[1]
+                gate = two[3].columns(two[3].shape[1] - channels, two[3].shape[1]) if len(ins) == 4 else None
+                run = lambda: hip.selective_scan(two[0], two[1], dp["A"], two[2].columns(wide - 2 * half, wide - half), two[2].columns(wide - half, wide), two[-1], batch,
+                                                 at["states"], dp["skip"], gate, dp["dt_bias"], at["softplus"], at["reverse"])
+                nbytes = 4 * (len(ins) * n_out + two[0].shape[0] * 2 * half)
         elif k == "pad":
             hip.fill_(O, l.attrs["constant"])  # the border is written once, here; forward copies the interior
             n_in = int(np.prod(l.parents[0].out_shape))

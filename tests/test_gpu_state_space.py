@@ -381,3 +381,212 @@ def test_empty_calls(hip):
     hip.causal_conv(X, hip.full((8, 4), 1.0), None, Y, none)
     hip.selective_scan(X, X, hip.full((8, 4), 1.0), V, V, Y, none)
     assert np.all(Y.numpy() == -7.0)
+
+
+# ------------------------------------------------------------------------------------------------- graphs, networks, large tensors
+def test_recorded_steps_follow_the_batch(hip):
+    """A recorded convolution and scan, replayed while offsets, lengths and slots change: every replay equals the eager calls on the same states, with the program's own
+    work between the replays."""
+    rng = np.random.default_rng(20)
+    channels, n, width, seqs = 40, 16, 4, 3
+    for most in (1, 40, 700):
+        batch = Ragged(rng, [most] * seqs, before=0, behind=0, apart=False)
+        case = _scan_case(rng, batch, channels, n, 1)
+        d = lambda t: hip.array(t)
+        X, W, U, Y, dt, A, B, C, D, G, bias = d(case["x"]), d(rng.standard_normal((channels, width))), hip.empty(case["x"].shape), hip.empty(case["x"].shape), d(case["dt"]), d(case["A"]), \
+            d(case["B"]), d(case["C"]), d(case["skip"]), d(case["gate"]), d(case["dt_bias"])
+        inputs, states = rng.standard_normal((batch.pool, width - 1, channels), dtype=np.float32), rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+        P, S, b = d(inputs), d(states), batch.on(hip, most)
+
+        def step():
+            hip.causal_conv(X, W, None, U, b, states=P, activation="silu")
+            hip.selective_scan(U, dt, A, B, C, Y, b, states=S, skip=D, gate=G, dt_bias=bias)
+            hip.group_norm(Y, Y, 8, image_rows=batch.rows)
+
+        step()
+        graph = hip.record(step)
+        for turn in range(3):
+            news = np.minimum(np.array([[most, most, most], [most, 0, most // 2], [1, most, 0]][turn]), most)
+            b.offsets.copy_from(np.concatenate([[0], np.cumsum(news)]))
+            b.lengths.copy_from(news + [5, 0, 7])
+            b.slots.copy_from(rng.permutation(batch.pool)[:seqs])
+            got = []
+            for run in (step, graph.launch):
+                P.copy_from(inputs)
+                S.copy_from(states)
+                hip.fill_(Y, 0.5)
+                X.copy_from(case["x"] * (turn + 1))
+                run()
+                got.append((Y.numpy(), P.numpy(), S.numpy()))
+            for e, g in zip(*got):
+                assert np.array_equal(e, g), (most, turn)
+
+
+def test_calls_on_changing_streams(hip):
+    """Divided groups and divided sequences share the library's workspace: calls on two streams in turn give the bits of calls on one."""
+    import ctypes
+    rng = np.random.default_rng(21)
+    streams = [ctypes.c_void_p() for _ in range(2)]
+    for s in streams:
+        assert hip.lib.hipStreamCreateWithFlags(ctypes.byref(s), 1) == 0
+    batch = Ragged(rng, [3000], kept=False)
+    case = _scan_case(rng, batch, 24, 16, 1)
+    X = hip.array(rng.standard_normal((1, 2, 400, 300)))
+    try:
+        Y, want = hip.empty(X.shape), None
+        for turn in range(6):
+            hip._check(hip.lib.eddlhip_set_stream(hip.dev, streams[turn % 2]))
+            hip.group_norm(X, Y, 2)
+            got = (_scan(hip, case, batch, np.zeros((batch.pool, 24, 16), np.float32), False)[0], Y.numpy())
+            want = want or got
+            assert all(np.array_equal(a, b) for a, b in zip(want, got)), turn
+    finally:
+        hip._check(hip.lib.eddlhip_set_stream(hip.dev, None))
+        for s in streams:
+            hip.lib.hipStreamDestroy(s)
+
+
+def test_net_of_state_space_blocks(hip):
+    """A network that scans the tokens of images both ways between group norms: norm, dense, convolution, dense, scan forwards; the same backwards; Add, dense, Add, norm with
+    SiLU.  The fused plan, the layer walk and a captured plan give the same bits, and the network in 64 bits within 2e-5 of its largest output (some tens of EPS a stage)."""
+    from eddl_amd import net as L
+    rng = np.random.default_rng(22)
+    images, tokens, cols, inner, n, rank = 3, 49, 32, 48, 8, 4
+
+    def build(fuse):
+        x = L.Input([tokens, cols], images)
+        xz = L.Dense(L.GroupNormalization(x, 8), 2 * inner, use_bias=False)
+        sides = []
+        for reverse in (False, True):
+            u = L.CausalConvolution(xz, 4, channels=inner, reverse=reverse)
+            proj = L.Dense(u, rank + 2 * n, use_bias=False)
+            sides.append(L.SelectiveScan(u, L.Dense(u, inner, use_bias=False), proj, n, gate=xz, reverse=reverse))
+        s = L.Add(x, L.Dense(L.Add(*sides), cols))
+        net = L.Net([x], [L.GroupNormalization(s, 4, activation="silu"), L.ReLu(L.GroupNormalization(s, 1, affine=False))])
+        r = np.random.default_rng(23)
+        for l in net.layers:
+            for k, v in l.params.items():
+                if k != "A":
+                    scale = 1 / np.sqrt(v.shape[0]) if l.kind == "dense" and k == "W" else 0.5 if k == "W" else 0.1
+                    l.params[k] = ((1.0 if k in ("w", "skip") else -2.0 if k == "dt_bias" else 0.0) + scale * r.standard_normal(v.shape)).astype(np.float32)
+        return net.build(hip, fuse=fuse)
+
+    fused, walk = build(True), build(False)
+    assert sum(op.kind == "relu" for op in walk.ops) == 1 and not any(op.kind == "relu" for op in fused.ops)
+    x = rng.standard_normal((images, tokens, cols), dtype=np.float32)
+    got = fused.predict(x)
+    graph = fused.capture()
+    for a, b in zip(walk.predict(x), got):
+        assert np.array_equal(a, b)
+    for turn in range(2):
+        fused.input_tensor().copy_from(x)
+        fused.run_graph()
+        for o, b in zip(fused.lout, got):
+            assert np.array_equal(fused.output_of(o).numpy(), b)
+    # in 64 bits
+    by = lambda kind: [{k: v.astype(np.float64) for k, v in l.params.items()} for l in fused.layers if l.kind == kind]
+    norms, denses, convs, scans = by("group_norm"), [l for l in fused.layers if l.kind == "dense"], [l for l in fused.layers if l.kind == "causal_conv"], \
+        [l for l in fused.layers if l.kind == "selective_scan"]
+    W = lambda l: {k: v.astype(np.float64) for k, v in l.params.items()}
+
+    def norm(t, groups, p, eps):
+        v = t.reshape(images, tokens, groups, -1)
+        v = (v - v.mean((1, 3), keepdims=True)) / np.sqrt(v.var((1, 3), keepdims=True) + eps)
+        v = v.reshape(t.shape)
+        return v * p["w"] + p["b"] if p else v
+    layer = {id(l): l for l in fused.layers}
+    assert len(layer) == len(fused.layers)
+    first = [l for l in fused.layers if l.kind == "group_norm" and l.parents[0].kind == "input"][0]
+    z = norm(x.astype(np.float64), 8, W(first), 1e-3) @ W([l for l in denses if l.parents[0] is first][0])["W"]
+    total = 0
+    for conv in convs:
+        scan = [l for l in scans if l.parents[0] is conv][0]
+        c, p, flip = W(conv), W(scan), slice(None, None, -1 if conv.attrs["reverse"] else 1)
+        u = np.concatenate([np.zeros((images, 3, inner)), z[:, flip, :inner]], 1)
+        u = sum(u[:, k:k + tokens] * c["W"][:, k] for k in range(4)) + c["bias"]
+        u = u / (1 + np.exp(-u))
+        dt = np.logaddexp(u @ W(scan.parents[1])["W"] + p["dt_bias"], 0)
+        v = u @ W(scan.parents[2])["W"]
+        h, out = np.zeros((images, inner, n)), []
+        for t in range(tokens):
+            h = np.exp(dt[:, t, :, None] * p["A"]) * h + (dt[:, t] * u[:, t])[:, :, None] * v[:, t, None, rank:rank + n]
+            out.append((h * v[:, t, None, rank + n:]).sum(2) + p["skip"] * u[:, t])
+        total = total + np.stack(out, 1)[:, flip] * (z[:, :, inner:] / (1 + np.exp(-z[:, :, inner:])))
+    last = [l for l in denses if l.parents[0].kind == "sum"][0]
+    s = x + total @ W(last)["W"] + W(last)["bias"]
+    a = norm(s, 4, W([l for l in fused.layers if l.kind == "group_norm" and l.attrs["activation"]][0]), 1e-3)
+    for g, w in zip(got, (a / (1 + np.exp(-a)), np.maximum(norm(s, 1, None, 1e-3), 0))):
+        assert np.abs(g - w).max() <= 2e-5 * np.abs(w).max(), np.abs(g - w).max() / np.abs(w).max()
+
+
+def test_net_of_group_norms_on_maps(hip):
+    """Convolution, group norm, ReLU: one launch for the last two in a fused plan, the same bits as the layer walk, another batch size behind it."""
+    from eddl_amd import net as L
+    rng = np.random.default_rng(24)
+    nets = []
+    for fuse in (True, False):
+        x = L.Input([6, 13, 11], 2)
+        net = L.Net([x], [L.ReLu(L.GroupNormalization(L.Conv2D(x, 12, [3, 3]), 4))])
+        r = np.random.default_rng(25)
+        for l in net.layers:
+            for k, v in l.params.items():
+                l.params[k] = (0.3 * r.standard_normal(v.shape)).astype(np.float32)
+        nets.append(net.build(hip, fuse=fuse))
+    assert [op.kind for op in nets[0].ops] == ["conv2d", "group_norm"] and [op.kind for op in nets[1].ops][-1] == "relu"
+    for batch in (2, 5):
+        x = rng.standard_normal((batch, 6, 13, 11), dtype=np.float32)
+        a, b = (net.predict(x)[0] for net in nets)
+        conv = nets[1].output_of([l for l in nets[1].layers if l.kind == "conv2d"][0]).numpy()
+        p = [l for l in nets[0].layers if l.kind == "group_norm"][0].params
+        want, err = group_norm(conv.reshape(batch, 12, -1), 4, p["w"], p["b"], 1e-3, None, None, "relu")
+        assert np.array_equal(a, b)
+        _check(a.reshape(want.shape), want, err)
+
+
+def test_places_beyond_32_bits(hip):
+    """Columns of a tensor of 2.4e9 numbers: the last rows lie beyond what 32 bits count, in numbers and in bytes."""
+    from eddl_amd.state_space import StateBatch
+    rng = np.random.default_rng(26)
+    rows, ld, channels, n = 600000, 4096, 8, 16
+    wide = hip.empty((rows, ld))
+    hip.fill_(wide, 1.0)
+    tail = 300
+    x = rng.standard_normal((tail, channels), dtype=np.float32)
+    flat = wide.reshape((rows * ld,))
+    for t in range(tail):  # the last rows, in the last columns
+        at = ((rows - tail + t) * ld + ld - channels) * 4
+        row = np.ascontiguousarray(x[t])
+        hip._check(hip.lib.eddlhip_memcpy_h2d(hip.dev, wide.ptr + at, row.ctypes.data, row.nbytes))
+    assert flat.size == rows * ld
+    X = wide.columns(ld - channels, ld)
+    offsets = np.array([rows - tail, rows - tail + 100, rows], np.int32)
+    batch = StateBatch(hip.array(offsets, "int32"), 200)
+    w = rng.standard_normal((channels, 4), dtype=np.float32)
+    Y = hip.full((rows, channels), -7.0)
+    hip.causal_conv(X, hip.array(w), None, Y, batch)
+    want, err, _ = causal_conv(x, w, None, [0, 100, tail], None, False)
+    y = Y.numpy()
+    _check(y[-tail:], want, err)
+    assert np.all(y[:-tail] == -7.0)
+    A, vectors = -np.ones((channels, n), np.float32), np.ones((tail, n), np.float32)
+    hip.fill_(Y, -7.0)
+    V = wide.columns(0, n)  # (ones)
+    hip.selective_scan(X, X, hip.array(A), V, V, Y, batch)
+    want, err = selective_scan(x, x, A, vectors, vectors, [0, 100, tail])[:2]
+    y = Y.numpy()
+    _check(y[-tail:], want, err)
+    assert np.all(y[:-tail] == -7.0)
+    hip.group_norm(X, Y, 2, image_rows=tail)
+    want, err = group_norm(np.ascontiguousarray(x.T)[None], 2, None, None, 1e-5, None, None, None)
+    _check(Y.numpy()[-tail:].T[None], want, err)
+    whole = hip.empty(wide.shape)  # and maps: a group of 1.2e9 numbers
+    hip.group_norm(wide.reshape((1, 2, rows // 2, ld)), whole.reshape((1, 2, rows // 2, ld)), 2, eps=1.0)
+    got = np.empty(4096, np.float32)
+    hip._check(hip.lib.eddlhip_memcpy_d2h(hip.dev, got.ctypes.data, whole.ptr + 4 * (rows * ld - 4096), got.nbytes))
+    # (the second group: ones, but for the tail's numbers)
+    total, count = x.astype(np.float64), rows * ld // 2
+    mean = 1 + (total - 1).sum() / count
+    var = ((1 - mean) ** 2 * (count - x.size) + ((total - mean) ** 2).sum()) / count
+    row = np.concatenate([np.ones(ld - channels), x[-1]])
+    want = (row - mean) / np.sqrt(var + 1.0)
+    assert np.abs(got - want).max() <= 128 * EPS * np.abs(row).max()

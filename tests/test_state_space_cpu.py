@@ -154,3 +154,30 @@ def test_shapes_of_selective_scan(hip):
     for bad in (dict(dt=t(1, 20, 9)), dict(dt=t(1, 19, 8)), dict(A=t(2, 9, 5)), dict(A=t(2, 40)), dict(B=t(3, 20, 11)), dict(B=t(3, 20, 11), C=t(4, 20, 11)), dict(B=t(3, 19, 10), C=t(4, 19, 10)),
                 dict(gate=t(8, 20, 4)), dict(skip=t(7, 9)), dict(dt_bias=t(7, 9)), dict(states=t(6, 5, 5, 8)), dict(Y=t(5, 21, 8)), dict(A=_Tensor((8, 5), "int32")), dict(A=t(2, 8, 0))):
         _refused(lambda: hip.selective_scan(**dict(ok, **bad)))
+
+
+def test_layers_check_their_parents():
+    from eddl_amd import net as L
+    x, t = L.Input([8, 5, 7], 3), L.Input([9, 24], 3)
+    g = L.GroupNormalization(x, 4)
+    assert g.out_shape == [3, 8, 5, 7] and g.params["w"].shape == (8,) and not L.GroupNormalization(t, 8, affine=False).params
+    assert L.GroupNormalization(t, 8, activation="silu").params["b"].shape == (24,)
+    for parent, groups, activation in ((x, 3, None), (t, 5, None), (x, 0, None), (x, 4, "gelu"), (L.Input([24], 3), 4, None)):
+        with pytest.raises(RuntimeError):
+            L.GroupNormalization(parent, groups, activation=activation)
+    c = L.CausalConvolution(t, 4, channels=16)
+    assert c.out_shape == [3, 9, 16] and c.params["W"].shape == (16, 4) and "bias" not in L.CausalConvolution(t, 2, use_bias=False).params
+    for parent, width, channels in ((t, 1, None), (t, 9, None), (t, 4, 25), (t, 4, 0), (x, 4, None)):
+        with pytest.raises(RuntimeError):
+            L.CausalConvolution(parent, width, channels)
+    with pytest.raises(RuntimeError):
+        L.CausalConvolution(t, 4, states=_Tensor((3, 3, 24)))
+    d, v, z = (L.Dense(c, n) for n in (16, 2 * 2 * 5 + 3, 16))
+    y = L.SelectiveScan(c, d, v, 5, groups=2, gate=z)
+    assert y.out_shape == [3, 9, 16] and y.params["A"].shape == (16, 5) and list(y.params) == ["A", "skip", "dt_bias"] and len(y.parents) == 4
+    assert y.params["A"][3].tolist() == [-1, -2, -3, -4, -5]
+    for bad in (dict(state=6), dict(groups=3), dict(dt=v), dict(gate=L.Dense(c, 15)), dict(state=0), dict(vectors=L.Input([8, 40], 3)), dict(parent=t), dict(state=65)):
+        with pytest.raises(RuntimeError):
+            L.SelectiveScan(**dict(dict(parent=c, dt=d, vectors=v, state=5, groups=2, gate=z), **bad))
+    with pytest.raises(RuntimeError):
+        L.SelectiveScan(c, d, v, 5, states=_Tensor((3, 16, 5)))
