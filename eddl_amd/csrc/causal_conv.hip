@@ -49,6 +49,7 @@ __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
 // state, so that no other thread meets it.
 template <int WIDTH, int UNIT>
 __global__ __launch_bounds__(256) void causal_conv_kernel(const ConvParams p) {
+    static_assert(CONV_TOKENS >= WIDTH - 1, "inputs of the state reach the first chunk only");
     // (neighbours in time share width - 1 rows)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
         const long long job = xcd_job(id);

@@ -81,9 +81,13 @@ __device__ __forceinline__ void keep_state(const ScanParams &p, const Sequence &
 }
 template <int NL, bool VEC>
 __device__ __forceinline__ void exponents(const ScanParams &p, int c, int n0, float (&a)[NL]) {
+    constexpr float MOST = 3.40282347e38f;
     get<NL, VEC>(p.A + (long long)c * p.n, n0, p.n, a);
 #pragma unroll
-    for (int i = 0; i < NL; i++) a[i] *= LOG2_E;
+    for (int i = 0; i < NL; i++) {
+        a[i] *= LOG2_E;
+        a[i] = a[i] > MOST ? MOST : a[i] < -MOST ? -MOST : a[i];  // (an infinite one would make NaN of the steps of 0 behind the last token)
+    }
 }
 
 // Few tokens a sequence: LANES lanes a channel, NL states each; token after token from memory.  VEC: vectors, states and A are read 16 bytes at a time.
@@ -182,6 +186,31 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             through[i] = 1.0f;
         }
         if (mine) exponents<NL, false>(p, c, n0, a);
+        if constexpr (PART == 2) {  // the parts before this one: a stretch of them by every wavefront, joined by the first (the second half is free until the second tile)
+            vec f, b;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                f[i] = 1.0f;
+                b[i] = 0.0f;
+            }
+            const int each = (part + WT - 1) / WT, end = min(part, (wt + 1) * each);
+            const long long step = (long long)p.channels * T::NP;
+            const float *factors = p.part_factors + ((long long)s * (int)p.parts * p.channels + c) * T::NP + n0;
+            const float *states = p.part_states + ((long long)s * ((int)p.parts + 1) * p.channels + c) * T::NP + n0;
+            if (mine)
+#pragma unroll 4
+                for (int j = wt * each; j < end; j++) {
+                    const vec pf = *reinterpret_cast<const vec *>(factors + j * step), pb = *reinterpret_cast<const vec *>(states + (j + 1) * step);
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        b[i] = __builtin_fmaf(pf[i], b[i], pb[i]);
+                        f[i] *= pf[i];
+                    }
+                }
+            factor[T::THREADS + wt * SETS + set] = f;
+            brought[T::THREADS + wt * SETS + set] = b;
+            __syncthreads();
+        }
         if (mine && wt == 0) {
             float *states = PART ? p.part_states + ((long long)s * ((int)p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
             if (PART == 0) {
@@ -194,13 +223,12 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                     for (int i = 0; i < NL; i++) states[i] = kept[i];
                 }
             } else {
-                const float *factors = p.part_factors + ((long long)s * (int)p.parts * p.channels + c) * T::NP + n0;
-                const long long step = (long long)p.channels * T::NP;
                 const vec v = *reinterpret_cast<const vec *>(states);
 #pragma unroll
                 for (int i = 0; i < NL; i++) h[i] = v[i];
-                for (int j = 0; j < part; j++) {
-                    const vec f = *reinterpret_cast<const vec *>(factors + j * step), b = *reinterpret_cast<const vec *>(states + (j + 1) * step);
+#pragma unroll 1
+                for (int w = 0; w < WT; w++) {
+                    const vec f = factor[T::THREADS + w * SETS + set], b = brought[T::THREADS + w * SETS + set];
 #pragma unroll
                     for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[i], h[i], b[i]);
                 }

@@ -581,7 +581,8 @@ int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R
  *     n = (x - mean) / sqrt(variance + eps) w + b,   Y = act(n (1 + mod) + shift).
  * channels_last == 0: maps X, Y [images][channels][pixels], ldx and ldy are not looked at.  Otherwise rows of tokens [images * pixels][channels] that lie
  * ldx and ldy floats apart.  Up to 4096 channels a group.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
- * whose group holds an infinity or NaN is NaN in that group; images and groups do not reach one another. */
+ * whose group holds an infinity or NaN is NaN in that group; images and groups do not reach one another.  Workspace: means and squared differences of the
+ * parts of a group of more than 32768 numbers. */
 int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last,
                        int groups, const float *w, const float *b, float eps, const float *mod, const float *shift, int activation);
 
@@ -609,7 +610,8 @@ int eddlhip_causal_conv(int dev, const float *X, long long ldx, const float *W, 
  *     h[c][i] = e^(d A[c][i]) h[c][i] + d x B[i],   Y = (sum_i C[i] h[c][i] + skip[c] x) silu(gate).
  * X, dt, gate, Y [rows][channels]; B and C [rows][groups * n], a vector for each of `groups` equal parts of the channels; A [channels][n]; skip and dt_bias
  * [channels] may be NULL (0), gate too (no factor).  The state is [pool][channels][n].  Y and the states lie on nothing else that is read.
- * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  Sums and states are fp32. */
+ * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  Sums and states
+ * are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups take. */
 int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
                            const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,
                            int rows, int channels, int n, int groups, int softplus, int reverse, float *states, int pool,

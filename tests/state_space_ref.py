@@ -116,7 +116,7 @@ def selective_scan(x, dt, A, B, C, offsets, skip=None, gate=None, dt_bias=None, 
                 arg = d[t][:, None] * A64
                 a = np.exp(arg)
                 put = (d[t] * f(x[row]))[:, None] * b
-                rel = ed[t][:, None] * np.abs(A64) + 4 * EPS * np.abs(arg) + 2 * EPS
+                rel = np.where(a > 0, ed[t][:, None] * np.abs(A64) + 4 * EPS * np.abs(arg) + 2 * EPS, 0)  # (a factor of 0 is exact)
                 relative = (ed[t] / np.where(d[t] != 0, np.abs(d[t]), 1))[:, None] + 3 * EPS
                 eh = a * (1 + rel) * eh + np.abs(h) * a * rel + np.abs(put) * relative
                 h = a * h + put

@@ -224,7 +224,7 @@ def test_selective_scan(hip, n, channels, groups):
                 assert np.array_equal(s[untouched], pool[untouched])
 
 
-@pytest.mark.parametrize("channels, n, news", [(16, 16, [5000]), (5, 16, [3001, 40]), (64, 16, [2000]), (128, 4, [1500, 1000]), (40, 1, [4000]), (33, 64, [1025]), (600, 16, [700, 30, 2, 650]), (16, 16, [9000]), (24, 8, [2100, 1, 1030]),
+@pytest.mark.parametrize("channels, n, news", [(16, 16, [5000]), (5, 16, [3001, 40]), (64, 16, [2000]), (128, 4, [1500, 1000]), (40, 1, [4000]), (33, 64, [1025]), (600, 16, [700, 30, 2, 650]), (16, 16, [9000]), (24, 8, [2100, 1, 1030]), (3, 16, [33000]), (2, 1, [20000, 9]),
                                                (1500, 8, [400] * 3)])
 def test_selective_scan_of_long_sequences(hip, channels, n, news):
     rng = np.random.default_rng([channels, n])
@@ -282,6 +282,21 @@ def test_gate_over_its_range(hip):
     want = v / (1 + np.exp(-v))
     off = np.abs(Y.numpy()[0] - want) / np.maximum(np.abs(want), 2.0 ** -100)
     assert off.max() <= 11 * EPS, off.max() / EPS
+
+
+def test_an_infinite_factor_wipes_the_state(hip):
+    """A of minus infinity: what a token finds is gone behind it, and the last token's product is what is kept, however many tokens fill the tiles."""
+    rng = np.random.default_rng(12)
+    for news in ([1, 2, 3], [5, 17, 130]):
+        batch = Ragged(rng, news)
+        case = _scan_case(rng, batch, 20, 6, 1)
+        case["A"][:, 2], case["A"][3] = -np.inf, -3e38
+        pool = rng.standard_normal((batch.pool, 20, 6), dtype=np.float32)
+        want, err, after, after_err = selective_scan(**case, **batch.reference(pool))
+        y, s = _scan(hip, case, batch, pool, False)
+        assert np.all(np.isfinite(want[batch.offsets[0]:batch.offsets[-1]])) and np.all(np.isfinite(after))
+        _check(y, want, err)
+        _check(s, after, after_err)
 
 
 @pytest.mark.parametrize("channels, n", [(20, 16), (64, 4), (7, 1), (130, 64)])
