@@ -655,9 +655,9 @@ class Backend:
         channels = shape[1]
         if shape != yshape or len(W.shape) != 2 or W.shape[0] != channels or W.dtype != "float32" or bias is not None and (bias.size != channels or bias.dtype != "float32"):
             raise ValueError("causal_conv shapes %s -> %s, weights %s, bias %s" % (shape, yshape, W.shape, getattr(bias, "shape", None)))
-        pool = _pool(states, batch, (W.shape[1] - 1, channels), "causal_conv")
-        self._check(self.lib.eddlhip_causal_conv(self.dev, x, ldx, W.ptr, _ptr(bias), y, ldy, shape[0], channels, W.shape[1], _activation(activation), int(bool(reverse)),
-                                                 *pool, *batch.arguments))
+        pool, slots = _pool(states, batch, W.shape[1] - 1, channels, "causal_conv")
+        self._check(self.lib.eddlhip_causal_conv(self.dev, x, ldx, W.ptr, _ptr(bias), y, ldy, shape[0], channels, W.shape[1], _activation(activation), 1 if reverse else 0,
+                                                 pool, slots, *batch.arguments))
 
     def selective_scan(self, X, dt, A, B, C, Y, batch, states=None, skip=None, gate=None, dt_bias=None, softplus=True, reverse=False):
         """The selective scan along the tokens of a ragged batch: ``X``, ``dt``, ``Y`` and ``gate`` (or None) [rows, channels], ``A`` [channels, n], ``B`` and ``C``
@@ -670,12 +670,12 @@ class Backend:
         n = A.shape[1] if len(A.shape) == 2 and A.dtype == "float32" else 0
         if not shape == dshape == yshape == gshape or bshape != cshape or bshape[0] != rows or A.shape[0] != channels or not n or bshape[1] % n:
             raise ValueError("selective_scan shapes x %s, dt %s, gate %s -> %s, A %s, B %s, C %s" % (shape, dshape, gshape, yshape, A.shape, bshape, cshape))
-        for t in (skip, dt_bias):
-            if t is not None and (t.size != channels or t.dtype != "float32"):
-                raise ValueError("selective_scan: skip or dt_bias %s %s for %d channels" % (t.dtype, t.shape, channels))
-        pool = _pool(states, batch, (channels, n), "selective_scan")
-        self._check(self.lib.eddlhip_selective_scan(self.dev, x, ldx, d, lddt, A.ptr, b, ldb, c, ldc, _ptr(skip), g, ldg, _ptr(dt_bias), y, ldy, rows, channels, n,
-                                                    bshape[1] // n, int(bool(softplus)), int(bool(reverse)), *pool, *batch.arguments))
+        if skip is not None and (skip.size != channels or skip.dtype != "float32") or dt_bias is not None and (dt_bias.size != channels or dt_bias.dtype != "float32"):
+            raise ValueError("selective_scan: skip or dt_bias not float32 numbers of %d channels" % channels)
+        pool, slots = _pool(states, batch, channels, n, "selective_scan")
+        self._check(self.lib.eddlhip_selective_scan(self.dev, x, ldx, d, lddt, A.ptr, b, ldb, c, ldc, None if skip is None else skip.ptr, g, ldg,
+                                                    None if dt_bias is None else dt_bias.ptr, y, ldy, rows, channels, n, bshape[1] // n, 1 if softplus else 0,
+                                                    1 if reverse else 0, pool, slots, *batch.arguments))
 
 
 _NORMS = {None: 0, "layer": 1, "rms": 2}
@@ -688,10 +688,11 @@ def _activation(name):
     return _ACTIVATIONS[name]
 
 
-def _pool(states, batch, each, what):
-    """(pointer, slots) of a pool of states of shape ``each``."""
+def _pool(states, batch, rows, cols, what):
+    """(pointer, slots) of a pool of states [rows, cols]."""
     if states is None:
         return None, 0
-    if len(states.shape) != 3 or tuple(states.shape[1:]) != each or states.dtype != "float32" or batch.slots is None:
-        raise ValueError("%s: states are float32 [slots, %d, %d] with a batch that names lengths and slots, not %s %s" % (what, *each, states.dtype, states.shape))
-    return states.ptr, states.shape[0]
+    shape = states.shape
+    if len(shape) != 3 or shape[1] != rows or shape[2] != cols or states.dtype != "float32" or batch.slots is None:
+        raise ValueError("%s: states are float32 [slots, %d, %d] with a batch that names lengths and slots, not %s %s" % (what, rows, cols, states.dtype, shape))
+    return states.ptr, shape[0]
