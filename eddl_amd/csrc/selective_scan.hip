@@ -407,24 +407,45 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             if constexpr (PART != 1) {
 #pragma unroll
                 for (int t = 0; t < T::TT; t += 4) {
-                    floatx4 dv, xv, y;
+                    // The exponentials of four tokens first: one after another, each would be waited for (32 sequences of 512 tokens of 2048 channels
+                    // 175 -> 165 us).
+                    float f[4][NL], u[4][NL];
                     if constexpr (WT == 1) {
-                        dv = *reinterpret_cast<const floatx4 *>(my_steps + t);
-                        xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+                        const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const vec bv = my_b[(t + j) * LANES];
+#pragma unroll
+                            for (int i = 0; i < NL; i++) {
+                                f[j][i] = __builtin_amdgcn_exp2f(dv[j] * a[i]);
+                                u[j][i] = xv[j] * bv[i];
+                            }
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+#pragma unroll
+                            for (int i = 0; i < NL; i++) {
+                                f[j][i] = kept[t + j][i];
+                                u[j][i] = put[t + j][i];
+                            }
                     }
+                    floatx4 y;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        vec bv;
-                        if constexpr (WT == 1) bv = my_b[(t + j) * LANES];
                         const vec cv = my_c[(t + j) * LANES];
                         float sum = 0.0f;
 #pragma unroll
                         for (int i = 0; i < NL; i++) {
-                            if constexpr (WT == 1) h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dv[j] * a[i]), h[i], xv[j] * bv[i]);
-                            else h[i] = __builtin_fmaf(kept[t + j][i], h[i], put[t + j][i]);
+                            h[i] = __builtin_fmaf(f[j][i], h[i], u[j][i]);
                             sum = i ? __builtin_fmaf(cv[i], h[i], sum) : cv[i] * h[i];
                         }
-                        y[j] = lane_sum<LANES>(sum);
+                        y[j] = sum;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        y[j] = lane_sum<LANES>(y[j]);
                         asm volatile("" : "+v"(y[j]));  // (or the last addition goes into the branch below, apart from its swap)
                     }
                     if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
