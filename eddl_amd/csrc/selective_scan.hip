@@ -17,7 +17,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 struct ScanParams {
     const float *X, *dt, *gate, *B, *C, *A, *skip, *dt_bias;
     float *Y, *states;
-    float *part_states, *part_factors;  // [sequence][part + 1][channel][NP], [sequence][part][channel][NP]
+    float *part_states, *part_factors;  // [sequence][the state that it continues, parts, pieces of them][channel][NP], [sequence][parts, pieces][channel][NP]
     long long ldx, lddt, ldg, ldb, ldc, ldy;
     int channels, n, per;  // channels that share B and C
     unsigned blocks, group_blocks, parts;
@@ -149,19 +149,23 @@ __device__ __forceinline__ void in_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups: PART 1 brings the state of every part from
-// zeros and the factor of what comes before it, PART 2 takes in the parts before its own and brings the outputs.
+// PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups, and a workgroup's part over its wavefronts, which
+// walk their pieces on their own: PART 1 brings the state of every piece and part from zeros and the factor of what comes before it, PART 2 takes in what lies
+// before its own and brings the outputs.
 template <int LANES, int NL, int WAVES, int WT, bool VEC, int PART>
-__global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan_tile_kernel(const ScanParams p) {
+__global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && LANES == 16) ? 2 : 4) void scan_tile_kernel(const ScanParams p) {
     using T = ScanTile<LANES, NL, WAVES, WT>;
     constexpr int U = T::U;
     typedef float vec __attribute__((ext_vector_type(NL)));
     typedef float unit __attribute__((ext_vector_type(U)));
+    static_assert(PART == 0 || WT == 1, "pieces of a part are walked on their own");
     constexpr int SETS = 64 * (WAVES / WT);  // lanes that walk the same tokens
+    constexpr int PIECES = PART ? WAVES : 1;
     __shared__ __attribute__((aligned(16))) float all_steps[WAVES][T::CH * T::STRIDE], all_inputs[WAVES][T::CH * T::STRIDE];  // d and d x, whose place the outputs take
     __shared__ __attribute__((aligned(16))) vec all_b[WAVES][T::VECTORS], all_c[WAVES][PART == 1 ? 1 : T::VECTORS];
     // (two of each: a wavefront may be a tile ahead of the slowest one)
-    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 ? 2 * T::THREADS : 1], factor[WT > 1 ? 2 * T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
+    __shared__ __attribute__((aligned(16))) vec brought[WT > 1 || PART == 2 ? 2 * T::THREADS : PART ? T::THREADS : 1],
+        factor[WT > 1 || PART == 2 ? 2 * T::THREADS : PART ? T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
 
     // (workgroups side by side in channels share lines of memory, and B and C)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
@@ -170,77 +174,22 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
         const unsigned rest = (unsigned)job / p.blocks;  // (fewer than 2^31 jobs)
         const int block = (unsigned)job % p.blocks, group = block / p.group_blocks, part = rest % p.parts, s = rest / p.parts;
         const Sequence q = sequence(p.batch, s);
-        const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + (int)p.parts - 1) / (int)p.parts;  // (of a part)
-        const int tile0 = min(tiles, part * share), tile1 = min(tiles, tile0 + share);
-        if (tile0 == tile1) continue;
+        const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + (int)p.parts * PIECES - 1) / ((int)p.parts * PIECES);  // (of a piece)
+        if (part * PIECES * share >= tiles) continue;
 
-        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wc = wave / WT, set = wc * 64 + lane;
-        const int c0 = group * p.per + (int)(block % p.group_blocks) * T::CHANNELS + wc * T::CH, cend = (group + 1) * p.per;  // the wavefront's first channel
+        const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wc = PART ? 0 : wave / WT, set = wc * 64 + lane;
+        const int tile0 = PART ? min(tiles, (part * PIECES + wave) * share) : 0, tile1 = PART ? min(tiles, tile0 + share) : tiles;
+        const int c0 = group * p.per + (int)(block % p.group_blocks) * (PART ? T::CH : T::CHANNELS) + wc * T::CH, cend = (group + 1) * p.per;  // the wavefront's first channel
         const int ch = lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
         const bool mine = c < cend;
 
-        float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a part)
+        float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a piece)
 #pragma unroll
         for (int i = 0; i < NL; i++) {
             a[i] = h[i] = 0.0f;
             through[i] = 1.0f;
         }
         if (mine) exponents<NL, false>(p, c, n0, a);
-        if constexpr (PART == 2) {  // the parts before this one: a stretch of them by every wavefront, joined by the first (the second half is free until the second tile)
-            vec f, b;
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                f[i] = 1.0f;
-                b[i] = 0.0f;
-            }
-            const int each = (part + WT - 1) / WT, end = min(part, (wt + 1) * each);
-            const long long step = (long long)p.channels * T::NP;
-            const float *factors = p.part_factors + ((long long)s * (int)p.parts * p.channels + c) * T::NP + n0;
-            const float *states = p.part_states + ((long long)s * ((int)p.parts + 1) * p.channels + c) * T::NP + n0;
-            if (mine)
-#pragma unroll 4
-                for (int j = wt * each; j < end; j++) {
-                    const vec pf = *reinterpret_cast<const vec *>(factors + j * step), pb = *reinterpret_cast<const vec *>(states + (j + 1) * step);
-#pragma unroll
-                    for (int i = 0; i < NL; i++) {
-                        b[i] = __builtin_fmaf(pf[i], b[i], pb[i]);
-                        f[i] *= pf[i];
-                    }
-                }
-            factor[T::THREADS + wt * SETS + set] = f;
-            brought[T::THREADS + wt * SETS + set] = b;
-            __syncthreads();
-        }
-        if (mine && wt == 0) {
-            float *states = PART ? p.part_states + ((long long)s * ((int)p.parts + 1) * p.channels + c) * T::NP + n0 : nullptr;
-            if (PART == 0) {
-                first_state<NL, false>(p, q, c, n0, h);
-            } else if (PART == 1) {
-                if (part == 0) {  // kept for the second launch, in which the slot may be written already
-                    float kept[NL];
-                    first_state<NL, false>(p, q, c, n0, kept);
-#pragma unroll
-                    for (int i = 0; i < NL; i++) states[i] = kept[i];
-                }
-            } else {
-                const vec v = *reinterpret_cast<const vec *>(states);
-#pragma unroll
-                for (int i = 0; i < NL; i++) h[i] = v[i];
-#pragma unroll 1
-                for (int w = 0; w < WT; w++) {
-                    const vec f = factor[T::THREADS + w * SETS + set], b = brought[T::THREADS + w * SETS + set];
-#pragma unroll
-                    for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[i], h[i], b[i]);
-                }
-            }
-            if (WT > 1 && PART != 1) {
-                vec v;
-#pragma unroll
-                for (int i = 0; i < NL; i++) v[i] = h[i];
-                begin[set] = v;
-            }
-        }
-
         // What a lane brings of a tile, one tile ahead.  Its places are pointers that go on by a tile's rows.
         unit x[T::PER], d[T::PER], g[T::PER];
         vec b[T::VPER], cc[T::VPER];
@@ -333,7 +282,63 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
         float *my_inputs = inputs + ch * T::STRIDE;
         const vec *my_b = vb + ln, *my_c = vc + (PART == 1 ? 0 : ln);
 
-        fetch(tile0);
+        if (tile0 < tile1) fetch(tile0);
+
+        // Workspace of a sequence: the state that it continues, the states of its parts, those of its pieces; the factors of both.
+        const long long step = (long long)p.channels * T::NP, at0 = (long long)c * T::NP + n0;
+        const int all = (int)p.parts * (PIECES + 1);
+        float *states = PART ? p.part_states + (long long)s * (all + 1) * step + at0 : nullptr, *factors = PART ? p.part_factors + (long long)s * all * step + at0 : nullptr;
+        auto take_in = [&](vec &f, vec &b, int which) {  // a part or piece behind what f and b hold
+            const vec pf = *reinterpret_cast<const vec *>(factors + which * step), pb = *reinterpret_cast<const vec *>(states + (which + 1) * step);
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                b[i] = __builtin_fmaf(pf[i], b[i], pb[i]);
+                f[i] *= pf[i];
+            }
+        };
+        if constexpr (PART == 0) {
+            if (mine && wt == 0) first_state<NL, false>(p, q, c, n0, h);
+            if (WT > 1 && wt == 0) {
+                vec v;
+#pragma unroll
+                for (int i = 0; i < NL; i++) v[i] = h[i];
+                begin[set] = v;
+            }
+        } else if constexpr (PART == 1) {
+            if (mine && part == 0 && wave == 0) {  // kept for the second launch, in which the slot may be written already
+                float kept[NL];
+                first_state<NL, false>(p, q, c, n0, kept);
+#pragma unroll
+                for (int i = 0; i < NL; i++) states[i] = kept[i];
+            }
+        } else {  // a stretch of the parts before this one and a piece of its own by every wavefront, joined by all of them
+            vec f, b, v, pf, pb;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                f[i] = pf[i] = 1.0f;
+                b[i] = v[i] = pb[i] = 0.0f;
+            }
+            const int each = (part + WAVES - 1) / WAVES, end = min(part, (wave + 1) * each);
+            if (mine) {
+                v = *reinterpret_cast<const vec *>(states);
+                take_in(pf, pb, (int)p.parts + part * PIECES + wave);
+#pragma unroll 4
+                for (int j = wave * each; j < end; j++) take_in(f, b, j);
+            }
+            factor[tid] = f;
+            brought[tid] = b;
+            factor[T::THREADS + tid] = pf;
+            brought[T::THREADS + tid] = pb;
+            __syncthreads();
+            for (int w = 0; w < WAVES + wave; w++) {
+                const vec wf = factor[w * 64 + lane], wb = brought[w * 64 + lane];
+#pragma unroll
+                for (int i = 0; i < NL; i++) v[i] = __builtin_fmaf(wf[i], v[i], wb[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < NL; i++) h[i] = v[i];
+        }
+
         for (int tile = tile0; tile < tile1; tile++) {
             in_order();
             stage(tile);
@@ -345,7 +350,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
             }
             if (tile + 1 < tile1) fetch(tile + 1);
             in_order();
-            float kept[WT > 1 ? T::TT : 1][NL], put[WT > 1 && PART != 1 ? T::TT : 1][NL];  // factors and products of the tokens
+            float kept[WT > 1 ? T::TT : 1][NL], put[WT > 1 ? T::TT : 1][NL];  // factors and products of the tokens
             if constexpr (WT > 1) {
                 float local[NL], sum = 0.0f;
 #pragma unroll
@@ -362,7 +367,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                             const float f = __builtin_amdgcn_exp2f(dv[j] * a[i]), u = xv[j] * bv[i];
                             local[i] = __builtin_fmaf(f, local[i], u);
                             kept[t + j][i] = f;
-                            if (PART != 1) put[t + j][i] = u;
+                            put[t + j][i] = u;
                         }
                     }
                 }
@@ -377,12 +382,9 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                 all[wt * SETS] = v;
                 all_f[wt * SETS] = f;
                 __syncthreads();
-                const int before = PART == 1 ? (wt == 0 ? WT : 0) : wt;
-                if (PART != 1) {
-                    const vec v0 = begin[half * SETS + set];
+                const vec v0 = begin[half * SETS + set];
 #pragma unroll
-                    for (int i = 0; i < NL; i++) h[i] = v0[i];
-                }
+                for (int i = 0; i < NL; i++) h[i] = v0[i];
                 auto take = [&](int w, auto count) {  // (reads in flight together)
                     constexpr int N = decltype(count)::value;
                     vec wf[N], wb[N];
@@ -394,43 +396,47 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
 #pragma unroll
                     for (int k = 0; k < N; k++)
 #pragma unroll
-                        for (int i = 0; i < NL; i++) {
-                            h[i] = __builtin_fmaf(wf[k][i], h[i], wb[k][i]);
-                            if (PART == 1) through[i] *= wf[k][i];
-                        }
+                        for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(wf[k][i], h[i], wb[k][i]);
                 };
                 int w = 0;
-                for (; w + 4 <= before; w += 4) take(w, std::integral_constant<int, 4>());
-                if (before & 2) take(w, std::integral_constant<int, 2>()), w += 2;
-                if (before & 1) take(w, std::integral_constant<int, 1>());
+                for (; w + 4 <= wt; w += 4) take(w, std::integral_constant<int, 4>());
+                if (wt & 2) take(w, std::integral_constant<int, 2>()), w += 2;
+                if (wt & 1) take(w, std::integral_constant<int, 1>());
             }
-            if constexpr (PART != 1) {
+            float sum_d = 0.0f;
 #pragma unroll
-                for (int t = 0; t < T::TT; t += 4) {
-                    // The exponentials of four tokens first: one after another, each would be waited for (32 sequences of 512 tokens of 2048 channels
-                    // 175 -> 165 us).
-                    float f[4][NL], u[4][NL];
-                    if constexpr (WT == 1) {
-                        const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
+            for (int t = 0; t < T::TT; t += 4) {
+                // The exponentials of four tokens first: one after another, each would be waited for (32 sequences of 512 tokens of 2048 channels
+                // 175 -> 165 us).
+                float f[4][NL], u[4][NL];
+                if constexpr (WT == 1) {
+                    const floatx4 dv = *reinterpret_cast<const floatx4 *>(my_steps + t), xv = *reinterpret_cast<const floatx4 *>(my_inputs + t);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const vec bv = my_b[(t + j) * LANES];
+                    for (int j = 0; j < 4; j++) {
+                        const vec bv = my_b[(t + j) * LANES];
+                        if (PART == 1) sum_d += dv[j];
 #pragma unroll
-                            for (int i = 0; i < NL; i++) {
-                                f[j][i] = __builtin_amdgcn_exp2f(dv[j] * a[i]);
-                                u[j][i] = xv[j] * bv[i];
-                            }
+                        for (int i = 0; i < NL; i++) {
+                            f[j][i] = __builtin_amdgcn_exp2f(dv[j] * a[i]);
+                            u[j][i] = xv[j] * bv[i];
                         }
-                        __builtin_amdgcn_sched_barrier(0);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-#pragma unroll
-                            for (int i = 0; i < NL; i++) {
-                                f[j][i] = kept[t + j][i];
-                                u[j][i] = put[t + j][i];
-                            }
                     }
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int i = 0; i < NL; i++) {
+                            f[j][i] = kept[t + j][i];
+                            u[j][i] = put[t + j][i];
+                        }
+                }
+                if constexpr (PART == 1) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(f[j][i], h[i], u[j][i]);
+                } else {
                     floatx4 y;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
@@ -450,6 +456,11 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                     }
                     if (ln == 0) *reinterpret_cast<floatx4 *>(my_inputs + t) = y;
                 }
+            }
+            if constexpr (PART == 1) {
+#pragma unroll
+                for (int i = 0; i < NL; i++) through[i] *= __builtin_amdgcn_exp2f(sum_d * a[i]);
+            } else {
                 if (WT > 1 && wt == WT - 1) {
                     vec v;
 #pragma unroll
@@ -484,17 +495,34 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 ? 2 : 4) void scan
                 py += T::TOKENS * my;
             }
         }
-        if (PART == 1) {
-            if (mine && wt == 0) {
-                float *states = p.part_states + (((long long)s * ((int)p.parts + 1) + part + 1) * p.channels + c) * T::NP + n0;
-                float *factors = p.part_factors + (((long long)s * (int)p.parts + part) * p.channels + c) * T::NP + n0;
+        if constexpr (PART == 1) {  // the piece's, and by the first wavefront all pieces' together
+            vec f, b;
 #pragma unroll
-                for (int i = 0; i < NL; i++) {
-                    states[i] = h[i];
-                    factors[i] = through[i];
-                }
+            for (int i = 0; i < NL; i++) {
+                f[i] = through[i];
+                b[i] = h[i];
             }
-        } else if (mine && wt == WT - 1 && tile1 == tiles) {
+            auto keep = [&](int which) {
+                *reinterpret_cast<vec *>(factors + which * step) = f;
+                *reinterpret_cast<vec *>(states + (which + 1) * step) = b;
+            };
+            if (mine) keep((int)p.parts + part * PIECES + wave);
+            factor[tid] = f;
+            brought[tid] = b;
+            __syncthreads();
+            if (mine && wave == 0) {
+#pragma unroll
+                for (int w = 1; w < WAVES; w++) {
+                    const vec wf = factor[w * 64 + lane], wb = brought[w * 64 + lane];
+#pragma unroll
+                    for (int i = 0; i < NL; i++) {
+                        b[i] = __builtin_fmaf(wf[i], b[i], wb[i]);
+                        f[i] *= wf[i];
+                    }
+                }
+                keep(part);
+            }
+        } else if (mine && wt == WT - 1 && tile0 < tile1 && tile1 == tiles) {
             keep_state<NL, false>(p, q, c, n0, h);
         }
         __syncthreads();  // (the next job's states)
@@ -530,20 +558,10 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
         p.blocks = groups * p.group_blocks;
         return (long long)p.blocks * seqs;
     };
-    auto divided = [&](auto tile, auto first, auto second, int parts) {
-        using T = decltype(tile);
-        p.parts = parts;
-        const size_t each = (size_t)p.channels * T::NP * sizeof(float);
-        void *ws = nullptr;
-        EH_TRY(get_workspace(dev, each * seqs * (2 * (size_t)parts + 1), &ws));
-        p.part_states = (float *)ws;
-        p.part_factors = (float *)((char *)ws + each * seqs * (parts + 1));
-        EH_TRY(launch(first, T::THREADS));
-        return launch(second, T::THREADS);
-    };
     // By the workgroups that there are, in multiples of the compute units: four wavefronts of different channels do the least work a token; where that leaves
     // the device half empty, they divide the tokens of a quarter of the channels (512 tokens of 2048 channels, us: 16 sequences 107 against 128, 12 105 and 95, 4 84 and
-    // 36); where that would, too, eight do (2 sequences 28 and 22); and where those do not meet every unit, sequences are divided over workgroups.
+    // 36); where that would, too, eight do (2 sequences 28 and 22); and where those do not meet every unit, sequences are divided over workgroups (1000 tokens of
+    // 1024 channels: not divided 39 us, divided 20; 8192 of 4096, as many workgroups as units: 215 and 276, since all exponentials are formed twice).
     using Alone = ScanTile<LANES, NL, 4, 1>;
     using Four = ScanTile<LANES, NL, 4, 4>;
     using Eight = ScanTile<LANES, NL, 8, 8>;
@@ -554,13 +572,16 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
     const long long parts = num_cu / workgroups, tiles = (tokens + Eight::TOKENS - 1) / Eight::TOKENS;
     if (parts < 2 || tiles < 4)
         return launch(vec ? scan_tile_kernel<LANES, NL, 8, 8, true, 0> : scan_tile_kernel<LANES, NL, 8, 8, false, 0>, Eight::THREADS);
-    // (4096 tokens of 1024 channels: not divided 125 us, 4 parts of eight wavefronts 63, 8 of four 57; 1000 tokens 39, 24 and 25)
-    if (tiles >= 8 * parts)
-        return vec ? divided(Four(), scan_tile_kernel<LANES, NL, 4, 4, true, 1>, scan_tile_kernel<LANES, NL, 4, 4, true, 2>, (int)(2 * parts))
-                   : divided(Four(), scan_tile_kernel<LANES, NL, 4, 4, false, 1>, scan_tile_kernel<LANES, NL, 4, 4, false, 2>, (int)(2 * parts));
-    const int n = (int)std::min(parts, tiles);
-    return vec ? divided(Eight(), scan_tile_kernel<LANES, NL, 8, 8, true, 1>, scan_tile_kernel<LANES, NL, 8, 8, true, 2>, n)
-               : divided(Eight(), scan_tile_kernel<LANES, NL, 8, 8, false, 1>, scan_tile_kernel<LANES, NL, 8, 8, false, 2>, n);
+    // Eight wavefronts a part; two parts a unit where they are long (a workgroup and two a unit, us: 65536 tokens of 256 channels 164 and 140, 4096 of 1024 49 and 45,
+    // 1000 of 1024 20.5 and 21.8).
+    p.parts = (unsigned)(tiles >= 8 * parts ? 2 * parts : std::min(parts, tiles));
+    const size_t each = (size_t)p.channels * Eight::NP * sizeof(float) * seqs, all = (size_t)p.parts * 9;  // (parts and their pieces)
+    void *ws = nullptr;
+    EH_TRY(get_workspace(dev, each * (2 * all + 1), &ws));
+    p.part_states = (float *)ws;
+    p.part_factors = (float *)((char *)ws + each * (all + 1));
+    EH_TRY(launch(vec ? scan_tile_kernel<LANES, NL, 8, 1, true, 1> : scan_tile_kernel<LANES, NL, 8, 1, false, 1>, Eight::THREADS));
+    return launch(vec ? scan_tile_kernel<LANES, NL, 8, 1, true, 2> : scan_tile_kernel<LANES, NL, 8, 1, false, 2>, Eight::THREADS);
 }
 
 }  // namespace

@@ -610,8 +610,9 @@ int eddlhip_causal_conv(int dev, const float *X, long long ldx, const float *W, 
  *     h[c][i] = e^(d A[c][i]) h[c][i] + d x B[i],   Y = (sum_i C[i] h[c][i] + skip[c] x) silu(gate).
  * X, dt, gate, Y [rows][channels]; B and C [rows][groups * n], a vector for each of `groups` equal parts of the channels; A [channels][n]; skip and dt_bias
  * [channels] may be NULL (0), gate too (no factor).  The state is [pool][channels][n].  Y and the states lie on nothing else that is read.
- * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  Sums and states
- * are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups take. */
+ * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  Factors are multiplied over runs of
+ * tokens: where e^(d A), d A summed over tokens one after another, passes the largest number, the state may be infinite or NaN, also one of zeros (it does not where no d A is
+ * positive).  Sums and states are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups take. */
 int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
                            const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,
                            int rows, int channels, int n, int groups, int softplus, int reverse, float *states, int pool,
