@@ -268,6 +268,8 @@ def CausalConvolution(parent, width, channels=None, use_bias=True, activation="s
     n = shape[-1] if channels is None else int(channels)
     if len(shape) != 3 or not 1 <= n <= shape[2] or not 2 <= int(width) <= 8:
         msg("CausalConvolution needs [batch, tokens, columns] with %s channels and a width of 2 to 8, not %s and %s" % (channels, shape, width), "CausalConvolution")
+    if activation not in (None, "relu", "silu"):
+        msg("CausalConvolution knows no activation %s" % activation, "CausalConvolution")
     if states is not None and batch is None:
         msg("states come with a batch", "CausalConvolution")
     l = Layer("causal_conv", [parent], shape[:2] + [n], name, activation=activation, reverse=bool(reverse), batch=batch, states=states)

@@ -605,3 +605,88 @@ def test_places_beyond_32_bits(hip):
     row = np.concatenate([np.ones(ld - channels), x[-1]])
     want = (row - mean) / np.sqrt(var + 1.0)
     assert np.abs(got - want).max() <= 128 * EPS * np.abs(row).max()
+
+
+# ------------------------------------------------------------------------------------------------- sequences whose parts several workgroups take
+@pytest.mark.parametrize("channels, n, news", [(12, 16, [1200, 0, 700]), (40, 3, [2100, 17, 900, 1]), (5, 40, [2500])])
+def test_divided_sequences(hip, channels, n, news):
+    """Sequences with tokens and without, short and long, whose states come from other slots than they go to; with a bound below and far above the new
+    tokens, and several sequences that continue one slot."""
+    rng = np.random.default_rng([channels, n, 1])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, 1)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    for fork in (False, True):
+        if fork:
+            batch.slots = np.full(len(news), batch.slots[0], np.int32)
+            batch.lengths = (batch.news + 3).astype(np.int32)
+        for reverse in (False, True):
+            want, err, after, after_err = selective_scan(reverse=reverse, **case, **batch.reference(pool))
+            for most in (None, 600, 1 << 20):
+                y, s = _scan(hip, case, batch, pool, reverse, most)
+                _check(y, want, err, (fork, most))
+                _check(s, after, after_err, (fork, most, "state"))
+                assert np.all(batch.outside(y) == -7.0)
+
+
+def test_not_finite_numbers_of_divided_sequences(hip):
+    """As in short sequences: nothing changes by a bit before the token, in other channels and in other sequences; a state outside the pool makes its sequence NaN."""
+    rng = np.random.default_rng(31)
+    channels, n = 20, 16
+    batch = Ragged(rng, [3000, 900])
+    batch.lengths[:] = batch.news + 2
+    case = _scan_case(rng, batch, channels, n, 1)
+    case["A"] = np.maximum(case["A"], -2)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    y, s = _scan(hip, case, batch, pool, False)
+    for value in (np.inf, np.nan):
+        for token in (0, 1234, 2999):
+            bad = dict(case, x=case["x"].copy())
+            at, end = int(batch.offsets[0]) + token, int(batch.offsets[1])
+            bad["x"][at, 2] = value
+            y2, s2 = _scan(hip, bad, batch, pool, False)
+            assert not np.any(np.isfinite(y2[at:end, 2])) and not np.any(np.isfinite(s2[batch.out_slots[0], 2]))
+            y2[at:end, 2], s2[batch.out_slots[0], 2] = y[at:end, 2], s[batch.out_slots[0], 2]
+            assert np.array_equal(y, y2) and np.array_equal(s, s2)
+    batch.slots[0], batch.out_slots[1] = -1, batch.pool
+    y2, s2 = _scan(hip, case, batch, pool, False)
+    first, second = (slice(*batch.offsets[k:k + 2]) for k in (0, 1))
+    assert np.all(np.isnan(y2[first])) and np.array_equal(y2[second], y[second]) and np.all(np.isnan(s2[batch.out_slots[0]]))
+
+
+def test_a_larger_call_outgrows_a_recorded_one(hip):
+    """Divided sequences and groups take the workspace: one that would have to grow is refused while a graph is recorded, and a graph whose workspace was
+    replaced is refused at its launch."""
+    from eddl_amd.backend import EddlHipError
+    rng = np.random.default_rng(32)
+    batch = Ragged(rng, [2000], before=0, behind=0, kept=False)
+    case = _scan_case(rng, batch, 16, 16, 1)
+    d, b = (lambda t: hip.array(t)), batch.on(hip)
+    X, dt, A, B, C, Y = d(case["x"]), d(case["dt"]), d(case["A"]), d(case["B"]), d(case["C"]), hip.empty(case["x"].shape)
+    big = hip.empty((1, 4, 600, 512))
+    hip.fill_(big, 1.0)
+
+    def small():
+        hip.selective_scan(X, dt, A, B, C, Y, b)
+
+    hip.workspace_trim()
+    small()
+    want = Y.numpy()
+    graph = hip.record(small)
+    hip.group_norm(big, big, 2)  # (fits the workspace that stands)
+    hip.fill_(Y, 0.0)
+    graph.launch()
+    assert np.array_equal(Y.numpy(), want)
+    many = Ragged(rng, [600] * 6, before=0, behind=0, kept=False)
+    wide = _scan_case(rng, many, 60, 64, 1)
+    m = many.on(hip)
+    W = [d(wide[k]) for k in ("x", "dt", "A", "B", "C")] + [hip.empty(wide["x"].shape)]
+    with pytest.raises(EddlHipError, match="before recording"):
+        hip.record(lambda: hip.selective_scan(*W, m))
+    hip.selective_scan(*W, m)
+    with pytest.raises(EddlHipError, match="record again"):
+        graph.launch()
+    graph = hip.record(small)
+    hip.fill_(Y, 0.0)
+    graph.launch()
+    assert np.array_equal(Y.numpy(), want)

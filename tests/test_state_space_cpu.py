@@ -181,3 +181,9 @@ def test_layers_check_their_parents():
             L.SelectiveScan(**dict(dict(parent=c, dt=d, vectors=v, state=5, groups=2, gate=z), **bad))
     with pytest.raises(RuntimeError):
         L.SelectiveScan(c, d, v, 5, states=_Tensor((3, 16, 5)))
+
+
+def test_layer_refuses_an_unknown_activation():
+    from eddl_amd import net as L
+    with pytest.raises(RuntimeError):
+        L.CausalConvolution(L.Input([9, 24], 3), 4, activation="gelu")
