@@ -163,7 +163,7 @@ __device__ __forceinline__ void in_order() {
 // PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups, and a workgroup's part over its wavefronts, which
 // walk their pieces on their own: PART 1 brings the state of every piece and part from zeros and the factor of what comes before it, PART 2 takes in what lies
 // before its own and brings the outputs.
-template <int LANES, int NL, int WAVES, int WT, bool VEC, int PART>
+template <int LANES, int NL, int WAVES, int WT, int PART>
 __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && LANES == 16) ? 2 : 4) void scan_tile_kernel(const ScanParams p) {
     using T = ScanTile<LANES, NL, WAVES, WT>;
     constexpr int U = T::U;
@@ -217,7 +217,6 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
         const bool has = c0 + at < cend, hasv = av < p.n, wholev = av + NL <= p.n;
         const bool whole = c0 + at + U <= cend;  // (wherever rows begin, since 16 bytes are read from any multiple of four: 7 ragged sequences of 1002 channels 26.1 -> 22.2 us)
         auto get_unit = [&](const float *from) {
-            if (VEC) return *reinterpret_cast<const unit *>(from);
             unit v;
             if (whole) {
                 v = *reinterpret_cast<const loose_unit *>(from);
@@ -501,9 +500,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
                             for (int i = 0; i < U; i++) y[i] *= silu(g0[k][i]);
                         }
                         float *to = py + k * APART * my;
-                        if (VEC) {
-                            *reinterpret_cast<unit *>(to) = y;
-                        } else if (whole) {
+                        if (whole) {
                             *reinterpret_cast<loose_unit *>(to) = y;
                         } else {
 #pragma unroll
@@ -553,7 +550,7 @@ constexpr int MOST_STATES = 64;
 constexpr int FEW_TOKENS = 3;  // up to here token after token from memory (32 sequences of 2 tokens of 2048 channels 8.8 us, as tiles 10.9; of 8 19.0 and 12.1)
 
 template <int LANES, int NL>
-int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
+int launch_scan(int dev, ScanParams &p, int seqs, int tokens) {
     const hipStream_t st = state(dev).stream;
     if (tokens <= FEW_TOKENS) {
         hipLaunchKernelGGL((p.n % NL == 0 ? scan_tokens_kernel<LANES, NL, true> : scan_tokens_kernel<LANES, NL, false>), dim3((unsigned)(((long long)p.channels * LANES + 255) / 256), seqs), dim3(256), 0, st, p);
@@ -585,12 +582,12 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
     using Four = ScanTile<LANES, NL, 4, 4>;
     using Eight = ScanTile<LANES, NL, 8, 8>;
     if (sized(Alone()) >= 2 * num_cu || tokens <= Alone::TOKENS)
-        return launch(vec ? scan_tile_kernel<LANES, NL, 4, 1, true, 0> : scan_tile_kernel<LANES, NL, 4, 1, false, 0>, Alone::THREADS);
+        return launch(scan_tile_kernel<LANES, NL, 4, 1, 0>, Alone::THREADS);
     const long long workgroups = sized(Four());  // (as many as of eight wavefronts, which have as many channels)
-    if (2 * workgroups >= 3 * num_cu) return launch(vec ? scan_tile_kernel<LANES, NL, 4, 4, true, 0> : scan_tile_kernel<LANES, NL, 4, 4, false, 0>, Four::THREADS);
+    if (2 * workgroups >= 3 * num_cu) return launch(scan_tile_kernel<LANES, NL, 4, 4, 0>, Four::THREADS);
     const long long parts = num_cu / workgroups, tiles = (tokens + Eight::TOKENS - 1) / Eight::TOKENS;
     if (parts < 2 || tiles < 4)
-        return launch(vec ? scan_tile_kernel<LANES, NL, 8, 8, true, 0> : scan_tile_kernel<LANES, NL, 8, 8, false, 0>, Eight::THREADS);
+        return launch(scan_tile_kernel<LANES, NL, 8, 8, 0>, Eight::THREADS);
     // Eight wavefronts a part; two parts a unit where they are long (a workgroup and two a unit, us: 65536 tokens of 256 channels 164 and 140, 4096 of 1024 49 and 45,
     // 1000 of 1024 20.5 and 21.8).
     p.parts = (unsigned)(tiles >= 8 * parts ? 2 * parts : std::min(parts, tiles));
@@ -599,8 +596,8 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens, bool vec) {
     EH_TRY(get_workspace(dev, each * (2 * all + 1), &ws));
     p.part_states = (float *)ws;
     p.part_factors = (float *)((char *)ws + each * (all + 1));
-    EH_TRY(launch(vec ? scan_tile_kernel<LANES, NL, 8, 1, true, 1> : scan_tile_kernel<LANES, NL, 8, 1, false, 1>, Eight::THREADS));
-    return launch(vec ? scan_tile_kernel<LANES, NL, 8, 1, true, 2> : scan_tile_kernel<LANES, NL, 8, 1, false, 2>, Eight::THREADS);
+    EH_TRY(launch(scan_tile_kernel<LANES, NL, 8, 1, 1>, Eight::THREADS));
+    return launch(scan_tile_kernel<LANES, NL, 8, 1, 2>, Eight::THREADS);
 }
 
 }  // namespace
@@ -657,15 +654,11 @@ extern "C" int eddlhip_selective_scan(int dev, const float *X, long long ldx, co
     p.per = channels / groups;
     p.softplus = softplus != 0;
     p.batch = StateBatch{offsets, lengths, slots, out_slots, rows, pool, reverse != 0};
-    // (a group's first channel, too, has to be aligned)
-    uintptr_t rows16 = 0;
-    for (const void *at : {(const void *)X, (const void *)dt, (const void *)gate, (const void *)Y, (const void *)skip, (const void *)dt_bias}) rows16 |= (uintptr_t)at;
-    const bool vec = (rows16 & 15) == 0 && p.per % 4 == 0 && ldx % 4 == 0 && lddt % 4 == 0 && ldy % 4 == 0 && (!gate || ldg % 4 == 0);
     const int tokens = std::max(1, std::min(max_new, rows));
-    if (n == 1) return launch_scan<1, 1>(dev, p, seqs, tokens, vec);
-    if (n <= 4) return launch_scan<1, 4>(dev, p, seqs, tokens, vec);
-    if (n <= 8) return launch_scan<2, 4>(dev, p, seqs, tokens, vec);
-    if (n <= 16) return launch_scan<4, 4>(dev, p, seqs, tokens, vec);
-    if (n <= 32) return launch_scan<8, 4>(dev, p, seqs, tokens, vec);
-    return launch_scan<16, 4>(dev, p, seqs, tokens, vec);
+    if (n == 1) return launch_scan<1, 1>(dev, p, seqs, tokens);
+    if (n <= 4) return launch_scan<1, 4>(dev, p, seqs, tokens);
+    if (n <= 8) return launch_scan<2, 4>(dev, p, seqs, tokens);
+    if (n <= 16) return launch_scan<4, 4>(dev, p, seqs, tokens);
+    if (n <= 32) return launch_scan<8, 4>(dev, p, seqs, tokens);
+    return launch_scan<16, 4>(dev, p, seqs, tokens);
 }
