@@ -14,7 +14,7 @@ using namespace eddlhip;
 
 namespace {
 
-typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4), aligned(4)));  // (the hardware reads and writes 16 bytes at any multiple of four)
 
 struct ConvParams {
     const float *X, *W, *bias;
@@ -43,79 +43,87 @@ __device__ __forceinline__ Unit<UNIT> get(const float *from) {
     }
     return u;
 }
+// Outputs are written past the caches (4096 tokens of 4096 channels 38 -> 30 us; rows that begin inside a line too: 16 x 2048 of 2044 channels 114 -> 109).
 template <int UNIT>
 __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u) {
-    if constexpr (UNIT == 4) __builtin_nontemporal_store(floatx4{u.v[0], u.v[1], u.v[2], u.v[3]}, reinterpret_cast<floatx4 *>(to));  // (4096 tokens of 4096 channels 38 -> 30 us)
+    if constexpr (UNIT == 4) __builtin_nontemporal_store(floatx4{u.v[0], u.v[1], u.v[2], u.v[3]}, reinterpret_cast<floatx4 *>(to));
     else *to = u.v[0];
 }
 
-// A thread takes UNIT channels of eight tokens, all of whose inputs it asks for at once; the first tokens' thread also reads and writes the
+// UNIT channels of a sequence from c on, of eight tokens, all of whose inputs are asked for at once; the first tokens' thread also reads and writes the
 // state, so that no other thread meets it.
 template <int WIDTH, int UNIT>
-__global__ __launch_bounds__(256) void causal_conv_kernel(const ConvParams p) {
+__device__ __forceinline__ void convolve(const ConvParams &p, const Sequence &q, int c, long long from) {
     static_assert(CONV_TOKENS >= WIDTH - 1, "inputs of the state reach the first chunk only");
+    Unit<UNIT> w[WIDTH], bias;  // w[k].v[i]: number i * WIDTH + k of the channels' weights
+    {
+        Unit<UNIT> in[WIDTH];
+#pragma unroll
+        for (int k = 0; k < WIDTH; k++) in[k] = get<UNIT>(p.W + (long long)c * WIDTH + k * UNIT);
+#pragma unroll
+        for (int k = 0; k < WIDTH; k++)
+#pragma unroll
+            for (int i = 0; i < UNIT; i++) w[k].v[i] = in[(i * WIDTH + k) / UNIT].v[(i * WIDTH + k) % UNIT];
+#pragma unroll
+        for (int i = 0; i < UNIT; i++) bias.v[i] = 0.0f;
+        if (p.bias) bias = get<UNIT>(p.bias + c);
+    }
+    for (; from < q.fresh; from += (long long)p.chunks * CONV_TOKENS) {
+        const int t0 = (int)from;
+        Unit<UNIT> x[WIDTH - 1 + CONV_TOKENS];  // x[k]: the input of token t0 - (WIDTH - 1) + k
+#pragma unroll
+        for (int k = 0; k < WIDTH - 1 + CONV_TOKENS; k++) {
+            const int t = t0 - (WIDTH - 1) + k;
+#pragma unroll
+            for (int i = 0; i < UNIT; i++) x[k].v[i] = k < WIDTH - 1 && t < 0 && q.read == -2 ? __builtin_nanf("") : 0.0f;
+            if (k >= WIDTH - 1 ? t < q.fresh : t >= 0) x[k] = get<UNIT>(p.X + q.row(t) * p.ldx + c);
+            else if (k < WIDTH - 1 && q.read >= 0) x[k] = get<UNIT>(p.states + ((long long)q.read * (WIDTH - 1) + k) * p.channels + c);
+        }
+        if (t0 == 0 && q.write >= 0) {
+#pragma unroll
+            for (int k = 0; k < WIDTH - 1; k++) {
+                const int t = q.fresh - (WIDTH - 1) + k;  // of an input that is kept
+                Unit<UNIT> kept;
+                if (t >= 0) {
+                    kept = get<UNIT>(p.X + q.row(t) * p.ldx + c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < WIDTH - 1; j++)
+                        if (t == j - (WIDTH - 1)) kept = x[j];
+                }
+                set<UNIT>(p.states + ((long long)q.write * (WIDTH - 1) + k) * p.channels + c, kept);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < CONV_TOKENS; j++) {
+            if (t0 + j < q.fresh) {
+                Unit<UNIT> y = bias;
+#pragma unroll
+                for (int i = 0; i < UNIT; i++) {
+#pragma unroll
+                    for (int k = 0; k < WIDTH; k++) y.v[i] = __builtin_fmaf(w[k].v[i], x[j + k].v[i], y.v[i]);
+                    y.v[i] = activated(y.v[i], p.activation);
+                }
+                set<UNIT>(p.Y + q.row(t0 + j) * p.ldy + c, y);
+            }
+        }
+    }
+}
+
+// Four channels a thread; those behind the last four one a thread (16 sequences of 2048 tokens of 2046 channels, us: all one a thread 151, so 117).
+template <int WIDTH>
+__global__ __launch_bounds__(256) void causal_conv_kernel(const ConvParams p) {
     // (neighbours in time share width - 1 rows)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
         const long long job = xcd_job(id);
         if (job >= p.jobs) continue;
         const unsigned chunk = (unsigned)job % p.chunks, rest = (unsigned)job / p.chunks;  // (fewer than 2^31 jobs)
         const Sequence q = sequence(p.batch, rest / p.blocks);
-        const int c = (rest % p.blocks * 256 + threadIdx.x) * UNIT;
-        long long from = (long long)chunk * CONV_TOKENS;
-        if (c >= p.channels || from >= q.fresh) continue;
-        Unit<UNIT> w[WIDTH], bias;  // w[k].v[i]: number i * WIDTH + k of the channels' weights
-        {
-            Unit<UNIT> in[WIDTH];
-#pragma unroll
-            for (int k = 0; k < WIDTH; k++) in[k] = get<UNIT>(p.W + (long long)c * WIDTH + k * UNIT);
-#pragma unroll
-            for (int k = 0; k < WIDTH; k++)
-#pragma unroll
-                for (int i = 0; i < UNIT; i++) w[k].v[i] = in[(i * WIDTH + k) / UNIT].v[(i * WIDTH + k) % UNIT];
-#pragma unroll
-            for (int i = 0; i < UNIT; i++) bias.v[i] = 0.0f;
-            if (p.bias) bias = get<UNIT>(p.bias + c);
-        }
-        for (; from < q.fresh; from += (long long)p.chunks * CONV_TOKENS) {
-            const int t0 = (int)from;
-            Unit<UNIT> x[WIDTH - 1 + CONV_TOKENS];  // x[k]: the input of token t0 - (WIDTH - 1) + k
-#pragma unroll
-            for (int k = 0; k < WIDTH - 1 + CONV_TOKENS; k++) {
-                const int t = t0 - (WIDTH - 1) + k;
-#pragma unroll
-                for (int i = 0; i < UNIT; i++) x[k].v[i] = k < WIDTH - 1 && t < 0 && q.read == -2 ? __builtin_nanf("") : 0.0f;
-                if (k >= WIDTH - 1 ? t < q.fresh : t >= 0) x[k] = get<UNIT>(p.X + q.row(t) * p.ldx + c);
-                else if (k < WIDTH - 1 && q.read >= 0) x[k] = get<UNIT>(p.states + ((long long)q.read * (WIDTH - 1) + k) * p.channels + c);
-            }
-            if (t0 == 0 && q.write >= 0) {
-#pragma unroll
-                for (int k = 0; k < WIDTH - 1; k++) {
-                    const int t = q.fresh - (WIDTH - 1) + k;  // of an input that is kept
-                    Unit<UNIT> kept;
-                    if (t >= 0) {
-                        kept = get<UNIT>(p.X + q.row(t) * p.ldx + c);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < WIDTH - 1; j++)
-                            if (t == j - (WIDTH - 1)) kept = x[j];
-                    }
-                    set<UNIT>(p.states + ((long long)q.write * (WIDTH - 1) + k) * p.channels + c, kept);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < CONV_TOKENS; j++) {
-                if (t0 + j < q.fresh) {
-                    Unit<UNIT> y = bias;
-#pragma unroll
-                    for (int i = 0; i < UNIT; i++) {
-#pragma unroll
-                        for (int k = 0; k < WIDTH; k++) y.v[i] = __builtin_fmaf(w[k].v[i], x[j + k].v[i], y.v[i]);
-                        y.v[i] = activated(y.v[i], p.activation);
-                    }
-                    set<UNIT>(p.Y + q.row(t0 + j) * p.ldy + c, y);
-                }
-            }
-        }
+        const int unit = rest % p.blocks * 256 + threadIdx.x, units = p.channels / 4, single = unit - (units + 63) / 64 * 64;  // (those one a thread are in a wavefront of their own)
+        const long long from = (long long)chunk * CONV_TOKENS;
+        if (from >= q.fresh) continue;
+        if (unit < units) convolve<WIDTH, 4>(p, q, unit * 4, from);
+        else if (single >= 0 && single < p.channels % 4) convolve<WIDTH, 1>(p, q, units * 4 + single, from);
     }
 }
 
@@ -156,15 +164,13 @@ extern "C" int eddlhip_causal_conv(int dev, const float *X, long long ldx, const
     p.activation = activation;
     p.batch = StateBatch{offsets, lengths, slots, out_slots, rows, pool, reverse != 0};
     typedef void (*kernel)(ConvParams);
-    static const kernel kernels[2][MOST_WIDTH - 1] = {
-        {causal_conv_kernel<2, 1>, causal_conv_kernel<3, 1>, causal_conv_kernel<4, 1>, causal_conv_kernel<5, 1>, causal_conv_kernel<6, 1>, causal_conv_kernel<7, 1>, causal_conv_kernel<8, 1>},
-        {causal_conv_kernel<2, 4>, causal_conv_kernel<3, 4>, causal_conv_kernel<4, 4>, causal_conv_kernel<5, 4>, causal_conv_kernel<6, 4>, causal_conv_kernel<7, 4>, causal_conv_kernel<8, 4>}};
-    const bool vec = (((uintptr_t)X | (uintptr_t)Y | (uintptr_t)W | (uintptr_t)bias | (uintptr_t)states) & 15) == 0 && channels % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0;
-    p.blocks = (channels + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+    static const kernel kernels[MOST_WIDTH - 1] = {causal_conv_kernel<2>, causal_conv_kernel<3>, causal_conv_kernel<4>, causal_conv_kernel<5>,
+                                                   causal_conv_kernel<6>, causal_conv_kernel<7>, causal_conv_kernel<8>};
+    p.blocks = ((channels / 4 + 63) / 64 * 64 + channels % 4 + 255) / 256;
     // (jobs that a 31-bit number counts: a thread walks the chunks beyond)
     p.chunks = (unsigned)std::min<long long>((std::max(1, std::min(max_new, rows)) + CONV_TOKENS - 1) / CONV_TOKENS, ((1LL << 31) - 1) / ((long long)p.blocks * seqs));
     p.jobs = (long long)p.blocks * p.chunks * seqs;
-    hipLaunchKernelGGL(kernels[vec][width - 2], dim3(xcd_grid(p.jobs, 256)), dim3(256), 0, state(dev).stream, p);
+    hipLaunchKernelGGL(kernels[width - 2], dim3(xcd_grid(p.jobs, 256)), dim3(256), 0, state(dev).stream, p);
     EH_CHECK_LAUNCH();
     return 0;
 }
