@@ -64,7 +64,7 @@ struct Unit {
 };
 template <int UNIT>
 __device__ __forceinline__ Unit<UNIT> get(const float *from) {
-    typedef float vec __attribute__((ext_vector_type(UNIT)));
+    typedef float vec __attribute__((ext_vector_type(UNIT), aligned(4)));  // (the hardware reads and writes 16 bytes at any multiple of four)
     const vec v = *reinterpret_cast<const vec *>(from);
     Unit<UNIT> u;
 #pragma unroll
@@ -75,7 +75,7 @@ __device__ __forceinline__ Unit<UNIT> get(const float *from) {
 // (24 channels a group 27 -> 21).
 template <int UNIT>
 __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u, bool lines) {
-    typedef float vec __attribute__((ext_vector_type(UNIT)));
+    typedef float vec __attribute__((ext_vector_type(UNIT), aligned(4)));
     vec v;
 #pragma unroll
     for (int i = 0; i < UNIT; i++) v[i] = u.v[i];
@@ -428,11 +428,11 @@ int launch_rows(int dev, GroupNormParams &p) {
     return launch_divided(dev, p, group_norm_rows_kernel<256, NV, UNIT, ONE, SUMS>, group_norm_rows_kernel<256, NV, UNIT, ONE, APPLY>, groups, 0);
 }
 
-// Maps: a group begins at a multiple of UNIT numbers, which meet two channels at most.
-int launch_maps(int dev, GroupNormParams &p, int aligned) {
+// Maps: a group is a number of UNITs, which meet two channels at most.
+int launch_maps(int dev, GroupNormParams &p) {
     const long long count = (long long)p.per * p.pixels;
-    if (aligned == 4 && count % 4 == 0 && p.pixels >= 4) return launch_groups<4, false>(dev, p);
-    if (aligned >= 2 && count % 2 == 0 && p.pixels >= 2) return launch_groups<2, false>(dev, p);
+    if (count % 4 == 0 && p.pixels >= 4) return launch_groups<4, false>(dev, p);
+    if (count % 2 == 0 && p.pixels >= 2) return launch_groups<2, false>(dev, p);
     return launch_groups<1, false>(dev, p);
 }
 template <int UNIT>
@@ -481,12 +481,7 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     p.together = 1;
     p.blocks = groups;
     p.eps = eps;
-    // (numbers that may be read at a time)
-    const uintptr_t bits = (uintptr_t)X | (uintptr_t)Y;
-    const int aligned = bits % 16 == 0 ? 4 : bits % 8 == 0 ? 2 : 1;
     p.lines = !channels_last || (p.per % 32 == 0 && ldy % 32 == 0 && (uintptr_t)Y % 128 == 0);
-    if (!channels_last) return launch_maps(dev, p, aligned);
-    if (aligned == 4 && p.per % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0) return launch_tokens<4>(dev, p);
-    if (aligned >= 2 && p.per % 2 == 0 && ldx % 2 == 0 && ldy % 2 == 0) return launch_tokens<2>(dev, p);
-    return launch_tokens<1>(dev, p);
+    if (!channels_last) return launch_maps(dev, p);
+    return p.per % 4 == 0 ? launch_tokens<4>(dev, p) : p.per % 2 == 0 ? launch_tokens<2>(dev, p) : launch_tokens<1>(dev, p);
 }
