@@ -88,13 +88,32 @@ __device__ __forceinline__ void set(float *to, const Unit<UNIT> &u, bool lines) 
     }
 }
 
-// y = act((x - mean) slope + lift) for a channel of an image
-__device__ __forceinline__ void coefficients(const GroupNormParams &p, int image, int c, float scale, float &slope, float &lift) {
-    const long long at = (long long)image * p.channels + c;
-    const float more = p.mod ? 1.0f + p.mod[at] : 1.0f;
-    slope = scale * (p.w ? p.w[c] : 1.0f) * more;
-    lift = (p.b ? p.b[c] : 0.0f) * more + (p.shift ? p.shift[at] : 0.0f);
-}
+// y = act((x - mean) slope + lift) for UNIT channels of an image.  What they are made of is asked for before the sums, behind which it would be waited for.
+template <int UNIT>
+struct Coefficients {
+    Unit<UNIT> w, b, mod, shift;
+
+    __device__ __forceinline__ void ask(const GroupNormParams &p, int image, int c) {
+        const long long at = (long long)image * p.channels + c;
+#pragma unroll
+        for (int i = 0; i < UNIT; i++) {
+            w.v[i] = 1.0f;
+            b.v[i] = mod.v[i] = shift.v[i] = 0.0f;
+        }
+        if (p.w) w = get<UNIT>(p.w + c);
+        if (p.b) b = get<UNIT>(p.b + c);
+        if (p.mod) mod = get<UNIT>(p.mod + at);
+        if (p.shift) shift = get<UNIT>(p.shift + at);
+    }
+    __device__ __forceinline__ void make(float scale, float *slope, float *lift) const {
+#pragma unroll
+        for (int i = 0; i < UNIT; i++) {
+            const float more = 1.0f + mod.v[i];
+            slope[i] = scale * w.v[i] * more;
+            lift[i] = b.v[i] * more + shift.v[i];
+        }
+    }
+};
 
 // Mean and squared differences of n more numbers taken into those of `count`.
 __device__ __forceinline__ void join(double &count, float &mean, float &squares, double n, float mean_n, float squares_n) {
@@ -144,10 +163,18 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
         float *Y = p.Y + (ROWS ? (long long)image * p.pixels * p.ldy + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float mean = 0.0f, squares = 0.0f;
         double seen = 0.0;
+        Coefficients<1> own;
+        auto ask = [&](int c) {
+            if (WHAT != SUMS && c < p.per) own.ask(p, image, c0 + c);
+        };
+        ask(threadIdx.x);
         auto prepare = [&]() {  // slopes and lifts of the group's channels
             const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
             if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
-            for (int c = threadIdx.x; c < p.per; c += THREADS) coefficients(p, image, c0 + c, scale, slopes[c], lifts[c]);
+            for (int c = threadIdx.x; c < p.per; c += THREADS) {
+                own.make(scale, slopes + c, lifts + c);
+                ask(c + THREADS);
+            }
             __syncthreads();
         };
         for (long long at = first; at < last; at += TILE) {
@@ -275,11 +302,10 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
         };
         float mean = 0.0f, squares = 0.0f, slope[UNIT], lift[UNIT];
         double seen = 0.0;
+        Coefficients<UNIT> own;
+        if (WHAT != SUMS && mine) own.ask(p, image, c);
         auto prepare = [&]() {
-            const float scale = 1.0f / sqrtf(squares / (float)total + p.eps);
-#pragma unroll
-            for (int i = 0; i < UNIT; i++)
-                if (mine) coefficients(p, image, c + i, scale, slope[i], lift[i]);
+            if (mine) own.make(1.0f / sqrtf(squares / (float)total + p.eps), slope, lift);
         };
         for (long long at = first; at < last; at += (long long)rows_at_once * NV) {
             const long long step_x = rows_at_once * p.ldx, step_y = rows_at_once * p.ldy;
