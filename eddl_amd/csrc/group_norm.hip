@@ -122,19 +122,35 @@ __device__ __forceinline__ void join(double &count, float &mean, float &squares,
     squares += squares_n + delta * delta * (float)count * share;
     count += n;
 }
+constexpr int MOST_PARTS = 256;  // of a group
+
 // Those of all parts of a group of `total` numbers, parts of `part` each, by a wavefront; in all of its lanes.
-__device__ __forceinline__ void join_parts(const float2 *parts, int split, long long part, long long total, float &mean, float &squares) {
-    const int lane = threadIdx.x & 63;
-    float sum = 0.0f;
-    for (int k = lane; k < split; k += 64) sum += parts[k].x * ((float)min(part, total - k * part) / (float)total);
-    mean = wave_sum(sum);
-    sum = 0.0f;
-    for (int k = lane; k < split; k += 64) {
-        const float2 v = parts[k];
-        sum += v.y + (v.x - mean) * (v.x - mean) * (float)min(part, total - k * part);
+struct Parts {
+    float2 v[MOST_PARTS / 64];
+
+    __device__ __forceinline__ void ask(const float2 *parts, int split) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < MOST_PARTS / 64; k++) {
+            v[k] = float2{0.0f, 0.0f};
+            if (lane + k * 64 < split) v[k] = parts[lane + k * 64];
+        }
     }
-    squares = wave_sum(sum);
-}
+    __device__ __forceinline__ void join(int split, long long part, long long total, float &mean, float &squares) const {
+        const int lane = threadIdx.x & 63;
+        float sum = 0.0f, n[MOST_PARTS / 64];
+#pragma unroll
+        for (int k = 0; k < MOST_PARTS / 64; k++) {
+            n[k] = lane + k * 64 < split ? (float)min(part, total - (lane + k * 64) * part) : 0.0f;
+            sum += v[k].x * (n[k] / (float)total);
+        }
+        mean = wave_sum(sum);
+        sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < MOST_PARTS / 64; k++) sum += v[k].y + (v[k].x - mean) * (v[k].x - mean) * n[k];
+        squares = wave_sum(sum);
+    }
+};
 
 constexpr int SHORT = 16;  // channels of a group in rows: with fewer, 64 bytes of a row are taken together
 
@@ -168,6 +184,8 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
             if (WHAT != SUMS && c < p.per) own.ask(p, image, c0 + c);
         };
         ask(threadIdx.x);
+        Parts parts;  // (what comes back first is asked for first)
+        if (WHAT == APPLY) parts.ask(p.parts + (long long)which * (int)p.split, (int)p.split);
         auto prepare = [&]() {  // slopes and lifts of the group's channels
             const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
             if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
@@ -207,7 +225,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 }
             }
             if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
-                join_parts(p.parts + (long long)which * (int)p.split, (int)p.split, p.part, count, mean, squares);
+                parts.join((int)p.split, p.part, count, mean, squares);
                 prepare();
             }
             if (WHAT != APPLY) {
@@ -304,6 +322,9 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
         double seen = 0.0;
         Coefficients<UNIT> own;
         if (WHAT != SUMS && mine) own.ask(p, image, c);
+        const float2 *all_parts = p.parts + ((long long)image * (int)p.groups + g0) * (int)p.split;
+        Parts parts;  // (what comes back first is asked for first)
+        if (WHAT == APPLY && ONE) parts.ask(all_parts, (int)p.split);
         auto prepare = [&]() {
             if (mine) own.make(1.0f / sqrtf(squares / (float)total + p.eps), slope, lift);
         };
@@ -324,13 +345,13 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                 asm volatile("" : "+v"(x));  // (one place that goes on: all of them at once take two registers each)
             }
             if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
-                const float2 *parts = p.parts + ((long long)image * (int)p.groups + g0) * (int)p.split;
                 if constexpr (ONE) {
-                    join_parts(parts, (int)p.split, p.part * p.per, total, mean, squares);
+                    parts.join((int)p.split, p.part * p.per, total, mean, squares);
                 } else {
                     __syncthreads();
                     for (int j = wave; j < here; j += THREADS / 64) {
-                        join_parts(parts + j * (int)p.split, (int)p.split, p.part * p.per, total, mean, squares);
+                        parts.ask(all_parts + j * (int)p.split, (int)p.split);
+                        parts.join((int)p.split, p.part * p.per, total, mean, squares);
                         if (lane == 0) {
                             red[j] = mean;
                             stat[j] = squares;
@@ -406,7 +427,7 @@ int launch_divided(int dev, GroupNormParams &p, Kernel sums, Kernel apply, long 
     return launch(dev, p, apply, 256, groups, lds);
 }
 
-constexpr int MOST_PARTS = 256, WORKGROUPS = 4096;  // parts of a group; workgroups after which groups are not divided further
+constexpr int WORKGROUPS = 4096;  // after which groups are not divided further
 
 // The kernels of a group of `count` numbers: the smallest workgroup that holds it in registers, up to 32 numbers a thread.
 struct Size {
