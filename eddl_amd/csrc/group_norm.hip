@@ -446,7 +446,7 @@ int launch_groups(int dev, GroupNormParams &p) {
     p.part = count;
     for (const Size &s : sizes)
         if (count <= (long long)s.threads * s.numbers) return launch(dev, p, s.fn, s.threads, groups, lds);
-    constexpr int TILE = 256 * 32;
+    constexpr int TILE = 256 * 16;  // parts of half of what a workgroup's registers hold (maps of 2 x 256 x 64 x 64, 32 channels a group: 13.0 -> 12.1 us; of a quarter 1 x 64 x 256 x 256 15 -> 17)
     const long long tiles = (count + TILE - 1) / TILE, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
     p.part = (tiles + parts - 1) / parts * TILE;
     p.split = (unsigned)((count + p.part - 1) / p.part);
@@ -468,7 +468,7 @@ int launch_rows(int dev, GroupNormParams &p) {
     p.part = p.pixels;
     for (const Size &s : sizes)
         if (p.pixels <= (long long)(s.threads / wide) * (s.numbers / UNIT)) return launch(dev, p, s.fn, s.threads, groups, 0);
-    const int tile = 256 / wide * NV;  // rows
+    const int tile = 256 / wide * NV / 2;  // rows: parts of half of what a workgroup's registers hold (1 and 4 x 4096 x 640, 20 channels a group: 15.6 -> 14.3 us and 32 -> 29)
     const long long tiles = (p.pixels + tile - 1) / tile, parts = std::max(1LL, std::min<long long>({tiles, MOST_PARTS, WORKGROUPS / groups}));
     p.part = (tiles + parts - 1) / parts * tile;
     p.split = (unsigned)((p.pixels + p.part - 1) / p.part);
