@@ -8,8 +8,8 @@
 // joins them and reads the numbers again, from the last one to the first: what was read last may still be in the last-level cache.  The variance is that of differences
 // from a mean, never a difference of squares.
 //
-// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 19.6 us (3.9 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 129 us (41 of
-// sums at 6.6 TB/s, 81 of outputs); rows of 3 x 1369 x 330, groups of 41070, 10.9 us, two launches of 4.1 and 6.8; 1 x 512 x 7 x 7 5.3 us, the host's call.
+// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.4 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 128 us (41 of
+// sums and 82 of outputs, both 6.5 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.8 us, two launches of 4.3 and 6.8; 1 x 512 x 7 x 7 4.8 us, the host's call.
 #include <math.h>
 
 #include <algorithm>

@@ -9,7 +9,7 @@
 // Bound: memory where the tokens are few (a single token reads and writes its channel's state: 128 sequences of 4096 channels of 16 states 15 us, 4.5 TB/s).  Along
 // many tokens 16 bytes of memory stand beside n exponentials and four more instructions a state: with 16 states the vector instructions bind (cycles of a SIMD
 // an instruction, measured: exponential 8.3; other fp32 ones 2.5 to 3 with eight wavefronts of a SIMD, 3 to 4 with four; 4.8 with a DPP operand).  64 sequences of 196 tokens of 768
-// channels: 53 us (2.9 TB/s); a vector instruction is at work in 71 % of the cycles, 22 of 35 of them for the states, the others for softplus, silu and places in LDS.
+// channels: 53 us (2.9 TB/s); a vector instruction is at work in 70 % of the cycles, 22 of 35 of them for the states, the others for softplus, silu and places in LDS.
 // Rounding: fp32 throughout; 1e-7 of the outputs against 64 bits (2-norm), where the products of a long run take the rounding of one exponential instead of hundreds.
 #include <algorithm>
 
