@@ -1,7 +1,7 @@
 // The short causal convolution of every channel along the tokens of a ragged batch of sequences, whose last inputs lie in slots of a pool:
 //     Y[t][c] = act(bias[c] + sum_k W[c][k] x[t - width + 1 + k][c]).
 // Bound: memory, 8 bytes a number.  A thread keeps its channels' weights and walks along the tokens, so that an input is read from memory once and the width - 1 rows
-// that two threads share come from the L2.  Eight ragged sequences of up to 2048 tokens of 2048 channels: 21.5 us for 86 MB, 4.0 TB/s; 32 single tokens 4.3 us in
+// that two threads share come from the L2.  Eight ragged sequences of up to 2048 tokens of 2048 channels: 21.5 us for 86 MB, 4.0 TB/s; 32 single tokens 4.6 us in
 // the kernel, a chain of the batch's numbers, weights and states.
 #include <algorithm>
 
