@@ -1,7 +1,7 @@
 // The short causal convolution of every channel along the tokens of a ragged batch of sequences, whose last inputs lie in slots of a pool:
 //     Y[t][c] = act(bias[c] + sum_k W[c][k] x[t - width + 1 + k][c]).
 // Bound: memory, 8 bytes a number.  A thread keeps its channels' weights and walks along the tokens, so that an input is read from memory once and the width - 1 rows
-// that two threads share come from the L2.  Eight ragged sequences of up to 2048 tokens of 2048 channels: 21.5 us for 86 MB, 4.0 TB/s; 32 single tokens 4.6 us in
+// that two threads share come from the L2.  Eight ragged sequences of up to 2048 tokens of 2048 channels: 20 us for 86 MB, 4.3 TB/s; 32 single tokens 4.6 us in
 // the kernel, a chain of the batch's numbers, weights and states.
 #include <algorithm>
 
@@ -115,7 +115,7 @@ template <int WIDTH>
 __global__ __launch_bounds__(256) void causal_conv_kernel(const ConvParams p) {
     // (neighbours in time share width - 1 rows)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
-        const long long job = xcd_job(id);
+        const long long job = xcd_job<true>(id);
         if (job >= p.jobs) continue;
         const unsigned chunk = (unsigned)job % p.chunks, rest = (unsigned)job / p.chunks;  // (fewer than 2^31 jobs)
         const Sequence q = sequence(p.batch, rest / p.blocks);
@@ -167,8 +167,10 @@ extern "C" int eddlhip_causal_conv(int dev, const float *X, long long ldx, const
     static const kernel kernels[MOST_WIDTH - 1] = {causal_conv_kernel<2>, causal_conv_kernel<3>, causal_conv_kernel<4>, causal_conv_kernel<5>,
                                                    causal_conv_kernel<6>, causal_conv_kernel<7>, causal_conv_kernel<8>};
     p.blocks = ((channels / 4 + 63) / 64 * 64 + channels % 4 + 255) / 256;
-    // (jobs that a 31-bit number counts: a thread walks the chunks beyond)
-    p.chunks = (unsigned)std::min<long long>((std::max(1, std::min(max_new, rows)) + CONV_TOKENS - 1) / CONV_TOKENS, ((1LL << 31) - 1) / ((long long)p.blocks * seqs));
+    // Chunks of the longest sequence that the host allows, as far as the rows are worth it: a thread walks the chunks beyond, and workgroups without tokens cost time too
+    // (2048 sequences of 3 tokens of 1024 channels, 8192 allowed: all chunks 1325 us, so 57).
+    const long long each = (long long)p.blocks * seqs, chunks = (std::max(1, std::min(max_new, rows)) + CONV_TOKENS - 1) / CONV_TOKENS;
+    p.chunks = (unsigned)std::min(chunks, std::max(1LL, std::max(32768LL, (long long)rows * p.blocks) / each));
     p.jobs = (long long)p.blocks * p.chunks * seqs;
     hipLaunchKernelGGL(kernels[width - 2], dim3(xcd_grid(p.jobs, 256)), dim3(256), 0, state(dev).stream, p);
     EH_CHECK_LAUNCH();

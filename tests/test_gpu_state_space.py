@@ -690,3 +690,37 @@ def test_a_larger_call_outgrows_a_recorded_one(hip):
     hip.fill_(Y, 0.0)
     graph.launch()
     assert np.array_equal(Y.numpy(), want)
+
+
+@pytest.mark.parametrize("most", [1, 9, 1 << 20])
+def test_as_many_sequences_as_there_may_be(hip, most):
+    """65535 sequences of no to three tokens, whatever bound the host gives; a last one of 400."""
+    from eddl_amd.state_space import StateBatch
+    rng = np.random.default_rng(41)
+    seqs, channels, n = 65535, 5, 3
+    news = rng.integers(0, 4, seqs)
+    news[-1] = 400
+    offsets = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    rows = int(offsets[-1])
+    r = lambda *s: rng.standard_normal(s, dtype=np.float32)
+    x, dt, A, B, C, w = r(rows, channels), np.exp(0.3 * r(rows, channels) - 1), -np.exp(r(channels, n)), r(rows, n), r(rows, n), r(channels, 4)
+    token = np.arange(rows) - np.repeat(offsets[:-1], news)
+    X, Y, batch = hip.array(x), hip.full((rows, channels), -7.0), StateBatch(hip.array(offsets, "int32"), most)
+    hip.causal_conv(X, hip.array(w), None, Y, batch)
+    want, size = np.zeros((rows, channels)), np.zeros((rows, channels))
+    for back in range(4):
+        there = np.flatnonzero(token >= back)
+        product = x[there - back].astype(np.float64) * w[:, 3 - back]
+        want[there] += product
+        size[there] += np.abs(product)
+    _check(Y.numpy(), want, 8 * EPS * size)
+    hip.fill_(Y, -7.0)
+    d = lambda t: hip.array(t)
+    hip.selective_scan(X, d(dt), d(A), d(B), d(C), Y, batch, softplus=False)
+    y = Y.numpy()
+    for length in (1, 2, 3, 400):
+        for s in np.flatnonzero(news == length)[::500]:
+            rows_of = slice(int(offsets[s]), int(offsets[s + 1]))
+            want, err = selective_scan(x[rows_of], dt[rows_of], A, B[rows_of], C[rows_of], [0, length], softplus=False)[:2]
+            _check(y[rows_of], want, err, (length, s))
+    assert np.all(np.isfinite(y)) and not np.any(y == -7.0)
