@@ -11,6 +11,8 @@
 // an instruction, measured: exponential 8.3; other fp32 ones 2.5 to 3 with eight wavefronts of a SIMD, 3 to 4 with four; 4.8 with a DPP operand).  64 sequences of 196 tokens of 768
 // channels: 53 us (2.9 TB/s); a vector instruction is at work in 70 % of the cycles, 22 of 35 of them for the states, the others for softplus, silu and places in LDS.
 // Rounding: fp32 throughout; 1e-7 of the outputs against 64 bits (2-norm), where the products of a long run take the rounding of one exponential instead of hundreds.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "common.h"
@@ -32,6 +34,8 @@ struct ScanParams {
     int channels, n, per;  // channels that share B and C
     unsigned blocks, group_blocks, parts;
     long long jobs;
+    const int *list;  // tiles: the sequences that are meant (-1: none), or NULL: all of up to `most` new tokens
+    int most;
     bool softplus;
     StateBatch batch;
 };
@@ -160,6 +164,29 @@ __device__ __forceinline__ void in_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// The sequences of `least` new tokens or more, one after another, and -1 behind them, `count` numbers in all.
+constexpr int LIST_THREADS = 1024;
+__global__ __launch_bounds__(LIST_THREADS) void list_sequences_kernel(const StateBatch batch, int seqs, int least, int *list, int count) {
+    __shared__ int found[LIST_THREADS / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0;
+    for (int first = 0; first < seqs; first += LIST_THREADS) {
+        const int s = first + (int)threadIdx.x;
+        const bool is = s < seqs && sequence_rows(batch.offsets[s], batch.offsets[s + 1], batch.rows).fresh >= least;
+        const unsigned long long all = __ballot(is);
+        __syncthreads();
+        if (lane == 0) found[wave] = __popcll(all);
+        __syncthreads();
+        int at = before + __popcll(all & ((1ull << lane) - 1));
+        for (int w = 0; w < LIST_THREADS / 64; w++) {
+            if (w < wave) at += found[w];
+            before += found[w];
+        }
+        if (is && at < count) list[at] = s;
+    }
+    for (int k = before + (int)threadIdx.x; k < count; k += LIST_THREADS) list[k] = -1;
+}
+
 // PART 0: the whole scan of a sequence.  A long one that would leave the device empty is divided over workgroups, and a workgroup's part over its wavefronts, which
 // walk their pieces on their own: PART 1 brings the state of every piece and part from zeros and the factor of what comes before it, PART 2 takes in what lies
 // before its own and brings the outputs.
@@ -185,10 +212,12 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
         const long long job = xcd_job(id);
         if (job >= p.jobs) continue;
         const unsigned rest = (unsigned)job / p.blocks;  // (fewer than 2^31 jobs)
-        const int block = (unsigned)job % p.blocks, group = block / p.group_blocks, part = rest % p.parts, s = rest / p.parts;
+        const int block = (unsigned)job % p.blocks, group = block / p.group_blocks, part = rest % p.parts, place = rest / p.parts;
+        const int s = p.list ? p.list[place] : place;
+        if (s < 0) continue;
         const Sequence q = sequence(p.batch, s);
         const int tiles = (int)(((long long)q.fresh + T::TOKENS - 1) / T::TOKENS), share = (tiles + (int)p.parts * PIECES - 1) / ((int)p.parts * PIECES);  // (of a piece)
-        if (part * PIECES * share >= tiles) continue;
+        if (part * PIECES * share >= tiles || q.fresh > p.most) continue;
 
         const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave % WT, wc = PART ? 0 : wave / WT, set = wc * 64 + lane;
         const int tile0 = PART ? min(tiles, (part * PIECES + wave) * share) : 0, tile1 = PART ? min(tiles, tile0 + share) : tiles;
@@ -304,7 +333,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
         // Workspace of a sequence: the state that it continues, the states of its parts, those of its pieces; the factors of both.
         const long long step = (long long)p.channels * T::NP, at0 = (long long)c * T::NP + n0;
         const int all = (int)p.parts * (PIECES + 1);
-        float *states = PART ? p.part_states + (long long)s * (all + 1) * step + at0 : nullptr, *factors = PART ? p.part_factors + (long long)s * all * step + at0 : nullptr;
+        float *states = PART ? p.part_states + (long long)place * (all + 1) * step + at0 : nullptr, *factors = PART ? p.part_factors + (long long)place * all * step + at0 : nullptr;
         auto take_in = [&](vec &f, vec &b, int which) {  // a part or piece behind what f and b hold
             const vec pf = *reinterpret_cast<const vec *>(factors + which * step), pb = *reinterpret_cast<const vec *>(states + (which + 1) * step);
 #pragma unroll
@@ -549,8 +578,10 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
 constexpr int MOST_STATES = 64;
 constexpr int FEW_TOKENS = 3;  // up to here token after token from memory (32 sequences of 2 tokens of 2048 channels 8.8 us, as tiles 10.9; of 8 19.0 and 12.1)
 
+constexpr int MIXED_TOKENS = 128;  // of the longest sequence, from which on long and short sequences are taken apart
+
 template <int LANES, int NL>
-int launch_scan(int dev, ScanParams &p, int seqs, int tokens) {
+int launch_scan(int dev, ScanParams &p, int seqs, int rows, int tokens) {
     const hipStream_t st = state(dev).stream;
     if (tokens <= FEW_TOKENS) {
         hipLaunchKernelGGL((p.n % NL == 0 ? scan_tokens_kernel<LANES, NL, true> : scan_tokens_kernel<LANES, NL, false>), dim3((unsigned)(((long long)p.channels * LANES + 255) / 256), seqs), dim3(256), 0, st, p);
@@ -559,20 +590,12 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens) {
     }
     const int groups = p.channels / p.per;
     const long long num_cu = state(dev).num_cu;
-    auto launch = [&](auto fn, int threads) {
-        p.jobs = (long long)p.blocks * p.parts * seqs;
+    auto launch = [&](auto fn, int threads, long long count) {
+        p.jobs = (long long)p.blocks * p.parts * (p.list ? count : seqs);
         EH_REQUIRE(p.jobs < (1LL << 31), "selective_scan: %d sequences of %d channels in %d groups are out of range", seqs, p.channels, groups);
         hipLaunchKernelGGL(fn, dim3(xcd_grid(p.jobs, threads)), dim3(threads), 0, st, p);
         EH_CHECK_LAUNCH();
         return 0;
-    };
-    // (workgroups of a call without parts)
-    auto sized = [&](auto tile) {
-        using T = decltype(tile);
-        p.parts = 1;
-        p.group_blocks = (p.per + T::CHANNELS - 1) / T::CHANNELS;
-        p.blocks = groups * p.group_blocks;
-        return (long long)p.blocks * seqs;
     };
     // By the workgroups that there are, in multiples of the compute units: four wavefronts of different channels do the least work a token; where that leaves
     // the device half empty, they divide the tokens of a quarter of the channels (512 tokens of 2048 channels, us: 16 sequences 107 against 128, 12 105 and 95, 4 84 and
@@ -581,23 +604,47 @@ int launch_scan(int dev, ScanParams &p, int seqs, int tokens) {
     using Alone = ScanTile<LANES, NL, 4, 1>;
     using Four = ScanTile<LANES, NL, 4, 4>;
     using Eight = ScanTile<LANES, NL, 8, 8>;
-    if (sized(Alone()) >= 2 * num_cu || tokens <= Alone::TOKENS)
-        return launch(scan_tile_kernel<LANES, NL, 4, 1, 0>, Alone::THREADS);
-    const long long workgroups = sized(Four());  // (as many as of eight wavefronts, which have as many channels)
-    if (2 * workgroups >= 3 * num_cu) return launch(scan_tile_kernel<LANES, NL, 4, 4, 0>, Four::THREADS);
-    const long long parts = num_cu / workgroups, tiles = (tokens + Eight::TOKENS - 1) / Eight::TOKENS;
-    if (parts < 2 || tiles < 4)
-        return launch(scan_tile_kernel<LANES, NL, 8, 8, 0>, Eight::THREADS);
-    // Eight wavefronts a part; two parts a unit where they are long (a workgroup and two a unit, us: 65536 tokens of 256 channels 164 and 140, 4096 of 1024 49 and 45,
-    // 1000 of 1024 20.5 and 21.8).
-    p.parts = (unsigned)(tiles >= 8 * parts ? 2 * parts : std::min(parts, tiles));
-    const size_t each = (size_t)p.channels * Eight::NP * sizeof(float) * seqs, all = (size_t)p.parts * 9;  // (parts and their pieces)
-    void *ws = nullptr;
-    EH_TRY(get_workspace(dev, each * (2 * all + 1), &ws));
-    p.part_states = (float *)ws;
-    p.part_factors = (float *)((char *)ws + each * (all + 1));
-    EH_TRY(launch(scan_tile_kernel<LANES, NL, 8, 1, 1>, Eight::THREADS));
-    return launch(scan_tile_kernel<LANES, NL, 8, 1, 2>, Eight::THREADS);
+    auto blocks = [&](auto tile) { return (p.per + decltype(tile)::CHANNELS - 1) / decltype(tile)::CHANNELS; };  // of a group
+    const long long wide = (long long)groups * blocks(Alone()), narrow = (long long)groups * blocks(Four());     // workgroups a sequence (eight wavefronts have as many channels as four)
+    auto wavefronts = [&](long long seqs, int tokens) { return wide * seqs >= 2 * num_cu || tokens <= Alone::TOKENS ? 1 : 2 * narrow * seqs >= 3 * num_cu ? 4 : 8; };
+    // The sequences of least to most tokens, `count` of them at most, of up to `tokens`; least 0: all up to most.
+    auto run = [&](long long count, int tokens, int least, int most) {
+        const int kind = wavefronts(count, tokens);
+        p.group_blocks = kind == 1 ? blocks(Alone()) : blocks(Four());
+        p.blocks = groups * p.group_blocks;
+        const long long parts = num_cu / (narrow * count), tiles = (tokens + Eight::TOKENS - 1) / Eight::TOKENS;
+        const bool divided = kind == 8 && parts >= 2 && tiles >= 4;
+        // Eight wavefronts a part; two parts a unit where they are long (a workgroup and two a unit, us: 65536 tokens of 256 channels 164 and 140, 4096 of 1024 49 and 45,
+        // 1000 of 1024 20.5 and 21.8).
+        p.parts = (unsigned)(!divided ? 1 : tiles >= 8 * parts ? 2 * parts : std::min(parts, tiles));
+        const size_t all = (size_t)p.parts * 9, each = (size_t)p.channels * Eight::NP * sizeof(float) * count;  // (parts and their pieces)
+        const size_t part_bytes = divided ? each * (2 * all + 1) : 0, list_bytes = least > 0 ? (size_t)count * sizeof(int) : 0;
+        void *ws = nullptr;
+        if (part_bytes + list_bytes > 0) EH_TRY(get_workspace(dev, part_bytes + list_bytes, &ws));
+        p.part_states = (float *)ws;
+        p.part_factors = (float *)((char *)ws + each * (all + 1));
+        p.most = most;
+        p.list = nullptr;
+        if (least > 0) {
+            int *list = (int *)((char *)ws + part_bytes);
+            hipLaunchKernelGGL(list_sequences_kernel, dim3(1), dim3(LIST_THREADS), 0, st, p.batch, seqs, least, list, (int)count);
+            EH_CHECK_LAUNCH();
+            p.list = list;
+        }
+        if (kind == 1) return launch(scan_tile_kernel<LANES, NL, 4, 1, 0>, Alone::THREADS, count);
+        if (kind == 4) return launch(scan_tile_kernel<LANES, NL, 4, 4, 0>, Four::THREADS, count);
+        if (!divided) return launch(scan_tile_kernel<LANES, NL, 8, 8, 0>, Eight::THREADS, count);
+        EH_TRY(launch(scan_tile_kernel<LANES, NL, 8, 1, 1>, Eight::THREADS, count));
+        return launch(scan_tile_kernel<LANES, NL, 8, 1, 2>, Eight::THREADS, count);
+    };
+    // A few long sequences among many short ones would be walked as if there were many long ones.  Of more than half the longest's tokens there are no more than the rows
+    // hold: where they are few, and would be walked by more wavefronts, they are taken by themselves (31
+    // single tokens and a prompt of 2048 of 2048 channels 255 us, so 61; 255 of 3 tokens and one of 8192 of 1024 channels 998 and 110; 60 of 20 and 4 of 500 of 768 71 and 37).
+    const int half = tokens / 2;
+    const long long few = std::max(1, std::min(seqs, rows / (half + 1)));
+    const bool mixed = tokens >= MIXED_TOKENS && 4 * few <= seqs && wavefronts(few, tokens) != wavefronts(seqs, tokens);
+    if (mixed) EH_TRY(run(seqs, half, 0, half));
+    return mixed ? run(few, tokens, half + 1, INT_MAX) : run(seqs, tokens, 0, INT_MAX);
 }
 
 }  // namespace
@@ -655,10 +702,10 @@ extern "C" int eddlhip_selective_scan(int dev, const float *X, long long ldx, co
     p.softplus = softplus != 0;
     p.batch = StateBatch{offsets, lengths, slots, out_slots, rows, pool, reverse != 0};
     const int tokens = std::max(1, std::min(max_new, rows));
-    if (n == 1) return launch_scan<1, 1>(dev, p, seqs, tokens);
-    if (n <= 4) return launch_scan<1, 4>(dev, p, seqs, tokens);
-    if (n <= 8) return launch_scan<2, 4>(dev, p, seqs, tokens);
-    if (n <= 16) return launch_scan<4, 4>(dev, p, seqs, tokens);
-    if (n <= 32) return launch_scan<8, 4>(dev, p, seqs, tokens);
-    return launch_scan<16, 4>(dev, p, seqs, tokens);
+    if (n == 1) return launch_scan<1, 1>(dev, p, seqs, rows, tokens);
+    if (n <= 4) return launch_scan<1, 4>(dev, p, seqs, rows, tokens);
+    if (n <= 8) return launch_scan<2, 4>(dev, p, seqs, rows, tokens);
+    if (n <= 16) return launch_scan<4, 4>(dev, p, seqs, rows, tokens);
+    if (n <= 32) return launch_scan<8, 4>(dev, p, seqs, rows, tokens);
+    return launch_scan<16, 4>(dev, p, seqs, rows, tokens);
 }

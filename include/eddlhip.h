@@ -612,7 +612,8 @@ int eddlhip_causal_conv(int dev, const float *X, long long ldx, const float *W, 
  * [channels] may be NULL (0), gate too (no factor).  The state is [pool][channels][n].  Y and the states lie on nothing else that is read.
  * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  Factors are multiplied over runs of
  * tokens: where e^(d A), d A summed over tokens one after another, passes the largest number, the state may be infinite or NaN, also one of zeros (it does not where no d A is
- * positive).  Sums and states are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups take. */
+ * positive).  Sums and states are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups
+ * take, and the list of long sequences among many short ones. */
 int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
                            const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,
                            int rows, int channels, int n, int groups, int softplus, int reverse, float *states, int pool,

@@ -724,3 +724,52 @@ def test_as_many_sequences_as_there_may_be(hip, most):
             want, err = selective_scan(x[rows_of], dt[rows_of], A, B[rows_of], C[rows_of], [0, length], softplus=False)[:2]
             _check(y[rows_of], want, err, (length, s))
     assert np.all(np.isfinite(y)) and not np.any(y == -7.0)
+
+
+MIXED = [(1500, 16, [1] * 20 + [300] + [2] * 20), (100, 16, [2] * 200 + [0] * 60 + [2000] + [1] * 100), (40, 40, [3] * 550 + [700, 600] + [0, 1] * 40), (520, 1, [1] * 90 + [129]),
+         (300, 4, [150] + [7] * 150 + [140, 0])]
+
+
+@pytest.mark.parametrize("channels, n, news", MIXED)
+def test_long_sequences_among_short_ones(hip, channels, n, news):
+    """A few long sequences are walked in a launch of their own, whatever the host's bound is and wherever they stand."""
+    rng = np.random.default_rng([channels, n, 2])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, 1)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    for reverse in (False, True):
+        want, err, after, after_err = selective_scan(reverse=reverse, **case, **batch.reference(pool))
+        for most in (None, max(news) // 3, 1 << 20):
+            y, s = _scan(hip, case, batch, pool, reverse, most)
+            _check(y, want, err, (reverse, most))
+            _check(s, after, after_err, (reverse, most, "state"))
+            assert np.all(batch.outside(y) == -7.0)
+
+
+def test_a_recorded_mixed_batch_follows_its_offsets(hip):
+    """The long sequences are looked up when the kernels run: replays after the program moved them, made more of them or none equal the eager calls."""
+    rng = np.random.default_rng(51)
+    channels, n, seqs, most = 600, 16, 64, 400
+    batch = Ragged(rng, [1] * (seqs - 1) + [most], before=0, behind=0, apart=False)
+    case = _scan_case(rng, batch, channels, n, 1)
+    d = lambda t: hip.array(t)
+    X, dt, A, B, C, Y, b = d(case["x"]), d(case["dt"]), d(case["A"]), d(case["B"]), d(case["C"]), hip.empty(case["x"].shape), batch.on(hip, most)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    S = d(pool)
+    step = lambda: hip.selective_scan(X, dt, A, B, C, Y, b, states=S)
+    step()
+    graph = hip.record(step)
+    places = [[(5, 400)], [(0, 210), (63, 190)], [], [(k, 7) for k in range(seqs)]]
+    for long in places:
+        news = np.ones(seqs, int)
+        for k, length in long:
+            news[k] = length
+        b.offsets.copy_from(np.minimum(np.concatenate([[0], np.cumsum(news)]), batch.rows))
+        b.lengths.copy_from(news + 3)
+        got = []
+        for run in (step, graph.launch):
+            S.copy_from(pool)
+            hip.fill_(Y, 0.5)
+            run()
+            got.append((Y.numpy(), S.numpy()))
+        assert all(np.array_equal(e, g) for e, g in zip(*got)), long
