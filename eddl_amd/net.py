@@ -303,10 +303,12 @@ def SelectiveScan(parent, dt, vectors, state, groups=1, gate=None, softplus=True
 # ---------------------------------------------------------------------------- the net
 class Op:
     """One launch group of the built plan.  ``flops``/``bytes`` are the algorithmic figures
-    (convolution: 2*N*K*C*R*S*P*Q and 4*(in + filters + out); bandwidth operators: bytes moved once)."""
+    (convolution: 2*N*K*C*R*S*P*Q and 4*(in + filters + out); bandwidth operators: bytes moved once).
+    ``rehearse``: the same launches without a trace in what the program keeps between runs (``run``, where there is none)."""
 
-    def __init__(self, kind, name, run, flops=0, nbytes=0, layers=()):
+    def __init__(self, kind, name, run, flops=0, nbytes=0, layers=(), rehearse=None):
         self.kind, self.name, self.run, self.flops, self.bytes, self.layers = kind, name, run, flops, nbytes, list(layers)
+        self.rehearse = rehearse or run
 
 
 class Net:
@@ -716,6 +718,7 @@ class Net:
             return
         O = hip.empty(l.out_shape)
         self.out[id(l)] = O
+        rehearse = None
         if k == "batchnorm":
             dp = self.dparams[id(l)]
             C = l.out_shape[1]
@@ -767,21 +770,24 @@ class Net:
             at, dp, batch, channels = l.attrs, self.dparams[id(l)], self._sequences(l), l.out_shape[2]
             two = [t.reshape((l.out_shape[0] * l.out_shape[1], t.shape[2])) for t in ins + [O]]
             if k == "causal_conv":
-                run = lambda: hip.causal_conv(two[0].columns(0, channels), dp["W"], dp.get("bias"), two[1], batch, at["states"], at["activation"], at["reverse"])
+                step = lambda b: hip.causal_conv(two[0].columns(0, channels), dp["W"], dp.get("bias"), two[1], b, at["states"], at["activation"], at["reverse"])
                 nbytes = 8 * n_out
             else:
                 half, wide = at["groups"] * at["state"], two[2].shape[1]
                 gate = two[3].columns(two[3].shape[1] - channels, two[3].shape[1]) if len(ins) == 4 else None
-                run = lambda: hip.selective_scan(two[0], two[1], dp["A"], two[2].columns(wide - 2 * half, wide - half), two[2].columns(wide - half, wide), two[-1], batch,
-                                                 at["states"], dp["skip"], gate, dp["dt_bias"], at["softplus"], at["reverse"])
+                step = lambda b: hip.selective_scan(two[0], two[1], dp["A"], two[2].columns(wide - 2 * half, wide - half), two[2].columns(wide - half, wide), two[-1], b,
+                                                    at["states"], dp["skip"], gate, dp["dt_bias"], at["softplus"], at["reverse"])
                 nbytes = 4 * (len(ins) * n_out + two[0].shape[0] * 2 * half)
+            run = lambda: step(batch)
+            if at["states"] is not None:
+                rehearse = lambda: step(batch.unkept())
         elif k == "pad":
             hip.fill_(O, l.attrs["constant"])  # the border is written once, here; forward copies the interior
             n_in = int(np.prod(l.parents[0].out_shape))
             run, nbytes = (lambda: hip.pad(ins[0], O, l.attrs["pads"])), 8 * n_in
         else:
             msg("layer kind %s has no forward on this backend" % k, "Net::build")
-        self.ops.append(Op(k, l.name, run, 0, nbytes, [l]))
+        self.ops.append(Op(k, l.name, run, 0, nbytes, [l], rehearse))
 
     # ---- run
     def resize(self, batch):
@@ -822,9 +828,11 @@ class Net:
     def capture(self):
         """Records the plan as a graph (one call replays every launch): for plans whose kernels are so short
         that queueing them one at a time takes longer than running them.  Runs the plan once first, so that
-        the library's workspace has its final size.  The graph names this net's tensors: capture again after
-        ``resize``."""
-        self.run()
+        the library's workspace has its final size; states that layers keep between runs stay as they are (a
+        paged cache gets the keys and values of the batch as it stands).  The graph names this net's
+        tensors: capture again after ``resize``."""
+        for op in self.ops:
+            op.rehearse()
         self.graph = self.backend.record(self.run)
         return self.graph
 

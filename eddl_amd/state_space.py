@@ -1,4 +1,5 @@
 """What the state space operators of ``Backend`` take: the batch of sequences whose tokens ``causal_conv`` and ``selective_scan`` mix."""
+import numpy as np
 
 
 class StateBatch:
@@ -18,3 +19,7 @@ class StateBatch:
                              % (offsets.shape, [getattr(t, "shape", None) for t in (lengths, slots, out_slots)]))
         self.offsets, self.lengths, self.slots, self.out_slots, self.max_new = offsets, lengths, slots, out_slots, int(max_new)
         self.arguments = (offsets.address, *(t.address if t is not None else None for t in (lengths, slots, out_slots)), seqs, self.max_new)
+
+    def unkept(self):
+        """The same sequences, whose states go nowhere."""
+        return StateBatch(self.offsets, self.max_new, self.lengths, self.slots, self.slots.backend.array(np.full(self.slots.shape, -1), "int32"))
