@@ -630,7 +630,8 @@ class Backend:
     def group_norm(self, X, Y, groups, weight=None, bias=None, eps=1e-5, activation=None, mod=None, shift=None, image_rows=None):
         """Y = act(n (1 + mod) + shift), n the norm of ``groups`` groups of channels over the pixels of an image, its ``weight`` and ``bias`` [channels].
         ``X``, ``Y``: maps [images, channels, height, width], or rows of tokens [rows, channels], ``image_rows`` rows an image (all, unless
-        given); ``Y`` may be ``X``.  ``activation`` None, "relu" or "silu"; ``mod``, ``shift`` [images, channels] or None."""
+        given); ``Y`` may be ``X``.  ``activation`` None, "relu" (NaN stays), "relu_layer" (as ``Backend.relu``, which makes 0 of it) or "silu"; ``mod``,
+        ``shift`` [images, channels] or None."""
         if len(X.shape) == 4 and len(Y.shape) == 4 and image_rows is None:
             if X.dtype != "float32" or X.shape != Y.shape:
                 raise ValueError("group_norm shapes %s -> %s" % (X.shape, Y.shape))
@@ -646,7 +647,7 @@ class Backend:
             if t is not None and (t.size != size or t.dtype != "float32"):
                 raise ValueError("group_norm: weight, bias, mod or shift %s %s for %d images of %d channels" % (t.dtype, t.shape, images, channels))
         self._check(self.lib.eddlhip_group_norm(self.dev, x, ldx, y, ldy, images, channels, pixels, last, groups, _ptr(weight), _ptr(bias), eps, _ptr(mod), _ptr(shift),
-                                                _activation(activation)))
+                                                _activation(activation, _NORM_ACTIVATIONS)))
 
     def causal_conv(self, X, W, bias, Y, batch, states=None, activation=None, reverse=False):
         """The short convolution of every channel along the tokens of a ragged batch: ``X`` -> ``Y`` [rows, channels], ``W`` [channels, width],
@@ -680,12 +681,13 @@ class Backend:
 
 _NORMS = {None: 0, "layer": 1, "rms": 2}
 _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2}
+_NORM_ACTIVATIONS = dict(_ACTIVATIONS, relu_layer=4)
 
 
-def _activation(name):
-    if name not in _ACTIVATIONS:
-        raise ValueError("no activation %r: None, \"relu\" or \"silu\"" % (name,))
-    return _ACTIVATIONS[name]
+def _activation(name, known=_ACTIVATIONS):
+    if name not in known:
+        raise ValueError("no activation %r: %s" % (name, ", ".join(map(repr, known))))
+    return known[name]
 
 
 def _pool(states, batch, rows, cols, what):

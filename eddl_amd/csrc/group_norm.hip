@@ -495,7 +495,7 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     EH_REQUIRE(images >= 0 && channels > 0 && pixels > 0, "group_norm: %d images of %d channels of %d pixels", images, channels, pixels);
     EH_REQUIRE(groups > 0 && channels % groups == 0 && channels / groups <= MOST_CHANNELS, "group_norm: %d channels in %d groups (of up to %d)", channels, groups, MOST_CHANNELS);
     EH_REQUIRE((long long)images * pixels <= 0x7fffffffLL && (long long)images * channels <= 0x7fffffffLL, "group_norm: %d images of %d channels of %d pixels are out of range", images, channels, pixels);
-    EH_REQUIRE(activation == EDDLHIP_ACT_NONE || activation == EDDLHIP_ACT_RELU || activation == EDDLHIP_ACT_SILU, "group_norm: unknown activation %d", activation);
+    EH_REQUIRE(activation == EDDLHIP_ACT_NONE || activation == EDDLHIP_ACT_RELU || activation == EDDLHIP_ACT_SILU || activation == EDDLHIP_ACT_RELU_LAYER, "group_norm: unknown activation %d", activation);
     EH_REQUIRE(!channels_last || (ldx >= channels && ldy >= channels), "group_norm: rows shorter than %d channels", channels);
     if (images == 0) return 0;
     EH_REQUIRE(X && Y, "group_norm: NULL tensor");

@@ -687,7 +687,7 @@ class Net:
         last, activation = l, at["activation"]
         c = sole_child(l)
         if fuse and activation is None and c is not None and c.kind == "relu":
-            last, activation = c, "relu"
+            last, activation = c, "relu_layer"
             absorbed.add(id(c))
         X, O, dp = self.out[id(l.parents[0])], hip.empty(last.out_shape), self.dparams[id(l)]
         self.out[id(last)] = O

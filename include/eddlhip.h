@@ -572,16 +572,18 @@ int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R
  * What networks need whose blocks mix the tokens of an image or video by a state instead of attention (or beside it), and the group norm that
  * image networks put between their convolutions.  No counterpart in the reference's forward path.  Inference only, fp32.
  *
- * Activations are EDDLHIP_ACT_NONE, _RELU (max(x, 0); NaN stays) or _SILU (x / (1 + e^-x)). */
+ * Activations are EDDLHIP_ACT_NONE, _RELU (max(x, 0); NaN stays) or _SILU (x / (1 + e^-x)); group norms also know _RELU_LAYER, which is eddlhip_relu
+ * bit for bit (a NaN becomes 0): what a plan needs that folds that layer into the norm before it. */
 #define EDDLHIP_ACT_NONE 0
 #define EDDLHIP_ACT_RELU 1
 #define EDDLHIP_ACT_SILU 2
+#define EDDLHIP_ACT_RELU_LAYER 4
 
 /* The norm of groups of channels side by side, over all pixels of an image, and its activation:
  *     n = (x - mean) / sqrt(variance + eps) w + b,   Y = act(n (1 + mod) + shift).
  * channels_last == 0: maps X, Y [images][channels][pixels], ldx and ldy are not looked at.  Otherwise rows of tokens [images * pixels][channels] that lie
  * ldx and ldy floats apart.  Up to 4096 channels a group.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
- * whose group holds an infinity or NaN is NaN in that group; images and groups do not reach one another.  Workspace: means and squared differences of the
+ * whose group holds an infinity or NaN is NaN in that group (0 behind _RELU_LAYER); images and groups do not reach one another.  Workspace: means and squared differences of the
  * parts of a group of more than 32768 numbers. */
 int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last,
                        int groups, const float *w, const float *b, float eps, const float *mod, const float *shift, int activation);

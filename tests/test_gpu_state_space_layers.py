@@ -105,3 +105,25 @@ def test_capture_leaves_the_states(hip, tokens):
     net.input_tensor().copy_from(xs[0])  # and capturing it again, between two steps
     net.capture()
     assert np.array_equal(blocks.P.numpy(), want[-1][1]) and np.array_equal(blocks.S.numpy(), want[-1][2])
+
+
+@pytest.mark.parametrize("maps", [True, False])
+def test_a_relu_behind_a_group_norm_is_the_relu_layer(hip, maps):
+    """A plan that folds a ReLU layer into the norm before it gives that layer's bits, for groups that are NaN too (the layer makes 0 of a NaN); a norm whose own activation is a
+    ReLU leaves NaN as it is."""
+    from eddl_amd import net as L
+    rng = np.random.default_rng(6)
+    shape, at = ([6, 5, 7], (1, 4, 3, 2)) if maps else ([35, 6], (1, 17, 4))
+    x = rng.standard_normal([3] + shape, dtype=np.float32)
+    x[at], x[2][tuple(np.array(at[1:]) // 2)] = np.nan, np.inf
+    outs = []
+    for fuse in (True, False):
+        i = L.Input(shape, 3)
+        net = L.Net([i], [L.ReLu(L.GroupNormalization(i, 3)), L.GroupNormalization(i, 3, activation="relu")]).build(hip, fuse=fuse)
+        assert sum(op.kind == "relu" for op in net.ops) == (0 if fuse else 1)
+        outs.append(net.predict(x))
+    assert not np.any(np.isnan(outs[1][0])) and np.isnan(outs[1][1]).sum() == 2 * 2 * 35
+    for a, b in zip(*outs):
+        assert np.array_equal(a, b, equal_nan=True)
+    fine = ~np.isnan(outs[0][1])
+    assert np.array_equal(outs[0][0][fine], outs[0][1][fine])
