@@ -643,6 +643,7 @@ class Backend:
             if shape != yshape or pixels < 0 or (shape[0] % pixels if pixels else shape[0]):
                 raise ValueError("group_norm: rows %s -> %s in images of %s rows" % (shape, yshape, image_rows))
             images, pixels = (shape[0] // pixels, pixels) if shape[0] else (0, 1)
+        _ints("group_norm", images, channels, pixels, groups)
         for t, size in ((weight, channels), (bias, channels), (mod, images * channels), (shift, images * channels)):
             if t is not None and (t.size != size or t.dtype != "float32"):
                 raise ValueError("group_norm: weight, bias, mod or shift %s %s for %d images of %d channels" % (t.dtype, t.shape, images, channels))
@@ -657,6 +658,7 @@ class Backend:
         if shape != yshape or len(W.shape) != 2 or W.shape[0] != channels or W.dtype != "float32" or bias is not None and (bias.size != channels or bias.dtype != "float32"):
             raise ValueError("causal_conv shapes %s -> %s, weights %s, bias %s" % (shape, yshape, W.shape, getattr(bias, "shape", None)))
         pool, slots = _pool(states, batch, W.shape[1] - 1, channels, "causal_conv")
+        _ints("causal_conv", *shape, W.shape[1], slots)
         self._check(self.lib.eddlhip_causal_conv(self.dev, x, ldx, W.ptr, _ptr(bias), y, ldy, shape[0], channels, W.shape[1], _activation(activation), 1 if reverse else 0,
                                                  pool, slots, *batch.arguments))
 
@@ -674,6 +676,7 @@ class Backend:
         if skip is not None and (skip.size != channels or skip.dtype != "float32") or dt_bias is not None and (dt_bias.size != channels or dt_bias.dtype != "float32"):
             raise ValueError("selective_scan: skip or dt_bias not float32 numbers of %d channels" % channels)
         pool, slots = _pool(states, batch, channels, n, "selective_scan")
+        _ints("selective_scan", *shape, bshape[1], slots)
         self._check(self.lib.eddlhip_selective_scan(self.dev, x, ldx, d, lddt, A.ptr, b, ldb, c, ldc, None if skip is None else skip.ptr, g, ldg,
                                                     None if dt_bias is None else dt_bias.ptr, y, ldy, rows, channels, n, bshape[1] // n, 1 if softplus else 0,
                                                     1 if reverse else 0, pool, slots, *batch.arguments))
@@ -688,6 +691,12 @@ def _activation(name, known=_ACTIVATIONS):
     if name not in known:
         raise ValueError("no activation %r: %s" % (name, ", ".join(map(repr, known))))
     return known[name]
+
+
+def _ints(what, *sizes):
+    """Refuses sizes that the library's ints do not hold: they would arrive as other ones."""
+    if any(not -2 ** 31 <= size < 2 ** 31 for size in sizes):
+        raise ValueError("%s: a size of %s is out of range" % (what, max(sizes, key=abs)))
 
 
 def _pool(states, batch, rows, cols, what):

@@ -14,10 +14,12 @@ class StateBatch:
             out_slots = slots
         seqs = offsets.shape[0] - 1 if len(offsets.shape) == 1 else -1
         kept = [t for t in (lengths, slots, out_slots) if t is not None]
-        if seqs < 0 or len(kept) not in (0, 3) or any(tuple(t.shape) != (seqs,) for t in kept) or any(t.dtype != "int32" for t in (offsets, *kept)):
+        if not 0 <= seqs < 2 ** 31 or len(kept) not in (0, 3) or any(tuple(t.shape) != (seqs,) for t in kept) or any(t.dtype != "int32" for t in (offsets, *kept)):
             raise ValueError("a batch is int32 offsets [sequences + 1] and no or both of lengths and slots [sequences], not %s %s"
                              % (offsets.shape, [getattr(t, "shape", None) for t in (lengths, slots, out_slots)]))
-        self.offsets, self.lengths, self.slots, self.out_slots, self.max_new = offsets, lengths, slots, out_slots, int(max_new)
+        if int(max_new) < 0:
+            raise ValueError("a bound of %d new tokens" % int(max_new))
+        self.offsets, self.lengths, self.slots, self.out_slots, self.max_new = offsets, lengths, slots, out_slots, min(int(max_new), 2 ** 31 - 1)  # (an int of the library)
         self.arguments = (offsets.address, *(t.address if t is not None else None for t in (lengths, slots, out_slots)), seqs, self.max_new)
 
     def unkept(self):
