@@ -26,9 +26,7 @@ __device__ __forceinline__ float softplus(float x) {
 
 // The activations of EDDLHIP_ACT_*.
 __device__ __forceinline__ float activated(float x, int kind) {
-    if (kind == EDDLHIP_ACT_SILU) return silu(x);
-    if (kind == EDDLHIP_ACT_RELU) return x > 0.0f || x != x ? x : 0.0f;
-    return kind == EDDLHIP_ACT_RELU_LAYER && !(x > 0.0f) ? 0.0f : x;
+    return kind == EDDLHIP_ACT_SILU ? silu(x) : kind == EDDLHIP_ACT_RELU ? (x > 0.0f || x != x ? x : 0.0f) : x;
 }
 
 }  // namespace eddlhip

@@ -38,8 +38,14 @@ struct GroupNormParams {
     long long jobs;       // of the launch
     int together;         // groups of a workgroup (short rows)
     bool lines;           // a workgroup writes whole lines of memory
-    float eps;
+    float eps, of_nan;    // what a ReLU makes of NaN
 };
+
+// A ReLU that keeps NaN and one that does not differ in a number, not in a branch (which every number would take: 17.3 -> 18.1 us, 6.0 -> 6.4).
+__device__ __forceinline__ float activated(float x, const GroupNormParams &p) {
+    if (p.activation == EDDLHIP_ACT_SILU) return silu(x);
+    return p.activation == EDDLHIP_ACT_RELU ? (x != x ? p.of_nan : x > 0.0f ? x : 0.0f) : x;
+}
 
 __device__ __forceinline__ float wave_sum(float x) {
 #pragma unroll
@@ -271,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                                 slope = slopes[c];
                                 lift = lifts[c];
                             }
-                            v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope, lift), p.activation);
+                            v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope, lift), p);
                         }
                         set<UNIT>(ROWS ? Y + hi * p.ldy + lo : y + k * STEP, v[k], p.lines);
                     }
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                 for (int k = 0; k < NV; k++) {
                     if (k * rows_at_once < left) {
 #pragma unroll
-                        for (int i = 0; i < UNIT; i++) v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope[i], lift[i]), p.activation);
+                        for (int i = 0; i < UNIT; i++) v[k].v[i] = activated(__builtin_fmaf(v[k].v[i] - mean, slope[i], lift[i]), p);
                         set<UNIT>(y, v[k], p.lines);
                     }
                     y += step_y;
@@ -522,7 +528,8 @@ extern "C" int eddlhip_group_norm(int dev, const float *X, long long ldx, float 
     p.channels = channels;
     p.pixels = pixels;
     p.groups = groups;
-    p.activation = activation;
+    p.activation = activation == EDDLHIP_ACT_RELU_LAYER ? EDDLHIP_ACT_RELU : activation;
+    p.of_nan = activation == EDDLHIP_ACT_RELU_LAYER ? 0.0f : NAN;
     p.per = channels / groups;
     p.parts = nullptr;
     p.together = 1;
