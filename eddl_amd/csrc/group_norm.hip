@@ -47,21 +47,46 @@ __device__ __forceinline__ float activated(float x, const GroupNormParams &p) {
     return p.activation == EDDLHIP_ACT_RELU ? (x != x ? p.of_nan : x > 0.0f ? x : 0.0f) : x;
 }
 
-__device__ __forceinline__ float wave_sum(float x) {
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) x += __shfl_xor(x, step);
-    return x;
+// The sum over a wavefront, in all lanes: across the 16 lanes of a row by operands of other lanes, the four rows one after another.
+template <int CTRL>
+__device__ __forceinline__ float swapped(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
-template <int THREADS>
-__device__ __forceinline__ float block_sum(float x, float *red) {
+__device__ __forceinline__ float wave_sum(float x) {
+    x += swapped<0xB1>(x);   // the neighbour
+    x += swapped<0x4E>(x);   // the other pair of four
+    x += swapped<0x141>(x);  // the other four of eight, mirrored
+    x += swapped<0x140>(x);  // the other eight of sixteen, mirrored
+    float row[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++) row[r] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 16 * r));
+    return (row[0] + row[1]) + (row[2] + row[3]);
+}
+__device__ __forceinline__ float2 wave_sum(float2 x) { return float2{wave_sum(x.x), wave_sum(x.y)}; }
+__device__ __forceinline__ void add(float &x, float y) { x += y; }
+__device__ __forceinline__ void add(float2 &x, float2 y) {
+    x.x += y.x;
+    x.y += y.y;
+}
+template <int THREADS, typename T>
+__device__ __forceinline__ T block_sum(T x, float2 *place) {
+    T *red = reinterpret_cast<T *>(place);
     x = wave_sum(x);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
     __syncthreads();
     x = red[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; w++) x += red[w];
+    for (int w = 1; w < THREADS / 64; w++) add(x, red[w]);
     return x;
+}
+
+// Of n numbers, nth = 1 / n, whose sum gave `mean`: `off` holds the sum of their differences from it and that of the differences' squares.  The first is what the mean lost to rounding, so
+// that equal numbers have their own value as their mean, and nothing but the bias is left of them (of 1234.567, 32768 times, the mean's last bits made 0.04).
+__device__ __forceinline__ void settle(float &mean, float &squares, float nth, float2 off) {
+    const float more = off.x * nth, left = off.y - more * off.x;
+    mean += more;
+    squares = left < 0.0f ? 0.0f : left;
 }
 
 template <int UNIT>
@@ -144,13 +169,14 @@ struct Parts {
     }
     __device__ __forceinline__ void join(int split, long long part, long long total, float &mean, float &squares) const {
         const int lane = threadIdx.x & 63;
+        const float first = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v[0].x)));  // (differences from it: equal means are the mean)
         float sum = 0.0f, n[MOST_PARTS / 64];
 #pragma unroll
         for (int k = 0; k < MOST_PARTS / 64; k++) {
             n[k] = lane + k * 64 < split ? (float)min(part, total - (lane + k * 64) * part) : 0.0f;
-            sum += v[k].x * (n[k] / (float)total);
+            sum += (v[k].x - first) * (n[k] / (float)total);
         }
-        mean = wave_sum(sum);
+        mean = first + wave_sum(sum);
         sum = 0.0f;
 #pragma unroll
         for (int k = 0; k < MOST_PARTS / 64; k++) sum += v[k].y + (v[k].x - mean) * (v[k].x - mean) * n[k];
@@ -165,7 +191,7 @@ constexpr int MOST_CHANNELS = 4096;  // of a group: their slopes and lifts lie i
 // A workgroup a group of an image or a part of one.  UNIT numbers are read at a time; ROWS: the numbers are counted along the group's pieces of the rows.
 template <int THREADS, int NV, int UNIT, bool ROWS, int WHAT>
 __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormParams p) {
-    __shared__ float red[THREADS / 64];
+    __shared__ float2 red[THREADS / 64];
     extern __shared__ float slopes[];  // of the group's channels, and their lifts
     float *lifts = slopes + p.per;
     constexpr int STEP = THREADS * UNIT, TILE = STEP * NV;
@@ -241,18 +267,20 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                     else if constexpr (UNIT == 2) sum += v[k].v[0] + v[k].v[1];
                     else sum += v[k].v[0];
                 }
-                const float n = (float)min((long long)TILE, last - at), mean_n = block_sum<THREADS>(sum, red) / n;
-                float sq = 0.0f;
+                const float n = (float)min((long long)TILE, last - at), nth = 1.0f / n;
+                float mean_n = block_sum<THREADS>(sum, red) * nth, squares_n;
+                float2 off = {0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < NV; k++)
                     if (k * STEP < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) {
                             const float d = v[k].v[i] - mean_n;
-                            sq = __builtin_fmaf(d, d, sq);
+                            off.x += d;
+                            off.y = __builtin_fmaf(d, d, off.y);
                         }
                     }
-                const float squares_n = block_sum<THREADS>(sq, red);
+                settle(mean_n, squares_n, nth, block_sum<THREADS>(off, red));
                 if (WHAT == SUMS) {
                     join(seen, mean, squares, n, mean_n, squares_n);
                 } else {
@@ -294,7 +322,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
 // pieces of a row would be short.
 template <int THREADS, int NV, int UNIT, bool ONE, int WHAT>
 __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNormParams p) {
-    __shared__ float red[ONE ? THREADS / 64 : THREADS], stat[ONE ? 1 : 2 * SHORT];
+    __shared__ float2 red[ONE ? THREADS / 64 : THREADS], stat[ONE ? 1 : 2 * SHORT];
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
         long long job = xcd_job(id);
         if (job >= p.jobs) continue;
@@ -307,21 +335,23 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
         const long long first = piece * p.part, last = min((long long)p.pixels, first + p.part), total = (long long)p.per * p.pixels;
         const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
         // the sums of the groups over all threads; of several groups by the wavefronts in turn
-        auto group_sum = [&](float x) {
+        auto group_sum = [&](auto x) {
+            using T = decltype(x);
             if constexpr (ONE) {
                 return block_sum<THREADS>(x, red);
             } else {
+                T *all = reinterpret_cast<T *>(red), *sums = reinterpret_cast<T *>(stat);
                 __syncthreads();
-                red[threadIdx.x] = x;
+                all[threadIdx.x] = x;
                 __syncthreads();
                 for (int j = wave; j < here; j += THREADS / 64) {
-                    float s = 0.0f;
-                    for (int k = lane; k < rows_at_once * units; k += 64) s += red[k / units * wide + j * units + k % units];
+                    T s = T();
+                    for (int k = lane; k < rows_at_once * units; k += 64) add(s, all[k / units * wide + j * units + k % units]);
                     s = wave_sum(s);
-                    if (lane == 0) stat[j] = s;
+                    if (lane == 0) sums[j] = s;
                 }
                 __syncthreads();
-                return stat[mine ? g : 0];
+                return sums[mine ? g : 0];
             }
         };
         float mean = 0.0f, squares = 0.0f, slope[UNIT], lift[UNIT];
@@ -358,14 +388,11 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                     for (int j = wave; j < here; j += THREADS / 64) {
                         parts.ask(all_parts + j * (int)p.split, (int)p.split);
                         parts.join((int)p.split, p.part * p.per, total, mean, squares);
-                        if (lane == 0) {
-                            red[j] = mean;
-                            stat[j] = squares;
-                        }
+                        if (lane == 0) stat[j] = float2{mean, squares};
                     }
                     __syncthreads();
-                    mean = red[mine ? g : 0];
-                    squares = stat[mine ? g : 0];
+                    mean = stat[mine ? g : 0].x;
+                    squares = stat[mine ? g : 0].y;
                 }
                 prepare();
             }
@@ -377,18 +404,20 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
             }
             if (WHAT != APPLY) {
                 const double n = (double)min((long long)rows_at_once * NV, last - at) * p.per;
-                const float mean_n = group_sum(sum) / (float)n;
-                float sq = 0.0f;
+                const float nth = 1.0f / (float)n;
+                float mean_n = group_sum(sum) * nth, squares_n;
+                float2 off = {0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < NV; k++)
                     if (k * rows_at_once < left) {
 #pragma unroll
                         for (int i = 0; i < UNIT; i++) {
                             const float d = v[k].v[i] - mean_n;
-                            sq = __builtin_fmaf(d, d, sq);
+                            off.x += d;
+                            off.y = __builtin_fmaf(d, d, off.y);
                         }
                     }
-                const float squares_n = group_sum(sq);
+                settle(mean_n, squares_n, nth, group_sum(off));
                 if (WHAT == SUMS) {
                     join(seen, mean, squares, n, mean_n, squares_n);
                 } else {

@@ -75,3 +75,21 @@ def test_every_form_of_the_scan(hip, form, n):
 @pytest.mark.parametrize("kind", [None, "relu", "silu"])
 def test_more_shapes_of_group_norm(hip, images, channels, height, width, groups, kind):
     base.test_group_norm(hip, images, channels, height, width, groups, kind)
+
+
+@pytest.mark.parametrize("channels, pixels, groups", [(8, 100, 4), (6, 49, 6), (64, 1500, 4), (128, 16, 1), (30, 333, 2), (99, 63, 3), (6, 40000, 2), (33, 1300, 1), (24, 12000, 3),
+                                                      (4, 2500, 4), (40, 4000, 40), (2, 60000, 1)])
+def test_constant_groups_are_their_bias(hip, channels, pixels, groups):
+    """A group of equal numbers has their value as its mean, to the bit, whatever the value and however the group is read: what is left is the bias."""
+    rng = np.random.default_rng([channels, pixels])
+    values = np.array([1234.567, -0.1, 3.3e7, 1e4, 7.7e-5, -98765.4], np.float32)
+    per = channels // groups
+    x = np.repeat(np.resize(values, (2, groups))[:, :, None], per * pixels, 2).reshape(2, channels, pixels)
+    b = rng.standard_normal(channels, dtype=np.float32)
+    want = np.broadcast_to(b[None, :, None], x.shape)
+    X = hip.array(x.reshape(2, channels, pixels, 1))
+    hip.group_norm(X, X, groups, bias=hip.array(b))
+    assert np.array_equal(X.numpy().reshape(x.shape), want), "maps"
+    R = hip.array(x.transpose(0, 2, 1).reshape(-1, channels))
+    hip.group_norm(R, R, groups, bias=hip.array(b), image_rows=pixels)
+    assert np.array_equal(R.numpy().reshape(2, pixels, channels).transpose(0, 2, 1), want), "rows"
