@@ -29,7 +29,7 @@ typedef float floatx4 __attribute__((ext_vector_type(4)));
 struct ScanParams {
     const float *X, *dt, *gate, *B, *C, *A, *skip, *dt_bias;
     float *Y, *states;
-    float *part_states, *part_factors;  // [sequence][the state that it continues, parts, pieces of them][channel][NP], [sequence][parts, pieces][channel][NP]
+    float *part_states, *part_exponents;  // [sequence][the state that it continues, parts, pieces of them][channel][NP], [sequence][parts, pieces][channel][NP]: half the exponents
     long long ldx, lddt, ldg, ldb, ldc, ldy;
     int channels, n, per;  // channels that share B and C
     unsigned blocks, group_blocks, parts;
@@ -103,6 +103,14 @@ __device__ __forceinline__ void exponents(const ScanParams &p, int c, int n0, fl
         a[i] = a[i] > MOST ? MOST : a[i] < -MOST ? -MOST : a[i];  // (an infinite one would make NaN of the steps of 0 behind the last token)
     }
 }
+
+// A run of tokens is joined to a state by its factor 2^l, which passes the largest number where the run's steps grow, though no token's does: times a state of zeros it would be NaN,
+// and whether a batch's tokens are joined in runs is not the formula's.  So the state is multiplied by the root 2^(l/2) twice: 0 stays 0, and past 2^254 any other is
+// infinite (those below the normal numbers aside).  Sums of steps stay finite, so that A of 0 has l = 0.  (The factor itself would be cheaper: 8192 tokens of 4096 channels
+// 215 us, by roots 221; 4102 tokens of 128 channels 24.7 and 25.0.)
+__device__ __forceinline__ float within(float steps) { return __builtin_amdgcn_fmed3f(steps, -3.40282347e38f, 3.40282347e38f); }
+__device__ __forceinline__ float run_root(float half_exponent) { return __builtin_amdgcn_exp2f(__builtin_amdgcn_fmed3f(half_exponent, -150.0f, 127.0f)); }
+__device__ __forceinline__ float behind_run(float root, float h, float brought) { return __builtin_fmaf(root * h, root, brought); }
 
 // Few tokens a sequence: LANES lanes a channel, NL states each; token after token from memory.  WHOLE: loads that no branch
 // parts (128 sequences of 4096 channels 17.3 -> 16.1 us).
@@ -206,6 +214,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
     // (two of each: a wavefront may be a tile ahead of the slowest one)
     __shared__ __attribute__((aligned(16))) vec brought[WT > 1 || PART == 2 ? 2 * T::THREADS : PART ? T::THREADS : 1],
         factor[WT > 1 || PART == 2 ? 2 * T::THREADS : PART ? T::THREADS : 1], begin[WT > 1 ? 2 * SETS : 1];
+    __shared__ float halves[PART == 1 ? T::THREADS : 1];
 
     // (workgroups side by side in channels share lines of memory, and B and C)
     for (long long id = blockIdx.x; id < xcd_padded(p.jobs); id += gridDim.x) {
@@ -225,12 +234,9 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
         const int ch = lane / LANES, c = c0 + ch, ln = lane % LANES, n0 = ln * NL;
         const bool mine = c < cend;
 
-        float a[NL], h[NL], through[NL];  // (through: the factor of all tokens of a piece)
+        float a[NL], h[NL], through = 0.0f, through_low = 0.0f;  // (through: the steps of all tokens of a piece, and what their sum lost to rounding)
 #pragma unroll
-        for (int i = 0; i < NL; i++) {
-            a[i] = h[i] = 0.0f;
-            through[i] = 1.0f;
-        }
+        for (int i = 0; i < NL; i++) a[i] = h[i] = 0.0f;
         if (mine) exponents<NL, false>(p, c, n0, a);
         // What a lane brings of a tile, one tile ahead.  Its places are pointers that go on by a tile's rows.
         unit x[T::PER], d[T::PER], g[T::PER];
@@ -330,16 +336,16 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
 
         if (tile0 < tile1) fetch(tile0);
 
-        // Workspace of a sequence: the state that it continues, the states of its parts, those of its pieces; the factors of both.
+        // Workspace of a sequence: the state that it continues, the states of its parts, those of its pieces; half the exponents of both (runs side by side have the sum of theirs).
         const long long step = (long long)p.channels * T::NP, at0 = (long long)c * T::NP + n0;
         const int all = (int)p.parts * (PIECES + 1);
-        float *states = PART ? p.part_states + (long long)place * (all + 1) * step + at0 : nullptr, *factors = PART ? p.part_factors + (long long)place * all * step + at0 : nullptr;
+        float *states = PART ? p.part_states + (long long)place * (all + 1) * step + at0 : nullptr, *halves_of = PART ? p.part_exponents + (long long)place * all * step + at0 : nullptr;
         auto take_in = [&](vec &f, vec &b, int which) {  // a part or piece behind what f and b hold
-            const vec pf = *reinterpret_cast<const vec *>(factors + which * step), pb = *reinterpret_cast<const vec *>(states + (which + 1) * step);
+            const vec pf = *reinterpret_cast<const vec *>(halves_of + which * step), pb = *reinterpret_cast<const vec *>(states + (which + 1) * step);
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                b[i] = __builtin_fmaf(pf[i], b[i], pb[i]);
-                f[i] *= pf[i];
+                b[i] = behind_run(run_root(pf[i]), b[i], pb[i]);
+                f[i] += pf[i];
             }
         };
         if constexpr (PART == 0) {
@@ -360,16 +366,18 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
         } else {  // a stretch of the parts before this one and a piece of its own by every wavefront, joined by all of them
             vec f, b, v, pf, pb;
 #pragma unroll
-            for (int i = 0; i < NL; i++) {
-                f[i] = pf[i] = 1.0f;
-                b[i] = v[i] = pb[i] = 0.0f;
-            }
+            for (int i = 0; i < NL; i++) f[i] = pf[i] = b[i] = v[i] = pb[i] = 0.0f;
             const int each = (part + WAVES - 1) / WAVES, end = min(part, (wave + 1) * each);
             if (mine) {
                 v = *reinterpret_cast<const vec *>(states);
                 take_in(pf, pb, (int)p.parts + part * PIECES + wave);
 #pragma unroll 4
                 for (int j = wave * each; j < end; j++) take_in(f, b, j);
+            }
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                f[i] = run_root(f[i]);
+                pf[i] = run_root(pf[i]);
             }
             factor[tid] = f;
             brought[tid] = b;
@@ -379,7 +387,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
             for (int w = 0; w < WAVES + wave; w++) {
                 const vec wf = factor[w * 64 + lane], wb = brought[w * 64 + lane];
 #pragma unroll
-                for (int i = 0; i < NL; i++) v[i] = __builtin_fmaf(wf[i], v[i], wb[i]);
+                for (int i = 0; i < NL; i++) v[i] = behind_run(wf[i], v[i], wb[i]);
             }
 #pragma unroll
             for (int i = 0; i < NL; i++) h[i] = v[i];
@@ -417,11 +425,12 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
                         }
                     }
                 }
+                const float half_sum = 0.5f * within(sum);
                 vec v, f;
 #pragma unroll
                 for (int i = 0; i < NL; i++) {
                     v[i] = local[i];
-                    f[i] = __builtin_amdgcn_exp2f(sum * a[i]);
+                    f[i] = run_root(half_sum * a[i]);
                 }
                 const int half = tile - tile0 & 1;
                 vec *all = brought + half * T::THREADS + set, *all_f = factor + half * T::THREADS + set;
@@ -442,7 +451,7 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
 #pragma unroll
                     for (int k = 0; k < N; k++)
 #pragma unroll
-                        for (int i = 0; i < NL; i++) h[i] = __builtin_fmaf(wf[k][i], h[i], wb[k][i]);
+                        for (int i = 0; i < NL; i++) h[i] = behind_run(wf[k][i], h[i], wb[k][i]);
                 };
                 int w = 0;
                 for (; w + 4 <= wt; w += 4) take(w, std::integral_constant<int, 4>());
@@ -504,8 +513,9 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
                 }
             }
             if constexpr (PART == 1) {
-#pragma unroll
-                for (int i = 0; i < NL; i++) through[i] *= __builtin_amdgcn_exp2f(sum_d * a[i]);
+                const float sum = within(through + sum_d), of_tile = sum - through;
+                through_low += (through - (sum - of_tile)) + (sum_d - of_tile);
+                through = sum;
             } else {
                 if (WT > 1 && wt == WT - 1) {
                     vec v;
@@ -542,30 +552,35 @@ __global__ __launch_bounds__(64 * WAVES, WT > 1 || LANES == 1 || (PART == 2 && L
             }
         }
         if constexpr (PART == 1) {  // the piece's, and by the first wavefront all pieces' together
+            float half = 0.5f * within(through + through_low);
             vec f, b;
 #pragma unroll
             for (int i = 0; i < NL; i++) {
-                f[i] = through[i];
+                f[i] = half * a[i];
                 b[i] = h[i];
             }
             auto keep = [&](int which) {
-                *reinterpret_cast<vec *>(factors + which * step) = f;
+                *reinterpret_cast<vec *>(halves_of + which * step) = f;
                 *reinterpret_cast<vec *>(states + (which + 1) * step) = b;
             };
             if (mine) keep((int)p.parts + part * PIECES + wave);
+#pragma unroll
+            for (int i = 0; i < NL; i++) f[i] = run_root(f[i]);
             factor[tid] = f;
             brought[tid] = b;
+            halves[tid] = half;
             __syncthreads();
             if (mine && wave == 0) {
 #pragma unroll
                 for (int w = 1; w < WAVES; w++) {
                     const vec wf = factor[w * 64 + lane], wb = brought[w * 64 + lane];
+                    half += halves[w * 64 + lane];
 #pragma unroll
-                    for (int i = 0; i < NL; i++) {
-                        b[i] = __builtin_fmaf(wf[i], b[i], wb[i]);
-                        f[i] *= wf[i];
-                    }
+                    for (int i = 0; i < NL; i++) b[i] = behind_run(wf[i], b[i], wb[i]);
                 }
+                half = within(half);
+#pragma unroll
+                for (int i = 0; i < NL; i++) f[i] = half * a[i];
                 keep(part);
             }
         } else if (mine && wt == WT - 1 && tile0 < tile1 && tile1 == tiles) {
@@ -622,7 +637,7 @@ int launch_scan(int dev, ScanParams &p, int seqs, int rows, int tokens) {
         void *ws = nullptr;
         if (part_bytes + list_bytes > 0) EH_TRY(get_workspace(dev, part_bytes + list_bytes, &ws));
         p.part_states = (float *)ws;
-        p.part_factors = (float *)((char *)ws + each * (all + 1));
+        p.part_exponents = (float *)((char *)ws + each * (all + 1));
         p.most = most;
         p.list = nullptr;
         if (least > 0) {

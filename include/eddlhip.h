@@ -612,9 +612,10 @@ int eddlhip_causal_conv(int dev, const float *X, long long ldx, const float *W, 
  *     h[c][i] = e^(d A[c][i]) h[c][i] + d x B[i],   Y = (sum_i C[i] h[c][i] + skip[c] x) silu(gate).
  * X, dt, gate, Y [rows][channels]; B and C [rows][groups * n], a vector for each of `groups` equal parts of the channels; A [channels][n]; skip and dt_bias
  * [channels] may be NULL (0), gate too (no factor).  The state is [pool][channels][n].  Y and the states lie on nothing else that is read.
- * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  Factors are multiplied over runs of
- * tokens: where e^(d A), d A summed over tokens one after another, passes the largest number, the state may be infinite or NaN, also one of zeros (it does not where no d A is
- * positive).  Sums and states are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups
+ * Once a state is infinite or NaN, what its channel brings from there on is infinite or NaN.  An infinite A counts as the largest number.  A token whose own e^(d A) passes the
+ * largest number makes any state infinite or NaN, also one of zeros.  Tokens are joined in runs of 8 and more, which ones is for the kernels to choose: a state that grows is what the formula gives
+ * as long as it is a number (0 stays 0), but may be NaN where the formula's is infinite; and where steps of both signs (softplus == 0) let a state pass the largest number and come back,
+ * it may be a number, infinite or NaN behind that.  Sums and states are fp32.  Workspace: the states between the parts of a long sequence of few channels, whose parts several workgroups
  * take, and the list of long sequences among many short ones. */
 int eddlhip_selective_scan(int dev, const float *X, long long ldx, const float *dt, long long lddt, const float *A, const float *B, long long ldb,
                            const float *C, long long ldc, const float *skip, const float *gate, long long ldg, const float *dt_bias, float *Y, long long ldy,

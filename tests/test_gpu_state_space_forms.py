@@ -68,6 +68,71 @@ def test_every_form_of_the_scan(hip, form, n):
         assert np.array_equal(y, y2) and np.array_equal(s, s2)
 
 
+def _bounds_of_runs(case, batch, pool):
+    """Bounds of outputs and states where runs of tokens are joined: F h + H, F a run's factor, H its state from zeros.
+
+    The recurrence's own bound takes errors relative to the state that it has: a token's rel |h|.  Joined, F h and H are off relative to themselves.  Where they cancel and the
+    state grows, F h may be large, and carry the errors of all of the run's tokens, beside a small F h + H: of h = 1 and a first product of -1 the recurrence carries one token's error
+    on, F h those of 8 or 16.  But every term, h or a product, times the factors behind it, is off by at most the sum of these tokens' errors relative to itself, in any order of
+    joining; and that is what the recurrence's bound is where nothing cancels: with the magnitudes of states, inputs, B and C."""
+    sizes = dict(case, x=np.abs(case["x"]), B=np.abs(case["B"]), C=np.abs(case["C"]))
+    _, err, _, after_err = selective_scan(**sizes, **batch.reference(np.abs(pool)))
+    return err, after_err
+
+
+@pytest.mark.parametrize("n", [1, 4, 8, 16, 32, 64])
+@pytest.mark.parametrize("form", FORMS)
+def test_growing_states_in_every_form(hip, form, n):
+    """Positive A, whose factors over a tile's or a sequence's tokens pass the largest number: a state of zeros stays zeros until its first input, one of 1e-30 grows as the
+    formula says, whichever kernel the batch takes."""
+    channels, groups, news = _sizes(form, n)
+    rng = np.random.default_rng([n, channels, 5])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, groups, softplus=False, gate=False, skip=False)
+    case["A"] = (0.5 + rng.random((channels, n))).astype(np.float32)
+    last = np.concatenate([np.arange(b - min(4, k), b) for b, k in zip(batch.offsets[1:], news)])  # four tokens of every sequence
+    # steps of 9: a factor of up to e^13 a token; the inputs come last
+    zero = dict(case, x=np.zeros_like(case["x"]), dt=np.full_like(case["dt"], 9.0))
+    zero["x"][last], zero["dt"][last] = case["x"][last], 0.3
+    batch.lengths[:] = batch.news  # (every sequence begins)
+    pool = np.zeros((batch.pool, channels, n), np.float32)
+    want, err, after, after_err = selective_scan(**zero, **batch.reference(pool))
+    y, s = _scan(hip, zero, batch, pool, False)
+    _check(y, want, err, "zeros")
+    _check(s, after, after_err, "zeros, state")
+    # states and inputs of 1e-30, a growth of e^60 to e^130 over the longest sequence
+    tiny = dict(case, x=case["x"] * np.float32(1e-30), dt=np.full_like(case["dt"], 88.0 / max(news)))
+    batch.lengths[:] = batch.news + 5
+    pool = (1e-30 * rng.standard_normal((batch.pool, channels, n))).astype(np.float32)
+    want, _, after, _ = selective_scan(**tiny, **batch.reference(pool))
+    err, after_err = _bounds_of_runs(tiny, batch, pool)
+    assert np.abs(want[batch.offsets[0]:batch.offsets[-1]]).max() < 1e32
+    y, s = _scan(hip, tiny, batch, pool, False)
+    _check(y, want, err, "1e-30")
+    _check(s, after, after_err, "1e-30, state")
+
+
+@pytest.mark.parametrize("n", [1, 4, 8, 16, 32, 64])
+@pytest.mark.parametrize("form", FORMS)
+def test_steps_whose_sum_passes_the_largest_number(hip, form, n):
+    """Steps of 1e38: negative A leaves nothing of what came before, A of 0 all of it."""
+    channels, groups, news = _sizes(form, n)
+    rng = np.random.default_rng([n, channels, 6])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, groups, softplus=False)
+    case["A"] = -np.exp(rng.standard_normal((channels, n), dtype=np.float32))
+    case["A"][::2, 0] = 0
+    case["dt"][:], case["x"] = 1e38, case["x"] * np.float32(1e-38)
+    batch.lengths[:] = batch.news + 5
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    for reverse in (False, True):
+        want, err, after, after_err = selective_scan(reverse=reverse, **case, **batch.reference(pool))
+        y, s = _scan(hip, case, batch, pool, reverse)
+        _check(y, want, err, reverse)
+        _check(s, after, after_err, (reverse, "state"))
+        assert np.all(np.isfinite(s)) and np.all(np.isfinite(y[batch.offsets[0]:batch.offsets[-1]]))
+
+
 # ------------------------------------------------------------------------------------------------- group norm
 # odd wide rows, whole and divided; odd maps, divided; even wide rows, whole; short groups of rows two numbers at a time; one group of them
 @pytest.mark.parametrize("images, channels, height, width, groups", [(2, 99, 9, 7, 3), (1, 45, 33, 31, 1), (1, 1, 257, 255, 1), (1, 3, 201, 199, 1), (2, 132, 5, 5, 2), (3, 30, 7, 5, 5),
