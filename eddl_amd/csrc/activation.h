@@ -1,5 +1,5 @@
-// exp, silu and softplus of the state space and group norm kernels: fp32, errors of a few roundings of the result over the whole range, infinities
-// and NaN as the formulas bring them.
+// exp, silu and softplus of the state space and group norm kernels: fp32, off by a few roundings of the result or, where that is more, by 2^-119: below the normal numbers the
+// instructions give 0, and with them what stands on 1 / (1 + e^-x) from x = -87 down.  Infinities and NaN as the formulas bring them.
 #pragma once
 
 namespace eddlhip {

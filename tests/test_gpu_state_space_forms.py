@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import test_gpu_state_space as base
-from state_space_ref import selective_scan
+from state_space_ref import EPS, selective_scan
 from test_gpu_state_space import Ragged, _check, _scan, _scan_case
 
 pytestmark = pytest.mark.gpu
@@ -158,3 +158,15 @@ def test_constant_groups_are_their_bias(hip, channels, pixels, groups):
     R = hip.array(x.transpose(0, 2, 1).reshape(-1, channels))
     hip.group_norm(R, R, groups, bias=hip.array(b), image_rows=pixels)
     assert np.array_equal(R.numpy().reshape(2, pixels, channels).transpose(0, 2, 1), want), "rows"
+
+
+def test_gate_where_its_exponential_passes_the_largest_number(hip):
+    """silu from -80 to -300: its size falls from 1e-33 below the smallest normal number; off by 2^-119 at most there, not by a share of itself."""
+    from eddl_amd.state_space import StateBatch
+    v = np.concatenate([np.linspace(-89, -80, 4000), np.linspace(-300, -89, 1000)]).astype(np.float32)
+    X, none, A = hip.full((1, len(v)), 1.0), hip.full((1, 1), 0.0), hip.full((len(v), 1), 0.0)
+    Y = hip.empty(X.shape)
+    hip.selective_scan(X, X, A, none, none, Y, StateBatch(hip.array(np.array([0, 1]), "int32"), 1), skip=hip.full((len(v),), 1.0), gate=hip.array(v[None]), softplus=False)
+    x = v.astype(np.float64)
+    want = x * np.exp(x) / (1 + np.exp(x))
+    assert np.all(np.abs(Y.numpy()[0] - want) <= 11 * EPS * np.abs(want) + 2.0 ** -119)
