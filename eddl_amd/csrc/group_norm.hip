@@ -3,10 +3,10 @@
 // Maps [images][channels][pixels], where a group is one stretch of memory, or rows of tokens [images * pixels][channels], where it is a
 // piece of every row.
 //
-// Bound: memory, 8 bytes a number, if a group is read once.  A group of up to 32768 numbers stays in the registers of a workgroup between its
-// sums and its outputs (group_norm_kernel, WHOLE).  A larger one is divided: the first launch brings mean and squared differences of every part, the second
-// joins them and reads the numbers again, from the last one to the first: what was read last may still be in the last-level cache.  The variance is that of differences
-// from a mean, never a difference of squares.
+// Bound: memory, 8 bytes a number, if a group is read once.  A group of up to 32768 numbers (in rows about 32000, where threads stay in their columns; of groups of
+// few channels all that are taken together) stays in the registers of a workgroup between its sums and its outputs (WHOLE).  A larger one is divided: the first launch
+// brings mean and squared differences of every part, the second joins them and reads the numbers again, from the last one to the first: what was read last may still be in the
+// last-level cache.  The variance is that of differences from a mean, never a difference of squares.
 //
 // Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.4 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 128 us (41 of
 // sums and 82 of outputs, both 6.5 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.8 us, two launches of 4.3 and 6.8; 1 x 512 x 7 x 7 4.8 us, the host's call.
@@ -184,7 +184,7 @@ struct Parts {
     }
 };
 
-constexpr int SHORT = 16;  // channels of a group in rows: with fewer, 64 bytes of a row are taken together
+constexpr int SHORT = 16;  // channels of a group in rows: of smaller ones as many are taken together as make 2 * SHORT channels, 128 bytes of a row
 
 constexpr int MOST_CHANNELS = 4096;  // of a group: their slopes and lifts lie in LDS
 

@@ -170,3 +170,20 @@ def test_gate_where_its_exponential_passes_the_largest_number(hip):
     x = v.astype(np.float64)
     want = x * np.exp(x) / (1 + np.exp(x))
     assert np.all(np.abs(Y.numpy()[0] - want) <= 11 * EPS * np.abs(want) + 2.0 ** -119)
+
+
+@pytest.mark.parametrize("per", [1, 2, 3, 4, 7, 8, 9, 13, 14, 15, 16, 17, 19, 27, 32, 33, 62, 96, 124, 130])
+def test_which_norms_take_the_workspace(hip, per):
+    """Groups of more than 32768 numbers of maps, of about 32000 of rows, groups side by side of fewer than 16 channels from 704 rows an image on: what the header says."""
+    def taken(rows, groups, tokens):
+        X = hip.full((rows, groups * per) if tokens else (1, groups * per, rows, 1), 1.0)
+        hip.workspace_trim()
+        hip.group_norm(X, X, groups)
+        return hip.workspace_bytes() > 0
+
+    assert not taken(32768 // per, 2, False) and taken(32768 // per + 1, 2, False)
+    assert not taken(31968 // per, 1, True) and taken(32768 // per + 1, 1, True)
+    if per < 16:
+        assert not taken(704, 40, True) and taken(1057, 40, True)
+    else:
+        assert not taken(31968 // per, 2, True) and taken(32768 // per + 1, 2, True)
