@@ -270,8 +270,8 @@ def CausalConvolution(parent, width, channels=None, use_bias=True, activation="s
         msg("CausalConvolution needs [batch, tokens, columns] with %s channels and a width of 2 to 8, not %s and %s" % (channels, shape, width), "CausalConvolution")
     if activation not in (None, "relu", "silu"):
         msg("CausalConvolution knows no activation %s" % activation, "CausalConvolution")
-    if states is not None and batch is None:
-        msg("states come with a batch", "CausalConvolution")
+    if states is not None and (batch is None or batch.slots is None):
+        msg("states come with a batch that names lengths and slots", "CausalConvolution")
     l = Layer("causal_conv", [parent], shape[:2] + [n], name, activation=activation, reverse=bool(reverse), batch=batch, states=states)
     l.params["W"] = np.zeros((n, int(width)), np.float32)
     if use_bias:
@@ -290,8 +290,8 @@ def SelectiveScan(parent, dt, vectors, state, groups=1, gate=None, softplus=True
             or vectors.out_shape[2] < need or (gate is not None and gate.out_shape[2] < shape[2]):
         msg("SelectiveScan needs [batch, tokens, channels], time steps of the same shape, %d columns of vectors and as many of a gate as channels, not %s"
             % (need, [l.out_shape for l in (parent, dt, *others)]), "SelectiveScan")
-    if states is not None and batch is None:
-        msg("states come with a batch", "SelectiveScan")
+    if states is not None and (batch is None or batch.slots is None):
+        msg("states come with a batch that names lengths and slots", "SelectiveScan")
     l = Layer("selective_scan", [parent, dt, vectors] + ([gate] if gate is not None else []), shape, name, state=n, groups=int(groups), softplus=bool(softplus), reverse=bool(reverse),
               batch=batch, states=states)
     l.params["A"] = np.repeat(-np.arange(1, n + 1, dtype=np.float32)[None], shape[2], 0)

@@ -1,4 +1,4 @@
-"""Sizes beyond 32 bits are refused by the group norm and state space operators: the library counts in ints."""
+"""Sizes beyond 32 bits are refused by the group norm and state space operators, whose library counts in ints; states by layers whose batch has no place for them."""
 import pytest
 
 from test_state_space_cpu import P, _Tensor, _passes, _refused, hip  # noqa: F401
@@ -40,3 +40,15 @@ def test_rows_slots_and_bounds_of_a_batch(hip):  # noqa: F811
             batch(most)
     with pytest.raises(ValueError):
         StateBatch(_Tensor((BIG + 4,), "int32", P[30]), 9)
+
+
+def test_layers_refuse_states_without_slots():
+    from eddl_amd import net as L
+    from eddl_amd.state_space import StateBatch
+    x, bare = L.Input([9, 24], 3), StateBatch(_Tensor((4,), "int32", P[30]), 9)
+    kept = StateBatch(_Tensor((4,), "int32", P[30]), 9, _Tensor((3,), "int32", P[31]), _Tensor((3,), "int32", P[32]))
+    layers = (lambda batch: L.CausalConvolution(x, 4, batch=batch, states=_Tensor((5, 3, 24))), lambda batch: L.SelectiveScan(x, x, x, 5, batch=batch, states=_Tensor((5, 24, 5))))
+    for layer in layers:
+        assert layer(kept).attrs["states"] is not None
+        with pytest.raises(RuntimeError, match="slots"):
+            layer(bare)
