@@ -133,6 +133,53 @@ def test_steps_whose_sum_passes_the_largest_number(hip, form, n):
         assert np.all(np.isfinite(s)) and np.all(np.isfinite(y[batch.offsets[0]:batch.offsets[-1]]))
 
 
+@pytest.mark.parametrize("n", [1, 4, 8, 16, 32, 64])
+@pytest.mark.parametrize("form", FORMS)
+def test_steps_of_both_signs_in_every_form(hip, form, n):
+    """Without softplus steps may be negative: states decay and grow in turns, by some e^9 over the longest sequence."""
+    channels, groups, news = _sizes(form, n)
+    rng = np.random.default_rng([n, channels, 7])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, groups, softplus=False)
+    case["dt"], case["A"] = 0.3 * rng.standard_normal(case["dt"].shape, dtype=np.float32), -rng.random((channels, n), dtype=np.float32)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    want, _, after, _ = selective_scan(**case, **batch.reference(pool))
+    err, after_err = _bounds_of_runs(case, batch, pool)
+    y, s = _scan(hip, case, batch, pool, False)
+    _check(y, want, err)
+    _check(s, after, after_err, "state")
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_inputs_and_outputs_of_one_tensor(hip, form):
+    """A block's numbers as columns of one tensor, the output's columns between the inputs'; a step without gate, skip and bias beside it gives other outputs, the states' bits."""
+    n = 16
+    channels, groups, news = _sizes(form, n)
+    rng = np.random.default_rng([channels, 8])
+    batch = Ragged(rng, news)
+    case = _scan_case(rng, batch, channels, n, groups)
+    pool = rng.standard_normal((batch.pool, channels, n), dtype=np.float32)
+    y, s = _scan(hip, case, batch, pool, False)
+    parts, at = {}, 1
+    for k in ("x", "B", "y", "dt", "C", "gate"):
+        width = channels if k == "y" else case[k].shape[1]
+        parts[k], at = (at, at + width), at + width
+    wide = np.full((batch.rows, at + 2), 5.0, np.float32)
+    for k, (a, b) in parts.items():
+        wide[:, a:b] = -7.0 if k == "y" else case[k]
+    T, S, d = hip.array(wide), hip.array(pool), lambda k: hip.array(case[k])
+    c = {k: T.columns(*ab) for k, ab in parts.items()}
+    hip.selective_scan(c["x"], c["dt"], d("A"), c["B"], c["C"], c["y"], batch.on(hip), states=S, skip=d("skip"), gate=c["gate"], dt_bias=d("dt_bias"))
+    wide[:, slice(*parts["y"])] = y
+    assert np.array_equal(T.numpy(), wide) and np.array_equal(S.numpy(), s)
+    S, Y = hip.array(pool), hip.full((batch.rows, channels), -7.0)
+    hip.selective_scan(c["x"], c["dt"], d("A"), c["B"], c["C"], Y, batch.on(hip), states=S, dt_bias=d("dt_bias"))
+    bare = dict(case, gate=None, skip=None)
+    want, err, after, after_err = selective_scan(**bare, **batch.reference(pool))
+    _check(Y.numpy(), want, err)
+    assert np.array_equal(S.numpy(), s) and np.all(batch.outside(Y.numpy()) == -7.0)
+
+
 # ------------------------------------------------------------------------------------------------- group norm
 # odd wide rows, whole and divided; odd maps, divided; even wide rows, whole; short groups of rows two numbers at a time; one group of them
 @pytest.mark.parametrize("images, channels, height, width, groups", [(2, 99, 9, 7, 3), (1, 45, 33, 31, 1), (1, 1, 257, 255, 1), (1, 3, 201, 199, 1), (2, 132, 5, 5, 2), (3, 30, 7, 5, 5),
