@@ -5,11 +5,11 @@
 //
 // Bound: memory, 8 bytes a number, if a group is read once.  A group of up to 32768 numbers (in rows about 32000, where threads stay in their columns; of groups of
 // few channels all that are taken together) stays in the registers of a workgroup between its sums and its outputs (WHOLE).  A larger one is divided: the first launch
-// brings mean and squared differences of every part, the second joins them and reads the numbers again, from the last one to the first: what was read last may still be in the
+// brings mean and variance of every part, the second joins them and reads the numbers again, from the last one to the first: what was read last may still be in the
 // last-level cache.  The variance is that of differences from a mean, never a difference of squares.
 //
-// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.4 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 128 us (41 of
-// sums and 82 of outputs, both 6.5 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.8 us, two launches of 4.3 and 6.8; 1 x 512 x 7 x 7 4.8 us, the host's call.
+// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.2 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 128 us (sums 40 and
+// outputs 82, both 6.5 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.4 us, two launches of 4.4 and 6.6; 1 x 512 x 7 x 7 4.9 us, the host's call.
 #include <math.h>
 
 #include <algorithm>
@@ -27,7 +27,7 @@ enum { WHOLE, SUMS, APPLY };  // what a launch does
 struct GroupNormParams {
     const float *X, *w, *b, *mod, *shift;
     float *Y;
-    float2 *parts;  // mean and squared differences of every part
+    float2 *parts;  // mean and variance of every part
     long long ldx, ldy;
     int images, channels, pixels, activation;
     unsigned groups;
@@ -83,10 +83,10 @@ __device__ __forceinline__ T block_sum(T x, float2 *place) {
 
 // Of n numbers, nth = 1 / n, whose sum gave `mean`: `off` holds the sum of their differences from it and that of the differences' squares.  The first is what the mean lost to rounding, so
 // that equal numbers have their own value as their mean, and nothing but the bias is left of them (of 1234.567, 32768 times, the mean's last bits made 0.04).
-__device__ __forceinline__ void settle(float &mean, float &squares, float nth, float2 off) {
+__device__ __forceinline__ void settle(float &mean, float &variance, float nth, float2 off) {
     const float more = off.x * nth, left = off.y - more * off.x;
     mean += more;
-    squares = left < 0.0f ? 0.0f : left;
+    variance = left < 0.0f ? 0.0f : left * nth;
 }
 
 template <int UNIT>
@@ -146,11 +146,11 @@ struct Coefficients {
     }
 };
 
-// Mean and squared differences of n more numbers taken into those of `count`.
-__device__ __forceinline__ void join(double &count, float &mean, float &squares, double n, float mean_n, float squares_n) {
+// Mean and variance of n more numbers taken into those of `count`: no sum of squares, which passes the largest number before the variance does.
+__device__ __forceinline__ void join(double &count, float &mean, float &variance, double n, float mean_n, float variance_n) {
     const float delta = mean_n - mean, share = (float)(n / (count + n));
     mean = __builtin_fmaf(delta, share, mean);
-    squares += squares_n + delta * delta * (float)count * share;
+    variance = variance * (1.0f - share) + variance_n * share + delta * (share * (1.0f - share)) * delta;  // (of the first n numbers nothing but their own, also of 1e20, whose square is infinite)
     count += n;
 }
 constexpr int MOST_PARTS = 256;  // of a group
@@ -167,20 +167,20 @@ struct Parts {
             if (lane + k * 64 < split) v[k] = parts[lane + k * 64];
         }
     }
-    __device__ __forceinline__ void join(int split, long long part, long long total, float &mean, float &squares) const {
+    __device__ __forceinline__ void join(int split, long long part, long long total, float &mean, float &variance) const {
         const int lane = threadIdx.x & 63;
         const float first = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v[0].x)));  // (differences from it: equal means are the mean)
-        float sum = 0.0f, n[MOST_PARTS / 64];
+        float sum = 0.0f, share[MOST_PARTS / 64];
 #pragma unroll
         for (int k = 0; k < MOST_PARTS / 64; k++) {
-            n[k] = lane + k * 64 < split ? (float)min(part, total - (lane + k * 64) * part) : 0.0f;
-            sum += (v[k].x - first) * (n[k] / (float)total);
+            share[k] = lane + k * 64 < split ? (float)min(part, total - (lane + k * 64) * part) / (float)total : 0.0f;
+            sum += (v[k].x - first) * share[k];
         }
         mean = first + wave_sum(sum);
         sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < MOST_PARTS / 64; k++) sum += v[k].y + (v[k].x - mean) * (v[k].x - mean) * n[k];
-        squares = wave_sum(sum);
+        for (int k = 0; k < MOST_PARTS / 64; k++) sum += v[k].y * share[k] + (v[k].x - mean) * share[k] * (v[k].x - mean);
+        variance = wave_sum(sum);
     }
 };
 
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
         const int image = which / p.groups, c0 = (int)(which % p.groups) * p.per;
         const float *X = p.X + (ROWS ? (long long)image * p.pixels * p.ldx + c0 : ((long long)image * p.channels + c0) * p.pixels);
         float *Y = p.Y + (ROWS ? (long long)image * p.pixels * p.ldy + c0 : ((long long)image * p.channels + c0) * p.pixels);
-        float mean = 0.0f, squares = 0.0f;
+        float mean = 0.0f, variance = 0.0f;
         double seen = 0.0;
         Coefficients<1> own;
         auto ask = [&](int c) {
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
         Parts parts;  // (what comes back first is asked for first)
         if (WHAT == APPLY) parts.ask(p.parts + (long long)which * (int)p.split, (int)p.split);
         auto prepare = [&]() {  // slopes and lifts of the group's channels
-            const float scale = 1.0f / sqrtf(squares / (float)count + p.eps);
+            const float scale = 1.0f / sqrtf(variance + p.eps);
             if (WHAT == APPLY) __syncthreads();  // (the job before may still read them)
             for (int c = threadIdx.x; c < p.per; c += THREADS) {
                 own.make(scale, slopes + c, lifts + c);
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 }
             }
             if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
-                parts.join((int)p.split, p.part, count, mean, squares);
+                parts.join((int)p.split, p.part, count, mean, variance);
                 prepare();
             }
             if (WHAT != APPLY) {
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                     else sum += v[k].v[0];
                 }
                 const float n = (float)min((long long)TILE, last - at), nth = 1.0f / n;
-                float mean_n = block_sum<THREADS>(sum, red) * nth, squares_n;
+                float mean_n = block_sum<THREADS>(sum, red) * nth, variance_n;
                 float2 off = {0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < NV; k++)
@@ -280,12 +280,12 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                             off.y = __builtin_fmaf(d, d, off.y);
                         }
                     }
-                settle(mean_n, squares_n, nth, block_sum<THREADS>(off, red));
+                settle(mean_n, variance_n, nth, block_sum<THREADS>(off, red));
                 if (WHAT == SUMS) {
-                    join(seen, mean, squares, n, mean_n, squares_n);
+                    join(seen, mean, variance, n, mean_n, variance_n);
                 } else {
                     mean = mean_n;
-                    squares = squares_n;
+                    variance = variance_n;
                     prepare();
                 }
             }
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_kernel(const GroupNormPara
                 }
             }
         }
-        if (WHAT == SUMS && threadIdx.x == 0) p.parts[(long long)which * (int)p.split + (int)piece] = float2{mean, squares};
+        if (WHAT == SUMS && threadIdx.x == 0) p.parts[(long long)which * (int)p.split + (int)piece] = float2{mean, variance};
     }
 }
 
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                 return sums[mine ? g : 0];
             }
         };
-        float mean = 0.0f, squares = 0.0f, slope[UNIT], lift[UNIT];
+        float mean = 0.0f, variance = 0.0f, slope[UNIT], lift[UNIT];
         double seen = 0.0;
         Coefficients<UNIT> own;
         if (WHAT != SUMS && mine) own.ask(p, image, c);
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
         Parts parts;  // (what comes back first is asked for first)
         if (WHAT == APPLY && ONE) parts.ask(all_parts, (int)p.split);
         auto prepare = [&]() {
-            if (mine) own.make(1.0f / sqrtf(squares / (float)total + p.eps), slope, lift);
+            if (mine) own.make(1.0f / sqrtf(variance + p.eps), slope, lift);
         };
         for (long long at = first; at < last; at += (long long)rows_at_once * NV) {
             const long long step_x = rows_at_once * p.ldx, step_y = rows_at_once * p.ldy;
@@ -382,17 +382,17 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
             }
             if (WHAT == APPLY && at == first) {  // (while the first numbers are on their way)
                 if constexpr (ONE) {
-                    parts.join((int)p.split, p.part * p.per, total, mean, squares);
+                    parts.join((int)p.split, p.part * p.per, total, mean, variance);
                 } else {
                     __syncthreads();
                     for (int j = wave; j < here; j += THREADS / 64) {
                         parts.ask(all_parts + j * (int)p.split, (int)p.split);
-                        parts.join((int)p.split, p.part * p.per, total, mean, squares);
-                        if (lane == 0) stat[j] = float2{mean, squares};
+                        parts.join((int)p.split, p.part * p.per, total, mean, variance);
+                        if (lane == 0) stat[j] = float2{mean, variance};
                     }
                     __syncthreads();
                     mean = stat[mine ? g : 0].x;
-                    squares = stat[mine ? g : 0].y;
+                    variance = stat[mine ? g : 0].y;
                 }
                 prepare();
             }
@@ -405,7 +405,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
             if (WHAT != APPLY) {
                 const double n = (double)min((long long)rows_at_once * NV, last - at) * p.per;
                 const float nth = 1.0f / (float)n;
-                float mean_n = group_sum(sum) * nth, squares_n;
+                float mean_n = group_sum(sum) * nth, variance_n;
                 float2 off = {0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < NV; k++)
@@ -417,12 +417,12 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                             off.y = __builtin_fmaf(d, d, off.y);
                         }
                     }
-                settle(mean_n, squares_n, nth, group_sum(off));
+                settle(mean_n, variance_n, nth, group_sum(off));
                 if (WHAT == SUMS) {
-                    join(seen, mean, squares, n, mean_n, squares_n);
+                    join(seen, mean, variance, n, mean_n, variance_n);
                 } else {
                     mean = mean_n;
-                    squares = squares_n;
+                    variance = variance_n;
                     prepare();
                 }
             }
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(THREADS) void group_norm_rows_kernel(const GroupNor
                 }
             }
         }
-        if (WHAT == SUMS && tr == 0 && cu % units == 0) p.parts[((long long)image * (int)p.groups + g0 + g) * (int)p.split + (int)piece] = float2{mean, squares};
+        if (WHAT == SUMS && tr == 0 && cu % units == 0) p.parts[((long long)image * (int)p.groups + g0 + g) * (int)p.split + (int)piece] = float2{mean, variance};
     }
 }
 

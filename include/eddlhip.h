@@ -583,8 +583,9 @@ int eddlhip_norm_residual(int dev, const float *X, long long ldx, const float *R
  *     n = (x - mean) / sqrt(variance + eps) w + b,   Y = act(n (1 + mod) + shift).
  * channels_last == 0: maps X, Y [images][channels][pixels], ldx and ldy are not looked at.  Otherwise rows of tokens [images * pixels][channels] that lie
  * ldx and ldy floats apart.  Up to 4096 channels a group.  w, b [channels], mod and shift [images][channels]; NULL: 1, 0, 0, 0.  Y may be X (rows of the same distance).  An image
- * whose group holds an infinity or NaN is NaN in that group (0 behind _RELU_LAYER); images and groups do not reach one another.  Workspace: means and squared differences of the
- * parts of a group that a workgroup's registers do not hold: of more than 32768 numbers in maps, of about 32000 in rows, and in rows whose groups have fewer than 16 channels, some of
+ * whose group holds an infinity or NaN is NaN in that group (0 behind _RELU_LAYER); images and groups do not reach one another.  Sums are fp32, over
+ * 32768 numbers at most before they are divided: where such a sum of the differences' squares passes the largest number, n is b, where one of the numbers does, NaN.  Workspace: means and
+ * variances of the parts of a group that a workgroup's registers do not hold: of more than 32768 numbers in maps, of about 32000 in rows, and in rows whose groups have fewer than 16 channels, some of
  * which share a workgroup, from about 700 pixels an image on.  A step with such norms runs once before it is recorded. */
 int eddlhip_group_norm(int dev, const float *X, long long ldx, float *Y, long long ldy, int images, int channels, int pixels, int channels_last,
                        int groups, const float *w, const float *b, float eps, const float *mod, const float *shift, int activation);

@@ -234,3 +234,38 @@ def test_which_norms_take_the_workspace(hip, per):
         assert not taken(704, 40, True) and taken(1057, 40, True)
     else:
         assert not taken(31968 // per, 2, True) and taken(32768 // per + 1, 2, True)
+
+
+@pytest.mark.parametrize("pixels", [50, 30000])
+def test_large_numbers_of_small_spread(hip, pixels):
+    """Numbers about 3e20, 1e17 apart: a mean whose square is beyond the largest number, differences whose squares are not.  And equal ones of 1e20."""
+    rng = np.random.default_rng(pixels)
+    x = (3e20 + 1e17 * rng.standard_normal((2, 4, pixels))).astype(np.float32)
+    x[1, 2:] = 1e20
+    b = rng.standard_normal(4, dtype=np.float32)
+    want, err = base.group_norm(x, 2, None, b, 1e-5, None, None, None)
+    err[1, 2:] = 0
+    want[1, 2:] = b[2:, None]
+    X = hip.array(x.reshape(2, 4, pixels, 1))
+    hip.group_norm(X, X, 2, bias=hip.array(b))
+    _check(X.numpy().reshape(x.shape), want, err, "maps")
+    R = hip.array(x.transpose(0, 2, 1).reshape(-1, 4))
+    hip.group_norm(R, R, 2, bias=hip.array(b), image_rows=pixels)
+    _check(R.numpy().reshape(2, pixels, 4).transpose(0, 2, 1), want, err, "rows")
+
+
+@pytest.mark.parametrize("pixels", [50, 30000])
+def test_squares_beyond_the_largest_number(hip, pixels):
+    """What the header says of numbers that fp32 sums do not hold: squares beyond it leave the bias, sums beyond it NaN; the other group is as it was."""
+    rng = np.random.default_rng(pixels)
+    x = rng.standard_normal((1, 4, pixels), dtype=np.float32)
+    b = rng.standard_normal(4, dtype=np.float32)
+    for scale, left in ((1e21, b), (2e38, np.nan * b)):
+        big = x.copy()
+        big[0, :2] = scale * (np.abs(x[0, :2]) / np.abs(x[0, :2]).max() if scale > 1e30 else x[0, :2])
+        X, plain = hip.array(big.reshape(1, 4, pixels, 1)), hip.array(x.reshape(1, 4, pixels, 1))
+        for t in (X, plain):
+            hip.group_norm(t, t, 2, bias=hip.array(b))
+        got = X.numpy()[0, :, :, 0]
+        assert np.array_equal(got[:2], np.broadcast_to(left[:2, None], (2, pixels)), equal_nan=True)
+        assert np.array_equal(got[2:], plain.numpy()[0, 2:, :, 0])
