@@ -8,8 +8,8 @@
 // brings mean and variance of every part, the second joins them and reads the numbers again, from the last one to the first: what was read last may still be in the
 // last-level cache.  The variance is that of differences from a mean, never a difference of squares.
 //
-// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.2 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 128 us (sums 40 and
-// outputs 82, both 6.5 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.4 us, two launches of 4.4 and 6.6; 1 x 512 x 7 x 7 4.9 us, the host's call.
+// Measured: rows of 64 images of 196 tokens of 768 channels, modulated, 17.2 us (4.5 TB/s); maps of 4 x 64 x 512 x 512, groups of 524288 numbers, 126 us (sums 39 and
+// outputs 80, both 6.7 TB/s); rows of 3 x 1369 x 330, groups of 41070, 10.4 us, two launches of 4.4 and 6.6; 1 x 512 x 7 x 7 4.9 us, the host's call.
 #include <math.h>
 
 #include <algorithm>

@@ -615,7 +615,7 @@ int launch_scan(int dev, ScanParams &p, int seqs, int rows, int tokens) {
     // By the workgroups that there are, in multiples of the compute units: four wavefronts of different channels do the least work a token; where that leaves
     // the device half empty, they divide the tokens of a quarter of the channels (512 tokens of 2048 channels, us: 16 sequences 107 against 128, 12 105 and 95, 4 84 and
     // 36); where that would, too, eight do (2 sequences 28 and 22); and where those do not meet every unit, sequences are divided over workgroups (1000 tokens of
-    // 1024 channels: not divided 39 us, divided 20; 8192 of 4096, as many workgroups as units: 215 and 276, since all exponentials are formed twice).
+    // 1024 channels: not divided 39 us, divided 20; 8192 of 4096, as many workgroups as units: 221 and 276, since all exponentials are formed twice).
     using Alone = ScanTile<LANES, NL, 4, 1>;
     using Four = ScanTile<LANES, NL, 4, 4>;
     using Eight = ScanTile<LANES, NL, 8, 8>;
