@@ -127,3 +127,22 @@ def test_a_relu_behind_a_group_norm_is_the_relu_layer(hip, maps):
         assert np.array_equal(a, b, equal_nan=True)
     fine = ~np.isnan(outs[0][1])
     assert np.array_equal(outs[0][0][fine], outs[0][1][fine])
+
+
+@pytest.mark.parametrize("channels, pixels, groups", [(6, 35, 3), (8, 20000, 2), (30, 1500, 2), (96, 400, 2), (4, 3000, 2)])
+def test_relu_layer_of_a_norm_is_the_relu(hip, channels, pixels, groups):
+    """The "relu_layer" is the norm without an activation and ``Backend.relu`` behind it, bit for bit; NaN among the numbers, groups whole and divided, maps and rows."""
+    rng = np.random.default_rng([channels, pixels])
+    x = rng.standard_normal((2, channels, pixels), dtype=np.float32)
+    x[1, 0, pixels // 2] = np.nan
+    w, b = (hip.array(rng.standard_normal(channels, dtype=np.float32)) for _ in range(2))
+    for t, tokens in ((x.reshape(2, channels, pixels, 1), None), (x.transpose(0, 2, 1).reshape(-1, channels), pixels)):
+        X = hip.array(t)
+        plain, want, got, kept = (hip.full(t.shape, -7.0) for _ in range(4))
+        hip.group_norm(X, plain, groups, w, b, image_rows=tokens)
+        hip.relu(plain, want)
+        hip.group_norm(X, got, groups, w, b, activation="relu_layer", image_rows=tokens)
+        hip.group_norm(X, kept, groups, w, b, activation="relu", image_rows=tokens)
+        n, k = plain.numpy(), kept.numpy()
+        assert np.isnan(n).sum() == channels // groups * pixels
+        assert np.array_equal(got.numpy(), want.numpy()) and np.array_equal(np.isnan(k), np.isnan(n)) and np.array_equal(np.nan_to_num(k), want.numpy())
