@@ -5,6 +5,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <vector>
+
 #include "common.h"
 
 namespace eddlhip {
@@ -48,17 +50,39 @@ int use_device(int dev) {
     return 0;
 }
 
+// Whether the program captures the device's stream into a graph of its own.
+static bool program_is_capturing(const DeviceState &s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (s.stream == nullptr || s.capturing) return false;
+    if (hipStreamIsCapturing(s.stream, &status) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return status != hipStreamCaptureStatusNone;
+}
+
+// A graph of the program's that names the workspace can be launched at any time, and nothing tells the library: such memory stays until the shutdown.
+static std::vector<void *> g_named[EDDLHIP_MAX_DEVICES];
+static int leave_workspace(int dev) {
+    DeviceState &s = g_state[dev];
+    if (s.program_names_workspace) g_named[dev].push_back(s.workspace);
+    else EH_TRY_HIP(hipFree(s.workspace));
+    s.workspace = nullptr;
+    s.workspace_bytes = 0;
+    s.program_names_workspace = false;
+    return 0;
+}
+
 int get_workspace(int dev, size_t bytes, void **ptr) {
     DeviceState &s = g_state[dev];
+    const bool program = bytes > 0 && program_is_capturing(s);
     if (bytes > s.workspace_bytes) {
-        if (s.capturing)
+        if (s.capturing || program)
             return set_error(EDDLHIP_EINVAL, "the workspace would have to grow to %zu bytes while a graph is being recorded: "
                              "run the same calls once before recording them", bytes);
         if (s.workspace) {
             EH_TRY_HIP(hipStreamSynchronize(s.stream));
-            EH_TRY_HIP(hipFree(s.workspace));
-            s.workspace = nullptr;
-            s.workspace_bytes = 0;
+            EH_TRY(leave_workspace(dev));
         }
         size_t want = (bytes + (size_t(1) << 20) - 1) & ~((size_t(1) << 20) - 1);
         hipError_t e = hipMalloc(&s.workspace, want);
@@ -70,6 +94,7 @@ int get_workspace(int dev, size_t bytes, void **ptr) {
         s.workspace_generation++;
     }
     if (s.capturing && bytes > 0) s.capture_used_workspace = true;
+    if (program) s.program_names_workspace = true;
     *ptr = s.workspace;
     return 0;
 }
@@ -78,9 +103,7 @@ int release_workspace(int dev) {
     DeviceState &s = g_state[dev];
     if (s.workspace == nullptr) return 0;
     EH_TRY_HIP(hipStreamSynchronize(s.stream));
-    EH_TRY_HIP(hipFree(s.workspace));
-    s.workspace = nullptr;
-    s.workspace_bytes = 0;
+    EH_TRY(leave_workspace(dev));
     s.workspace_generation++;  // graphs recorded before name memory that is gone
     return 0;
 }
@@ -112,6 +135,10 @@ int eddlhip_shutdown(int dev) {
     EH_TRY_HIP(hipDeviceSynchronize());
     EH_TRY(eddlhip_conv2d_uncache_filters(dev, nullptr));
     if (s.workspace) EH_TRY_HIP(hipFree(s.workspace));
+    while (!g_named[dev].empty()) {
+        EH_TRY_HIP(hipFree(g_named[dev].back()));
+        g_named[dev].pop_back();
+    }
     if (s.flag) EH_TRY_HIP(hipFree(s.flag));
     for (hipStream_t cs : s.copy_stream)
         if (cs) EH_TRY_HIP(hipStreamDestroy(cs));
@@ -132,6 +159,7 @@ int eddlhip_workspace_bytes(int dev, size_t *bytes) {
 int eddlhip_workspace_trim(int dev) {
     EH_TRY(use_device(dev));
     EH_NOT_CAPTURING(dev, "eddlhip_workspace_trim");
+    EH_REQUIRE(!program_is_capturing(state(dev)), "eddlhip_workspace_trim is not possible while the program captures the stream");
     return release_workspace(dev);
 }
 

@@ -59,7 +59,8 @@ int eddlhip_pointer_device(const void *ptr, int *device);
  * device, because calls share the workspace and counters and must not overlap, whatever their streams; the old stream may have been
  * destroyed.  A program that captures the new stream into a graph of its own (and not by eddlhip_graph_begin) is not made to wait,
  * and neither is its next change of stream: it sees to that order itself, and that such a graph's replays do not overlap with
- * the library's calls on the device. */
+ * the library's calls on the device.  The same calls run once before, as before eddlhip_graph_begin: a workspace that would have to grow is refused.  The workspace that such a graph
+ * names stays as it is when a larger call takes another or eddlhip_workspace_trim lets it go, until eddlhip_shutdown. */
 int eddlhip_set_stream(int dev, void *hip_stream);
 int eddlhip_synchronize(int dev);
 int eddlhip_malloc(int dev, size_t bytes, void **dev_ptr);
